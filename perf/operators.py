@@ -119,7 +119,9 @@ def _logits(case, gen, dev):
     rows, vocab = case["rows"], case["vocab"]
     width = -(-vocab // 64) * 64 if case["padded"] else vocab
     x = torch.randn(rows, width, generator=gen, device=dev, dtype=torch.float32).mul_(2.2).sub_(3.0)
-    liked = torch.randint(0, vocab, (rows, 6), generator=gen, device=dev)
+    # one in each sixth of the vocabulary: different tokens, since a scatter to the same place twice keeps either
+    sixth = vocab // 6
+    liked = torch.randint(0, sixth, (rows, 6), generator=gen, device=dev) + torch.arange(6, device=dev) * sixth
     x.scatter_(1, liked, torch.rand(rows, 6, generator=gen, device=dev) * 16.0)
     x[:, vocab:] = 0.0
     return x.to(DTYPES[case["dtype"]])[:, :vocab], liked
