@@ -41,6 +41,10 @@ static inline int64_t round_up(int64_t v, int64_t a) { return (v + a - 1) / a * 
 // elements of 4 bytes in an unsigned 32-bit register (8 * 2^26 * 4 = 2^31).
 constexpr int kMaxN = 1 << 26;
 
+// Rows of logits: a thread counts a row's elements in an int, with some thousands to spare; a row's place in
+// 64 bits.
+constexpr int64_t kMaxVocab = 1ll << 30, kMaxPitch = 1ll << 40;
+
 // Workspace plan of one GEMM: where the packed weight and (if needed) the
 // packed activations live.
 struct LinearPlan {
@@ -458,6 +462,97 @@ int gptmi_softmax(const void* x, void* out, int64_t M, int64_t H, int dtype, voi
   }
   launch_softmax(x, out, M, (int)H, dtype == GPTMI_F16, (hipStream_t)stream);
   return check_launch("softmax");
+}
+
+// What the operators on rows of logits ask of them.
+static int check_logits(const char* what, const void* x, int64_t ld, float temperature, int64_t M, int64_t V,
+                        int dtype) {
+  if (!x || M <= 0 || V <= 0 || ld < 0 || !dtype_ok(dtype) || !(temperature > 0.0f) || isinf(temperature) ||
+      ((uintptr_t)x & (dtype == GPTMI_F16 ? 1 : 3)) != 0) {
+    set_error("%s: invalid argument", what);
+    return GPTMI_ERR_INVALID;
+  }
+  if (M >= 1ll << 31 || V > kMaxVocab || ld > kMaxPitch) {
+    set_error("%s: %lld rows of %lld logits at a pitch of %lld are beyond the supported 2^31 - 1, 2^30 and 2^40", what,
+              (long long)M, (long long)V, (long long)ld);
+    return GPTMI_ERR_UNSUPPORTED;
+  }
+  return GPTMI_OK;
+}
+
+static int check_logits_gradient(const char* what, const void* grad, int64_t ld_grad, int64_t M, int64_t V, int dtype) {
+  if (!grad || (M > 1 && ld_grad < V) || ((uintptr_t)grad & (dtype == GPTMI_F16 ? 1 : 3)) != 0) {
+    set_error("%s: invalid gradient", what);
+    return GPTMI_ERR_INVALID;
+  }
+  if (ld_grad > kMaxPitch) {
+    set_error("%s: a pitch of %lld is beyond the supported 2^40", what, (long long)ld_grad);
+    return GPTMI_ERR_UNSUPPORTED;
+  }
+  return GPTMI_OK;
+}
+
+static LogitRows logit_rows(const void* x, int64_t ld, float temperature, int64_t M, int64_t V, int dtype) {
+  return LogitRows{x, ld, M, (int)V, temperature, dtype == GPTMI_F16};
+}
+
+int gptmi_token_log_probs(const void* logits, int64_t ld, const int64_t* tokens, float temperature, float* log_probs,
+                          float* entropy, int64_t top, float* top_log_probs, int64_t* top_tokens, int64_t M, int64_t V,
+                          int dtype, void* stream) {
+  const int rc = check_logits("token_log_probs", logits, ld, temperature, M, V, dtype);
+  if (rc) return rc;
+  if ((log_probs && !tokens) || top < 0 || top > V || (top > 0 && (!top_log_probs || !top_tokens)) ||
+      (!log_probs && !entropy && top == 0)) {
+    set_error("token_log_probs: invalid argument");
+    return GPTMI_ERR_INVALID;
+  }
+  if (top > GPTMI_MAX_TOP) {
+    set_error("token_log_probs: %lld top tokens are beyond the supported %d", (long long)top, GPTMI_MAX_TOP);
+    return GPTMI_ERR_UNSUPPORTED;
+  }
+  launch_token_log_probs(logit_rows(logits, ld, temperature, M, V, dtype), tokens, (int)top, log_probs, entropy,
+                         top_log_probs, top_tokens, (hipStream_t)stream);
+  return check_launch("token_log_probs");
+}
+
+int gptmi_token_log_probs_backward(const void* logits, int64_t ld, const int64_t* tokens, float temperature,
+                                   const float* d_log_probs, const float* d_entropy, int64_t top,
+                                   const int64_t* top_tokens, const float* d_top_log_probs, void* grad,
+                                   int64_t ld_grad, int64_t M, int64_t V, int dtype, void* stream) {
+  int rc = check_logits("token_log_probs_backward", logits, ld, temperature, M, V, dtype);
+  if (!rc) rc = check_logits_gradient("token_log_probs_backward", grad, ld_grad, M, V, dtype);
+  if (rc) return rc;
+  if ((d_log_probs && !tokens) || top < 0 || (top > 0 && (!top_tokens || !d_top_log_probs))) {
+    set_error("token_log_probs_backward: invalid argument");
+    return GPTMI_ERR_INVALID;
+  }
+  if (top > GPTMI_MAX_TOP) {
+    set_error("token_log_probs_backward: %lld top tokens are beyond the supported %d", (long long)top, GPTMI_MAX_TOP);
+    return GPTMI_ERR_UNSUPPORTED;
+  }
+  launch_token_log_probs_backward(logit_rows(logits, ld, temperature, M, V, dtype), tokens, d_log_probs, d_entropy,
+                                  (int)top, top_tokens, d_top_log_probs, grad, ld_grad, (hipStream_t)stream);
+  return check_launch("token_log_probs_backward");
+}
+
+int gptmi_distillation_loss(const void* logits, int64_t ld, const int64_t* teacher_tokens, const void* teacher_logits,
+                            int64_t k, float temperature, const float* weights, float* losses, void* grad,
+                            int64_t ld_grad, int64_t M, int64_t V, int dtype, int teacher_dtype, void* stream) {
+  int rc = check_logits("distillation_loss", logits, ld, temperature, M, V, dtype);
+  if (!rc && grad) rc = check_logits_gradient("distillation_loss", grad, ld_grad, M, V, dtype);
+  if (rc) return rc;
+  if (!teacher_tokens || !teacher_logits || k <= 0 || (!losses && !grad) || !dtype_ok(teacher_dtype) ||
+      ((uintptr_t)teacher_logits & (teacher_dtype == GPTMI_F16 ? 1 : 3)) != 0) {
+    set_error("distillation_loss: invalid argument");
+    return GPTMI_ERR_INVALID;
+  }
+  if (k > GPTMI_MAX_TOP) {
+    set_error("distillation_loss: %lld teacher's logits a row are beyond the supported %d", (long long)k, GPTMI_MAX_TOP);
+    return GPTMI_ERR_UNSUPPORTED;
+  }
+  launch_distillation(logit_rows(logits, ld, temperature, M, V, dtype), teacher_tokens, teacher_logits,
+                      teacher_dtype == GPTMI_F16, (int)k, weights, losses, grad, ld_grad, (hipStream_t)stream);
+  return check_launch("distillation_loss");
 }
 
 size_t gptmi_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, int wlayout) {

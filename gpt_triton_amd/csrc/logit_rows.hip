@@ -1,0 +1,549 @@
+// Rows of logits: log probabilities of given tokens with the row's entropy and its most likely tokens, their
+// gradient, and the distillation loss against a teacher's top logits with its gradient.
+//
+// One workgroup per row.  With z = x / temperature, m = max x, e_j = exp((x_j - m) / temperature), S = sum e_j:
+//   log p_j = (x_j - m) / temperature - log S          H = -sum p_j log p_j = log S - sum e_j log e_j / S
+// Every term of H's second form is at least 0, so neither loses bits to the other; S is 1 for each logit that
+// equals m plus the sum of the others, and log S = log1p of that sum where one does: a confident token's log
+// probability, -1e-5 say, keeps its bits.  Maximum, sums and logarithms are fp32.
+#include "common.h"
+
+namespace gptmi {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr int kMaxTop = 128;     // top tokens, and a teacher's entries
+constexpr int kCandidates = 2048;
+
+template <typename T> struct RowVec;
+template <> struct RowVec<_Float16> {
+  typedef h8 V;
+  static constexpr int N = 8;
+};
+template <> struct RowVec<float> {
+  typedef f4 V;
+  static constexpr int N = 4;
+};
+
+// A row as the workgroup's threads share it: 16-byte chunks from the first aligned address on, dealt one behind
+// the other, and in front and behind at most 2 (N - 1) single elements, one for each of the first threads.
+template <typename T, int NT>
+struct Row {
+  typedef typename RowVec<T>::V V;
+  static constexpr int N = RowVec<T>::N;
+  const T* x;
+  int vocab, lead, chunks, loose;  // loose: the index of this thread's single element, or -1
+  __device__ __forceinline__ Row(const T* row, int vocab_) : x(row), vocab(vocab_) {
+    const int ahead = (int)((-(intptr_t)row & 15) / (int)sizeof(T));
+    lead = ahead < vocab ? ahead : vocab;
+    chunks = (vocab - lead) / N;
+    const int t = threadIdx.x, singles = vocab - chunks * N;
+    loose = t < lead ? t : t < singles ? t + chunks * N : -1;
+  }
+  // f(values, index of the first of them, how many: N or 1) for this thread's part of the row
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    for (int c = threadIdx.x; c < chunks; c += NT) {
+      const V v = reinterpret_cast<const V*>(x + lead)[c];
+      float y[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) y[j] = (float)v[j];
+      f(y, lead + c * N, std::integral_constant<int, N>{});
+    }
+    if (loose >= 0) {
+      const float y[1] = {(float)x[loose]};
+      f(y, loose, std::integral_constant<int, 1>{});
+    }
+  }
+  __device__ __forceinline__ float at(int64_t i) const { return (float)x[i]; }
+};
+
+struct Sums {
+  float s, u, n;  // sum of e without the logits that equal the maximum, sum of e log2 e, how many equal it
+};
+
+template <int NT>
+struct Shared {
+  static constexpr int W = NT / kWave;
+  float max[W], low[W];
+  Sums sums[W];
+  int count, scan[W];
+};
+
+// What a row's softmax needs.
+struct Stats {
+  float m, shift, c, inv_tau;  // maximum; what is subtracted (0 where nothing is finite); log2(e) / tau; 1 / tau
+  float S, inv, log_s;         // all 0 where no token has any probability
+  float entropy;
+  __device__ __forceinline__ float log2_e(float x) const { return (x - shift) * c; }
+  __device__ __forceinline__ float log_p(float x) const {
+    return S == 0.f ? -INFINITY : (x - shift) * inv_tau - log_s;
+  }
+};
+
+// Sum of c over the threads in front of this one; total: over all.
+template <int NT>
+__device__ __forceinline__ int scan_exclusive(int c, Shared<NT>& sh, int& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int s = c;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int o = __shfl_up(s, d);
+    s += lane >= d ? o : 0;
+  }
+  __syncthreads();
+  if (lane == 63) sh.scan[wave] = s;
+  __syncthreads();
+  int front = 0;
+  total = 0;
+  for (int w = 0; w < Shared<NT>::W; ++w) {
+    front += w < wave ? sh.scan[w] : 0;
+    total += sh.scan[w];
+  }
+  return front + s - c;
+}
+
+// Maximum and sums of the row, in an order that depends on nothing but its place in memory and its length.
+// `groups` (a power of two up to NT, or 0): low becomes a value that at least `groups` logits reach, the least of the
+// maxima of so many groups of threads.
+template <typename T, int NT, bool ENTROPY>
+__device__ __forceinline__ Stats row_stats(const Row<T, NT>& row, float tau, int groups, float& low, Shared<NT>& sh) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int W = Shared<NT>::W;
+  float mine = -INFINITY;
+  row.each([&](const auto& y, int, auto n) {
+#pragma unroll
+    for (int j = 0; j < n.value; ++j) mine = fmaxf(mine, y[j]);
+  });
+  // groups of at most a wavefront: the least of the maxima of NT / groups lanes each
+  const int lanes = groups > W ? NT / groups : 64;
+  float g = mine;
+  for (int d = 1; d < lanes; d *= 2) g = fmaxf(g, __shfl_xor(g, d));
+  float least = g, most = g;
+  for (int d = lanes; d < 64; d *= 2) {
+    least = fminf(least, __shfl_xor(least, d));
+    most = fmaxf(most, __shfl_xor(most, d));
+  }
+  if (lane == 0) {
+    sh.max[wave] = most;
+    sh.low[wave] = least;
+  }
+  __syncthreads();
+  Stats st;
+  st.m = sh.max[0];
+  low = sh.low[0];
+#pragma unroll
+  for (int w = 1; w < W; ++w) {
+    st.m = fmaxf(st.m, sh.max[w]);
+    low = fminf(low, sh.low[w]);
+  }
+  st.inv_tau = 1.0f / tau;
+  st.c = kLog2e * st.inv_tau;
+  st.shift = st.m == -INFINITY ? 0.f : st.m;
+  Sums a = {0.f, 0.f, 0.f};
+  row.each([&](const auto& y, int, auto n) {
+#pragma unroll
+    for (int j = 0; j < n.value; ++j) {
+      const float t = st.log2_e(y[j]), e = __builtin_amdgcn_exp2f(t);
+      a.s += e;
+      if constexpr (ENTROPY) a.u = fmaf(e, fmaxf(t, -1e30f), a.u);  // 0 log 0 = 0
+    }
+  });
+  if (__any(mine == st.m) && fabsf(st.m) < INFINITY) {  // again without the maximum, for the few that have it
+    a.s = a.n = 0.f;
+    row.each([&](const auto& y, int, auto n) {
+#pragma unroll
+      for (int j = 0; j < n.value; ++j) {
+        const float e = __builtin_amdgcn_exp2f(st.log2_e(y[j]));
+        a.s += y[j] == st.m ? 0.f : e;
+        a.n += y[j] == st.m ? 1.f : 0.f;
+      }
+    });
+  }
+  a.s = wave_sum(a.s);
+  a.n = wave_sum(a.n);
+  if constexpr (ENTROPY) a.u = wave_sum(a.u);
+  if (lane == 0) sh.sums[wave] = a;
+  __syncthreads();
+  a = sh.sums[0];
+#pragma unroll
+  for (int w = 1; w < W; ++w) {
+    a.s += sh.sums[w].s;
+    a.n += sh.sums[w].n;
+    if constexpr (ENTROPY) a.u += sh.sums[w].u;
+  }
+  st.S = a.n + a.s;
+  st.inv = st.S == 0.f ? 0.f : 1.0f / st.S;
+  st.log_s = a.n == 1.f ? log1pf(a.s) : st.S == 0.f ? 0.f : logf(st.S);
+  st.entropy = ENTROPY ? st.log_s - kLn2 * a.u * st.inv : 0.f;
+  return st;
+}
+
+// Logits in their order as unsigned numbers (-0 as +0, NaN as -infinity), the lower index first among equal ones.
+__device__ __forceinline__ uint64_t top_key(float x, int index) {
+  const unsigned u = __float_as_uint(fmaxf(x, -INFINITY) + 0.0f);
+  const unsigned o = u & 0x80000000u ? ~u : u | 0x80000000u;
+  return (uint64_t)o << 32 | (0xffffffffu - (unsigned)index);
+}
+__device__ __forceinline__ float key_value(uint64_t key) {
+  const unsigned o = (unsigned)(key >> 32);
+  return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
+}
+__device__ __forceinline__ int key_index(uint64_t key) { return (int)(0xffffffffu - (unsigned)key); }
+
+// The k largest logits.  At least k reach `low` (row_stats); the ones above it are gathered, usually some k log k of
+// them, with the lowest-numbered of those that equal it where that leaves fewer than k.  Of more than 256 a
+// wavefront finds the k-th by bisection; what is left is ranked by counting.  found[r], r < k: the r-th.
+template <typename T, int NT>
+__device__ __forceinline__ void row_top(const Row<T, NT>& row, int k, float low, uint64_t* cand, uint64_t* found,
+                                        Shared<NT>& sh) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  auto gather = [&] {
+    __syncthreads();
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+    row.each([&](const auto& y, int first, auto n) {
+#pragma unroll
+      for (int j = 0; j < n.value; ++j)
+        if (y[j] > low) {
+          const int at = atomicAdd(&sh.count, 1);
+          if (at < kCandidates) cand[at] = top_key(y[j], first + j);
+        }
+    });
+    __syncthreads();
+    return sh.count;
+  };
+  int n = gather();
+  if (n > kCandidates) {
+    // the k-th largest value, bit by bit from the top: the largest that at least k reach
+    unsigned kth = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+      const unsigned trial = kth | 1u << bit;
+      int c = 0;
+      row.each([&](const auto& y, int, auto m) {
+#pragma unroll
+        for (int j = 0; j < m.value; ++j) c += (unsigned)(top_key(y[j], 0) >> 32) >= trial;
+      });
+      int total;
+      scan_exclusive<NT>(c, sh, total);
+      if (total >= k) kth = trial;
+    }
+    low = key_value((uint64_t)kth << 32);
+    n = gather();  // fewer than k are above it
+  }
+  if (n < k) {
+    // the first k - n of the logits that equal `low`, in the order of their indices
+    auto take = [&](bool one, int first, int elements, auto value) {
+      int c = 0, total;
+      if (one)
+        for (int j = 0; j < elements; ++j) c += fmaxf(value(j), -INFINITY) == low;
+      int at = n + scan_exclusive<NT>(c, sh, total);
+      if (one)
+        for (int j = 0; j < elements; ++j)
+          if (fmaxf(value(j), -INFINITY) == low) {
+            if (at < k) cand[at] = top_key(value(j), first + j);
+            ++at;
+          }
+      n += total;
+    };
+    auto at = [&](int first) { return [&row, first](int j) { return row.at(first + j); }; };
+    take(tid < row.lead, tid, 1, at(tid));
+    for (int c = 0; c < row.chunks && n < k; c += NT) {
+      const int first = row.lead + (c + tid) * Row<T, NT>::N;
+      take(c + tid < row.chunks, first, Row<T, NT>::N, at(first));
+    }
+    if (n < k) take(row.loose >= row.lead, row.loose, 1, at(row.loose));
+    n = k;
+    __syncthreads();
+  }
+  if (n > 256) {
+    if (tid < kWave) {
+      // keys differ, so exactly k reach the k-th; as soon as k reach a trial, those are the ones
+      uint64_t kth = 0;
+      for (int bit = 63; bit >= 0; --bit) {
+        const uint64_t trial = kth | 1ull << bit;
+        int c = 0;
+        for (int i = lane; i < n; i += kWave) c += cand[i] >= trial;
+        c = (int)wave_sum((float)c);
+        if (c >= k) kth = trial;
+        if (c == k) break;
+      }
+      int kept = 0;
+      for (int i = lane; i - lane < n; i += kWave) {
+        const uint64_t key = i < n ? cand[i] : 0;
+        const uint64_t in = __ballot(i < n && key >= kth);
+        // writes stay behind the reads: kept + 63 < i - lane + 64
+        if (in >> lane & 1) cand[kept + __popcll(in & ((1ull << lane) - 1))] = key;
+        kept += __popcll(in);
+      }
+    }
+    n = k;
+    __syncthreads();
+  }
+  for (int i = tid; i < n; i += NT) {
+    const uint64_t key = cand[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += cand[j] > key;
+    if (rank < k) found[rank] = key;
+  }
+  __syncthreads();
+}
+
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void token_log_probs_kernel(const T* __restrict__ x, int64_t ld, int vocab,
+                                                             const int64_t* __restrict__ tokens, float tau, int k,
+                                                             float* __restrict__ log_probs, float* __restrict__ entropy,
+                                                             float* __restrict__ top_log_probs,
+                                                             int64_t* __restrict__ top_tokens) {
+  __shared__ Shared<NT> sh;
+  __shared__ uint64_t cand[kCandidates], found[kMaxTop];
+  const int64_t r = blockIdx.x;
+  const Row<T, NT> row(x + r * ld, vocab);
+  int groups = 0;
+  if (k > 0)
+    for (groups = 1; groups < k; groups *= 2) {}
+  float low;
+  const Stats st = row_stats<T, NT, true>(row, tau, groups, low, sh);
+  if (log_probs != nullptr) {
+    const int64_t t = tokens[r];
+    const bool in = t >= 0 && t < vocab;
+    const float score = st.log_p(row.at(in ? t : 0));
+    if (threadIdx.x == 0) log_probs[r] = in ? score : 0.f;
+  }
+  if (entropy != nullptr && threadIdx.x == 0) entropy[r] = st.entropy;
+  if (k > 0) {
+    row_top<T, NT>(row, k, low, cand, found, sh);
+    for (int i = threadIdx.x; i < k; i += NT) {
+      top_log_probs[r * k + i] = st.log_p(key_value(found[i]));
+      top_tokens[r * k + i] = key_index(found[i]);
+    }
+  }
+}
+
+// Writes f(x_j, ...) of every logit of the row, then the entries of `ids` (count of them, in LDS, -1: none) as
+// f plus the sum of their `add`s: entries of one token share its place and write the same number there.
+template <typename T, int NT, typename F>
+__device__ __forceinline__ void write_gradient(const Row<T, NT>& row, T* __restrict__ out, const int* ids,
+                                               const float* add, int count, F f) {
+  typedef typename RowVec<T>::V V;
+  const bool whole = ((uintptr_t)out & 15) == ((uintptr_t)row.x & 15);
+  row.each([&](const auto& y, int first, auto n) {
+    if constexpr (n.value > 1) {
+      V v;
+#pragma unroll
+      for (int j = 0; j < n.value; ++j) v[j] = (T)f(y[j]);
+      if (whole) {
+        *reinterpret_cast<V*>(out + first) = v;
+      } else {
+#pragma unroll
+        for (int j = 0; j < n.value; ++j) out[first + j] = v[j];
+      }
+    } else {
+      out[first] = (T)f(y[0]);
+    }
+  });
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // another wavefront's store to the same place comes behind
+  __syncthreads();
+  for (int i = threadIdx.x; i < count; i += NT) {
+    const int id = ids[i];
+    if (id < 0) continue;
+    float sum = 0.f;
+    for (int j = 0; j < count; ++j) sum += ids[j] == id ? add[j] : 0.f;
+    out[id] = (T)(f(row.at(id)) + sum);
+  }
+}
+
+template <typename T, int NT>
+__device__ __forceinline__ void write_zeros(T* __restrict__ out, int vocab) {
+  const Row<T, NT> row(out, vocab);
+  typedef typename RowVec<T>::V V;
+  for (int c = threadIdx.x; c < row.chunks; c += NT) reinterpret_cast<V*>(out + row.lead)[c] = V(0);
+  if (row.loose >= 0) out[row.loose] = (T)0;
+}
+
+// dx_j = ([j = token] g + sum_i u_i [j = id_i] - p_j (g + sum_i u_i + h (log p_j + H))) / tau for the gradients g of
+// log p(token), h of the entropy and u_i of the top tokens' log probabilities.
+template <typename T, int NT, bool ENTROPY>
+__global__ __launch_bounds__(NT) void token_log_probs_backward_kernel(
+    const T* __restrict__ x, int64_t ld, int vocab, const int64_t* __restrict__ tokens, float tau,
+    const float* __restrict__ d_log_probs, const float* __restrict__ d_entropy, int k,
+    const int64_t* __restrict__ top_tokens, const float* __restrict__ d_top, T* __restrict__ out, int64_t ld_out) {
+  __shared__ Shared<NT> sh;
+  __shared__ int ids[kMaxTop + 1];
+  __shared__ float add[kMaxTop + 1];
+  const int64_t r = blockIdx.x;
+  const int count = k + 1;
+  // Where the condition is the same for all threads, and not in a thread's branch below: a load from one address is
+  // a scalar one, which a wavefront executes in a branch that none of its lanes takes.
+  int64_t token = -1;
+  float d_token = 0.f;
+  if (d_log_probs != nullptr) {
+    token = tokens[r];
+    d_token = d_log_probs[r];
+  }
+  for (int i = threadIdx.x; i < count; i += NT) {
+    int64_t t = token;
+    float d = d_token;
+    if (i < k) {
+      t = top_tokens[r * k + i];
+      d = d_top[r * k + i];
+    }
+    const bool in = t >= 0 && t < vocab;
+    ids[i] = in ? (int)t : -1;
+    add[i] = in ? d : 0.f;
+  }
+  __syncthreads();
+  float g = 0.f;
+  bool none = true;
+  for (int i = 0; i < count; ++i) {
+    g += add[i];
+    none &= add[i] == 0.f;
+  }
+  const float h = ENTROPY ? d_entropy[r] : 0.f;
+  T* o = out + r * ld_out;
+  if (none && h == 0.f) {  // padding: whatever its logits are
+    write_zeros<T, NT>(o, vocab);
+    return;
+  }
+  const Row<T, NT> row(x + r * ld, vocab);
+  float low;
+  const Stats st = row_stats<T, NT, ENTROPY>(row, tau, 0, low, sh);
+  __syncthreads();
+  for (int i = threadIdx.x; i < count; i += NT) add[i] *= st.inv_tau;
+  __syncthreads();
+  const float scale = st.inv * st.inv_tau, lift = st.entropy - st.log_s;
+  write_gradient<T, NT>(row, o, ids, add, st.S == 0.f ? 0 : count, [&](float y) {
+    const float t = st.log2_e(y), p = __builtin_amdgcn_exp2f(t) * scale;
+    return -p * (ENTROPY ? fmaf(h, fmaf(kLn2, fmaxf(t, -1e30f), lift), g) : g);
+  });
+}
+
+// q = softmax(teacher / tau) over the row's entries (an id outside the vocabulary is no entry), loss = w sum q (log q -
+// log p); gradient w / tau (p_j - sum of q over the entries of token j).
+template <typename T, typename S, int NT, bool GRAD>
+__global__ __launch_bounds__(NT) void distillation_kernel(const T* __restrict__ x, int64_t ld, int vocab,
+                                                          const int64_t* __restrict__ teacher_tokens,
+                                                          const S* __restrict__ teacher, int k, float tau,
+                                                          const float* __restrict__ weights, float* __restrict__ losses,
+                                                          T* __restrict__ out, int64_t ld_out) {
+  __shared__ Shared<NT> sh;
+  __shared__ int ids[kMaxTop];
+  __shared__ float add[kMaxTop], total;
+  const int64_t r = blockIdx.x;
+  const int tid = threadIdx.x;
+  const float w = weights != nullptr ? weights[r] : 1.f;
+  if (w == 0.f) {  // padding: whatever its logits are
+    if (tid == 0 && losses != nullptr) losses[r] = 0.f;
+    if constexpr (GRAD) write_zeros<T, NT>(out + r * ld_out, vocab);
+    return;
+  }
+  const Row<T, NT> row(x + r * ld, vocab);
+  constexpr int E = kMaxTop / kWave;  // a lane's entries, for the first wavefront
+  float q[E], log_q[E], student[E];
+  if (tid < kWave) {
+    const float inv_tau = 1.0f / tau;
+    float most = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const int at = tid + i * kWave;
+      const int64_t t = at < k ? teacher_tokens[r * k + at] : -1;
+      const bool in = t >= 0 && t < vocab;
+      log_q[i] = in ? (float)teacher[r * k + at] * inv_tau : -INFINITY;
+      student[i] = in ? row.at(t) : 0.f;
+      if (at < k) ids[at] = in ? (int)t : -1;
+      most = fmaxf(most, log_q[i]);
+    }
+    most = wave_max(most);
+    if (most == -INFINITY) most = 0.f;  // no entry: q = 0
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      log_q[i] -= most;
+      q[i] = expf(log_q[i]);
+      sum += q[i];
+    }
+    sum = wave_sum(sum);
+    const float log_sum = logf(sum), inv = sum == 0.f ? 0.f : 1.0f / sum;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      q[i] *= inv;
+      log_q[i] -= log_sum;
+      if (tid + i * kWave < k) add[tid + i * kWave] = -q[i] * w * inv_tau;
+    }
+    if (tid == 0) total = sum == 0.f ? 0.f : 1.f;
+  }
+  float low;
+  const Stats st = row_stats<T, NT, false>(row, tau, 0, low, sh);
+  if (tid < kWave && losses != nullptr) {
+    float loss = 0.f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) loss += q[i] == 0.f ? 0.f : q[i] * (log_q[i] - st.log_p(student[i]));
+    loss = wave_sum(loss);
+    if (tid == 0) losses[r] = total == 0.f ? 0.f : w * loss;
+  }
+  if constexpr (GRAD) {
+    const float scale = total == 0.f ? 0.f : w * st.inv * st.inv_tau;
+    write_gradient<T, NT>(row, out + r * ld_out, ids, add, st.S == 0.f ? 0 : k,
+                          [&](float y) { return __builtin_amdgcn_exp2f(st.log2_e(y)) * scale; });
+  }
+}
+
+constexpr int NT = 256;
+
+template <typename T>
+void launch_log_probs_t(const LogitRows& a, const int64_t* tokens, int top, float* log_probs, float* entropy,
+                        float* top_log_probs, int64_t* top_tokens, hipStream_t st) {
+  hipLaunchKernelGGL((token_log_probs_kernel<T, NT>), dim3((unsigned)a.rows), dim3(NT), 0, st, (const T*)a.x, a.ld,
+                     a.vocab, tokens, a.temperature, top, log_probs, entropy, top_log_probs, top_tokens);
+}
+
+template <typename T, bool ENTROPY>
+void launch_backward_t(const LogitRows& a, const int64_t* tokens, const float* d_log_probs, const float* d_entropy,
+                       int top, const int64_t* top_tokens, const float* d_top, void* grad, int64_t ld_grad,
+                       hipStream_t st) {
+  hipLaunchKernelGGL((token_log_probs_backward_kernel<T, NT, ENTROPY>), dim3((unsigned)a.rows), dim3(NT), 0, st,
+                     (const T*)a.x, a.ld, a.vocab, tokens, a.temperature, d_log_probs, d_entropy, top, top_tokens,
+                     d_top, (T*)grad, ld_grad);
+}
+
+template <typename T, typename S, bool GRAD>
+void launch_distillation_t(const LogitRows& a, const int64_t* teacher_tokens, const void* teacher, int k,
+                           const float* weights, float* losses, void* grad, int64_t ld_grad, hipStream_t st) {
+  hipLaunchKernelGGL((distillation_kernel<T, S, NT, GRAD>), dim3((unsigned)a.rows), dim3(NT), 0, st, (const T*)a.x,
+                     a.ld, a.vocab, teacher_tokens, (const S*)teacher, k, a.temperature, weights, losses, (T*)grad,
+                     ld_grad);
+}
+
+}  // namespace
+
+void launch_token_log_probs(const LogitRows& a, const int64_t* tokens, int top, float* log_probs, float* entropy,
+                            float* top_log_probs, int64_t* top_tokens, hipStream_t st) {
+  if (a.f16) launch_log_probs_t<_Float16>(a, tokens, top, log_probs, entropy, top_log_probs, top_tokens, st);
+  else launch_log_probs_t<float>(a, tokens, top, log_probs, entropy, top_log_probs, top_tokens, st);
+}
+
+void launch_token_log_probs_backward(const LogitRows& a, const int64_t* tokens, const float* d_log_probs,
+                                     const float* d_entropy, int top, const int64_t* top_tokens, const float* d_top,
+                                     void* grad, int64_t ld_grad, hipStream_t st) {
+  auto go = [&](auto type, auto entropy) {
+    launch_backward_t<decltype(type), decltype(entropy)::value>(a, tokens, d_log_probs, d_entropy, top, top_tokens,
+                                                                d_top, grad, ld_grad, st);
+  };
+  if (a.f16) d_entropy ? go(_Float16(), std::true_type()) : go(_Float16(), std::false_type());
+  else d_entropy ? go(float(), std::true_type()) : go(float(), std::false_type());
+}
+
+void launch_distillation(const LogitRows& a, const int64_t* teacher_tokens, const void* teacher, bool teacher_f16,
+                         int k, const float* weights, float* losses, void* grad, int64_t ld_grad, hipStream_t st) {
+  auto go = [&](auto type, auto teacher_type) {
+    typedef decltype(type) T;
+    typedef decltype(teacher_type) S;
+    if (grad != nullptr)
+      launch_distillation_t<T, S, true>(a, teacher_tokens, teacher, k, weights, losses, grad, ld_grad, st);
+    else
+      launch_distillation_t<T, S, false>(a, teacher_tokens, teacher, k, weights, losses, grad, ld_grad, st);
+  };
+  if (a.f16) teacher_f16 ? go(_Float16(), _Float16()) : go(_Float16(), float());
+  else teacher_f16 ? go(float(), _Float16()) : go(float(), float());
+}
+
+}  // namespace gptmi

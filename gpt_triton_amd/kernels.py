@@ -21,10 +21,12 @@ for the embedding, the flat index m*N + n for fused_ffn, query*Lk + key for the 
 weights (kernels.py:31-34, 65-70, 245-251, 457-460).
 """
 import array
+import collections
 import math
 import os
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -290,6 +292,208 @@ def lm_head(x, wte):
     assert H == wte.shape[1]
     z = x.new_empty((*shape[:-1], wte.shape[0]))
     return _linear(x, wte, None, None, z, False, 0.0, _lib.GPTMI_W_NK, "lm_head")
+
+
+# Top tokens a row of `token_log_probs`, and a teacher's logits a row of `distillation_loss`.
+MAX_TOP = 128
+
+TokenLogProbs = collections.namedtuple("TokenLogProbs", "log_probs entropy top_log_probs top_tokens")
+
+
+def _logit_rows(logits, what):
+    """(GPU, type code, rows, vocabulary, pitch) of logits [.., V] whose rows lie at one pitch, as `lm_head` returns
+    them: dense, or the front of padded rows."""
+    dev = _on_gpu(logits)
+    code = _dtype_code(logits, what)
+    V = logits.shape[-1]
+    assert V > 0 and (V == 1 or logits.stride(-1) == 1), "the logits of a row must lie side by side"
+    rows = logits.numel() // V
+    if logits.dim() == 2:
+        return dev, code, rows, V, logits.stride(0)
+    if logits.dim() == 1 or rows <= 1:
+        return dev, code, rows, V, V
+    try:
+        return dev, code, rows, V, logits.view(-1, V).stride(0)
+    except RuntimeError:
+        raise AssertionError(f"{what}: the rows of the logits must lie at one pitch") from None
+
+
+def _logit_gradient(logits, rows, V, ld):
+    """(a buffer for the gradient of rows of logits, its pitch, its view in the logits' shape).  Pitch and address equal
+    the logits' modulo 64 elements and 16 bytes, so that the kernels read and write in the same chunks."""
+    pitch = V + (ld - V) % 64
+    offset = logits.data_ptr() % 16 // logits.element_size()
+    buf = logits.new_empty(offset + max(rows - 1, 0) * pitch + V)
+    buf = buf.as_strided((rows, V), (pitch, 1), offset)
+    return buf, pitch, buf.view(logits.shape)
+
+
+def _check_row_tokens(t, shape, what):
+    if t.dtype != torch.int64:
+        raise TypeError(f"{what}: token ids must be int64, got {t.dtype}")
+    assert t.shape == shape, (t.shape, shape)
+    assert t.is_contiguous()
+
+
+def _maybe_check_row_tokens(t, V, what):
+    if os.environ.get("GPTMI_CHECK_IDS") == "1" and t.numel() > 0 and int(t.max()) >= V:
+        raise IndexError(f"{what}: token id {int(t.max())}, but a row has {V} logits")
+
+
+def _check_temperature(temperature, what):
+    if not 0.0 < temperature < math.inf:
+        raise ValueError(f"{what}: temperature {temperature} is not above 0 and finite")
+
+
+def _token_log_probs(logits, tokens, top, temperature):
+    dev, code, rows, V, ld = _logit_rows(logits, "token_log_probs")
+    lead = logits.shape[:-1]
+    _on_gpu(logits, tokens)
+    if tokens is not None:
+        _check_row_tokens(tokens, lead, "token_log_probs")
+        _maybe_check_row_tokens(tokens, V, "token_log_probs")
+    assert 0 <= top <= V, (top, V)
+    if top > MAX_TOP:
+        raise NotImplementedError(f"token_log_probs: at most {MAX_TOP} top tokens, got {top}")
+    _check_temperature(temperature, "token_log_probs")
+    entropy = logits.new_empty(lead, dtype=torch.float32)
+    log_probs = None if tokens is None else torch.empty_like(entropy)
+    top_log_probs = top_tokens = None
+    if top > 0:
+        top_log_probs = logits.new_empty((*lead, top), dtype=torch.float32)
+        top_tokens = logits.new_empty((*lead, top), dtype=torch.int64)
+    if rows > 0:
+        _call(dev, "token_log_probs", _lib.load().gptmi_token_log_probs, logits.data_ptr(), ld, _ptr(tokens),
+              temperature, _ptr(log_probs), entropy.data_ptr(), top, _ptr(top_log_probs), _ptr(top_tokens), rows, V,
+              code)
+    return log_probs, entropy, top_log_probs, top_tokens
+
+
+class _TokenLogProbsFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, top, temperature):
+        log_probs, entropy, top_log_probs, top_tokens = _token_log_probs(logits, tokens, top, temperature)
+        ctx.set_materialize_grads(False)
+        if top_tokens is not None:
+            ctx.mark_non_differentiable(top_tokens)
+        ctx.save_for_backward(logits, tokens, top_tokens)
+        ctx.temperature = temperature
+        return log_probs, entropy, top_log_probs, top_tokens
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_log_probs, d_entropy, d_top, _):
+        logits, tokens, top_tokens = ctx.saved_tensors
+        if d_log_probs is None and d_entropy is None and d_top is None:
+            return None, None, None, None
+        dev, code, rows, V, ld = _logit_rows(logits, "token_log_probs")
+        d_log_probs, d_entropy, d_top = (None if g is None else g.contiguous() for g in (d_log_probs, d_entropy, d_top))
+        buf, pitch, grad = _logit_gradient(logits, rows, V, ld)
+        if rows > 0:
+            _call(dev, "token_log_probs_backward", _lib.load().gptmi_token_log_probs_backward, logits.data_ptr(), ld,
+                  _ptr(tokens), ctx.temperature, _ptr(d_log_probs), _ptr(d_entropy),
+                  0 if d_top is None else top_tokens.shape[-1], _ptr(top_tokens), _ptr(d_top), buf.data_ptr(), pitch,
+                  rows, V, code)
+        return grad, None, None, None
+
+
+def token_log_probs(logits, tokens=None, top=0, temperature=1.0):
+    """Scores of rows of logits [.., V], as `lm_head` returns them, under softmax(logits / temperature):
+
+        log_probs      [..]       the log probability of tokens [..]; a token outside [0, V), such as the -100 of
+                                  padding, scores 0; None without tokens
+        entropy        [..]       of the row's distribution
+        top_log_probs  [.., top]  the `top` most likely tokens, the likeliest first, equal ones in the order of their
+        top_tokens     [.., top]  ids, at most MAX_TOP; None for top = 0
+
+    fp32 (the tokens int64) whatever the logits' type.  Logits of -infinity mark tokens that cannot occur.  Gradients flow
+    to the logits from all but top_tokens."""
+    temperature = float(temperature)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return TokenLogProbs(*_TokenLogProbsFunction.apply(logits, tokens, top, temperature))
+    return TokenLogProbs(*_token_log_probs(logits, tokens, top, temperature))
+
+
+def _distillation(logits, teacher_tokens, teacher_logits, temperature, weights, losses, gradient):
+    """(losses or None, gradient or None)."""
+    what = "distillation_loss"
+    dev, code, rows, V, ld = _logit_rows(logits, what)
+    _on_gpu(logits, teacher_tokens, teacher_logits, weights)
+    lead, k = logits.shape[:-1], teacher_tokens.shape[-1]
+    _check_row_tokens(teacher_tokens, (*lead, k), what)
+    _maybe_check_row_tokens(teacher_tokens, V, what)
+    assert teacher_logits.shape == teacher_tokens.shape, (teacher_logits.shape, teacher_tokens.shape)
+    assert teacher_logits.is_contiguous()
+    teacher_code = _dtype_code(teacher_logits, what)
+    assert k > 0
+    if k > MAX_TOP:
+        raise NotImplementedError(f"{what}: at most {MAX_TOP} of the teacher's logits a row, got {k}")
+    if weights is not None:
+        if weights.dtype != torch.float32:
+            raise TypeError(f"{what}: weights must be float32, got {weights.dtype}")
+        assert weights.shape == lead, (weights.shape, lead)
+        assert weights.is_contiguous()
+    _check_temperature(temperature, what)
+    out = logits.new_empty(lead, dtype=torch.float32) if losses else None
+    buf = grad = None
+    pitch = V
+    if gradient:
+        buf, pitch, grad = _logit_gradient(logits, rows, V, ld)
+    if rows > 0:
+        _call(dev, what, _lib.load().gptmi_distillation_loss, logits.data_ptr(), ld, teacher_tokens.data_ptr(),
+              teacher_logits.data_ptr(), k, temperature, _ptr(weights), _ptr(out), _ptr(buf), pitch, rows, V, code,
+              teacher_code)
+    return out, grad
+
+
+class _DistillationFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, teacher_tokens, teacher_logits, temperature, weights):
+        ctx.save_for_backward(logits, teacher_tokens, teacher_logits, weights)
+        ctx.temperature = temperature
+        return _distillation(logits, teacher_tokens, teacher_logits, temperature, weights, True, False)[0]
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_losses):
+        logits, teacher_tokens, teacher_logits, weights = ctx.saved_tensors
+        # the gradient of the sum of the losses under other weights; where a weight is 0, so is its product with
+        # whatever comes back
+        if weights is not None:
+            d_losses = torch.where(weights == 0, weights, d_losses * weights)
+        grad = _distillation(logits, teacher_tokens, teacher_logits, ctx.temperature, d_losses.contiguous(), False,
+                             True)[1]
+        return grad, None, None, None, None
+
+
+def _constants(*tensors):
+    assert not any(t is not None and t.requires_grad for t in tensors), "only the logits have a gradient"
+
+
+def distillation_loss(logits, teacher_tokens, teacher_logits, temperature=1.0, weights=None):
+    """Losses [..] (fp32) of a student's logits [.., V] against a teacher's top logits: with q the softmax of
+    teacher_logits [.., k] / temperature (float32 or float16; log probabilities serve as well) and p that of logits /
+    temperature,
+
+        weights * sum_i q_i (log q_i - log p[teacher_tokens_i])
+
+    k up to MAX_TOP.  An entry whose token is outside [0, V) or whose logit is -infinity counts for nothing.  weights [..]
+    (float32, all 1 if None): 0 marks padding, whose logits may be anything.  Gradients flow to the logits alone, which
+    are read again for them; `distillation_loss_and_grad` has both in one pass."""
+    _constants(teacher_logits, weights)
+    temperature = float(temperature)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _DistillationFunction.apply(logits, teacher_tokens, teacher_logits, temperature, weights)
+    return _distillation(logits, teacher_tokens, teacher_logits, temperature, weights, True, False)[0]
+
+
+@torch.no_grad()
+def distillation_loss_and_grad(logits, teacher_tokens, teacher_logits, temperature=1.0, weights=None):
+    """(losses, gradient of their sum with respect to the logits) of `distillation_loss` from one pass over the logits, for
+    steps that know the weights of their rows beforehand: `logits.backward(gradient)` goes on from there.  The
+    gradient has the logits' shape and type; the rows of padded logits' gradient are padded too."""
+    _constants(teacher_logits, weights)
+    return _distillation(logits, teacher_tokens, teacher_logits, float(temperature), weights, True, True)
 
 
 def matmul_and_split_qkv(x, weight, bias, num_heads):

@@ -132,6 +132,56 @@ int gptmi_layernorm(const void* x, const void* w, const void* b, void* out,
 int gptmi_softmax(const void* x, void* out, int64_t M, int64_t H, int dtype,
                   void* stream);
 
+/* Top tokens a row of gptmi_token_log_probs, and a teacher's logits a row of gptmi_distillation_loss. */
+#define GPTMI_MAX_TOP 128
+
+/*
+ * Scores of M rows of logits [V] at a pitch of ld elements (the padded rows of an LM head, a dense matrix, any
+ * alignment that the element type allows), z = logits / temperature, p = softmax(z) with fp32 maximum and sums:
+ *   log_probs[m] = log p[tokens[m]]        a token outside [0, V) (padding) reads no memory and scores 0
+ *   entropy[m]   = -sum p log p
+ *   top_tokens[m][0 .. top): the tokens with the largest logits, largest first, equal ones in the order of their ids
+ *   top_log_probs[m][0 .. top): log p of those
+ * Logits of -infinity are tokens that cannot occur: p = 0, nothing to the entropy.  A row of nothing else has entropy
+ * 0 and scores of -infinity; a row with a NaN or +infinity scores NaN (NaN counts as -infinity among the top tokens).
+ * log_probs (and tokens) or entropy may be NULL, top may be 0: 0 <= top <= min(V, GPTMI_MAX_TOP).  V up to 2^30.
+ *
+ * No counterpart in the reference, which ends in front of the logits (gpt.py:159-161, 172-179).
+ */
+int gptmi_token_log_probs(const void* logits, int64_t ld, const int64_t* tokens, float temperature,
+                          float* log_probs, float* entropy, int64_t top, float* top_log_probs,
+                          int64_t* top_tokens, int64_t M, int64_t V, int dtype, void* stream);
+
+/*
+ * The gradient of the logits for the gradients of log_probs, entropy and top_log_probs (NULL, or top 0: of nothing):
+ *   grad_j = ([j = token] g + sum_i [j = top_i] u_i - p_j (g + sum_i u_i + h (log p_j + H))) / temperature
+ * in the logits' type at a pitch of ld_grad >= V elements; it may not overlap the logits.  Rows of zero gradients are
+ * zeros whatever their logits are, rows without any probability too.  Fastest where grad and logits, and their pitches, are
+ * equal modulo 16 bytes.
+ */
+int gptmi_token_log_probs_backward(const void* logits, int64_t ld, const int64_t* tokens,
+                                   float temperature, const float* d_log_probs, const float* d_entropy,
+                                   int64_t top, const int64_t* top_tokens, const float* d_top_log_probs,
+                                   void* grad, int64_t ld_grad, int64_t M, int64_t V, int dtype,
+                                   void* stream);
+
+/*
+ * Distillation from a teacher's k top logits a row (1 <= k <= GPTMI_MAX_TOP), teacher_tokens, teacher_logits [M][k]:
+ *   q = softmax(teacher_logits / temperature) over the row's entries, p = softmax(logits / temperature) over V
+ *   losses[m] = weights[m] sum_i q_i (log q_i - log p[token_i])
+ *   grad_j    = weights[m] / temperature (p_j - sum_i [j = token_i] q_i)   of the sum of the losses
+ * in one pass over the logits.  Log probabilities serve as teacher_logits too (the softmax takes a constant out).  An
+ * entry whose token is outside [0, V) or whose logit is -infinity counts for nothing; a token that is there twice
+ * counts twice.  A row without entries, or of weight 0 (padding), has loss 0 and gradient 0 whatever its logits are; a student
+ * that gives the teacher's tokens no probability at all has loss +infinity.
+ * weights may be NULL (all 1), losses or grad may be NULL; grad as in gptmi_token_log_probs_backward.  teacher_dtype:
+ * the type of teacher_logits.
+ */
+int gptmi_distillation_loss(const void* logits, int64_t ld, const int64_t* teacher_tokens,
+                            const void* teacher_logits, int64_t k, float temperature, const float* weights,
+                            float* losses, void* grad, int64_t ld_grad, int64_t M, int64_t V, int dtype,
+                            int teacher_dtype, void* stream);
+
 /*
  * Bytes of workspace gptmi_linear / gptmi_linear_qkv need for these sizes
  * (0 if none).  The workspace holds the fp16, K-contiguous, zero-padded copy of
