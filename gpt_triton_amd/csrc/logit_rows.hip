@@ -25,14 +25,31 @@ template <> struct RowVec<float> {
   static constexpr int N = 4;
 };
 
+// The larger one, for numbers of which none is a NaN; one of two where one is.  By hand: the compiler's own maximum
+// quiets NaNs first, an operation more for each.
+__device__ __forceinline__ unsigned max_h2(unsigned a, unsigned b) {
+  unsigned r;
+  asm("v_pk_max_f16 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
+}
+__device__ __forceinline__ float max_f(float a, float b) {
+  float r;
+  asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
+}
+
 // A row as the workgroup's threads share it: 16-byte chunks from the first aligned address on, dealt one behind
 // the other, and in front and behind at most 2 (N - 1) single elements, one for each of the first threads.
-template <typename T, int NT>
+// CH > 0: it is read once and stays in registers, CH chunks a thread (-infinity where the row has ended).  CH = 0: rows
+// too long for that are read again by every pass.
+template <typename T, int NT, int CH>
 struct Row {
   typedef typename RowVec<T>::V V;
   static constexpr int N = RowVec<T>::N;
   const T* x;
   int vocab, lead, chunks, loose;  // loose: the index of this thread's single element, or -1
+  V held[CH > 0 ? CH : 1];
+  float single;
   __device__ __forceinline__ Row(const T* row, int vocab_) : x(row), vocab(vocab_) {
     const int ahead = (int)((-(intptr_t)row & 15) / (int)sizeof(T));
     lead = ahead < vocab ? ahead : vocab;
@@ -40,19 +57,72 @@ struct Row {
     const int t = threadIdx.x, singles = vocab - chunks * N;
     loose = t < lead ? t : t < singles ? t + chunks * N : -1;
   }
-  // f(values, index of the first of them, how many: N or 1) for this thread's part of the row
+  __device__ __forceinline__ void load() {
+    if constexpr (CH > 0) {
+      const V* p = reinterpret_cast<const V*>(x + lead) + threadIdx.x;
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        held[i] = V((T)-INFINITY);
+        if ((int)threadIdx.x + i * NT < chunks) held[i] = p[i * NT];
+      }
+      single = -INFINITY;
+      if (loose >= 0) single = (float)x[loose];
+    }
+  }
+  // In front of a pass: what the last one converted is not kept for this one, which is a register for each element.
+  __device__ __forceinline__ void renew() {
+    if constexpr (CH > 0) {
+#pragma unroll
+      for (int i = 0; i < CH; ++i) asm volatile("" : "+v"(held[i]));
+    }
+  }
+  // whether a wavefront has any of chunk i
+  __device__ __forceinline__ bool part(int i) const {
+    return i == 0 || __builtin_amdgcn_readfirstlane((int)threadIdx.x & -kWave) + i * NT < chunks;
+  }
+  // f(values, index of the first of them, how many: N or 1) for this thread's part of the row, with -infinity for what
+  // is not there (CH > 0)
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
-    for (int c = threadIdx.x; c < chunks; c += NT) {
-      const V v = reinterpret_cast<const V*>(x + lead)[c];
+    auto chunk = [&](const V& v, int c) {
       float y[N];
 #pragma unroll
       for (int j = 0; j < N; ++j) y[j] = (float)v[j];
       f(y, lead + c * N, std::integral_constant<int, N>{});
-    }
-    if (loose >= 0) {
-      const float y[1] = {(float)x[loose]};
+    };
+    if constexpr (CH > 0) {
+#pragma unroll
+      for (int i = 0; i < CH; ++i)
+        if (part(i)) chunk(held[i], threadIdx.x + i * NT);
+      const float y[1] = {single};
       f(y, loose, std::integral_constant<int, 1>{});
+    } else {
+      for (int c = threadIdx.x; c < chunks; c += NT) chunk(reinterpret_cast<const V*>(x + lead)[c], c);
+      if (loose >= 0) {
+        const float y[1] = {(float)x[loose]};
+        f(y, loose, std::integral_constant<int, 1>{});
+      }
+    }
+  }
+  // the largest of this thread's part, or -infinity
+  __device__ __forceinline__ float largest() const {
+    if constexpr (CH > 0 && sizeof(T) == 2) {
+      typedef unsigned u4v __attribute__((ext_vector_type(4)));
+      unsigned m = 0xfc00fc00u;  // -infinity twice
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        const u4v u = __builtin_bit_cast(u4v, held[i]);
+        m = max_h2(m, max_h2(max_h2(u[0], u[1]), max_h2(u[2], u[3])));
+      }
+      const h2 two = __builtin_bit_cast(h2, m);
+      return max_f(single, max_f((float)two[0], (float)two[1]));
+    } else {
+      float m = -INFINITY;
+      each([&](const auto& y, int, auto n) {
+#pragma unroll
+        for (int j = 0; j < n.value; ++j) m = max_f(m, y[j]);
+      });
+      return m;
     }
   }
   __device__ __forceinline__ float at(int64_t i) const { return (float)x[i]; }
@@ -69,6 +139,16 @@ struct Shared {
   Sums sums[W];
   int count, scan[W];
 };
+
+// op over the W values (a power of two up to 16) that lane l has the l % W-th of, for every lane.
+template <int W, typename Op>
+__device__ __forceinline__ float join(float v, Op op) {
+  if constexpr (W >= 16) v = op(v, row_rotate<8>(v));
+  if constexpr (W >= 8) v = op(v, row_rotate<4>(v));
+  if constexpr (W >= 4) v = op(v, row_rotate<2>(v));
+  if constexpr (W >= 2) v = op(v, row_rotate<1>(v));
+  return v;
+}
 
 // What a row's softmax needs.
 struct Stats {
@@ -96,6 +176,7 @@ __device__ __forceinline__ int scan_exclusive(int c, Shared<NT>& sh, int& total)
   __syncthreads();
   int front = 0;
   total = 0;
+#pragma unroll 1
   for (int w = 0; w < Shared<NT>::W; ++w) {
     front += w < wave ? sh.scan[w] : 0;
     total += sh.scan[w];
@@ -106,17 +187,13 @@ __device__ __forceinline__ int scan_exclusive(int c, Shared<NT>& sh, int& total)
 // Maximum and sums of the row, in an order that depends on nothing but its place in memory and its length.
 // `groups` (a power of two up to NT, or 0): low becomes a value that at least `groups` logits reach, the least of the
 // maxima of so many groups of threads.
-template <typename T, int NT, bool ENTROPY>
-__device__ __forceinline__ Stats row_stats(const Row<T, NT>& row, float tau, int groups, float& low, Shared<NT>& sh) {
+template <bool ENTROPY, typename T, int NT, int CH>
+__device__ __forceinline__ Stats row_stats(Row<T, NT, CH>& row, float tau, int groups, float& low, Shared<NT>& sh) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   constexpr int W = Shared<NT>::W;
-  float mine = -INFINITY;
-  row.each([&](const auto& y, int, auto n) {
-#pragma unroll
-    for (int j = 0; j < n.value; ++j) mine = fmaxf(mine, y[j]);
-  });
+  const float mine = row.largest();
   // groups of at most a wavefront: the least of the maxima of NT / groups lanes each
-  const int lanes = groups > W ? NT / groups : 64;
+  const int lanes = groups > NT ? 64 : groups > W ? NT / groups : 64;
   float g = mine;
   for (int d = 1; d < lanes; d *= 2) g = fmaxf(g, __shfl_xor(g, d));
   float least = g, most = g;
@@ -130,17 +207,14 @@ __device__ __forceinline__ Stats row_stats(const Row<T, NT>& row, float tau, int
   }
   __syncthreads();
   Stats st;
-  st.m = sh.max[0];
-  low = sh.low[0];
-#pragma unroll
-  for (int w = 1; w < W; ++w) {
-    st.m = fmaxf(st.m, sh.max[w]);
-    low = fminf(low, sh.low[w]);
-  }
+  st.m = join<W>(sh.max[lane % W], [](float a, float b) { return fmaxf(a, b); });
+  low = join<W>(sh.low[lane % W], [](float a, float b) { return fminf(a, b); });
+  if (groups > NT) low = -INFINITY;
   st.inv_tau = 1.0f / tau;
   st.c = kLog2e * st.inv_tau;
   st.shift = st.m == -INFINITY ? 0.f : st.m;
   Sums a = {0.f, 0.f, 0.f};
+  row.renew();
   row.each([&](const auto& y, int, auto n) {
 #pragma unroll
     for (int j = 0; j < n.value; ++j) {
@@ -151,6 +225,7 @@ __device__ __forceinline__ Stats row_stats(const Row<T, NT>& row, float tau, int
   });
   if (__any(mine == st.m) && fabsf(st.m) < INFINITY) {  // again without the maximum, for the few that have it
     a.s = a.n = 0.f;
+    row.renew();
     row.each([&](const auto& y, int, auto n) {
 #pragma unroll
       for (int j = 0; j < n.value; ++j) {
@@ -165,13 +240,11 @@ __device__ __forceinline__ Stats row_stats(const Row<T, NT>& row, float tau, int
   if constexpr (ENTROPY) a.u = wave_sum(a.u);
   if (lane == 0) sh.sums[wave] = a;
   __syncthreads();
-  a = sh.sums[0];
-#pragma unroll
-  for (int w = 1; w < W; ++w) {
-    a.s += sh.sums[w].s;
-    a.n += sh.sums[w].n;
-    if constexpr (ENTROPY) a.u += sh.sums[w].u;
-  }
+  auto add = [](float a, float b) { return a + b; };
+  a = sh.sums[lane % W];
+  a.s = join<W>(a.s, add);
+  a.n = join<W>(a.n, add);
+  if constexpr (ENTROPY) a.u = join<W>(a.u, add);
   st.S = a.n + a.s;
   st.inv = st.S == 0.f ? 0.f : 1.0f / st.S;
   st.log_s = a.n == 1.f ? log1pf(a.s) : st.S == 0.f ? 0.f : logf(st.S);
@@ -194,15 +267,15 @@ __device__ __forceinline__ int key_index(uint64_t key) { return (int)(0xffffffff
 // The k largest logits.  At least k reach `low` (row_stats); the ones above it are gathered, usually some k log k of
 // them, with the lowest-numbered of those that equal it where that leaves fewer than k.  Of more than 256 a
 // wavefront finds the k-th by bisection; what is left is ranked by counting.  found[r], r < k: the r-th.
-template <typename T, int NT>
-__device__ __forceinline__ void row_top(const Row<T, NT>& row, int k, float low, uint64_t* cand, uint64_t* found,
+template <typename T, int NT, int CH>
+__device__ __forceinline__ void row_top(Row<T, NT, CH>& row, int k, float low, uint64_t* cand, uint64_t* found,
                                         Shared<NT>& sh) {
   const int tid = threadIdx.x, lane = tid & 63;
-  auto gather = [&] {
+  auto gather = [&](auto& from) {
     __syncthreads();
     if (tid == 0) sh.count = 0;
     __syncthreads();
-    row.each([&](const auto& y, int first, auto n) {
+    from.each([&](const auto& y, int first, auto n) {
 #pragma unroll
       for (int j = 0; j < n.value; ++j)
         if (y[j] > low) {
@@ -213,14 +286,16 @@ __device__ __forceinline__ void row_top(const Row<T, NT>& row, int k, float low,
     __syncthreads();
     return sh.count;
   };
-  int n = gather();
+  row.renew();
+  int n = gather(row);
   if (n > kCandidates) {
+    const Row<T, NT, 0> again(row.x, row.vocab);  // seldom: from memory, for the registers' sake
     // the k-th largest value, bit by bit from the top: the largest that at least k reach
     unsigned kth = 0;
     for (int bit = 31; bit >= 0; --bit) {
       const unsigned trial = kth | 1u << bit;
       int c = 0;
-      row.each([&](const auto& y, int, auto m) {
+      again.each([&](const auto& y, int, auto m) {
 #pragma unroll
         for (int j = 0; j < m.value; ++j) c += (unsigned)(top_key(y[j], 0) >> 32) >= trial;
       });
@@ -229,7 +304,7 @@ __device__ __forceinline__ void row_top(const Row<T, NT>& row, int k, float low,
       if (total >= k) kth = trial;
     }
     low = key_value((uint64_t)kth << 32);
-    n = gather();  // fewer than k are above it
+    n = gather(again);  // fewer than k are above it
   }
   if (n < k) {
     // the first k - n of the logits that equal `low`, in the order of their indices
@@ -249,8 +324,8 @@ __device__ __forceinline__ void row_top(const Row<T, NT>& row, int k, float low,
     auto at = [&](int first) { return [&row, first](int j) { return row.at(first + j); }; };
     take(tid < row.lead, tid, 1, at(tid));
     for (int c = 0; c < row.chunks && n < k; c += NT) {
-      const int first = row.lead + (c + tid) * Row<T, NT>::N;
-      take(c + tid < row.chunks, first, Row<T, NT>::N, at(first));
+      const int first = row.lead + (c + tid) * Row<T, NT, CH>::N;
+      take(c + tid < row.chunks, first, Row<T, NT, CH>::N, at(first));
     }
     if (n < k) take(row.loose >= row.lead, row.loose, 1, at(row.loose));
     n = k;
@@ -289,21 +364,21 @@ __device__ __forceinline__ void row_top(const Row<T, NT>& row, int k, float low,
   __syncthreads();
 }
 
-template <typename T, int NT>
-__global__ __launch_bounds__(NT) void token_log_probs_kernel(const T* __restrict__ x, int64_t ld, int vocab,
+template <typename T, bool TOP, int NT, int CH, int WAVES>
+__global__ __launch_bounds__(NT, WAVES) void token_log_probs_kernel(const T* __restrict__ x, int64_t ld, int vocab,
                                                              const int64_t* __restrict__ tokens, float tau, int k,
                                                              float* __restrict__ log_probs, float* __restrict__ entropy,
                                                              float* __restrict__ top_log_probs,
                                                              int64_t* __restrict__ top_tokens) {
   __shared__ Shared<NT> sh;
-  __shared__ uint64_t cand[kCandidates], found[kMaxTop];
   const int64_t r = blockIdx.x;
-  const Row<T, NT> row(x + r * ld, vocab);
+  Row<T, NT, CH> row(x + r * ld, vocab);
+  row.load();
   int groups = 0;
-  if (k > 0)
+  if (TOP)
     for (groups = 1; groups < k; groups *= 2) {}
   float low;
-  const Stats st = row_stats<T, NT, true>(row, tau, groups, low, sh);
+  const Stats st = row_stats<true>(row, tau, groups, low, sh);
   if (log_probs != nullptr) {
     const int64_t t = tokens[r];
     const bool in = t >= 0 && t < vocab;
@@ -311,8 +386,9 @@ __global__ __launch_bounds__(NT) void token_log_probs_kernel(const T* __restrict
     if (threadIdx.x == 0) log_probs[r] = in ? score : 0.f;
   }
   if (entropy != nullptr && threadIdx.x == 0) entropy[r] = st.entropy;
-  if (k > 0) {
-    row_top<T, NT>(row, k, low, cand, found, sh);
+  if constexpr (TOP) {
+    __shared__ uint64_t cand[kCandidates], found[kMaxTop];
+    row_top(row, k, low, cand, found, sh);
     for (int i = threadIdx.x; i < k; i += NT) {
       top_log_probs[r * k + i] = st.log_p(key_value(found[i]));
       top_tokens[r * k + i] = key_index(found[i]);
@@ -322,13 +398,15 @@ __global__ __launch_bounds__(NT) void token_log_probs_kernel(const T* __restrict
 
 // Writes f(x_j, ...) of every logit of the row, then the entries of `ids` (count of them, in LDS, -1: none) as
 // f plus the sum of their `add`s: entries of one token share its place and write the same number there.
-template <typename T, int NT, typename F>
-__device__ __forceinline__ void write_gradient(const Row<T, NT>& row, T* __restrict__ out, const int* ids,
+template <typename T, int NT, int CH, typename F>
+__device__ __forceinline__ void write_gradient(Row<T, NT, CH>& row, T* __restrict__ out, const int* ids,
                                                const float* add, int count, F f) {
   typedef typename RowVec<T>::V V;
   const bool whole = ((uintptr_t)out & 15) == ((uintptr_t)row.x & 15);
+  row.renew();
   row.each([&](const auto& y, int first, auto n) {
     if constexpr (n.value > 1) {
+      if (first >= row.lead + row.chunks * n.value) return;
       V v;
 #pragma unroll
       for (int j = 0; j < n.value; ++j) v[j] = (T)f(y[j]);
@@ -338,7 +416,7 @@ __device__ __forceinline__ void write_gradient(const Row<T, NT>& row, T* __restr
 #pragma unroll
         for (int j = 0; j < n.value; ++j) out[first + j] = v[j];
       }
-    } else {
+    } else if (first >= 0) {
       out[first] = (T)f(y[0]);
     }
   });
@@ -355,7 +433,7 @@ __device__ __forceinline__ void write_gradient(const Row<T, NT>& row, T* __restr
 
 template <typename T, int NT>
 __device__ __forceinline__ void write_zeros(T* __restrict__ out, int vocab) {
-  const Row<T, NT> row(out, vocab);
+  const Row<T, NT, 0> row(out, vocab);
   typedef typename RowVec<T>::V V;
   for (int c = threadIdx.x; c < row.chunks; c += NT) reinterpret_cast<V*>(out + row.lead)[c] = V(0);
   if (row.loose >= 0) out[row.loose] = (T)0;
@@ -363,8 +441,8 @@ __device__ __forceinline__ void write_zeros(T* __restrict__ out, int vocab) {
 
 // dx_j = ([j = token] g + sum_i u_i [j = id_i] - p_j (g + sum_i u_i + h (log p_j + H))) / tau for the gradients g of
 // log p(token), h of the entropy and u_i of the top tokens' log probabilities.
-template <typename T, int NT, bool ENTROPY>
-__global__ __launch_bounds__(NT) void token_log_probs_backward_kernel(
+template <typename T, int NT, int CH, int WAVES>
+__global__ __launch_bounds__(NT, WAVES) void token_log_probs_backward_kernel(
     const T* __restrict__ x, int64_t ld, int vocab, const int64_t* __restrict__ tokens, float tau,
     const float* __restrict__ d_log_probs, const float* __restrict__ d_entropy, int k,
     const int64_t* __restrict__ top_tokens, const float* __restrict__ d_top, T* __restrict__ out, int64_t ld_out) {
@@ -399,31 +477,33 @@ __global__ __launch_bounds__(NT) void token_log_probs_backward_kernel(
     g += add[i];
     none &= add[i] == 0.f;
   }
-  const float h = ENTROPY ? d_entropy[r] : 0.f;
+  float h = 0.f;
+  if (d_entropy != nullptr) h = d_entropy[r];
   T* o = out + r * ld_out;
   if (none && h == 0.f) {  // padding: whatever its logits are
     write_zeros<T, NT>(o, vocab);
     return;
   }
-  const Row<T, NT> row(x + r * ld, vocab);
+  Row<T, NT, CH> row(x + r * ld, vocab);
+  row.load();
   float low;
-  const Stats st = row_stats<T, NT, ENTROPY>(row, tau, 0, low, sh);
+  const Stats st = row_stats<true>(row, tau, 0, low, sh);
   __syncthreads();
   for (int i = threadIdx.x; i < count; i += NT) add[i] *= st.inv_tau;
   __syncthreads();
   const float scale = st.inv * st.inv_tau, lift = st.entropy - st.log_s;
-  write_gradient<T, NT>(row, o, ids, add, st.S == 0.f ? 0 : count, [&](float y) {
+  write_gradient(row, o, ids, add, st.S == 0.f ? 0 : count, [&](float y) {
     const float t = st.log2_e(y), p = __builtin_amdgcn_exp2f(t) * scale;
-    return -p * (ENTROPY ? fmaf(h, fmaf(kLn2, fmaxf(t, -1e30f), lift), g) : g);
+    return -p * fmaf(h, fmaf(kLn2, fmaxf(t, -1e30f), lift), g);
   });
 }
 
 // q = softmax(teacher / tau) over the row's entries (an id outside the vocabulary is no entry), loss = w sum q (log q -
 // log p); gradient w / tau (p_j - sum of q over the entries of token j).
-template <typename T, typename S, int NT, bool GRAD>
-__global__ __launch_bounds__(NT) void distillation_kernel(const T* __restrict__ x, int64_t ld, int vocab,
+template <typename T, bool GRAD, int NT, int CH, int WAVES>
+__global__ __launch_bounds__(NT, WAVES) void distillation_kernel(const T* __restrict__ x, int64_t ld, int vocab,
                                                           const int64_t* __restrict__ teacher_tokens,
-                                                          const S* __restrict__ teacher, int k, float tau,
+                                                          const void* __restrict__ teacher, int teacher_f16, int k, float tau,
                                                           const float* __restrict__ weights, float* __restrict__ losses,
                                                           T* __restrict__ out, int64_t ld_out) {
   __shared__ Shared<NT> sh;
@@ -437,7 +517,8 @@ __global__ __launch_bounds__(NT) void distillation_kernel(const T* __restrict__ 
     if constexpr (GRAD) write_zeros<T, NT>(out + r * ld_out, vocab);
     return;
   }
-  const Row<T, NT> row(x + r * ld, vocab);
+  Row<T, NT, CH> row(x + r * ld, vocab);
+  row.load();
   constexpr int E = kMaxTop / kWave;  // a lane's entries, for the first wavefront
   float q[E], log_q[E], student[E];
   if (tid < kWave) {
@@ -448,7 +529,9 @@ __global__ __launch_bounds__(NT) void distillation_kernel(const T* __restrict__ 
       const int at = tid + i * kWave;
       const int64_t t = at < k ? teacher_tokens[r * k + at] : -1;
       const bool in = t >= 0 && t < vocab;
-      log_q[i] = in ? (float)teacher[r * k + at] * inv_tau : -INFINITY;
+      float value = -INFINITY;
+      if (in) value = teacher_f16 ? (float)((const _Float16*)teacher)[r * k + at] : ((const float*)teacher)[r * k + at];
+      log_q[i] = value * inv_tau;
       student[i] = in ? row.at(t) : 0.f;
       if (at < k) ids[at] = in ? (int)t : -1;
       most = fmaxf(most, log_q[i]);
@@ -472,7 +555,7 @@ __global__ __launch_bounds__(NT) void distillation_kernel(const T* __restrict__ 
     if (tid == 0) total = sum == 0.f ? 0.f : 1.f;
   }
   float low;
-  const Stats st = row_stats<T, NT, false>(row, tau, 0, low, sh);
+  const Stats st = row_stats<false>(row, tau, 0, low, sh);
   if (tid < kWave && losses != nullptr) {
     float loss = 0.f;
 #pragma unroll
@@ -482,68 +565,75 @@ __global__ __launch_bounds__(NT) void distillation_kernel(const T* __restrict__ 
   }
   if constexpr (GRAD) {
     const float scale = total == 0.f ? 0.f : w * st.inv * st.inv_tau;
-    write_gradient<T, NT>(row, out + r * ld_out, ids, add, st.S == 0.f ? 0 : k,
+    write_gradient(row, out + r * ld_out, ids, add, st.S == 0.f ? 0 : k,
                           [&](float y) { return __builtin_amdgcn_exp2f(st.log2_e(y)) * scale; });
   }
 }
 
-constexpr int NT = 256;
-
-template <typename T>
-void launch_log_probs_t(const LogitRows& a, const int64_t* tokens, int top, float* log_probs, float* entropy,
-                        float* top_log_probs, int64_t* top_tokens, hipStream_t st) {
-  hipLaunchKernelGGL((token_log_probs_kernel<T, NT>), dim3((unsigned)a.rows), dim3(NT), 0, st, (const T*)a.x, a.ld,
-                     a.vocab, tokens, a.temperature, top, log_probs, entropy, top_log_probs, top_tokens);
+// f(threads, chunks a thread, wavefronts a SIMD) as integral constants for rows of this many chunks.  A row takes 4 CH
+// registers a thread and some 26 more, so few threads with long parts keep the most rows on a CU: of 50257 fp16 logits (6283
+// chunks) 3 with 512 threads, 4 with 256, 2 with 1024; 1477 rows scored 44 / 49 / 45 us, 2048 rows' loss and gradient 100 /
+// 105 / 104.  50304 fp32 logits (12576 chunks), forward and backward of 2048 rows: 512 threads 255 us, 1024 310.
+template <typename F>
+void pick(int chunks, F f) {
+  auto go = [&](auto nt, auto ch, auto waves) { f(nt, ch, waves); };
+#define GPTMI_ROW(NT, CH, WAVES)                                                                             \
+  if (chunks <= NT * CH)                                                                                     \
+    return go(std::integral_constant<int, NT>(), std::integral_constant<int, CH>(), std::integral_constant<int, WAVES>())
+  GPTMI_ROW(64, 4, 4);
+  GPTMI_ROW(256, 4, 4);
+  GPTMI_ROW(256, 8, 4);
+  GPTMI_ROW(512, 8, 4);
+  GPTMI_ROW(512, 13, 6);
+  GPTMI_ROW(512, 16, 4);
+  GPTMI_ROW(512, 25, 4);
+  GPTMI_ROW(1024, 16, 4);
+  GPTMI_ROW(1024, 20, 4);
+#undef GPTMI_ROW
+  go(std::integral_constant<int, 1024>(), std::integral_constant<int, 0>(), std::integral_constant<int, 4>());
 }
 
-template <typename T, bool ENTROPY>
-void launch_backward_t(const LogitRows& a, const int64_t* tokens, const float* d_log_probs, const float* d_entropy,
-                       int top, const int64_t* top_tokens, const float* d_top, void* grad, int64_t ld_grad,
-                       hipStream_t st) {
-  hipLaunchKernelGGL((token_log_probs_backward_kernel<T, NT, ENTROPY>), dim3((unsigned)a.rows), dim3(NT), 0, st,
-                     (const T*)a.x, a.ld, a.vocab, tokens, a.temperature, d_log_probs, d_entropy, top, top_tokens,
-                     d_top, (T*)grad, ld_grad);
-}
-
-template <typename T, typename S, bool GRAD>
-void launch_distillation_t(const LogitRows& a, const int64_t* teacher_tokens, const void* teacher, int k,
-                           const float* weights, float* losses, void* grad, int64_t ld_grad, hipStream_t st) {
-  hipLaunchKernelGGL((distillation_kernel<T, S, NT, GRAD>), dim3((unsigned)a.rows), dim3(NT), 0, st, (const T*)a.x,
-                     a.ld, a.vocab, teacher_tokens, (const S*)teacher, k, a.temperature, weights, losses, (T*)grad,
-                     ld_grad);
+template <typename F>
+void pick_row(const LogitRows& a, F f) {
+  if (a.f16)
+    pick(a.vocab / 8, [&](auto nt, auto ch, auto waves) { f(_Float16(), nt, ch, waves); });
+  else
+    pick(a.vocab / 4, [&](auto nt, auto ch, auto waves) { f(float(), nt, ch, waves); });
 }
 
 }  // namespace
 
 void launch_token_log_probs(const LogitRows& a, const int64_t* tokens, int top, float* log_probs, float* entropy,
                             float* top_log_probs, int64_t* top_tokens, hipStream_t st) {
-  if (a.f16) launch_log_probs_t<_Float16>(a, tokens, top, log_probs, entropy, top_log_probs, top_tokens, st);
-  else launch_log_probs_t<float>(a, tokens, top, log_probs, entropy, top_log_probs, top_tokens, st);
+  pick_row(a, [&](auto type, auto nt, auto ch, auto waves) {
+    typedef decltype(type) T;
+    auto kernel = top > 0 ? token_log_probs_kernel<T, true, nt.value, ch.value, waves.value>
+                          : token_log_probs_kernel<T, false, nt.value, ch.value, waves.value>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)a.rows), dim3(nt.value), 0, st, (const T*)a.x, a.ld, a.vocab, tokens,
+                       a.temperature, top, log_probs, entropy, top_log_probs, top_tokens);
+  });
 }
 
 void launch_token_log_probs_backward(const LogitRows& a, const int64_t* tokens, const float* d_log_probs,
                                      const float* d_entropy, int top, const int64_t* top_tokens, const float* d_top,
                                      void* grad, int64_t ld_grad, hipStream_t st) {
-  auto go = [&](auto type, auto entropy) {
-    launch_backward_t<decltype(type), decltype(entropy)::value>(a, tokens, d_log_probs, d_entropy, top, top_tokens,
-                                                                d_top, grad, ld_grad, st);
-  };
-  if (a.f16) d_entropy ? go(_Float16(), std::true_type()) : go(_Float16(), std::false_type());
-  else d_entropy ? go(float(), std::true_type()) : go(float(), std::false_type());
+  pick_row(a, [&](auto type, auto nt, auto ch, auto waves) {
+    typedef decltype(type) T;
+    hipLaunchKernelGGL((token_log_probs_backward_kernel<T, nt.value, ch.value, waves.value>), dim3((unsigned)a.rows),
+                       dim3(nt.value), 0, st, (const T*)a.x, a.ld, a.vocab, tokens, a.temperature, d_log_probs,
+                       d_entropy, top, top_tokens, d_top, (T*)grad, ld_grad);
+  });
 }
 
 void launch_distillation(const LogitRows& a, const int64_t* teacher_tokens, const void* teacher, bool teacher_f16,
                          int k, const float* weights, float* losses, void* grad, int64_t ld_grad, hipStream_t st) {
-  auto go = [&](auto type, auto teacher_type) {
+  pick_row(a, [&](auto type, auto nt, auto ch, auto waves) {
     typedef decltype(type) T;
-    typedef decltype(teacher_type) S;
-    if (grad != nullptr)
-      launch_distillation_t<T, S, true>(a, teacher_tokens, teacher, k, weights, losses, grad, ld_grad, st);
-    else
-      launch_distillation_t<T, S, false>(a, teacher_tokens, teacher, k, weights, losses, grad, ld_grad, st);
-  };
-  if (a.f16) teacher_f16 ? go(_Float16(), _Float16()) : go(_Float16(), float());
-  else teacher_f16 ? go(float(), _Float16()) : go(float(), float());
+    auto kernel = grad != nullptr ? distillation_kernel<T, true, nt.value, ch.value, waves.value>
+                                  : distillation_kernel<T, false, nt.value, ch.value, waves.value>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)a.rows), dim3(nt.value), 0, st, (const T*)a.x, a.ld, a.vocab,
+                       teacher_tokens, teacher, (int)teacher_f16, k, a.temperature, weights, losses, (T*)grad, ld_grad);
+  });
 }
 
 }  // namespace gptmi
