@@ -57,6 +57,7 @@ SIGNATURES = {
     "gptmi_dropout_mask": (_int, [_vp, _i64, _f32, _u64, _vp]),
     "gptmi_flash_attn": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _f32, _f32,
                                 _u64, _int, _int, _vp]),
+    "gptmi_flash_attn_packed": (_int, [_vp] * 5 + [_i64] * 11 + [_f32, _int, _vp]),
 }
 
 _lib = None

@@ -754,6 +754,39 @@ int gptmi_flash_attn(const void* q, const void* k, const void* v, void* out, int
   return check_launch("flash_attn");
 }
 
+int gptmi_flash_attn_packed(const void* q, const void* k, const void* v, void* out, const int64_t* starts,
+                            int64_t sequences, int64_t T, int64_t N, int64_t G, int64_t d, int64_t q_row,
+                            int64_t q_head, int64_t k_row, int64_t k_head, int64_t v_row, int64_t v_head, float scale,
+                            int dtype, void* stream) {
+  if (!q || !k || !v || !out || !starts || sequences <= 0 || T <= 0 || N <= 0 || G <= 0 || N % G != 0 || d <= 0 ||
+      !dtype_ok(dtype) || !(scale > 0.0f) || isinf(scale) || ((uintptr_t)starts & 7) != 0) {
+    set_error("flash_attn_packed: invalid argument");
+    return GPTMI_ERR_INVALID;
+  }
+  if (dtype != GPTMI_F16) {
+    set_error("flash_attn_packed: fp16 only");
+    return GPTMI_ERR_UNSUPPORTED;
+  }
+  const uintptr_t all = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out;
+  if ((all & 15) != 0 || ((q_row | q_head | k_row | k_head | v_row | v_head) & 7) != 0) {
+    set_error("flash_attn_packed: q, k, v and out must be 16-byte aligned, and their pitches multiples of 8");
+    return GPTMI_ERR_INVALID;
+  }
+  // the kernel's offsets of a tile's 64 rows are 32-bit numbers of bytes
+  const auto pitch_ok = [](int64_t row) { return row >= 0 && row <= 1 << 24; };
+  const auto head_ok = [](int64_t head) { return head >= 0 && head <= 1ll << 40; };
+  if (!pitch_ok(q_row) || !pitch_ok(k_row) || !pitch_ok(v_row) || !head_ok(q_head) || !head_ok(k_head) ||
+      !head_ok(v_head) || T >= 1ll << 31 || sequences >= 1ll << 31 || N > 1 << 20) {
+    set_error("flash_attn_packed: sizes or pitches beyond the supported");
+    return GPTMI_ERR_UNSUPPORTED;
+  }
+  const int rc = launch_flash_attn_packed(
+      PackedAttention{q, k, v, out, starts, sequences, T, N, G, q_row, q_head, k_row, k_head, v_row, v_head, scale},
+      (int)d, (hipStream_t)stream);
+  if (rc) return rc;
+  return check_launch("flash_attn_packed");
+}
+
 size_t gptmi_dropout_mask_bytes(int64_t n) {
   return n > 0 && n <= kMaxMaskBits ? (size_t)((n + 31) / 32 + 4) * 4 : 0;
 }

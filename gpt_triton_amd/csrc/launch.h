@@ -83,6 +83,17 @@ int launch_gemm_layernorm(const void* x, const void* ln_w, const void* ln_b, flo
                           const void* Bt, int64_t M, int N, int H, const GemmEpilogue& ep,
                           hipStream_t st);
 
+// Causal attention over sequences one behind the other (packed_attn.hip), fp16; pitches in elements.
+struct PackedAttention {
+  const void *q, *k, *v;
+  void* out;
+  const int64_t* starts;
+  int64_t sequences, rows, heads, kv_heads;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+  float scale;
+};
+int launch_flash_attn_packed(const PackedAttention& p, int d, hipStream_t st);
+
 // Rows of logits: x [rows][vocab] at a pitch of ld elements, no alignment beyond the element's.
 struct LogitRows {
   const void* x;

@@ -635,6 +635,54 @@ def flash_attention_v1(q, k, v, dropout_prob=0.0, *, merged_heads_layout=False):
     return buf.transpose(1, 2) if merged_heads_layout else buf
 
 
+def flash_attention_packed(q, k, v, starts, scale=None, out=None):
+    """Causal attention over whole prompts of different lengths, one behind the other without padding, with grouped
+    heads: q [T, N, d], k and v [T, G, d], N a multiple of G -> [T, N, d].  Sequence s is the rows starts[s] ..
+    starts[s + 1] - 1 (int64 on the GPU, S + 1 of them, not decreasing, from 0 to T; a sequence may be empty), scale
+    1 / sqrt(d) if None.
+
+    fp16 (fp32 storage would round q, k and v to it).  A head's d elements lie side by side; rows and heads may be
+    views of something larger at 16-byte aligned pitches, such as the columns of a q, k, v product.  Rows that belong to no
+    sequence are not read, and of `out` (dense; allocated if None) not written."""
+    assert q.dim() == k.dim() == 3 and k.shape == v.shape, (q.shape, k.shape, v.shape)
+    T, N, d = q.shape
+    G = k.shape[1]
+    assert k.shape[0] == T and k.shape[2] == d, (q.shape, k.shape)
+    assert N > 0 and G > 0 and N % G == 0, (N, G)
+    assert d in HEAD_SIZES
+    assert starts.dim() == 1 and starts.shape[0] >= 2 and starts.is_contiguous()
+    if not q.dtype == k.dtype == v.dtype:
+        raise TypeError("flash_attention_packed: q, k and v must share a dtype")
+    if q.dtype != torch.float16:
+        _dtype_code(q, "flash_attention_packed")
+        raise NotImplementedError("flash_attention_packed: fp16 operands only")
+    if starts.dtype != torch.int64:
+        raise TypeError(f"flash_attention_packed: starts must be int64, got {starts.dtype}")
+    dev = _on_gpu(q, k, v, starts, out)
+    pitches = []
+    for t in (q, k, v):
+        row, head, one = t.stride()
+        assert one == 1, "the elements of a head must lie side by side"
+        if (row | head) & 7 or t.data_ptr() & 15:
+            raise NotImplementedError("flash_attention_packed: heads must start at multiples of 16 bytes")
+        pitches += (row, head)
+    if scale is None:
+        scale = d ** -0.5
+    if not 0.0 < scale < math.inf:
+        raise ValueError(f"flash_attention_packed: scale {scale} is not above 0 and finite")
+    if out is None:
+        out = q.new_empty((T, N, d))
+    else:
+        assert out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous()
+        if out.data_ptr() & 15:
+            raise NotImplementedError("flash_attention_packed: out must start at a multiple of 16 bytes")
+    if T > 0:
+        _call(dev, "flash_attention_packed", _lib.load().gptmi_flash_attn_packed, q.data_ptr(), k.data_ptr(),
+              v.data_ptr(), out.data_ptr(), starts.data_ptr(), starts.shape[0] - 1, T, N, G, d, *pitches, scale,
+              _lib.GPTMI_F16)
+    return out
+
+
 class DropoutMask:
     """Bits of the dropout mask that `fused_ffn` (offset m * N + n) and `flash_attention_v1` (offset
     query * Lk + key) draw for probability p: both count flat indices from 0 under one seed, so the

@@ -331,6 +331,25 @@ int gptmi_flash_attn(const void* q, const void* k, const void* v, void* out,
                      void* stream);
 
 /*
+ * Causal attention over whole prompts of different lengths that lie one behind the other, without padding, and with
+ * grouped heads:
+ *   out[i][n] = sum_j w_ij v[j][n G / N],  w_i = softmax(scale q[i][n] . k[j][n G / N]) over the keys j <= i of i's
+ *   sequence; sequence s is the rows starts[s] .. starts[s + 1] - 1, and may be empty
+ *   q [T][N][d] at row and head pitches q_row, q_head (elements, multiples of 8, rows up to 2^24; the columns of a
+ *   q, k, v product as they are), k, v [T][G][d] at theirs, out [T][N][d] dense; N a multiple of G; d = 16, 32, 64, 128 or 256
+ *   starts: sequences + 1 int64 on the device, not decreasing, from 0 to T.  Rows in front of the first and behind the
+ *   last sequence are not read and not written.  (Starts that break these rules reach no row outside [0, T).)
+ * fp16 storage; scores, softmax and sums are fp32, the weights are rounded to fp16 for the product with v (they lie in a
+ * result of that type).  What hidden keys and values hold, infinities and NaN included, plays no part.  scale > 0.
+ * Extends flash_attention_v1 -> kernels.py:477-525, which takes one length and as many key heads as heads.
+ */
+int gptmi_flash_attn_packed(const void* q, const void* k, const void* v, void* out,
+                            const int64_t* starts, int64_t sequences, int64_t T, int64_t N,
+                            int64_t G, int64_t d, int64_t q_row, int64_t q_head, int64_t k_row,
+                            int64_t k_head, int64_t v_row, int64_t v_head, float scale, int dtype,
+                            void* stream);
+
+/*
  * The dropout mask of gptmi_linear and gptmi_flash_attn as bits: bit o % 32 of 32-bit word o / 32 is set
  * iff offset o < n is kept, rand(seed, o) > p.  Both count flat indices from 0, so one mask of the
  * largest matrix serves all the layers of a forward; 1 <= n <= 2^32.  gptmi_dropout_mask_bytes(n) is what

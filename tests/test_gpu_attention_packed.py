@@ -1,0 +1,295 @@
+"""flash_attention_packed against its formula in 64 bits.
+
+Tolerance, from the arithmetic (u = 2^-24, half a step of fp32; h = 2^-11, half a step of fp16):
+  * a score is a sum of d products in fp32: off by (d + 8) u times the sum of their sizes, times the scale.  Its exponent is
+    rounded twice more, relative to itself and to the row's maximum.  Both move a weight by E relative, E the
+    largest such error of the row in natural units, and the hardware's exponential by 2 u;
+  * a weight is rounded to fp16 for the product with v, relative to the row's largest weight: h of itself, or 2^-25 where
+    it is a subnormal number, while the denominator sums L of them in fp32;
+  * an output is rounded to fp16: h of itself, at least 2^-25.
+With A = sum w |v|: |error| <= (h + 2 E + 8 u + L u) A + L 2^-25 max |v| + h |out| + 2^-25."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U, H = 2.0**-24, 2.0**-11
+
+
+@pytest.fixture(scope="module")
+def K(gpu_device):
+    from gpt_triton_amd import kernels
+
+    return kernels
+
+
+def want(q, k, v, scale):
+    """(out, tolerance) of one sequence, [L, N, d] fp16 tensors, in 64 bits."""
+    L, n, d = q.shape
+    rep = n // k.shape[1]
+    out, tol = torch.empty(L, n, d, dtype=torch.float64, device=q.device), torch.empty(L, n, d, dtype=torch.float64,
+                                                                                       device=q.device)
+    past = torch.ones(L, L, dtype=torch.bool, device=q.device).tril_()
+    for i in range(n):
+        a, b, c = q[:, i].double(), k[:, i // rep].double(), v[:, i // rep].double()
+        s = torch.where(past, torch.mm(a, b.t().contiguous()) * scale, -math.inf)
+        w = torch.softmax(s, 1)
+        size = torch.where(past, torch.mm(a.abs(), b.abs().t().contiguous()) * scale, 0.0).amax(1, keepdim=True)
+        e = (d + 16) * U * size
+        out[:, i] = torch.mm(w, c)
+        A = torch.mm(w, c.abs())
+        tol[:, i] = ((H + 2 * e + (8 + L) * U) * A + L * 2.0**-25 * c.abs().amax() + H * out[:, i].abs() + 2.0**-25)
+    return out, tol
+
+
+def make(r, total, n, g, d, fused, device, spread=1.0):
+    sizes = (n, g, g)
+    if fused:
+        y = torch.from_numpy((r.standard_normal((total, sum(sizes), d)) * spread).astype(np.float16)).to(device)
+        return y.split(sizes, dim=1)
+    return tuple(torch.from_numpy((r.standard_normal((total, s, d)) * spread).astype(np.float16)).to(device) for s in sizes)
+
+
+def starts_of(lengths, device, first=0):
+    return torch.tensor([first] + [first + int(x) for x in np.cumsum(lengths)], dtype=torch.int64, device=device)
+
+
+def check(K, q, k, v, lengths, scale=None, first=0):
+    out = K.flash_attention_packed(q, k, v, starts_of(lengths, q.device, first), scale=scale)
+    assert out.shape == q.shape and out.is_contiguous()
+    at = first
+    for L in lengths:
+        rows = slice(at, at + L)
+        at += L
+        if L:
+            w, tol = want(q[rows], k[rows], v[rows], q.shape[2] ** -0.5 if scale is None else scale)
+            err = (out[rows].double() - w).abs()
+            assert torch.all(err <= tol), (L, float((err / tol).max()))
+    return out
+
+
+LENGTHS = [[1], [2], [31], [32, 33], [63, 64, 65], [127, 1, 128, 129], [0, 5, 0, 0, 257, 1, 0], [191, 320, 640, 7],
+           [1] * 40, [1000, 1, 383]]
+
+
+@pytest.mark.parametrize("d", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("heads", [(12, 12), (8, 2), (25, 25)])
+@pytest.mark.parametrize("fused", [True, False])
+def test_lengths(K, gpu_device, d, heads, fused):
+    r = np.random.default_rng(d)
+    for lengths in LENGTHS:
+        if heads[0] == 25 and sum(lengths) > 400:
+            continue
+        check(K, *make(r, sum(lengths), *heads, d, fused, gpu_device), lengths)
+
+
+@pytest.mark.parametrize("d", [16, 64, 128, 256])
+@pytest.mark.parametrize("heads", [(1, 1), (7, 7), (8, 8), (9, 9), (32, 8), (6, 1), (36, 9), (64, 16)])
+def test_heads(K, gpu_device, d, heads):
+    r = np.random.default_rng(heads[0])
+    lengths = [150, 64, 3, 97]
+    check(K, *make(r, sum(lengths), *heads, d, True, gpu_device), lengths)
+
+
+@pytest.mark.parametrize("d", [16, 32, 64, 128, 256])
+def test_long(K, gpu_device, d):
+    r = np.random.default_rng(7)
+    lengths = [3001, 5, 1500]
+    check(K, *make(r, sum(lengths), 2, 1, d, True, gpu_device), lengths)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("scale,spread", [(0.02, 1.0), (1.0, 1.0), (0.125, 6.0), (0.125, 0.01)])
+def test_sharp_and_flat_weights(K, gpu_device, d, scale, spread):
+    """Scores of up to some hundred, where a weight or two are left of a row, and ones that are all alike."""
+    r = np.random.default_rng(8)
+    lengths = [700, 33]
+    check(K, *make(r, sum(lengths), 2, 2, d, False, gpu_device, spread), lengths, scale=scale)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_scores_that_rise_and_fall(K, gpu_device, d):
+    """The running maximum moves in every tile, or never after the first; and leaps by more than weights reach."""
+    r = np.random.default_rng(9)
+    L = 900
+    q, k, v = make(r, L, 2, 2, d, False, gpu_device)
+    q[:] = 0
+    q[:, :, 0] = 1.0
+    ramp = torch.arange(L, device=gpu_device)
+    for values in (ramp * 0.25, -ramp * 0.25, (ramp // 100) * 40.0, (ramp % 130) * 1.0, 200.0 - (ramp // 64) * 14.0):
+        k[:, :, 0] = values[:, None].half()
+        check(K, q, k, v, [L], scale=1.0)
+
+
+@pytest.mark.parametrize("count", [63, 64, 65, 130, 1000, 5000])
+def test_many_sequences(K, gpu_device, count):
+    r = np.random.default_rng(count)
+    lengths = r.integers(0, 4, count).tolist()
+    lengths[count // 3] = 150
+    q, k, v = make(r, sum(lengths), 2, 1, 64, True, gpu_device)
+    out = K.flash_attention_packed(q, k, v, starts_of(lengths, gpu_device))
+    # each against the same rows on their own
+    ends = np.cumsum(lengths)
+    for s in {0, 1, 62, count // 3, count // 2, count - 2, count - 1}:
+        rows = slice(int(ends[s]) - lengths[s], int(ends[s]))
+        if lengths[s]:
+            w, tol = want(q[rows], k[rows], v[rows], 0.125)
+            assert torch.all((out[rows].double() - w).abs() <= tol), s
+    ones = np.flatnonzero(np.array(lengths) == 1)
+    rows = torch.from_numpy(ends[ones] - 1).to(gpu_device)
+    assert torch.equal(out[rows], v[rows].expand(-1, 2, -1))  # a key alone has all the weight
+
+
+@pytest.mark.parametrize("d", [16, 32, 64, 128, 256])
+def test_hidden_keys_play_no_part(K, gpu_device, d):
+    """Infinities and NaN in later tokens, other sequences, and rows of none: the bits of finite ones there."""
+    r = np.random.default_rng(10)
+    lengths, first = [70, 33, 300, 1], 5
+    total = first + sum(lengths) + 9
+    q, k, v = (t.clone() for t in make(r, total, 3, 3, d, False, gpu_device))
+    starts = starts_of(lengths, gpu_device, first)
+    clean = K.flash_attention_packed(q, k, v, starts)
+    end = first + sum(lengths)
+    for bad in (math.nan, math.inf, -math.inf):
+        a, b, c = q.clone(), k.clone(), v.clone()
+        for t in (a, b, c):
+            t[:first] = bad
+            t[end:] = bad
+        assert torch.equal(K.flash_attention_packed(a, b, c, starts)[first:end], clean[first:end])
+        for spoilt in (first + 69, first + 70 + 20, first + 103 + 130, first + 103 + 255):
+            for which in (1, 2):  # a key, a value
+                x = [q, k.clone(), v.clone()]
+                x[which][spoilt] = bad
+                got = K.flash_attention_packed(*x, starts)
+                s = int(torch.searchsorted(starts, spoilt, right=True)) - 1
+                behind = torch.zeros(total, dtype=torch.bool, device=gpu_device)
+                behind[spoilt:int(starts[s + 1])] = True
+                there = torch.zeros_like(behind)
+                there[first:end] = True
+                fine = there & ~behind
+                # the wavefronts that met it form their rows another way: roundings, not bits
+                assert torch.all((got[fine].double() - clean[fine].double()).abs() <= 4 * H * clean[fine].double().abs() + 2e-3)
+                far = fine.clone()
+                far[spoilt - 32:spoilt] = False
+                assert torch.equal(got[far], clean[far])
+                if which == 2:
+                    assert not torch.any(torch.isfinite(got[behind]))
+                elif math.isnan(bad):
+                    assert torch.all(torch.isnan(got[behind]))
+
+
+def test_rows_of_no_sequence_stay(K, gpu_device):
+    r = np.random.default_rng(11)
+    for d in (16, 64, 128, 256):
+        q, k, v = make(r, 400, 4, 2, d, True, gpu_device)
+        out = torch.full((400, 4, d), 7.0, dtype=torch.float16, device=gpu_device)
+        got = K.flash_attention_packed(q, k, v, torch.tensor([100, 170, 170, 301], device=gpu_device), out=out)
+        assert got is out and torch.all(out[:100] == 7) and torch.all(out[301:] == 7)
+        w, tol = want(q[100:170], k[100:170], v[100:170], d ** -0.5)
+        assert torch.all((out[100:170].double() - w).abs() <= tol)
+
+
+def test_starts_that_are_wrong_reach_no_row_outside(K, gpu_device):
+    r = np.random.default_rng(12)
+    q, k, v = make(r, 300, 2, 2, 64, False, gpu_device)
+    for starts in ([-50, 20, 300], [0, 200, 100, 300], [0, 100, 5000], [400, 500], [-10, -5], [10**12, 0, 300], [-10**12, 10**12]):
+        buf = torch.full((302, 2, 64), 7.0, dtype=torch.float16, device=gpu_device)
+        out = K.flash_attention_packed(q, k, v, torch.tensor(starts, device=gpu_device), out=buf[1:301])
+        assert torch.all(buf[0] == 7) and torch.all(buf[301] == 7)
+        assert torch.all(torch.isfinite(out))
+
+
+def test_views_and_pitches(K, gpu_device):
+    """Heads in front of rows, every other row, more than one token's room between rows."""
+    r = np.random.default_rng(13)
+    lengths = [77, 140]
+    total = sum(lengths)
+    q, k, v = make(r, total, 4, 2, 64, False, gpu_device)
+    base = K.flash_attention_packed(q, k, v, starts_of(lengths, gpu_device))
+    heads_first = tuple(t.transpose(0, 1).contiguous().transpose(0, 1) for t in (q, k, v))
+    assert torch.equal(K.flash_attention_packed(*heads_first, starts_of(lengths, gpu_device)), base)
+
+    def spaced(t):
+        big = torch.full((2 * total, t.shape[1], 64 + 8), math.nan, dtype=torch.float16, device=gpu_device)
+        big[::2, :, 8:] = t
+        return big[::2, :, 8:]
+
+    assert torch.equal(K.flash_attention_packed(spaced(q), spaced(k), spaced(v), starts_of(lengths, gpu_device)), base)
+    one_key_head = k[:, :1].expand(-1, 2, -1)  # a pitch of 0
+    check(K, q, one_key_head, v, lengths)
+
+
+def test_rows_beyond_32_bits(K, gpu_device):
+    r = np.random.default_rng(14)
+    lengths = [200, 140, 60]
+    total, pitch = sum(lengths), 12_000_000  # 400 rows: 4.8e9 elements
+    buf = torch.empty((total - 1) * pitch + 3 * 64, dtype=torch.float16, device=gpu_device)
+    y = buf.as_strided((total, 3, 64), (pitch, 64, 1))
+    y.copy_(torch.from_numpy(r.standard_normal((total, 3, 64)).astype(np.float16)))
+    check(K, y[:, :1], y[:, 1:2], y[:, 2:], lengths)
+
+
+def test_equal_lengths_as_flash_attention_v1(K, gpu_device):
+    r = np.random.default_rng(15)
+    for B, n, L, d in ((3, 4, 200, 64), (2, 3, 77, 128)):
+        q, k, v = make(r, B * L, n, n, d, True, gpu_device)
+        got = check(K, q, k, v, [L] * B)
+        batch = [t.reshape(B, L, n, d).transpose(1, 2).contiguous() for t in (q, k, v)]
+        other = K.flash_attention_v1(*batch).transpose(1, 2).reshape(B * L, n, d)
+        assert float((got.double() - other.double()).abs().max()) <= 4 * 2.0**-10 * float(other.abs().max())
+
+
+def test_streams_and_graphs(K, gpu_device):
+    """Captured once, replayed for other lengths: the starts are read on the GPU."""
+    r = np.random.default_rng(16)
+    q, k, v = make(r, 700, 12, 12, 64, True, gpu_device)
+    starts = starts_of([300, 400, 0, 0], gpu_device)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = K.flash_attention_packed(q, k, v, starts)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(other, K.flash_attention_packed(q, k, v, starts))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = K.flash_attention_packed(q, k, v, starts)
+    for lengths in ([300, 400, 0, 0], [1, 1, 1, 697], [0, 0, 700, 0], [175] * 4):
+        starts.copy_(starts_of(lengths, gpu_device))
+        q.copy_(torch.randn_like(q))
+        graph.replay()
+        assert torch.equal(out, K.flash_attention_packed(q, k, v, starts))
+        torch.cuda.synchronize()
+
+
+def test_texts_scored_together(K, gpu_device):
+    """A layer's operators on texts of different lengths: product, attention, projection, LM head, scores."""
+    r = np.random.default_rng(17)
+    lengths, width, heads, V = [40, 1, 100, 23], 256, 4, 1003
+    total = sum(lengths)
+
+    def weight(*shape):
+        return torch.from_numpy((r.standard_normal(shape) / math.sqrt(shape[0])).astype(np.float16)).to(gpu_device)
+
+    x = torch.from_numpy(r.standard_normal((total, width)).astype(np.float16)).to(gpu_device)
+    w_qkv, w_proj, wte = weight(width, 3 * width), weight(width, width), weight(width, V).t().contiguous()
+    starts = starts_of(lengths, gpu_device)
+    y = K.fused_ffn(x, w_qkv)
+    q, k, v = y.view(total, 3, heads, 64).unbind(1)
+    z = K.flash_attention_packed(q, k, v, starts)
+    hidden = K.fused_ffn(z.view(total, width), w_proj, residual=x)
+    logits = K.lm_head(hidden, K.pack_lm_head(wte))
+    tokens = torch.from_numpy(r.integers(0, V, total)).to(gpu_device)
+    together = K.token_log_probs(logits, tokens, top=5)
+    at = 0
+    for L in lengths:  # each text on its own, by the operators for one length
+        rows = slice(at, at + L)
+        at += L
+        a, b, c = K.matmul_and_split_qkv(x[rows].contiguous().view(1, L, width), w_qkv, None, heads)
+        o = K.flash_attention_v1(a, b, c).transpose(1, 2).reshape(L, width).contiguous()
+        h = K.fused_ffn(o, w_proj, residual=x[rows].contiguous())
+        s = K.token_log_probs(K.lm_head(h, wte), tokens[rows], top=5)
+        # both round attention, hidden state and logits to fp16 at the same places: a few steps of a logit (below 8)
+        assert torch.all((s.log_probs - together.log_probs[rows]).abs() <= 8 * 8 * H)
