@@ -467,7 +467,7 @@ int gptmi_softmax(const void* x, void* out, int64_t M, int64_t H, int dtype, voi
 // What the operators on rows of logits ask of them.
 static int check_logits(const char* what, const void* x, int64_t ld, float temperature, int64_t M, int64_t V,
                         int dtype) {
-  if (!x || M <= 0 || V <= 0 || ld < 0 || !dtype_ok(dtype) || !(temperature > 0.0f) || isinf(temperature) ||
+  if (!x || M <= 0 || V <= 0 || ld < 0 || !dtype_ok(dtype) || !(temperature >= 1e-30f) || isinf(temperature) ||
       ((uintptr_t)x & (dtype == GPTMI_F16 ? 1 : 3)) != 0) {
     set_error("%s: invalid argument", what);
     return GPTMI_ERR_INVALID;

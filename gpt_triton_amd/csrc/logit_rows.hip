@@ -1,11 +1,14 @@
 // Rows of logits: log probabilities of given tokens with the row's entropy and its most likely tokens, their
 // gradient, and the distillation loss against a teacher's top logits with its gradient.
 //
-// One workgroup per row.  With z = x / temperature, m = max x, e_j = exp((x_j - m) / temperature), S = sum e_j:
-//   log p_j = (x_j - m) / temperature - log S          H = -sum p_j log p_j = log S - sum e_j log e_j / S
-// Every term of H's second form is at least 0, so neither loses bits to the other; S is 1 for each logit that
-// equals m plus the sum of the others, and log S = log1p of that sum where one does: a confident token's log
-// probability, -1e-5 say, keeps its bits.  Maximum, sums and logarithms are fp32.
+// One workgroup per row.  With z = x / temperature, m = max x and c = log2(e) / temperature, the logits are taken as
+// e_j = 2^t_j, t_j = x_j c - b, b = m c rounded to fp32; one logit that equals m is left out of the sums
+//   s = sum e_j,   u = sum e_j t_j       and is 2^d itself, d = m c - b (what the rounding left)
+// so that, with S = 2^d + s and L = log1p(s 2^-d) = log(S) - d log 2,
+//   log p_j = (x_j - m) / temperature - L       H = -sum p_j log p_j = L - log 2 (u - d s) / S       p_j = e_j / S
+// L is the logarithm of a number near 1 where one token has nearly all the probability, and keeps its bits there (a log
+// probability of -1e-5, say); H's two terms are both positive, so neither loses bits to the other.
+// Maximum, sums and logarithms are fp32.
 #include "common.h"
 
 namespace gptmi {
@@ -25,18 +28,11 @@ template <> struct RowVec<float> {
   static constexpr int N = 4;
 };
 
-// The larger one, for numbers of which none is a NaN; one of two where one is.  By hand: the compiler's own maximum
-// quiets NaNs first, an operation more for each.
-__device__ __forceinline__ unsigned max_h2(unsigned a, unsigned b) {
-  unsigned r;
-  asm("v_pk_max_f16 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
-  return r;
-}
-__device__ __forceinline__ float max_f(float a, float b) {
-  float r;
-  asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
-  return r;
-}
+// Maximum and minimum of which any NaN makes a NaN (one instruction each, two for the price of one in fp16).
+template <typename A>
+__device__ __forceinline__ A most_of(A a, A b) { return __builtin_elementwise_maximum(a, b); }
+template <typename A>
+__device__ __forceinline__ A least_of(A a, A b) { return __builtin_elementwise_minimum(a, b); }
 
 // A row as the workgroup's threads share it: 16-byte chunks from the first aligned address on, dealt one behind
 // the other, and in front and behind at most 2 (N - 1) single elements, one for each of the first threads.
@@ -49,7 +45,7 @@ struct Row {
   const T* x;
   int vocab, lead, chunks, loose;  // loose: the index of this thread's single element, or -1
   V held[CH > 0 ? CH : 1];
-  float single;
+  T single;
   __device__ __forceinline__ Row(const T* row, int vocab_) : x(row), vocab(vocab_) {
     const int ahead = (int)((-(intptr_t)row & 15) / (int)sizeof(T));
     lead = ahead < vocab ? ahead : vocab;
@@ -65,9 +61,15 @@ struct Row {
         held[i] = V((T)-INFINITY);
         if ((int)threadIdx.x + i * NT < chunks) held[i] = p[i * NT];
       }
-      single = -INFINITY;
-      if (loose >= 0) single = (float)x[loose];
+      single = (T)-INFINITY;
+      if (loose >= 0) single = x[loose];
     }
+  }
+  __device__ __forceinline__ T lone() const {
+    if constexpr (CH > 0) return single;
+    T y = (T)-INFINITY;
+    if (loose >= 0) y = x[loose];
+    return y;
   }
   // In front of a pass: what the last one converted is not kept for this one, which is a register for each element.
   __device__ __forceinline__ void renew() {
@@ -94,7 +96,7 @@ struct Row {
 #pragma unroll
       for (int i = 0; i < CH; ++i)
         if (part(i)) chunk(held[i], threadIdx.x + i * NT);
-      const float y[1] = {single};
+      const float y[1] = {(float)single};
       f(y, loose, std::integral_constant<int, 1>{});
     } else {
       for (int c = threadIdx.x; c < chunks; c += NT) chunk(reinterpret_cast<const V*>(x + lead)[c], c);
@@ -104,39 +106,37 @@ struct Row {
       }
     }
   }
-  // the largest of this thread's part, or -infinity
-  __device__ __forceinline__ float largest() const {
-    if constexpr (CH > 0 && sizeof(T) == 2) {
-      typedef unsigned u4v __attribute__((ext_vector_type(4)));
-      unsigned m = 0xfc00fc00u;  // -infinity twice
+  // f(chunks, how many: up to G) for this thread's part of the row but for the single element, the first as soon as
+  // they are there
+  template <int G, typename F>
+  __device__ __forceinline__ void groups(F f) const {
+    if constexpr (CH > 0) {
+      constexpr int REST = CH % G;
 #pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        const u4v u = __builtin_bit_cast(u4v, held[i]);
-        m = max_h2(m, max_h2(max_h2(u[0], u[1]), max_h2(u[2], u[3])));
-      }
-      const h2 two = __builtin_bit_cast(h2, m);
-      return max_f(single, max_f((float)two[0], (float)two[1]));
+      for (int i = 0; i + G <= CH; i += G)
+        if (part(i)) f(held + i, std::integral_constant<int, G>{});
+      if constexpr (REST > 0)
+        if (part(CH - REST)) f(held + CH - REST, std::integral_constant<int, REST>{});
     } else {
-      float m = -INFINITY;
-      each([&](const auto& y, int, auto n) {
+      const V* p = reinterpret_cast<const V*>(x + lead);
+      for (int c = threadIdx.x; c < chunks; c += G * NT) {
+        V v[G];
 #pragma unroll
-        for (int j = 0; j < n.value; ++j) m = max_f(m, y[j]);
-      });
-      return m;
+        for (int k = 0; k < G; ++k) {
+          v[k] = V((T)-INFINITY);
+          if (c + k * NT < chunks) v[k] = p[c + k * NT];
+        }
+        f(v, std::integral_constant<int, G>{});
+      }
     }
   }
   __device__ __forceinline__ float at(int64_t i) const { return (float)x[i]; }
 };
 
-struct Sums {
-  float s, u, n;  // sum of e without the logits that equal the maximum, sum of e log2 e, how many equal it
-};
-
 template <int NT>
 struct Shared {
   static constexpr int W = NT / kWave;
-  float max[W], low[W];
-  Sums sums[W];
+  float top[W], s[W], u[W], low[W];
   int count, scan[W];
 };
 
@@ -150,14 +150,42 @@ __device__ __forceinline__ float join(float v, Op op) {
   return v;
 }
 
+// t = x c - b.  fp16: one operation from the logit as it is, b rounded once for all of a row (65504 c is finite for
+// any temperature above 1e-30).  fp32, whose m c may overflow: the difference, which is 0 for m, and its multiple.
+template <typename T>
+struct Exponent {
+  float c, ref, b;
+  __device__ __forceinline__ Exponent(float c_, float ref_) : c(c_) { at(ref_); }
+  __device__ __forceinline__ void at(float r) {  // 0 in the place of -infinity: nothing is above it
+#pragma clang fp contract(off)  // b is the rounded product wherever it is used
+    ref = r == -INFINITY ? 0.f : r;
+    b = ref * c;
+  }
+  __device__ __forceinline__ float operator()(float x) const {
+    if constexpr (sizeof(T) == 2) return fmaf(x, c, -b);
+    else return (x - ref) * c;
+  }
+  // what the operator gives for the reference itself
+  __device__ __forceinline__ float rest() const { return (*this)(ref); }
+  // how far the exponents move when the reference goes from o's to this one: not above 0 once there is any sum, and
+  // finite, so that nothing is left of one and not a NaN
+  __device__ __forceinline__ float down(const Exponent& o) const {
+#pragma clang fp contract(off)
+    return fmaxf(fminf(sizeof(T) == 2 ? o.b - b : (o.ref - ref) * c, 0.f), -1e25f);
+  }
+};
+// e t with 0 where e is: tokens that cannot occur
+__device__ __forceinline__ float entropy_term(float e, float t, float u) { return fmaf(e, fmaxf(t, -1e30f), u); }
+
 // What a row's softmax needs.
+template <typename T>
 struct Stats {
-  float m, shift, c, inv_tau;  // maximum; what is subtracted (0 where nothing is finite); log2(e) / tau; 1 / tau
-  float S, inv, log_s;         // all 0 where no token has any probability
+  float m, inv_tau;   // maximum, 1 / tau
+  Exponent<T> t;      // with reference m
+  float S, inv, log_s;  // S, 1 / S, L; S = 0 where no token has any probability
   float entropy;
-  __device__ __forceinline__ float log2_e(float x) const { return (x - shift) * c; }
   __device__ __forceinline__ float log_p(float x) const {
-    return S == 0.f ? -INFINITY : (x - shift) * inv_tau - log_s;
+    return S == 0.f ? -INFINITY : (x - m) * inv_tau - log_s;
   }
 };
 
@@ -184,71 +212,136 @@ __device__ __forceinline__ int scan_exclusive(int c, Shared<NT>& sh, int& total)
   return front + s - c;
 }
 
-// Maximum and sums of the row, in an order that depends on nothing but its place in memory and its length.
-// `groups` (a power of two up to NT, or 0): low becomes a value that at least `groups` logits reach, the least of the
-// maxima of so many groups of threads.
+// Maximum and sums of the row, in an order that depends on nothing but its place in memory and its length.  One pass:
+// a thread takes its logits in groups of G chunks, of each first the maximum, which is then the reference of what it has
+// summed (so that no exponent is above 0 and u never changes sign), and keeps the largest logit so far out of the sums:
+// where a larger one comes, the old one goes in.  The groups' sums start while later groups are on their way.
+// `groups` (a power of two, or 0): low becomes a value that at least `groups` logits reach, the least of the maxima of so many
+// groups of threads.
 template <bool ENTROPY, typename T, int NT, int CH>
-__device__ __forceinline__ Stats row_stats(Row<T, NT, CH>& row, float tau, int groups, float& low, Shared<NT>& sh) {
+__device__ __forceinline__ Stats<T> row_stats(Row<T, NT, CH>& row, float tau, int groups, float& low, Shared<NT>& sh) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   constexpr int W = Shared<NT>::W;
-  const float mine = row.largest();
+  constexpr int E = sizeof(T) == 2 ? 2 : 1;  // largest logits kept out: one for each half of a register
+  typedef T Top __attribute__((ext_vector_type(E)));
+  const float inv_tau = 1.0f / tau, c = kLog2e * inv_tau;
+  Top top = Top((T)-INFINITY);
+  top[0] = row.lone();
+  Exponent<T> t(c, -INFINITY);
+  float s[E] = {}, u[E] = {};
+  row.template groups<4>([&](const auto* v, auto n) {
+    constexpr int N = Row<T, NT, CH>::N;
+    Top most = top;
+#pragma unroll
+    for (int k = 0; k < n.value; ++k)
+#pragma unroll
+      for (int j = 0; j < N; j += E) {
+        Top x;
+#pragma unroll
+        for (int i = 0; i < E; ++i) x[i] = v[k][j + i];
+        most = most_of(most, x);
+      }
+    const Exponent<T> old = t;
+    float ref = (float)most[0];
+#pragma unroll
+    for (int i = 1; i < E; ++i) ref = most_of(ref, (float)most[i]);
+    t.at(ref);
+    const float d = t.down(old), f = __builtin_amdgcn_exp2f(d);
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      if constexpr (ENTROPY) u[i] = fmaf(d, s[i], u[i]) * f;
+      s[i] *= f;
+    }
+#pragma unroll
+    for (int k = 0; k < n.value; ++k)
+#pragma unroll
+      for (int j = 0; j < N; j += E) {
+        Top x;
+#pragma unroll
+        for (int i = 0; i < E; ++i) x[i] = v[k][j + i];
+        const Top less = least_of(top, x);
+        top = most_of(top, x);
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          const float y = t((float)less[i]), e = __builtin_amdgcn_exp2f(y);
+          s[i] += e;
+          if constexpr (ENTROPY) u[i] = entropy_term(e, y, u[i]);
+        }
+      }
+  });
+  // the thread's: one largest logit, one sum (its reference may be that of no group at all)
+  float mine = (float)top[0];
+  {
+    const Exponent<T> old = t;
+    float less = -INFINITY;
+    if constexpr (E == 2) {
+      less = least_of(mine, (float)top[1]);
+      mine = most_of(mine, (float)top[1]);
+    }
+    t.at(mine);
+    const float d = t.down(old), f = __builtin_amdgcn_exp2f(d), y = t(less), e = __builtin_amdgcn_exp2f(y);
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      if constexpr (ENTROPY) u[i] = fmaf(d, s[i], u[i]) * f;
+      s[i] *= f;
+    }
+    if constexpr (E == 2) {
+      s[0] += s[1] + e;
+      if constexpr (ENTROPY) u[0] = entropy_term(e, y, u[0] + u[1]);
+    }
+  }
+  // of this lane's (largest, s, u) and others' whose largest is m: the sums for reference m, all but the first largest
+  auto rebase = [&](float& s, float& u, const Exponent<T>& from, const Exponent<T>& to, float largest, bool first) {
+    const float d = to.down(from), f = __builtin_amdgcn_exp2f(d);
+    const float y = to(largest), e = __builtin_amdgcn_exp2f(y);
+    if constexpr (ENTROPY) u = fmaf(d, s, u) * f;
+    s *= f;
+    if (!first) {
+      s += e;
+      if constexpr (ENTROPY) u = entropy_term(e, y, u);
+    }
+  };
   // groups of at most a wavefront: the least of the maxima of NT / groups lanes each
   const int lanes = groups > NT ? 64 : groups > W ? NT / groups : 64;
-  float g = mine;
+  float g = fmaxf(mine, -INFINITY);  // a NaN counts as -infinity
   for (int d = 1; d < lanes; d *= 2) g = fmaxf(g, __shfl_xor(g, d));
-  float least = g, most = g;
-  for (int d = lanes; d < 64; d *= 2) {
-    least = fminf(least, __shfl_xor(least, d));
-    most = fmaxf(most, __shfl_xor(most, d));
+  for (int d = lanes; d < 64; d *= 2) g = fminf(g, __shfl_xor(g, d));
+  const float m_wave = group_reduce<kWave>(mine, [](float a, float b) { return most_of(a, b); });
+  {
+    Exponent<T> to(c, m_wave);
+    const uint64_t largest = __ballot(mine == m_wave);
+    rebase(s[0], u[0], t, to, mine, largest != 0 && lane == __ffsll((unsigned long long)largest) - 1);
   }
+  s[0] = wave_sum(s[0]);
+  if constexpr (ENTROPY) u[0] = wave_sum(u[0]);
   if (lane == 0) {
-    sh.max[wave] = most;
-    sh.low[wave] = least;
+    sh.top[wave] = m_wave;
+    sh.s[wave] = s[0];
+    sh.u[wave] = u[0];
+    sh.low[wave] = g;
   }
   __syncthreads();
-  Stats st;
-  st.m = join<W>(sh.max[lane % W], [](float a, float b) { return fmaxf(a, b); });
-  low = join<W>(sh.low[lane % W], [](float a, float b) { return fminf(a, b); });
-  if (groups > NT) low = -INFINITY;
-  st.inv_tau = 1.0f / tau;
-  st.c = kLog2e * st.inv_tau;
-  st.shift = st.m == -INFINITY ? 0.f : st.m;
-  Sums a = {0.f, 0.f, 0.f};
-  row.renew();
-  row.each([&](const auto& y, int, auto n) {
-#pragma unroll
-    for (int j = 0; j < n.value; ++j) {
-      const float t = st.log2_e(y[j]), e = __builtin_amdgcn_exp2f(t);
-      a.s += e;
-      if constexpr (ENTROPY) a.u = fmaf(e, fmaxf(t, -1e30f), a.u);  // 0 log 0 = 0
-    }
-  });
-  if (__any(mine == st.m) && fabsf(st.m) < INFINITY) {  // again without the maximum, for the few that have it
-    a.s = a.n = 0.f;
-    row.renew();
-    row.each([&](const auto& y, int, auto n) {
-#pragma unroll
-      for (int j = 0; j < n.value; ++j) {
-        const float e = __builtin_amdgcn_exp2f(st.log2_e(y[j]));
-        a.s += y[j] == st.m ? 0.f : e;
-        a.n += y[j] == st.m ? 1.f : 0.f;
-      }
-    });
-  }
-  a.s = wave_sum(a.s);
-  a.n = wave_sum(a.n);
-  if constexpr (ENTROPY) a.u = wave_sum(a.u);
-  if (lane == 0) sh.sums[wave] = a;
-  __syncthreads();
+  const int w = lane % W;
   auto add = [](float a, float b) { return a + b; };
-  a = sh.sums[lane % W];
-  a.s = join<W>(a.s, add);
-  a.n = join<W>(a.n, add);
-  if constexpr (ENTROPY) a.u = join<W>(a.u, add);
-  st.S = a.n + a.s;
-  st.inv = st.S == 0.f ? 0.f : 1.0f / st.S;
-  st.log_s = a.n == 1.f ? log1pf(a.s) : st.S == 0.f ? 0.f : logf(st.S);
-  st.entropy = ENTROPY ? st.log_s - kLn2 * a.u * st.inv : 0.f;
+  mine = sh.top[w];
+  low = groups > NT ? -INFINITY : join<W>(sh.low[w], [](float a, float b) { return fminf(a, b); });
+  const float m = join<W>(mine, [](float a, float b) { return most_of(a, b); });
+  Stats<T> st = {m, inv_tau, Exponent<T>(c, m)};
+  float sum = sh.s[w], terms = sh.u[w];
+  const uint64_t largest = __ballot(mine == m);
+  rebase(sum, terms, Exponent<T>(c, mine), st.t, mine, largest != 0 && w == __ffsll((unsigned long long)largest) - 1);
+  sum = join<W>(sum, add);
+  if constexpr (ENTROPY) terms = join<W>(terms, add);
+  if (m == INFINITY) sum = NAN;
+  const float d = st.t.rest(), one = __builtin_amdgcn_exp2f(d);
+  if (m == -INFINITY) {
+    st.S = st.inv = st.log_s = st.entropy = 0.f;
+  } else {
+    st.S = one + sum;
+    st.inv = 1.0f / st.S;
+    st.log_s = log1pf(sum * __builtin_amdgcn_exp2f(-d));
+    st.entropy = ENTROPY ? st.log_s - kLn2 * fmaf(-d, sum, terms) * st.inv : 0.f;
+  }
   return st;
 }
 
@@ -378,7 +471,7 @@ __global__ __launch_bounds__(NT, WAVES) void token_log_probs_kernel(const T* __r
   if (TOP)
     for (groups = 1; groups < k; groups *= 2) {}
   float low;
-  const Stats st = row_stats<true>(row, tau, groups, low, sh);
+  const Stats<T> st = row_stats<true>(row, tau, groups, low, sh);
   if (log_probs != nullptr) {
     const int64_t t = tokens[r];
     const bool in = t >= 0 && t < vocab;
@@ -487,13 +580,13 @@ __global__ __launch_bounds__(NT, WAVES) void token_log_probs_backward_kernel(
   Row<T, NT, CH> row(x + r * ld, vocab);
   row.load();
   float low;
-  const Stats st = row_stats<true>(row, tau, 0, low, sh);
+  const Stats<T> st = row_stats<true>(row, tau, 0, low, sh);
   __syncthreads();
   for (int i = threadIdx.x; i < count; i += NT) add[i] *= st.inv_tau;
   __syncthreads();
-  const float scale = st.inv * st.inv_tau, lift = st.entropy - st.log_s;
+  const float scale = st.inv * st.inv_tau, lift = st.entropy - st.log_s - kLn2 * st.t.rest();
   write_gradient(row, o, ids, add, st.S == 0.f ? 0 : count, [&](float y) {
-    const float t = st.log2_e(y), p = __builtin_amdgcn_exp2f(t) * scale;
+    const float t = st.t(y), p = __builtin_amdgcn_exp2f(t) * scale;
     return -p * fmaf(h, fmaf(kLn2, fmaxf(t, -1e30f), lift), g);
   });
 }
@@ -555,7 +648,7 @@ __global__ __launch_bounds__(NT, WAVES) void distillation_kernel(const T* __rest
     if (tid == 0) total = sum == 0.f ? 0.f : 1.f;
   }
   float low;
-  const Stats st = row_stats<false>(row, tau, 0, low, sh);
+  const Stats<T> st = row_stats<false>(row, tau, 0, low, sh);
   if (tid < kWave && losses != nullptr) {
     float loss = 0.f;
 #pragma unroll
@@ -566,7 +659,7 @@ __global__ __launch_bounds__(NT, WAVES) void distillation_kernel(const T* __rest
   if constexpr (GRAD) {
     const float scale = total == 0.f ? 0.f : w * st.inv * st.inv_tau;
     write_gradient(row, out + r * ld_out, ids, add, st.S == 0.f ? 0 : k,
-                          [&](float y) { return __builtin_amdgcn_exp2f(st.log2_e(y)) * scale; });
+                          [&](float y) { return __builtin_amdgcn_exp2f(st.t(y)) * scale; });
   }
 }
 

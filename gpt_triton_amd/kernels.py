@@ -341,8 +341,8 @@ def _maybe_check_row_tokens(t, V, what):
 
 
 def _check_temperature(temperature, what):
-    if not 0.0 < temperature < math.inf:
-        raise ValueError(f"{what}: temperature {temperature} is not above 0 and finite")
+    if not 1e-30 <= temperature < 1e30:
+        raise ValueError(f"{what}: temperature {temperature} is not between 1e-30 and 1e30")
 
 
 def _token_log_probs(logits, tokens, top, temperature):
