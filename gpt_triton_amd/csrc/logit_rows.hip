@@ -16,7 +16,6 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kMaxTop = 128;     // top tokens, and a teacher's entries
-constexpr int kCandidates = 2048;
 
 template <typename T> struct RowVec;
 template <> struct RowVec<_Float16> {
@@ -137,7 +136,8 @@ template <int NT>
 struct Shared {
   static constexpr int W = NT / kWave;
   float top[W], s[W], u[W], low[W];
-  int count, scan[W];
+  float groups[64];  // maxima of groups of NT / 64 threads
+  int scan[W];
 };
 
 // op over the W values (a power of two up to 16) that lane l has the l % W-th of, for every lane.
@@ -174,6 +174,10 @@ struct Exponent {
     return fmaxf(fminf(sizeof(T) == 2 ? o.b - b : (o.ref - ref) * c, 0.f), -1e25f);
   }
 };
+// A number that is the same in all lanes, as a scalar: not a register of each thread.
+__device__ __forceinline__ float uniform(float v) {
+  return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v)));
+}
 // e t with 0 where e is: tokens that cannot occur
 __device__ __forceinline__ float entropy_term(float e, float t, float u) { return fmaf(e, fmaxf(t, -1e30f), u); }
 
@@ -216,10 +220,13 @@ __device__ __forceinline__ int scan_exclusive(int c, Shared<NT>& sh, int& total)
 // a thread takes its logits in groups of G chunks, of each first the maximum, which is then the reference of what it has
 // summed (so that no exponent is above 0 and u never changes sign), and keeps the largest logit so far out of the sums:
 // where a larger one comes, the old one goes in.  The groups' sums start while later groups are on their way.
-// `groups` (a power of two, or 0): low becomes a value that at least `groups` logits reach, the least of the maxima of so many
-// groups of threads.
-template <bool ENTROPY, typename T, int NT, int CH>
-__device__ __forceinline__ Stats<T> row_stats(Row<T, NT, CH>& row, float tau, int groups, float& low, Shared<NT>& sh) {
+// TOP: the maxima of 64 groups of threads go to sh.groups, `low` becomes the least of the maxima of 128 (of 64 where there
+// are no more threads); mine: this thread's maximum, a NaN as -infinity.
+struct Tops {
+  float low, mine;
+};
+template <bool ENTROPY, bool TOP, typename T, int NT, int CH>
+__device__ __forceinline__ Stats<T> row_stats(Row<T, NT, CH>& row, float tau, Shared<NT>& sh, Tops* tops = nullptr) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   constexpr int W = Shared<NT>::W;
   constexpr int E = sizeof(T) == 2 ? 2 : 1;  // largest logits kept out: one for each half of a register
@@ -301,11 +308,18 @@ __device__ __forceinline__ Stats<T> row_stats(Row<T, NT, CH>& row, float tau, in
       if constexpr (ENTROPY) u = entropy_term(e, y, u);
     }
   };
-  // groups of at most a wavefront: the least of the maxima of NT / groups lanes each
-  const int lanes = groups > NT ? 64 : groups > W ? NT / groups : 64;
-  float g = fmaxf(mine, -INFINITY);  // a NaN counts as -infinity
-  for (int d = 1; d < lanes; d *= 2) g = fmaxf(g, __shfl_xor(g, d));
-  for (int d = lanes; d < 64; d *= 2) g = fminf(g, __shfl_xor(g, d));
+  if constexpr (TOP) {
+    tops->mine = fmaxf(mine, -INFINITY);
+    float g = tops->mine;
+    constexpr int SMALL = NT >= 128 ? NT / 128 : 1, LANES = NT / 64;
+#pragma unroll
+    for (int d = 1; d < SMALL; d *= 2) g = fmaxf(g, __shfl_xor(g, d));
+    const float least = group_reduce<kWave>(g, [](float a, float b) { return fminf(a, b); });
+#pragma unroll
+    for (int d = SMALL; d < LANES; d *= 2) g = fmaxf(g, __shfl_xor(g, d));
+    if (lane == 0) sh.low[wave] = least;
+    if (lane % LANES == 0) sh.groups[threadIdx.x / LANES] = g;
+  }
   const float m_wave = group_reduce<kWave>(mine, [](float a, float b) { return most_of(a, b); });
   {
     Exponent<T> to(c, m_wave);
@@ -318,15 +332,16 @@ __device__ __forceinline__ Stats<T> row_stats(Row<T, NT, CH>& row, float tau, in
     sh.top[wave] = m_wave;
     sh.s[wave] = s[0];
     sh.u[wave] = u[0];
-    sh.low[wave] = g;
   }
   __syncthreads();
   const int w = lane % W;
   auto add = [](float a, float b) { return a + b; };
   mine = sh.top[w];
-  low = groups > NT ? -INFINITY : join<W>(sh.low[w], [](float a, float b) { return fminf(a, b); });
-  const float m = join<W>(mine, [](float a, float b) { return most_of(a, b); });
-  Stats<T> st = {m, inv_tau, Exponent<T>(c, m)};
+  if constexpr (TOP) tops->low = uniform(join<W>(sh.low[w], [](float a, float b) { return fminf(a, b); }));
+  const float m = uniform(join<W>(mine, [](float a, float b) { return most_of(a, b); }));
+  Stats<T> st = {m, uniform(inv_tau), Exponent<T>(uniform(c), m)};
+  st.t.b = uniform(st.t.b);
+  st.t.ref = uniform(st.t.ref);
   float sum = sh.s[w], terms = sh.u[w];
   const uint64_t largest = __ballot(mine == m);
   rebase(sum, terms, Exponent<T>(c, mine), st.t, mine, largest != 0 && w == __ffsll((unsigned long long)largest) - 1);
@@ -337,10 +352,10 @@ __device__ __forceinline__ Stats<T> row_stats(Row<T, NT, CH>& row, float tau, in
   if (m == -INFINITY) {
     st.S = st.inv = st.log_s = st.entropy = 0.f;
   } else {
-    st.S = one + sum;
-    st.inv = 1.0f / st.S;
-    st.log_s = log1pf(sum * __builtin_amdgcn_exp2f(-d));
-    st.entropy = ENTROPY ? st.log_s - kLn2 * fmaf(-d, sum, terms) * st.inv : 0.f;
+    st.S = uniform(one + sum);
+    st.inv = uniform(1.0f / st.S);
+    st.log_s = uniform(log1pf(sum * __builtin_amdgcn_exp2f(-d)));
+    st.entropy = ENTROPY ? uniform(st.log_s - kLn2 * fmaf(-d, sum, terms) * st.inv) : 0.f;
   }
   return st;
 }
@@ -357,104 +372,198 @@ __device__ __forceinline__ float key_value(uint64_t key) {
 }
 __device__ __forceinline__ int key_index(uint64_t key) { return (int)(0xffffffffu - (unsigned)key); }
 
-// The k largest logits.  At least k reach `low` (row_stats); the ones above it are gathered, usually some k log k of
-// them, with the lowest-numbered of those that equal it where that leaves fewer than k.  Of more than 256 a
-// wavefront finds the k-th by bisection; what is left is ranked by counting.  found[r], r < k: the r-th.
-template <typename T, int NT, int CH>
-__device__ __forceinline__ void row_top(Row<T, NT, CH>& row, int k, float low, uint64_t* cand, uint64_t* found,
-                                        Shared<NT>& sh) {
-  const int tid = threadIdx.x, lane = tid & 63;
-  auto gather = [&](auto& from) {
-    __syncthreads();
-    if (tid == 0) sh.count = 0;
-    __syncthreads();
-    from.each([&](const auto& y, int first, auto n) {
-#pragma unroll
-      for (int j = 0; j < n.value; ++j)
-        if (y[j] > low) {
-          const int at = atomicAdd(&sh.count, 1);
-          if (at < kCandidates) cand[at] = top_key(y[j], first + j);
-        }
-    });
-    __syncthreads();
-    return sh.count;
-  };
-  row.renew();
-  int n = gather(row);
-  if (n > kCandidates) {
-    const Row<T, NT, 0> again(row.x, row.vocab);  // seldom: from memory, for the registers' sake
-    // the k-th largest value, bit by bit from the top: the largest that at least k reach
-    unsigned kth = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-      const unsigned trial = kth | 1u << bit;
-      int c = 0;
-      again.each([&](const auto& y, int, auto m) {
-#pragma unroll
-        for (int j = 0; j < m.value; ++j) c += (unsigned)(top_key(y[j], 0) >> 32) >= trial;
-      });
-      int total;
-      scan_exclusive<NT>(c, sh, total);
-      if (total >= k) kth = trial;
-    }
-    low = key_value((uint64_t)kth << 32);
-    n = gather(again);  // fewer than k are above it
+template <int NT>
+struct TopShared {
+  static constexpr int kKeep = NT == 64 ? 512 : 1024;  // about 700 are kept of 128 groups of random logits
+  static constexpr int kBins = 256;
+  uint64_t kept[kKeep], fewer[kKeep];
+  int bins[kBins], count, count_fewer, cut, threads;
+  short thread[NT];
+  __device__ __forceinline__ void clear() {  // in front of a barrier in front of row_top
+    for (int i = threadIdx.x; i < kBins; i += NT) bins[i] = 0;
+    if (threadIdx.x == 0) count = count_fewer = threads = 0;
   }
-  if (n < k) {
-    // the first k - n of the logits that equal `low`, in the order of their indices
-    auto take = [&](bool one, int first, int elements, auto value) {
-      int c = 0, total;
-      if (one)
-        for (int j = 0; j < elements; ++j) c += fmaxf(value(j), -INFINITY) == low;
-      int at = n + scan_exclusive<NT>(c, sh, total);
-      if (one)
-        for (int j = 0; j < elements; ++j)
-          if (fmaxf(value(j), -INFINITY) == low) {
-            if (at < k) cand[at] = top_key(value(j), first + j);
-            ++at;
-          }
-      n += total;
-    };
-    auto at = [&](int first) { return [&row, first](int j) { return row.at(first + j); }; };
-    take(tid < row.lead, tid, 1, at(tid));
-    for (int c = 0; c < row.chunks && n < k; c += NT) {
-      const int first = row.lead + (c + tid) * Row<T, NT, CH>::N;
-      take(c + tid < row.chunks, first, Row<T, NT, CH>::N, at(first));
-    }
-    if (n < k) take(row.loose >= row.lead, row.loose, 1, at(row.loose));
-    n = k;
-    __syncthreads();
-  }
-  if (n > 256) {
-    if (tid < kWave) {
-      // keys differ, so exactly k reach the k-th; as soon as k reach a trial, those are the ones
-      uint64_t kth = 0;
-      for (int bit = 63; bit >= 0; --bit) {
-        const uint64_t trial = kth | 1ull << bit;
-        int c = 0;
-        for (int i = lane; i < n; i += kWave) c += cand[i] >= trial;
-        c = (int)wave_sum((float)c);
-        if (c >= k) kth = trial;
-        if (c == k) break;
-      }
-      int kept = 0;
-      for (int i = lane; i - lane < n; i += kWave) {
-        const uint64_t key = i < n ? cand[i] : 0;
-        const uint64_t in = __ballot(i < n && key >= kth);
-        // writes stay behind the reads: kept + 63 < i - lane + 64
-        if (in >> lane & 1) cand[kept + __popcll(in & ((1ull << lane) - 1))] = key;
-        kept += __popcll(in);
-      }
-    }
-    n = k;
-    __syncthreads();
-  }
-  for (int i = tid; i < n; i += NT) {
-    const uint64_t key = cand[i];
+};
+
+// found(r, key) of the k largest logits, r = 0 .. k - 1 in any order, by one thread each.  At least k logits reach `low`,
+// the k-th largest of the maxima of 64 groups of threads, or the least of 128 where k is larger: those are kept, little more
+// than k up to k = 40 or so and some 700 of 128 groups.  Where few threads have any, the wavefronts take these threads' logits
+// from memory, else the workgroup takes all.  Of more than 256 kept a histogram leaves the ones from the k-th's bin on.
+// The rest is ranked by counting.
+template <typename T, int NT, int CH, typename F>
+__device__ __forceinline__ void row_top(Row<T, NT, CH>& row, int k, Tops tops, float high, TopShared<NT>& top,
+                                        Shared<NT>& sh, F found) {
+  constexpr int kKeep = TopShared<NT>::kKeep, N = Row<T, NT, CH>::N, W = Shared<NT>::W;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  float low = tops.low;
+  if (k <= 64) {
+    // ranks of the 64 as numbers that differ: a maximum without its last 6 bits, and the group in their place; rounded down,
+    // the k-th is still reached by k
+    const unsigned key = (unsigned)(top_key(sh.groups[lane], 0) >> 32) & ~63u | (63 - lane);
     int rank = 0;
-    for (int j = 0; j < n; ++j) rank += cand[j] > key;
-    if (rank < k) found[rank] = key;
+#pragma unroll
+    for (int j = 0; j < 64; ++j) rank += (unsigned)__builtin_amdgcn_readlane((int)key, j) > key;
+    const uint64_t kth = __ballot(rank == k - 1);
+    const unsigned down = (unsigned)__shfl((int)key, __ffsll((unsigned long long)kth) - 1) & ~63u;
+    low = down < 0x007fffffu ? -INFINITY : uniform(key_value((uint64_t)down << 32));  // below -infinity's there are NaNs
+  } else if (NT == 64) {
+    low = -INFINITY;
   }
-  __syncthreads();
+  auto put = [&](int at, float y, int index) {
+    if (at < kKeep) top.kept[at] = top_key(y, index);
+  };
+  auto keep = [&](auto above) {
+    return [&, above](const auto& y, int first, auto n) {
+      int c = 0;
+#pragma unroll
+      for (int j = 0; j < n.value; ++j) c += above(y[j]);
+      if (c > 0) {
+        int at = atomicAdd(&top.count, c);
+#pragma unroll
+        for (int j = 0; j < n.value; ++j)
+          if (above(y[j])) put(at++, y[j], first + j);
+      }
+    };
+  };
+  const Row<T, NT, 0> again(row.x, row.vocab);  // from memory: held any longer, a row's registers are too many
+  auto recount = [&](auto above) {
+    __syncthreads();
+    if (tid == 0) top.count = 0;
+    __syncthreads();
+    again.each(keep(above));
+    __syncthreads();
+    return top.count;
+  };
+  auto reaches = [&](float y) { return y >= low; };
+  auto above = [&](float y) { return y > low; };
+  int n = kKeep + 1;  // all logits reach -infinity: not gathered
+  if (low > -INFINITY) {
+    const uint64_t in = __ballot(tops.mine >= low);
+    if (in) {
+      int base = 0;
+      if (lane == 0) base = atomicAdd(&top.threads, __popcll(in));
+      base = __builtin_amdgcn_readfirstlane(base);
+      if (in >> lane & 1) top.thread[base + __popcll(in & ((1ull << lane) - 1))] = (short)tid;
+    }
+    __syncthreads();
+    const int threads = top.threads;
+    if (threads <= 8 * W) {
+      const int part = (row.chunks + NT - 1) / NT * N + 1;  // logits of a thread, the last one single
+      const float per = 1.0f / (float)part;
+      for (int f = tid; f < threads * part; f += 4 * NT) {
+        float y[4];
+        int index[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int at = f + i * NT, nth = (int)(((float)at + 0.5f) * per), e = at - nth * part;
+          y[i] = -INFINITY;
+          if (at < threads * part) {
+            const int t = top.thread[nth], chunk = t + e / N * NT;
+            const bool single = e == part - 1;
+            index[i] = !single ? row.lead + chunk * N + e % N : t < row.lead ? t : t + row.chunks * N;
+            if (single ? t < row.vocab - row.chunks * N : chunk < row.chunks) y[i] = row.at(index[i]);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (y[i] >= low) put(atomicAdd(&top.count, 1), y[i], index[i]);
+      }
+      __syncthreads();
+      n = top.count;
+    } else {
+      n = recount(reaches);
+    }
+  }
+  if (n > kKeep) {
+    n = recount(above);
+    if (n > kKeep) {
+      // the k-th largest value, bit by bit from the top: the largest that at least k reach
+      unsigned kth = 0;
+      for (int bit = 31; bit >= 0; --bit) {
+        const unsigned trial = kth | 1u << bit;
+        int c = 0;
+        again.each([&](const auto& y, int, auto m) {
+#pragma unroll
+          for (int j = 0; j < m.value; ++j) c += (unsigned)(top_key(y[j], 0) >> 32) >= trial;
+        });
+        int total;
+        scan_exclusive<NT>(c, sh, total);
+        if (total >= k) kth = trial;
+      }
+      low = key_value((uint64_t)kth << 32);
+      n = recount(above);  // fewer than k
+    }
+    if (n < k) {
+      // the first k - n of the logits that equal `low`, in the order of their indices
+      auto take = [&](bool one, int first, int elements) {
+        int c = 0, total;
+        if (one)
+          for (int j = 0; j < elements; ++j) c += fmaxf(row.at(first + j), -INFINITY) == low;
+        int at = n + scan_exclusive<NT>(c, sh, total);
+        if (one)
+          for (int j = 0; j < elements; ++j)
+            if (fmaxf(row.at(first + j), -INFINITY) == low) {
+              if (at < k) top.kept[at] = top_key(row.at(first + j), first + j);
+              ++at;
+            }
+        n += total;
+      };
+      take(tid < row.lead, tid, 1);
+      for (int c = 0; c < row.chunks && n < k; c += NT) take(c + tid < row.chunks, row.lead + (c + tid) * N, N);
+      if (n < k) take(row.loose >= row.lead, row.loose, 1);
+      n = k;
+      __syncthreads();
+    }
+  }
+  const uint64_t* list = top.kept;
+  if (n > 256) {
+    // bins of the values between low and the largest; the list goes on with those from the bin on in which the k-th is
+    constexpr int kBins = TopShared<NT>::kBins;
+    const unsigned base = (unsigned)(top_key(low, 0) >> 32), range = (unsigned)(top_key(high, 0) >> 32) - base;
+    const int shift = max(0, 24 - __clz((int)(range | 1)));
+    auto bin_of = [&](uint64_t key) { return min(((unsigned)(key >> 32) - base) >> shift, kBins - 1u); };
+    for (int i = tid; i < n; i += NT) atomicAdd(&top.bins[bin_of(top.kept[i])], 1);
+    __syncthreads();
+    if (tid < kWave) {
+      int c[kBins / kWave], sum = 0;  // this lane's bins, the highest values first
+#pragma unroll
+      for (int i = 0; i < kBins / kWave; ++i) sum += c[i] = top.bins[kBins - 1 - (lane * (kBins / kWave) + i)];
+      int front = sum;
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) {
+        const int o = __shfl_up(front, d);
+        front += lane >= d ? o : 0;
+      }
+      front -= sum;
+#pragma unroll
+      for (int i = 0; i < kBins / kWave; ++i) {
+        if (front < k && front + c[i] >= k) top.cut = kBins - 1 - (lane * (kBins / kWave) + i);
+        front += c[i];
+      }
+    }
+    __syncthreads();
+    const unsigned cut = (unsigned)top.cut;
+    for (int i = tid; i < n; i += NT) {
+      const uint64_t key = top.kept[i];
+      if (bin_of(key) >= cut) top.fewer[atomicAdd(&top.count_fewer, 1)] = key;
+    }
+    __syncthreads();
+    n = top.count_fewer;
+    list = top.fewer;
+  }
+  // 2^split threads for a key, each for a part of the others
+  int split = 0;
+  while (split < 4 && (n << (split + 1)) <= NT) ++split;
+  const int parts = 1 << split, part = tid & (parts - 1);
+#pragma unroll 1
+  for (int i = tid >> split; i < ((n << split) + 63 & -64) >> split; i += NT >> split) {
+    const uint64_t key = list[i < n ? i : 0];
+    int rank = 0;
+#pragma unroll 8
+    for (int j = part; j < n; j += parts) rank += list[j] > key;
+    for (int d = 1; d < parts; d *= 2) rank += __shfl_xor(rank, d);
+    if (i < n && part == 0 && rank < k) found(rank, key);
+  }
 }
 
 template <typename T, bool TOP, int NT, int CH, int WAVES>
@@ -467,11 +576,14 @@ __global__ __launch_bounds__(NT, WAVES) void token_log_probs_kernel(const T* __r
   const int64_t r = blockIdx.x;
   Row<T, NT, CH> row(x + r * ld, vocab);
   row.load();
-  int groups = 0;
-  if (TOP)
-    for (groups = 1; groups < k; groups *= 2) {}
-  float low;
-  const Stats<T> st = row_stats<true>(row, tau, groups, low, sh);
+  TopShared<NT>* top_shared = nullptr;
+  if constexpr (TOP) {
+    __shared__ TopShared<NT> top;
+    top_shared = &top;
+    top.clear();
+  }
+  Tops tops;
+  const Stats<T> st = row_stats<true, TOP>(row, tau, sh, &tops);
   if (log_probs != nullptr) {
     const int64_t t = tokens[r];
     const bool in = t >= 0 && t < vocab;
@@ -479,21 +591,60 @@ __global__ __launch_bounds__(NT, WAVES) void token_log_probs_kernel(const T* __r
     if (threadIdx.x == 0) log_probs[r] = in ? score : 0.f;
   }
   if (entropy != nullptr && threadIdx.x == 0) entropy[r] = st.entropy;
-  if constexpr (TOP) {
-    __shared__ uint64_t cand[kCandidates], found[kMaxTop];
-    row_top(row, k, low, cand, found, sh);
-    for (int i = threadIdx.x; i < k; i += NT) {
-      top_log_probs[r * k + i] = st.log_p(key_value(found[i]));
-      top_tokens[r * k + i] = key_index(found[i]);
+  if constexpr (TOP)
+    row_top(row, k, tops, st.m, *top_shared, sh, [&](int rank, uint64_t key) {
+      top_log_probs[r * k + rank] = st.log_p(key_value(key));
+      top_tokens[r * k + rank] = key_index(key);
+    });
+}
+
+// Tokens of a row whose gradient has a part of its own: the token, its logit, its part, and the sum of the parts of all
+// entries of that token; first[t] and next[i] chain the entries whose logits thread t has.
+template <int NT>
+struct Special {
+  int id[kMaxTop + 1], next[kMaxTop + 1], first[NT];
+  float x[kMaxTop + 1], add[kMaxTop + 1], total[kMaxTop + 1];
+};
+
+// The entries lane, lane + 64, .. of a row, by the first wavefront and for all behind the next barrier: f(i, token, part, logit)
+// gives entry i, token -1 for none.
+template <typename T, int NT, int CH, typename F>
+__device__ __forceinline__ void set_special(const Row<T, NT, CH>& row, Special<NT>& sp, int count, F f) {
+  const int lane = threadIdx.x;
+  for (int t = lane; t < NT; t += kWave) sp.first[t] = -1;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+  for (int e = 0; e <= kMaxTop / kWave; ++e) {
+    const int i = lane + e * kWave;
+    if (i >= count) break;
+    int64_t token = -1;
+    float part = 0.f, x = 0.f;
+    f(e, i, token, part, x);
+    const bool in = token >= 0 && token < row.vocab;
+    const int id = in ? (int)token : -1, behind = id - row.lead;
+    sp.id[i] = id;
+    sp.add[i] = in ? part : 0.f;
+    sp.x[i] = x;
+    if (in) {
+      const int owner = behind < 0 ? id : behind < row.chunks * row.N ? behind / row.N % NT : id - row.chunks * row.N;
+      sp.next[i] = atomicExch(&sp.first[owner], i);
     }
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  for (int i = lane; i < count; i += kWave) {
+    const int id = sp.id[i];
+    float sum = 0.f;
+#pragma unroll 8
+    for (int j = 0; j < count; ++j) sum += sp.id[j] == id ? sp.add[j] : 0.f;
+    sp.total[i] = sum;
   }
 }
 
-// Writes f(x_j, ...) of every logit of the row, then the entries of `ids` (count of them, in LDS, -1: none) as
-// f plus the sum of their `add`s: entries of one token share its place and write the same number there.
+// Writes f(x_j) of every logit of the row, and of the special ones' f(x) + scale total: over what was written, by the thread
+// that wrote it, so that nothing has to be waited for.  Entries of one token write one number.
 template <typename T, int NT, int CH, typename F>
-__device__ __forceinline__ void write_gradient(Row<T, NT, CH>& row, T* __restrict__ out, const int* ids,
-                                               const float* add, int count, F f) {
+__device__ __forceinline__ void write_gradient(Row<T, NT, CH>& row, T* __restrict__ out, const Special<NT>& sp,
+                                               bool special, float scale, F f) {
   typedef typename RowVec<T>::V V;
   const bool whole = ((uintptr_t)out & 15) == ((uintptr_t)row.x & 15);
   row.renew();
@@ -513,15 +664,9 @@ __device__ __forceinline__ void write_gradient(Row<T, NT, CH>& row, T* __restric
       out[first] = (T)f(y[0]);
     }
   });
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // another wavefront's store to the same place comes behind
-  __syncthreads();
-  for (int i = threadIdx.x; i < count; i += NT) {
-    const int id = ids[i];
-    if (id < 0) continue;
-    float sum = 0.f;
-    for (int j = 0; j < count; ++j) sum += ids[j] == id ? add[j] : 0.f;
-    out[id] = (T)(f(row.at(id)) + sum);
-  }
+  asm volatile("" ::: "memory");
+  if (special)
+    for (int i = sp.first[threadIdx.x]; i >= 0; i = sp.next[i]) out[sp.id[i]] = (T)fmaf(scale, sp.total[i], f(sp.x[i]));
 }
 
 template <typename T, int NT>
@@ -540,52 +685,47 @@ __global__ __launch_bounds__(NT, WAVES) void token_log_probs_backward_kernel(
     const float* __restrict__ d_log_probs, const float* __restrict__ d_entropy, int k,
     const int64_t* __restrict__ top_tokens, const float* __restrict__ d_top, T* __restrict__ out, int64_t ld_out) {
   __shared__ Shared<NT> sh;
-  __shared__ int ids[kMaxTop + 1];
-  __shared__ float add[kMaxTop + 1];
+  __shared__ Special<NT> sp;
   const int64_t r = blockIdx.x;
   const int count = k + 1;
+  Row<T, NT, CH> row(x + r * ld, vocab);
   // Where the condition is the same for all threads, and not in a thread's branch below: a load from one address is
   // a scalar one, which a wavefront executes in a branch that none of its lanes takes.
   int64_t token = -1;
-  float d_token = 0.f;
+  float d_token = 0.f, h = 0.f;
   if (d_log_probs != nullptr) {
     token = tokens[r];
     d_token = d_log_probs[r];
   }
-  for (int i = threadIdx.x; i < count; i += NT) {
-    int64_t t = token;
-    float d = d_token;
-    if (i < k) {
-      t = top_tokens[r * k + i];
-      d = d_top[r * k + i];
-    }
-    const bool in = t >= 0 && t < vocab;
-    ids[i] = in ? (int)t : -1;
-    add[i] = in ? d : 0.f;
-  }
+  if (d_entropy != nullptr) h = d_entropy[r];
+  if (threadIdx.x < kWave)
+    set_special(row, sp, count, [&](int, int i, int64_t& t, float& part, float& logit) {
+      t = token;
+      part = d_token;
+      if (i < k) {
+        t = top_tokens[r * k + i];
+        part = d_top[r * k + i];
+      }
+      if (t >= 0 && t < vocab) logit = row.at(t);
+    });
   __syncthreads();
   float g = 0.f;
   bool none = true;
+#pragma unroll 8
   for (int i = 0; i < count; ++i) {
-    g += add[i];
-    none &= add[i] == 0.f;
+    g += sp.add[i];
+    none &= sp.add[i] == 0.f;
   }
-  float h = 0.f;
-  if (d_entropy != nullptr) h = d_entropy[r];
+  g = uniform(g);
   T* o = out + r * ld_out;
   if (none && h == 0.f) {  // padding: whatever its logits are
     write_zeros<T, NT>(o, vocab);
     return;
   }
-  Row<T, NT, CH> row(x + r * ld, vocab);
   row.load();
-  float low;
-  const Stats<T> st = row_stats<true>(row, tau, 0, low, sh);
-  __syncthreads();
-  for (int i = threadIdx.x; i < count; i += NT) add[i] *= st.inv_tau;
-  __syncthreads();
-  const float scale = st.inv * st.inv_tau, lift = st.entropy - st.log_s - kLn2 * st.t.rest();
-  write_gradient(row, o, ids, add, st.S == 0.f ? 0 : count, [&](float y) {
+  const Stats<T> st = row_stats<true, false>(row, tau, sh);
+  const float scale = uniform(st.inv * st.inv_tau), lift = uniform(st.entropy - st.log_s - kLn2 * st.t.rest());
+  write_gradient(row, o, sp, st.S != 0.f, st.inv_tau, [&](float y) {
     const float t = st.t(y), p = __builtin_amdgcn_exp2f(t) * scale;
     return -p * fmaf(h, fmaf(kLn2, fmaxf(t, -1e30f), lift), g);
   });
@@ -600,8 +740,8 @@ __global__ __launch_bounds__(NT, WAVES) void distillation_kernel(const T* __rest
                                                           const float* __restrict__ weights, float* __restrict__ losses,
                                                           T* __restrict__ out, int64_t ld_out) {
   __shared__ Shared<NT> sh;
-  __shared__ int ids[kMaxTop];
-  __shared__ float add[kMaxTop], total;
+  __shared__ Special<NT> sp;
+  __shared__ float total;
   const int64_t r = blockIdx.x;
   const int tid = threadIdx.x;
   const float w = weights != nullptr ? weights[r] : 1.f;
@@ -611,22 +751,35 @@ __global__ __launch_bounds__(NT, WAVES) void distillation_kernel(const T* __rest
     return;
   }
   Row<T, NT, CH> row(x + r * ld, vocab);
-  row.load();
   constexpr int E = kMaxTop / kWave;  // a lane's entries, for the first wavefront
+  __shared__ float entry_q[kMaxTop], entry_log_q[kMaxTop], entry_x[kMaxTop];  // not a register each of all wavefronts
   float q[E], log_q[E], student[E];
+  // the entries and their logits are requested first, and worked on while the row is on its way
+  int64_t entry[E];
+  if (tid < kWave) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const int at = tid + i * kWave;
+      entry[i] = -1;
+      log_q[i] = -INFINITY;
+      if (at < k) {
+        entry[i] = teacher_tokens[r * k + at];
+        log_q[i] = teacher_f16 ? (float)((const _Float16*)teacher)[r * k + at] : ((const float*)teacher)[r * k + at];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      student[i] = 0.f;
+      if (entry[i] >= 0 && entry[i] < vocab) student[i] = row.at(entry[i]);
+    }
+  }
+  row.load();
   if (tid < kWave) {
     const float inv_tau = 1.0f / tau;
     float most = -INFINITY, sum = 0.f;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      const int at = tid + i * kWave;
-      const int64_t t = at < k ? teacher_tokens[r * k + at] : -1;
-      const bool in = t >= 0 && t < vocab;
-      float value = -INFINITY;
-      if (in) value = teacher_f16 ? (float)((const _Float16*)teacher)[r * k + at] : ((const float*)teacher)[r * k + at];
-      log_q[i] = value * inv_tau;
-      student[i] = in ? row.at(t) : 0.f;
-      if (at < k) ids[at] = in ? (int)t : -1;
+      log_q[i] = entry[i] >= 0 && entry[i] < vocab ? log_q[i] * inv_tau : -INFINITY;
       most = fmaxf(most, log_q[i]);
     }
     most = wave_max(most);
@@ -642,24 +795,34 @@ __global__ __launch_bounds__(NT, WAVES) void distillation_kernel(const T* __rest
 #pragma unroll
     for (int i = 0; i < E; ++i) {
       q[i] *= inv;
-      log_q[i] -= log_sum;
-      if (tid + i * kWave < k) add[tid + i * kWave] = -q[i] * w * inv_tau;
+      entry_q[tid + i * kWave] = q[i];
+      entry_log_q[tid + i * kWave] = log_q[i] - log_sum;
+      entry_x[tid + i * kWave] = student[i];
     }
     if (tid == 0) total = sum == 0.f ? 0.f : 1.f;
+    if constexpr (GRAD)
+      set_special(row, sp, k, [&](int e, int, int64_t& token, float& part, float& logit) {
+        if (e >= E) return;
+        token = entry[e];
+        part = -q[e];
+        logit = student[e];
+      });
   }
-  float low;
-  const Stats<T> st = row_stats<false>(row, tau, 0, low, sh);
+  const Stats<T> st = row_stats<false, false>(row, tau, sh);
   if (tid < kWave && losses != nullptr) {
     float loss = 0.f;
 #pragma unroll
-    for (int i = 0; i < E; ++i) loss += q[i] == 0.f ? 0.f : q[i] * (log_q[i] - st.log_p(student[i]));
+    for (int i = 0; i < E; ++i) {
+      const int at = tid + i * kWave;
+      loss += entry_q[at] == 0.f ? 0.f : entry_q[at] * (entry_log_q[at] - st.log_p(entry_x[at]));
+    }
     loss = wave_sum(loss);
     if (tid == 0) losses[r] = total == 0.f ? 0.f : w * loss;
   }
   if constexpr (GRAD) {
-    const float scale = total == 0.f ? 0.f : w * st.inv * st.inv_tau;
-    write_gradient(row, out + r * ld_out, ids, add, st.S == 0.f ? 0 : k,
-                          [&](float y) { return __builtin_amdgcn_exp2f(st.t(y)) * scale; });
+    const float scale = uniform(total == 0.f ? 0.f : w * st.inv * st.inv_tau);
+    write_gradient(row, out + r * ld_out, sp, st.S != 0.f, w * st.inv_tau,
+                   [&](float y) { return __builtin_amdgcn_exp2f(st.t(y)) * scale; });
   }
 }
 

@@ -319,13 +319,14 @@ def _logit_rows(logits, what):
 
 
 def _logit_gradient(logits, rows, V, ld):
-    """(a buffer for the gradient of rows of logits, its pitch, its view in the logits' shape).  Pitch and address equal
-    the logits' modulo 64 elements and 16 bytes, so that the kernels read and write in the same chunks."""
+    """(a buffer for the gradient of rows of logits in their shape, its pitch).  Pitch and address equal the logits'
+    modulo 64 elements and 16 bytes, so that the kernels read and write in the same chunks."""
     pitch = V + (ld - V) % 64
     offset = logits.data_ptr() % 16 // logits.element_size()
+    if offset == 0 and (pitch == V or rows <= 1):
+        return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device), pitch
     buf = logits.new_empty(offset + max(rows - 1, 0) * pitch + V)
-    buf = buf.as_strided((rows, V), (pitch, 1), offset)
-    return buf, pitch, buf.view(logits.shape)
+    return buf.as_strided((rows, V), (pitch, 1), offset).view(logits.shape), pitch
 
 
 def _check_row_tokens(t, shape, what):
@@ -388,11 +389,11 @@ class _TokenLogProbsFunction(torch.autograd.Function):
             return None, None, None, None
         dev, code, rows, V, ld = _logit_rows(logits, "token_log_probs")
         d_log_probs, d_entropy, d_top = (None if g is None else g.contiguous() for g in (d_log_probs, d_entropy, d_top))
-        buf, pitch, grad = _logit_gradient(logits, rows, V, ld)
+        grad, pitch = _logit_gradient(logits, rows, V, ld)
         if rows > 0:
             _call(dev, "token_log_probs_backward", _lib.load().gptmi_token_log_probs_backward, logits.data_ptr(), ld,
                   _ptr(tokens), ctx.temperature, _ptr(d_log_probs), _ptr(d_entropy),
-                  0 if d_top is None else top_tokens.shape[-1], _ptr(top_tokens), _ptr(d_top), buf.data_ptr(), pitch,
+                  0 if d_top is None else top_tokens.shape[-1], _ptr(top_tokens), _ptr(d_top), grad.data_ptr(), pitch,
                   rows, V, code)
         return grad, None, None, None
 
@@ -435,13 +436,10 @@ def _distillation(logits, teacher_tokens, teacher_logits, temperature, weights, 
         assert weights.is_contiguous()
     _check_temperature(temperature, what)
     out = logits.new_empty(lead, dtype=torch.float32) if losses else None
-    buf = grad = None
-    pitch = V
-    if gradient:
-        buf, pitch, grad = _logit_gradient(logits, rows, V, ld)
+    grad, pitch = _logit_gradient(logits, rows, V, ld) if gradient else (None, V)
     if rows > 0:
         _call(dev, what, _lib.load().gptmi_distillation_loss, logits.data_ptr(), ld, teacher_tokens.data_ptr(),
-              teacher_logits.data_ptr(), k, temperature, _ptr(weights), _ptr(out), _ptr(buf), pitch, rows, V, code,
+              teacher_logits.data_ptr(), k, temperature, _ptr(weights), _ptr(out), _ptr(grad), pitch, rows, V, code,
               teacher_code)
     return out, grad
 
