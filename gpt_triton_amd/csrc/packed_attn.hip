@@ -119,22 +119,34 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
     for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const h8*>(p + ks * 16);
   }
 
-  // ---- tile loads: wavefronts 0-1 bring K, 2-3 V, 32 rows each
+  // ---- tile loads: wavefronts 0-1 bring K, 2-3 V, 32 rows each.  Load j's rows are RPI j further on, which the scalar
+  // base takes, and their keys differ by bits that are the same for all lanes; a sequence's last tile repeats its last row.
   const bool brings_v = wave >= 2;
   const int64_t pitch = (brings_v ? a.v_row : a.k_row) * 2;
-  const char* src = (const char*)(brings_v ? vp : kp);
+  const char* src = (const char*)(brings_v ? vp : kp) + (wave & 1) * 32 * pitch;
   const int lrow = lane / CH;
+  const unsigned lane_unit = (unsigned)((lane % CH) ^ (brings_v ? VMUL * (lrow & 3) : (lrow >> KSHIFT) & KMASK)) << 4;
+  const unsigned lane_row = (unsigned)lrow * (unsigned)pitch;
   auto issue_tile = [&](int t) {
     const unsigned dst = smem_base + (unsigned)((t & 1) * STAGE) + (brings_v ? (unsigned)TILE : 0u) +
                          (unsigned)((wave & 1) * NDMA) * 1024u;
     const char* base = src + (int64_t)t * kKeys * pitch;
-    const int rest = L - 1 - t * kKeys;
+    const int rest = L - 1 - t * kKeys - (wave & 1) * 32;  // the last row of this wavefront's 32
+    if (rest >= 31) {
 #pragma unroll
-    for (int j = 0; j < NDMA; ++j) {
-      const int r = (wave & 1) * 32 + j * RPI + lrow;
-      const int key = brings_v ? VMUL * (r & 3) : (r >> KSHIFT) & KMASK;
-      const unsigned unit = (unsigned)((lane % CH) ^ key) << 4;
-      load_lds16(base, (unsigned)min(r, rest) * (unsigned)pitch + unit, dst + j * 1024);
+      for (int j = 0; j < NDMA; ++j) {
+        const unsigned key = brings_v ? (unsigned)(VMUL * ((j * RPI) & 3)) : (unsigned)(((j * RPI) >> KSHIFT) & KMASK);
+        load_lds16(base, (lane_unit ^ (key << 4)) + lane_row, dst + j * 1024);
+        base += RPI * pitch;
+      }
+    } else {
+      base += (int64_t)min(rest, 0) * pitch;  // of 32 rows behind the end, row 0 is the sequence's last
+      const int last = max(rest, 0);
+#pragma unroll
+      for (int j = 0; j < NDMA; ++j) {
+        const unsigned key = brings_v ? (unsigned)(VMUL * ((j * RPI) & 3)) : (unsigned)(((j * RPI) >> KSHIFT) & KMASK);
+        load_lds16(base, (unsigned)min(j * RPI + lrow, last) * (unsigned)pitch + (lane_unit ^ (key << 4)), dst + j * 1024);
+      }
     }
   };
 
@@ -159,7 +171,11 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
   for (int i = 0; i < DB; ++i)
 #pragma unroll
     for (int r = 0; r < 16; ++r) oacc[i][r] = 0.f;
-  float mrun = -INFINITY, den = 0.f;
+  // The weights are 2^(c s - base), base = c ref - 6, for a reference that the running maximum may pass by 2^8 before it
+  // follows: the accumulator is rescaled in few tiles, a weight is at most 2^14, and one is a subnormal fp16 number, which
+  // has fewer bits, below 2^-20 of the reference.  The denominator adds the weights as rounded for the product with V.
+  float ref = -INFINITY, limit = -INFINITY, base = 0.f, den = 0.f;
+  const float room = 8.0f / c;
 
   // One 64-key tile.  MODE 0: both 32-key blocks entirely visible; 1: block 0 cut by the diagonal, block 1 hidden; 2:
   // block 0 visible, block 1 cut by the diagonal.
@@ -188,26 +204,31 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
 #pragma unroll
       for (int r = 0; r < 16; ++r) bmax = fmaxf(bmax, s[kb][r]);
     bmax = half_max(bmax);
-    const float mnew = fmaxf(bmax, mrun);
-    const float mult = __builtin_amdgcn_exp2f((mrun - mnew) * c), mb = mnew * c;
-    float psum = 0.f;
+    if (D > 128 || __any(bmax > limit)) {  // a branch there costs registers that there are none of
+      const float higher = fmaxf(bmax, ref), mult = __builtin_amdgcn_exp2f((ref - higher) * c);
+      ref = higher;
+      limit = higher + room;
+      base = fmaf(higher, c, -6.0f);
+      den *= mult;
+#pragma unroll
+      for (int i = 0; i < DB; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) oacc[i][r] *= mult;
+    }
     h8 pf[NKB][2];
 #pragma unroll
     for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
       for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float p = __builtin_amdgcn_exp2f(fmaf(s[kb][8 * tt + j], c, -mb));
-          psum += p;
-          pf[kb][tt][j] = (_Float16)p;
+        for (int j = 0; j < 8; j += 2) {
+          h2 p;
+          p[0] = (_Float16)__builtin_amdgcn_exp2f(fmaf(s[kb][8 * tt + j], c, -base));
+          p[1] = (_Float16)__builtin_amdgcn_exp2f(fmaf(s[kb][8 * tt + j + 1], c, -base));
+          pf[kb][tt][j] = p[0];
+          pf[kb][tt][j + 1] = p[1];
+          den = __builtin_amdgcn_fdot2(p, h2{1, 1}, den, false);
         }
-    mrun = mnew;
-    den = den * mult + half_sum(psum);
-#pragma unroll
-    for (int i = 0; i < DB; ++i)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) oacc[i][r] *= mult;
 #pragma unroll
     for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
@@ -251,7 +272,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
 
   // ---- an infinity or a NaN among the results: one of the inputs is none, and a hidden key's value, times its weight
   // of 0, may have spoilt queries in front of it.  Once more, key by key, for this wavefront.
-  const float inv = 1.0f / den;
+  const float inv = 1.0f / half_sum(den);
   float none = 0.f;
 #pragma unroll
   for (int i = 0; i < DB; ++i)
