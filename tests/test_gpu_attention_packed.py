@@ -173,7 +173,7 @@ def test_hidden_keys_play_no_part(K, gpu_device, d):
                 # the wavefronts that met it form their rows another way: roundings, not bits
                 assert torch.all((got[fine].double() - clean[fine].double()).abs() <= 4 * H * clean[fine].double().abs() + 2e-3)
                 far = fine.clone()
-                far[spoilt - 32:spoilt] = False
+                far[spoilt - 63:spoilt] = False  # a tile of 64 keys may have both in it
                 assert torch.equal(got[far], clean[far])
                 if which == 2:
                     assert not torch.any(torch.isfinite(got[behind]))
