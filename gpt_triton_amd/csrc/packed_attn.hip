@@ -23,7 +23,7 @@ struct PackedArgs {
   _Float16* out;
   const int64_t* starts;
   int64_t rows;               // T
-  int sequences, heads, kv_heads, slots;
+  int sequences, heads, kv_heads, slots, longest_first;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;  // pitches in elements
   float scale;
 };
@@ -71,6 +71,49 @@ __device__ __forceinline__ Block find_block(const PackedArgs& a, int slot) {
   return {first, block >= 0 && block * R < length ? (int)length : 0, (int)block};
 }
 
+// The nth block of all sequences' blocks in the order of their keys, the most first, for up to 64 kMany sequences.
+// Where all workgroups run at once or nearly, the last one to start decides when the launch ends.
+constexpr int kMany = 4;
+template <int R>
+__device__ __forceinline__ Block nth_longest(const PackedArgs& a, int nth) {
+  const int lane = threadIdx.x & 63;
+  int blocks[kMany], most = 0;  // of sequence lane + 64 i
+#pragma unroll
+  for (int i = 0; i < kMany; ++i) {
+    const int s = lane + i * kWave;
+    blocks[i] = 0;
+    if (i * kWave >= a.sequences) break;
+    if (s < a.sequences) {
+      const int64_t begin = a.starts[s], end = a.starts[s + 1];
+      const int64_t first = begin < 0 ? 0 : begin < a.rows ? begin : a.rows;
+      const int64_t last = end < first ? first : end < a.rows ? end : a.rows;
+      blocks[i] = (int)((last - first + R - 1) / R);
+    }
+    most = max(most, blocks[i]);
+  }
+  most = __builtin_amdgcn_readfirstlane((int)wave_max((float)most));  // below 2^24: the host sees to it
+  for (int block = most - 1; block >= 0; --block) {
+    int all = 0;
+#pragma unroll
+    for (int i = 0; i < kMany; ++i) {
+      if (i * kWave >= a.sequences) break;
+      const uint64_t have = __ballot(blocks[i] > block);
+      const int n = __popcll(have);
+      if (nth >= all && nth < all + n) {  // the (nth - all)th of these
+        const bool me = (have >> lane & 1) && __popcll(have & ((1ull << lane) - 1)) == nth - all;
+        const int s = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(me)) - 1 + i * kWave);
+        const int64_t begin = a.starts[s], end = a.starts[s + 1];
+        const int64_t first = begin < 0 ? 0 : begin < a.rows ? begin : a.rows;
+        const int64_t last = end < first ? first : end < a.rows ? end : a.rows;
+        return {first, (int)(last - first), block};
+      }
+      all += n;
+    }
+    nth -= all;
+  }
+  return {0, 0, 0};
+}
+
 template <int D, int QB>
 __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(PackedArgs a) {
   constexpr int R = 64 * QB;           // queries a workgroup
@@ -79,7 +122,6 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
   constexpr int CH = D / 8;            // 16-byte units of it
   constexpr int RPI = 1024 / ROWB;     // rows that a load instruction covers
   constexpr int TILE = kKeys * ROWB;   // bytes of a K (or V) tile
-  constexpr int STAGE = 2 * TILE;
   constexpr int NDMA = D / 16;         // load instructions a wavefront and tile
   // Unit u of K's row r lies at u ^ k_key(r), of V's at u ^ v_key(r).  A read of K takes one unit of rows 8 i + 0..3 (+ 4 b), i =
   // 0..3, a transposing read of V two units of rows 8 g + 0..3, two g at a time: the keys put these into different banks.
@@ -90,7 +132,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
   const auto v_key = [](int r) {
     return 2 * (CH >= 16 ? (r & 3) | (r >> 3 & 1) << 2 : CH == 8 ? (r >> 1 & 1) | (r >> 3 & 1) << 1 : CH == 4 ? r >> 3 & 1 : 0);
   };
-  extern __shared__ __attribute__((aligned(1024))) char smem[];  // 2 stages
+  extern __shared__ __attribute__((aligned(1024))) char smem[];  // K tiles of even and odd number, V tiles
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, g = lane >> 4;
@@ -101,7 +143,10 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
   // come first.
   const int id = (int)blockIdx.x, rep = a.heads / a.kv_heads, untied = (a.kv_heads & 7) * rep;
   int head, slot;
-  if (id < a.slots * untied) {
+  if (a.longest_first) {
+    slot = id / a.heads;
+    head = id - slot * a.heads;
+  } else if (id < a.slots * untied) {
     slot = id / untied;
     head = a.heads - untied + (id - slot * untied);
   } else {
@@ -109,7 +154,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
     slot = at - nth * a.slots;
     head = ((id & 7) + 8 * (nth / rep)) * rep + nth % rep;
   }
-  const Block block = find_block<R>(a, a.slots - 1 - slot);
+  const Block block = a.longest_first ? nth_longest<R>(a, slot) : find_block<R>(a, a.slots - 1 - slot);
   if (block.length == 0) return;
   const int L = block.length, q0 = block.block * R;
   const int qw0 = q0 + wave * 16 * QB;
@@ -143,8 +188,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
   const unsigned lane_unit = (unsigned)((lane % CH) ^ (brings_v ? v_key(lrow) : k_key(lrow))) << 4;
   const unsigned lane_row = (unsigned)lrow * (unsigned)pitch;
   auto issue_tile = [&](int t) {
-    const unsigned dst = smem_base + (unsigned)((t & 1) * STAGE) + (brings_v ? (unsigned)TILE : 0u) +
-                         (unsigned)((wave & 1) * NDMA) * 1024u;
+    const unsigned dst = smem_base + (unsigned)(((brings_v ? 2 : 0) + (t & 1)) * TILE) + (unsigned)((wave & 1) * NDMA) * 1024u;
     const char* base = src + (int64_t)t * kKeys * pitch;
     const int rest = L - 1 - t * kKeys - (wave & 1) * 32;  // the last row of this wavefront's 32
     if (rest >= 31) {
@@ -173,7 +217,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
   for (int ks = 0; ks < KV; ++ks) k_off[ks] = k_row * ROWB + (((4 * ks + (D >= 32 ? g : g & 1)) ^ k_key(k_row)) << 4);
 #pragma unroll
   for (int i = 0; i < VV; ++i)
-    v_off[i] = TILE + v_row * ROWB + (((2 * i + ((c & 3) >> 1)) ^ v_key(v_row)) << 4) + (c & 1) * 8;
+    v_off[i] = 2 * TILE + v_row * ROWB + (((2 * i + ((c & 3) >> 1)) ^ v_key(v_row)) << 4) + (c & 1) * 8;
   const float to_exp2 = a.scale * 1.4426950408889634f;
 
   f4 oacc[QB][DB];  // of query c of block n: d = 16 i + 4 g + 0..3
@@ -193,12 +237,10 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
   // One 64-key tile.  MASK: the one that the diagonal cuts, in which query x of the wavefront sees keys 0 .. edge + x;
   // KG = 1: none of them the second 32 of it.
   const int edge = qw0 & 63;
-  auto step = [&](auto mask, auto key_groups, const char* buf) {
-    constexpr bool MASK = decltype(mask)::value;
-    constexpr int KG = decltype(key_groups)::value;
-    f4 s[QB][2 * KG];  // [block][2 group + b]
+  f4 s[QB][4];  // scores, [block][2 group + b]
+  auto scores = [&](const char* buf) {
 #pragma unroll
-    for (int kb = 0; kb < 2 * KG; ++kb)
+    for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         h8 kf = *reinterpret_cast<const h8*>(buf + (kb >> 1) * 32 * ROWB + (kb & 1) * 4 * ROWB + k_off[ks % KV] + (ks / KV) * 256);
@@ -207,6 +249,11 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
         for (int n = 0; n < QB; ++n)
           s[n][kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[n][ks], ks == 0 ? f4(0.f) : s[n][kb], 0, 0, 0);
       }
+  };
+  h8 pf[QB][2];
+  auto softmax = [&](auto mask, auto key_groups) {
+    constexpr bool MASK = decltype(mask)::value;
+    constexpr int KG = decltype(key_groups)::value;
     float most[QB];
     bool higher = false;
 #pragma unroll
@@ -240,7 +287,6 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
         for (int i = 0; i < DB; ++i) oacc[n][i] *= mult;
       }
     }
-    h8 pf[QB][KG];
 #pragma unroll
     for (int n = 0; n < QB; ++n)
 #pragma unroll
@@ -256,6 +302,9 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
         }
 #pragma unroll
     for (int n = 0; n < QB; ++n) asm volatile("" : "+v"(den[n]));  // here, not with copies of the weights behind the barrier
+  };
+  auto weighted = [&](auto key_groups, const char* buf) {
+    constexpr int KG = decltype(key_groups)::value;
 #pragma unroll
     for (int kg = 0; kg < KG; ++kg)
 #pragma unroll
@@ -268,32 +317,51 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
           oacc[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[n][kg], oacc[n][i], 0, 0, 0);
       }
   };
-
   const int nfull = qw0 >> 6;  // key tiles entirely below this wavefront's diagonal
+  // The order inside a wavefront is softmax of tile t, the score products of tile t + 1, the P . V products of tile t,
+  // which the matrix pipe works through under the softmax of tile t + 1 and other wavefronts'.  So step t has K of tile t + 1
+  // and V of tile t, with K of t + 2 and V of t + 1 on their way: two places each.
+  // What this wavefront requested has landed; behind the barrier that holds for everyone, and the last step's tiles are free.
   auto arrive = [&] { asm volatile("s_waitcnt vmcnt(0)\n\ts_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
-  auto request = [&](int t) {
-    if (t + 1 < nt) issue_tile(t + 1);
+  auto request = [&](int k_tile) {  // and the V tile in front of it
+    const int t = brings_v ? k_tile - 1 : k_tile;
+    if (t < nt) issue_tile(t);
   };
+  auto tile = [&](int t) { return (const char*)smem + (t & 1) * TILE; };
   issue_tile(0);
+  if (!brings_v && nt > 1) issue_tile(1);
   arrive();
 #pragma unroll
   for (int n = 0; n < QB; ++n)  // they have landed too: no wait at their uses
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[n][ks]));
-  request(0);
+  constexpr std::integral_constant<int, 1> one{};
+  constexpr std::integral_constant<int, 2> two{};
+  if (wave_active) scores(tile(0));
+  if (nt > 1) {
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // everyone is done with K of tile 0
+    request(2);
+  }
   if (wave_active) {
     for (int t = 0; t < nfull; ++t) {
-      step(std::false_type{}, std::integral_constant<int, 2>{}, smem + (t & 1) * STAGE);
+      softmax(std::false_type{}, two);
+      __builtin_amdgcn_sched_barrier(0);
+      scores(tile(t + 1));
+      weighted(two, tile(t));
       arrive();
-      request(t + 1);
+      request(t + 3);
     }
-    const char* buf = smem + (nfull & 1) * STAGE;
-    if (D <= 64 && QB <= 2 && edge + 16 * QB <= 32) step(std::true_type{}, std::integral_constant<int, 1>{}, buf);
-    else step(std::true_type{}, std::integral_constant<int, 2>{}, buf);
+    if (D <= 64 && QB <= 2 && edge + 16 * QB <= 32) {
+      softmax(std::true_type{}, one);
+      weighted(one, tile(nfull));
+    } else {
+      softmax(std::true_type{}, two);
+      weighted(two, tile(nfull));
+    }
   }
-  for (int t = wave_active ? nfull + 1 : 1; t < nt; ++t) {
+  for (int t = wave_active ? nfull : 0; t < nt - 1; ++t) {
     arrive();
-    request(t);
+    request(t + 3);
   }
   if (!wave_active) return;
 
@@ -354,7 +422,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
 }
 
 template <int D, int QB>
-int launch_as(PackedArgs a, hipStream_t st) {
+int launch_as(PackedArgs a, bool longest_first, hipStream_t st) {
   constexpr int lds = 2 * 2 * kKeys * D * 2, R = 64 * QB;
   static bool attr_done = false;  // idempotent; a race only repeats the call
   if (!attr_done) {
@@ -373,6 +441,7 @@ int launch_as(PackedArgs a, hipStream_t st) {
     return -2;
   }
   a.slots = (int)slots;
+  a.longest_first = longest_first && a.sequences > 1 && a.sequences <= kMany * kWave && slots <= 512;
   hipLaunchKernelGGL((packed_attn_kernel<D, QB>), dim3((unsigned)(slots * a.heads)), dim3(256), lds, st, a);
   return 0;
 }
@@ -380,10 +449,11 @@ int launch_as(PackedArgs a, hipStream_t st) {
 template <int D>
 int launch_d(const PackedArgs& a, hipStream_t st) {
   const char* e = getenv("QBV");
-  const int qb = e ? atoi(e) : 2;
-  if (qb == 1) return launch_as<D, 1>(a, st);
-  if constexpr (D <= 64) if (qb == 4) return launch_as<D, 4>(a, st);
-  return launch_as<D, 2>(a, st);
+  const char* f = getenv("LF");
+  const int qb = e ? atoi(e) : 2, lf = f ? atoi(f) : 0;
+  if (qb == 1) return launch_as<D, 1>(a, lf, st);
+  if constexpr (D <= 64) if (qb == 4) return launch_as<D, 4>(a, lf, st);
+  return launch_as<D, 2>(a, lf, st);
 }
 
 }  // namespace
