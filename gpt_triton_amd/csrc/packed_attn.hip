@@ -143,9 +143,10 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
   // come first.
   const int id = (int)blockIdx.x, rep = a.heads / a.kv_heads, untied = (a.kv_heads & 7) * rep;
   int head, slot;
-  if (a.longest_first) {
+  if (a.longest_first) {  // a key head's heads 8 ids apart where that can be
     slot = id / a.heads;
-    head = id - slot * a.heads;
+    const int at = id - slot * a.heads, nth = at / a.kv_heads;
+    head = (at - nth * a.kv_heads) * rep + nth;
   } else if (id < a.slots * untied) {
     slot = id / untied;
     head = a.heads - untied + (id - slot * untied);
@@ -422,8 +423,8 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
 }
 
 template <int D, int QB>
-int launch_as(PackedArgs a, bool longest_first, hipStream_t st) {
-  constexpr int lds = 2 * 2 * kKeys * D * 2, R = 64 * QB;
+int launch_as(PackedArgs a, int64_t slots, hipStream_t st) {
+  constexpr int lds = 2 * 2 * kKeys * D * 2;
   static bool attr_done = false;  // idempotent; a race only repeats the call
   if (!attr_done) {
     hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(packed_attn_kernel<D, QB>),
@@ -434,26 +435,34 @@ int launch_as(PackedArgs a, bool longest_first, hipStream_t st) {
     }
     attr_done = true;
   }
-  const int64_t slots = a.rows / R + a.sequences;
-  if (slots * a.heads >= 1ll << 31) {
+  const int64_t blocks = slots * a.heads;
+  if (blocks >= 1ll << 31) {
     set_error("flash_attn_packed: %lld rows in %d sequences of %d heads exceed the grid", (long long)a.rows, a.sequences,
               a.heads);
     return -2;
   }
   a.slots = (int)slots;
-  a.longest_first = longest_first && a.sequences > 1 && a.sequences <= kMany * kWave && slots <= 512;
-  hipLaunchKernelGGL((packed_attn_kernel<D, QB>), dim3((unsigned)(slots * a.heads)), dim3(256), lds, st, a);
+  // Up to 10 workgroups a CU the heaviest first: whichever starts last ends the launch.  Beyond, a head's blocks one behind
+  // the other, whose K and V then come from one XCD's L2.  us, by slots / heaviest first: 2 x 8192 rows of 12 heads (1560
+  // workgroups) 252 / 230, 16 x 1024 (1728) 48.7 / 40.8, 40 x 512 (2400) 39.3 / 38.4, 200 x 64 (3600) 21.1 / 23.4, 8 x
+  // 4096 of 16 (4224) 329 / 338; d = 256, 4 x 1024 of 12 (432) 108 / 69.
+  a.longest_first = a.sequences > 1 && a.sequences <= kMany * kWave && slots <= 512 && blocks <= 2560;
+  hipLaunchKernelGGL((packed_attn_kernel<D, QB>), dim3((unsigned)blocks), dim3(256), lds, st, a);
   return 0;
 }
 
+// 16 queries a wavefront while the workgroups number at most 5 a CU: they all run at once, and a wavefront's chain through
+// its key tiles, which is then what the launch takes, is shorter (0.5 us a tile for 16 queries, 0.8 for 32).  32 beyond: K and V
+// are read from LDS for more queries at a time.  us, 16 / 32: 1 x 1024 rows of 12 heads (204 workgroups of 64 queries) 14.0 /
+// 18.0, 4 x 1024 (816) 17.3 / 20.1, 16 x 300 (1092) 10.6 / 12.5, 3 x 2048 (1188) 35.1 / 35.7, 48 of up to 1024 (1992) 21.6 /
+// 21.2, 2 x 8192 (3096) 263 / 230; d = 128, 32 heads over 8, 1 x 1024 (544) 24.4 / 28.7, 1 x 8192 (4128) 653 / 520.  64 queries
+// were slower: 1 x 16384 of 25 heads 997, 32 969, 16 1046.  d = 256 has one workgroup a CU either way.
 template <int D>
 int launch_d(const PackedArgs& a, hipStream_t st) {
-  const char* e = getenv("QBV");
-  const char* f = getenv("LF");
-  const int qb = e ? atoi(e) : 2, lf = f ? atoi(f) : 0;
-  if (qb == 1) return launch_as<D, 1>(a, lf, st);
-  if constexpr (D <= 64) if (qb == 4) return launch_as<D, 4>(a, lf, st);
-  return launch_as<D, 2>(a, lf, st);
+  const int64_t slots = a.rows / 64 + a.sequences;
+  if constexpr (D <= 128)
+    if (slots * a.heads <= 1280) return launch_as<D, 1>(a, slots, st);
+  return launch_as<D, 2>(a, a.rows / 128 + a.sequences, st);
 }
 
 }  // namespace

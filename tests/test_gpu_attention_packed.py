@@ -95,6 +95,28 @@ def test_heads(K, gpu_device, d, heads):
 
 
 @pytest.mark.parametrize("d", [16, 32, 64, 128, 256])
+def test_many_blocks(K, gpu_device, d):
+    """More blocks than run at once: 32 queries a wavefront, the heaviest blocks first (few sequences, few blocks) or in
+    the order of the slots (more than 256 sequences, more than 2560 blocks), with and without heads that one XCD has."""
+    r = np.random.default_rng(19)
+    for heads, lengths in (((64, 16), [700, 33, 0, 512, 255, 1]), ((20, 20), [65, 1000, 129, 0, 640, 2000]),
+                           ((48, 12), r.integers(0, 30, 300).tolist()), ((72, 9), [1500, 31, 900, 2100]), ((64, 64), [1600]),
+                           ((64, 8), [1] * 200 + [100, 200])):
+        q, k, v = make(r, sum(lengths), *heads, d, True, gpu_device)
+        out = K.flash_attention_packed(q, k, v, starts_of(lengths, gpu_device))
+        ends = np.cumsum(lengths)
+        for s in {0, 1, len(lengths) // 2, len(lengths) - 1, int(np.argmax(lengths))} & set(range(len(lengths))):
+            rows = slice(int(ends[s]) - lengths[s], int(ends[s]))
+            some = [0, heads[0] // 2, heads[0] - 1]
+            rep = heads[0] // heads[1]
+            for h in some:
+                if lengths[s]:
+                    w, tol = want(q[rows, h:h + 1], k[rows, h // rep:h // rep + 1], v[rows, h // rep:h // rep + 1], d ** -0.5)
+                    assert torch.all((out[rows, h:h + 1].double() - w).abs() <= tol), (heads, s, h)
+        assert torch.all(torch.isfinite(out))
+
+
+@pytest.mark.parametrize("d", [16, 32, 64, 128, 256])
 def test_long(K, gpu_device, d):
     r = np.random.default_rng(7)
     lengths = [3001, 5, 1500]
@@ -143,13 +165,14 @@ def test_many_sequences(K, gpu_device, count):
     assert torch.equal(out[rows], v[rows].expand(-1, 2, -1))  # a key alone has all the weight
 
 
+@pytest.mark.parametrize("heads", [3, 200])
 @pytest.mark.parametrize("d", [16, 32, 64, 128, 256])
-def test_hidden_keys_play_no_part(K, gpu_device, d):
+def test_hidden_keys_play_no_part(K, gpu_device, d, heads):
     """Infinities and NaN in later tokens, other sequences, and rows of none: the bits of finite ones there."""
     r = np.random.default_rng(10)
     lengths, first = [70, 33, 300, 1], 5
     total = first + sum(lengths) + 9
-    q, k, v = (t.clone() for t in make(r, total, 3, 3, d, False, gpu_device))
+    q, k, v = (t.clone() for t in make(r, total, heads, heads, d, False, gpu_device))
     starts = starts_of(lengths, gpu_device, first)
     clean = K.flash_attention_packed(q, k, v, starts)
     end = first + sum(lengths)
