@@ -35,9 +35,9 @@ __device__ __forceinline__ A least_of(A a, A b) { return __builtin_elementwise_m
 
 // A row as the workgroup's threads share it: 16-byte chunks from the first aligned address on, dealt one behind
 // the other, and in front and behind at most 2 (N - 1) single elements, one for each of the first threads.
-// CH > 0: it is read once and stays in registers, CH chunks a thread (-infinity where the row has ended).  CH = 0: rows
-// too long for that are read again by every pass.
-template <typename T, int NT, int CH>
+// It is read once and stays in registers, CH chunks a thread (-infinity where it has ended); OPEN: what a longer row has
+// behind those is read again by every pass.
+template <typename T, int NT, int CH, bool OPEN>
 struct Row {
   typedef typename RowVec<T>::V V;
   static constexpr int N = RowVec<T>::N;
@@ -52,91 +52,91 @@ struct Row {
     const int t = threadIdx.x, singles = vocab - chunks * N;
     loose = t < lead ? t : t < singles ? t + chunks * N : -1;
   }
-  __device__ __forceinline__ void load() {
-    if constexpr (CH > 0) {
-      const V* p = reinterpret_cast<const V*>(x + lead) + threadIdx.x;
-#pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        held[i] = V((T)-INFINITY);
-        if ((int)threadIdx.x + i * NT < chunks) held[i] = p[i * NT];
-      }
-      single = (T)-INFINITY;
-      if (loose >= 0) single = x[loose];
-    }
+  __device__ __forceinline__ V chunk(int c) const {
+    V v = V((T)-INFINITY);
+    if (c < chunks) v = reinterpret_cast<const V*>(x + lead)[c];
+    return v;
   }
-  __device__ __forceinline__ T lone() const {
-    if constexpr (CH > 0) return single;
-    T y = (T)-INFINITY;
-    if (loose >= 0) y = x[loose];
-    return y;
+  __device__ __forceinline__ void load() {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) held[i] = chunk(threadIdx.x + i * NT);
+    single = (T)-INFINITY;
+    if (loose >= 0) single = x[loose];
   }
   // In front of a pass: what the last one converted is not kept for this one, which is a register for each element.
   __device__ __forceinline__ void renew() {
-    if constexpr (CH > 0) {
 #pragma unroll
-      for (int i = 0; i < CH; ++i) asm volatile("" : "+v"(held[i]));
-    }
+    for (int i = 0; i < CH; ++i) asm volatile("" : "+v"(held[i]));
   }
   // whether a wavefront has any of chunk i
   __device__ __forceinline__ bool part(int i) const {
     return i == 0 || __builtin_amdgcn_readfirstlane((int)threadIdx.x & -kWave) + i * NT < chunks;
   }
-  // f(values, index of the first of them, how many: N or 1) for this thread's part of the row, with -infinity for what
-  // is not there (CH > 0)
-  template <typename F>
-  __device__ __forceinline__ void each(F f) const {
-    auto chunk = [&](const V& v, int c) {
-      float y[N];
+  // f(chunks, the first one's number, how many: up to G) for this thread's part of the row but for the single element, the
+  // first as soon as they are there, the others NT chunks further on each; -infinity for what is not there
+  template <int G, typename F>
+  __device__ __forceinline__ void groups(F f) const {
+    constexpr int REST = CH % G;
 #pragma unroll
-      for (int j = 0; j < N; ++j) y[j] = (float)v[j];
-      f(y, lead + c * N, std::integral_constant<int, N>{});
-    };
-    if constexpr (CH > 0) {
+    for (int i = 0; i + G <= CH; i += G)
+      if (part(i)) f(held + i, (int)threadIdx.x + i * NT, std::integral_constant<int, G>{});
+    if constexpr (REST > 0)
+      if (part(CH - REST)) f(held + CH - REST, (int)threadIdx.x + (CH - REST) * NT, std::integral_constant<int, REST>{});
+    if constexpr (OPEN) {
+      for (int c = threadIdx.x + CH * NT; c < chunks; c += G * NT) {
+        V v[G];
 #pragma unroll
-      for (int i = 0; i < CH; ++i)
-        if (part(i)) chunk(held[i], threadIdx.x + i * NT);
-      const float y[1] = {(float)single};
-      f(y, loose, std::integral_constant<int, 1>{});
-    } else {
-      for (int c = threadIdx.x; c < chunks; c += NT) chunk(reinterpret_cast<const V*>(x + lead)[c], c);
-      if (loose >= 0) {
-        const float y[1] = {(float)x[loose]};
-        f(y, loose, std::integral_constant<int, 1>{});
+        for (int k = 0; k < G; ++k) v[k] = chunk(c + k * NT);
+        f(v, c, std::integral_constant<int, G>{});
       }
     }
   }
-  // f(chunks, how many: up to G) for this thread's part of the row but for the single element, the first as soon as
-  // they are there
-  template <int G, typename F>
-  __device__ __forceinline__ void groups(F f) const {
-    if constexpr (CH > 0) {
-      constexpr int REST = CH % G;
+  // f(values, index of the first of them, how many: N or 1) for this thread's part of the row; a single element that is
+  // not there has index -1
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    groups<4>([&](const V* v, int c, auto n) {
 #pragma unroll
-      for (int i = 0; i + G <= CH; i += G)
-        if (part(i)) f(held + i, std::integral_constant<int, G>{});
-      if constexpr (REST > 0)
-        if (part(CH - REST)) f(held + CH - REST, std::integral_constant<int, REST>{});
-    } else {
-      const V* p = reinterpret_cast<const V*>(x + lead);
-      for (int c = threadIdx.x; c < chunks; c += G * NT) {
-        V v[G];
+      for (int k = 0; k < n.value; ++k)
+        if (part_of(c + k * NT)) {
+          float y[N];
 #pragma unroll
-        for (int k = 0; k < G; ++k) {
-          v[k] = V((T)-INFINITY);
-          if (c + k * NT < chunks) v[k] = p[c + k * NT];
+          for (int j = 0; j < N; ++j) y[j] = (float)v[k][j];
+          f(y, lead + (c + k * NT) * N, std::integral_constant<int, N>{});
         }
-        f(v, std::integral_constant<int, G>{});
-      }
-    }
+    });
+    const float y[1] = {(float)single};
+    f(y, loose, std::integral_constant<int, 1>{});
+  }
+  __device__ __forceinline__ bool part_of(int c) const {
+    return __builtin_amdgcn_readfirstlane(c & -kWave) < chunks;
   }
   __device__ __forceinline__ float at(int64_t i) const { return (float)x[i]; }
 };
+
+// All threads of a row: a workgroup, or a wavefront of one, whose LDS operations are in order as they stand.
+template <int NT>
+__device__ __forceinline__ void sync_row() {
+  if constexpr (NT == kWave) {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  } else {
+    __syncthreads();
+  }
+}
+// Rows of a workgroup, the one that a thread works on, and its part of an LDS array with an element a row.
+template <int NT>
+constexpr int kRowsOf = NT == kWave ? 4 : 1;
+template <int NT>
+__device__ __forceinline__ int row_in_group() {
+  return NT == kWave ? __builtin_amdgcn_readfirstlane((int)threadIdx.y) : 0;
+}
 
 template <int NT>
 struct Shared {
   static constexpr int W = NT / kWave;
   float top[W], s[W], u[W], low[W];
-  float groups[64];  // maxima of groups of NT / 64 threads
+  float groups[64], many[256];  // maxima of 64 groups of threads, and of 256 where there are so many
   int scan[W];
 };
 
@@ -203,9 +203,9 @@ __device__ __forceinline__ int scan_exclusive(int c, Shared<NT>& sh, int& total)
     const int o = __shfl_up(s, d);
     s += lane >= d ? o : 0;
   }
-  __syncthreads();
+  sync_row<NT>();
   if (lane == 63) sh.scan[wave] = s;
-  __syncthreads();
+  sync_row<NT>();
   int front = 0;
   total = 0;
 #pragma unroll 1
@@ -220,24 +220,24 @@ __device__ __forceinline__ int scan_exclusive(int c, Shared<NT>& sh, int& total)
 // a thread takes its logits in groups of G chunks, of each first the maximum, which is then the reference of what it has
 // summed (so that no exponent is above 0 and u never changes sign), and keeps the largest logit so far out of the sums:
 // where a larger one comes, the old one goes in.  The groups' sums start while later groups are on their way.
-// TOP: the maxima of 64 groups of threads go to sh.groups, `low` becomes the least of the maxima of 128 (of 64 where there
-// are no more threads); mine: this thread's maximum, a NaN as -infinity.
+// TOP: the maxima of 64 and of 256 groups of threads go to sh.groups and sh.many; low: the least of the latter above
+// -infinity; mine: this thread's maximum; a NaN counts as -infinity.
 struct Tops {
   float low, mine;
 };
-template <bool ENTROPY, bool TOP, typename T, int NT, int CH>
-__device__ __forceinline__ Stats<T> row_stats(Row<T, NT, CH>& row, float tau, Shared<NT>& sh, Tops* tops = nullptr) {
+template <bool ENTROPY, bool TOP, typename T, int NT, int CH, bool OPEN>
+__device__ __forceinline__ Stats<T> row_stats(Row<T, NT, CH, OPEN>& row, float tau, Shared<NT>& sh, Tops* tops = nullptr) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   constexpr int W = Shared<NT>::W;
   constexpr int E = sizeof(T) == 2 ? 2 : 1;  // largest logits kept out: one for each half of a register
   typedef T Top __attribute__((ext_vector_type(E)));
   const float inv_tau = 1.0f / tau, c = kLog2e * inv_tau;
   Top top = Top((T)-INFINITY);
-  top[0] = row.lone();
+  top[0] = row.single;
   Exponent<T> t(c, -INFINITY);
   float s[E] = {}, u[E] = {};
-  row.template groups<4>([&](const auto* v, auto n) {
-    constexpr int N = Row<T, NT, CH>::N;
+  row.template groups<4>([&](const auto* v, int, auto n) {
+    constexpr int N = RowVec<T>::N;
     Top most = top;
 #pragma unroll
     for (int k = 0; k < n.value; ++k)
@@ -311,13 +311,14 @@ __device__ __forceinline__ Stats<T> row_stats(Row<T, NT, CH>& row, float tau, Sh
   if constexpr (TOP) {
     tops->mine = fmaxf(mine, -INFINITY);
     float g = tops->mine;
-    constexpr int SMALL = NT >= 128 ? NT / 128 : 1, LANES = NT / 64;
+    constexpr int SMALL = NT >= 256 ? NT / 256 : 1, LANES = NT / 64;
 #pragma unroll
     for (int d = 1; d < SMALL; d *= 2) g = fmaxf(g, __shfl_xor(g, d));
-    const float least = group_reduce<kWave>(g, [](float a, float b) { return fminf(a, b); });
+    const float least = group_reduce<kWave>(g > -INFINITY ? g : INFINITY, [](float a, float b) { return fminf(a, b); });
+    if (lane == 0) sh.low[wave] = least;
+    if (NT >= 256 && lane % SMALL == 0) sh.many[threadIdx.x / SMALL] = g;
 #pragma unroll
     for (int d = SMALL; d < LANES; d *= 2) g = fmaxf(g, __shfl_xor(g, d));
-    if (lane == 0) sh.low[wave] = least;
     if (lane % LANES == 0) sh.groups[threadIdx.x / LANES] = g;
   }
   const float m_wave = group_reduce<kWave>(mine, [](float a, float b) { return most_of(a, b); });
@@ -333,7 +334,7 @@ __device__ __forceinline__ Stats<T> row_stats(Row<T, NT, CH>& row, float tau, Sh
     sh.s[wave] = s[0];
     sh.u[wave] = u[0];
   }
-  __syncthreads();
+  sync_row<NT>();
   const int w = lane % W;
   auto add = [](float a, float b) { return a + b; };
   mine = sh.top[w];
@@ -374,7 +375,7 @@ __device__ __forceinline__ int key_index(uint64_t key) { return (int)(0xffffffff
 
 template <int NT>
 struct TopShared {
-  static constexpr int kKeep = NT == 64 ? 512 : 1024;  // about 700 are kept of 128 groups of random logits
+  static constexpr int kKeep = NT == 64 ? 512 : 1024;
   static constexpr int kBins = 256;
   uint64_t kept[kKeep], fewer[kKeep];
   int bins[kBins], count, count_fewer, cut, threads;
@@ -385,70 +386,116 @@ struct TopShared {
   }
 };
 
-// found(r, key) of the k largest logits, r = 0 .. k - 1 in any order, by one thread each.  At least k logits reach `low`,
-// the k-th largest of the maxima of 64 groups of threads, or the least of 128 where k is larger: those are kept, little more
-// than k up to k = 40 or so and some 700 of 128 groups.  Where few threads have any, the wavefronts take these threads' logits
-// from memory, else the workgroup takes all.  Of more than 256 kept a histogram leaves the ones from the k-th's bin on.
-// The rest is ranked by counting.
-template <typename T, int NT, int CH, typename F>
-__device__ __forceinline__ void row_top(Row<T, NT, CH>& row, int k, Tops tops, float high, TopShared<NT>& top,
-                                        Shared<NT>& sh, F found) {
-  constexpr int kKeep = TopShared<NT>::kKeep, N = Row<T, NT, CH>::N, W = Shared<NT>::W;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  float low = tops.low;
-  if (k <= 64) {
-    // ranks of the 64 as numbers that differ: a maximum without its last 6 bits, and the group in their place; rounded down,
-    // the k-th is still reached by k
-    const unsigned key = (unsigned)(top_key(sh.groups[lane], 0) >> 32) & ~63u | (63 - lane);
-    int rank = 0;
+// The k-th largest of the numbers that lanes 0 .. G - 1 have, or a little below it: ranks of numbers that differ, a number
+// without its last 6 bits and the lane in their place.
+template <int G>
+__device__ __forceinline__ float kth_of_lanes(float v, int k) {
+  const int lane = threadIdx.x & 63;
+  const unsigned key = (unsigned)(top_key(v, 0) >> 32) & ~63u | (63 - lane);
+  int rank = 0;
 #pragma unroll
-    for (int j = 0; j < 64; ++j) rank += (unsigned)__builtin_amdgcn_readlane((int)key, j) > key;
-    const uint64_t kth = __ballot(rank == k - 1);
-    const unsigned down = (unsigned)__shfl((int)key, __ffsll((unsigned long long)kth) - 1) & ~63u;
-    low = down < 0x007fffffu ? -INFINITY : uniform(key_value((uint64_t)down << 32));  // below -infinity's there are NaNs
-  } else if (NT == 64) {
-    low = -INFINITY;
+  for (int j = 0; j < G; ++j) rank += (unsigned)__builtin_amdgcn_readlane((int)key, j) > key;
+  const uint64_t kth = __ballot(rank == k - 1 && lane < G);
+  const unsigned down = (unsigned)__builtin_amdgcn_readlane((int)key, __ffsll((unsigned long long)kth) - 1) & ~63u;
+  return down < 0x007fffffu ? -INFINITY : uniform(key_value((uint64_t)down << 32));  // below -infinity's there are NaNs
+}
+
+// found(r, key) of the k largest logits, r = 0 .. k - 1 in any order, by one thread each.  A bound that at least k of them
+// reach is the k-th largest of the maxima of some groups of threads: of the wavefronts for the least k, of 64 groups up to
+// k = 32, of 256, by a histogram, beyond.  The logits that reach it are gathered, little more than k (some 24 for k = 20, 180 for
+// 128), from memory, since a row's registers held any longer are too many: those of the few threads whose maximum reaches
+// it, or the whole row.  A histogram leaves of more than 256 those from the k-th's bin on, and the rest is ranked by
+// counting.  2048 rows of 50257 fp16 logits, us: no top tokens 42, 1 54, 20 60, 64 77, 128 113.
+template <typename T, int NT, int CH, bool OPEN, typename F>
+__device__ __forceinline__ void row_top(const Row<T, NT, CH, OPEN>& row, int k, Tops tops, float high, TopShared<NT>& top,
+                                        Shared<NT>& sh, F found) {
+  constexpr int kKeep = TopShared<NT>::kKeep, kBins = TopShared<NT>::kBins, N = RowVec<T>::N, W = Shared<NT>::W;
+  const int tid = threadIdx.x, lane = tid & 63;
+  // Bins of n keys between those of `from` and `high`, lower ones in the first: the lowest bin in which one of the k
+  // largest is.
+  unsigned base = 0;
+  int shift = 0;
+  auto bin_of = [&](unsigned key) { return key <= base ? 0u : min((key - base) >> shift, kBins - 1u); };
+  auto cut_bins = [&](int n, auto key_of, float from) {
+    base = (unsigned)(top_key(from, 0) >> 32);
+    const unsigned range = (unsigned)(top_key(high, 0) >> 32) - base;
+    shift = max(0, 24 - __clz((int)(range | 1)));
+    for (int i = tid; i < n; i += NT) atomicAdd(&top.bins[bin_of(key_of(i))], 1);
+    sync_row<NT>();
+    if (tid < kWave) {
+      int c[kBins / kWave], sum = 0;  // this lane's bins, the highest values first
+#pragma unroll
+      for (int i = 0; i < kBins / kWave; ++i) {
+        int& bin = top.bins[kBins - 1 - (lane * (kBins / kWave) + i)];
+        sum += c[i] = bin;
+        bin = 0;
+      }
+      int front = sum;
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) {
+        const int o = __shfl_up(front, d);
+        front += lane >= d ? o : 0;
+      }
+      front -= sum;
+#pragma unroll
+      for (int i = 0; i < kBins / kWave; ++i) {
+        if (front < k && front + c[i] >= k) top.cut = kBins - 1 - (lane * (kBins / kWave) + i);
+        front += c[i];
+      }
+    }
+    sync_row<NT>();
+    return (unsigned)top.cut;
+  };
+  float low = -INFINITY;
+  if (W >= 4 && 4 * k <= 3 * W) {
+    low = kth_of_lanes<W>(fmaxf(sh.top[lane % W], -INFINITY), k);
+  } else if (k <= 32 || (NT < 256 && k <= 64)) {
+    low = kth_of_lanes<64>(sh.groups[lane], k);
+  } else if (NT >= 256 && tops.low < INFINITY) {
+    const unsigned cut = cut_bins(256, [&](int i) { return (unsigned)(top_key(sh.many[i], 0) >> 32); }, tops.low);
+    if (cut > 0) low = key_value((uint64_t)(base + (cut << shift)) << 32);  // some in the first bin may be below its edge
   }
   auto put = [&](int at, float y, int index) {
     if (at < kKeep) top.kept[at] = top_key(y, index);
   };
-  auto keep = [&](auto above) {
-    return [&, above](const auto& y, int first, auto n) {
+  const Row<T, NT, 0, true> again = [&] {
+    Row<T, NT, 0, true> r(row.x, row.vocab);
+    r.single = row.single;
+    return r;
+  }();
+  auto recount = [&](auto reaches) {
+    sync_row<NT>();
+    if (tid == 0) top.count = 0;
+    sync_row<NT>();
+    again.each([&](const auto& y, int first, auto n) {
       int c = 0;
 #pragma unroll
-      for (int j = 0; j < n.value; ++j) c += above(y[j]);
+      for (int j = 0; j < n.value; ++j) c += reaches(y[j]);
+      if (first < 0) c = 0;
       if (c > 0) {
         int at = atomicAdd(&top.count, c);
 #pragma unroll
         for (int j = 0; j < n.value; ++j)
-          if (above(y[j])) put(at++, y[j], first + j);
+          if (reaches(y[j])) put(at++, y[j], first + j);
       }
-    };
-  };
-  const Row<T, NT, 0> again(row.x, row.vocab);  // from memory: held any longer, a row's registers are too many
-  auto recount = [&](auto above) {
-    __syncthreads();
-    if (tid == 0) top.count = 0;
-    __syncthreads();
-    again.each(keep(above));
-    __syncthreads();
+    });
+    sync_row<NT>();
     return top.count;
   };
-  auto reaches = [&](float y) { return y >= low; };
   auto above = [&](float y) { return y > low; };
   int n = kKeep + 1;  // all logits reach -infinity: not gathered
   if (low > -INFINITY) {
     const uint64_t in = __ballot(tops.mine >= low);
     if (in) {
-      int base = 0;
-      if (lane == 0) base = atomicAdd(&top.threads, __popcll(in));
-      base = __builtin_amdgcn_readfirstlane(base);
-      if (in >> lane & 1) top.thread[base + __popcll(in & ((1ull << lane) - 1))] = (short)tid;
+      int at = 0;
+      if (lane == 0) at = atomicAdd(&top.threads, __popcll(in));
+      at = __builtin_amdgcn_readfirstlane(at);
+      if (in >> lane & 1) top.thread[at + __popcll(in & ((1ull << lane) - 1))] = (short)tid;
     }
-    __syncthreads();
+    sync_row<NT>();
     const int threads = top.threads;
-    if (threads <= 8 * W) {
-      const int part = (row.chunks + NT - 1) / NT * N + 1;  // logits of a thread, the last one single
+    const int part = (row.chunks + NT - 1) / NT * N + 1;  // logits of a thread, the last one single
+    if (threads * part <= 32 * NT) {
       const float per = 1.0f / (float)part;
       for (int f = tid; f < threads * part; f += 4 * NT) {
         float y[4];
@@ -468,10 +515,10 @@ __device__ __forceinline__ void row_top(Row<T, NT, CH>& row, int k, Tops tops, f
         for (int i = 0; i < 4; ++i)
           if (y[i] >= low) put(atomicAdd(&top.count, 1), y[i], index[i]);
       }
-      __syncthreads();
+      sync_row<NT>();
       n = top.count;
     } else {
-      n = recount(reaches);
+      n = recount([&](float y) { return y >= low; });
     }
   }
   if (n > kKeep) {
@@ -482,9 +529,10 @@ __device__ __forceinline__ void row_top(Row<T, NT, CH>& row, int k, Tops tops, f
       for (int bit = 31; bit >= 0; --bit) {
         const unsigned trial = kth | 1u << bit;
         int c = 0;
-        again.each([&](const auto& y, int, auto m) {
+        again.each([&](const auto& y, int first, auto m) {
+          if (m.value == 1 && first < 0) return;
 #pragma unroll
-          for (int j = 0; j < m.value; ++j) c += (unsigned)(top_key(y[j], 0) >> 32) >= trial;
+          for (int j = 0; j < m.value; ++j) c += first + j < row.vocab && (unsigned)(top_key(y[j], 0) >> 32) >= trial;
         });
         int total;
         scan_exclusive<NT>(c, sh, total);
@@ -512,42 +560,17 @@ __device__ __forceinline__ void row_top(Row<T, NT, CH>& row, int k, Tops tops, f
       for (int c = 0; c < row.chunks && n < k; c += NT) take(c + tid < row.chunks, row.lead + (c + tid) * N, N);
       if (n < k) take(row.loose >= row.lead, row.loose, 1);
       n = k;
-      __syncthreads();
+      sync_row<NT>();
     }
   }
   const uint64_t* list = top.kept;
   if (n > 256) {
-    // bins of the values between low and the largest; the list goes on with those from the bin on in which the k-th is
-    constexpr int kBins = TopShared<NT>::kBins;
-    const unsigned base = (unsigned)(top_key(low, 0) >> 32), range = (unsigned)(top_key(high, 0) >> 32) - base;
-    const int shift = max(0, 24 - __clz((int)(range | 1)));
-    auto bin_of = [&](uint64_t key) { return min(((unsigned)(key >> 32) - base) >> shift, kBins - 1u); };
-    for (int i = tid; i < n; i += NT) atomicAdd(&top.bins[bin_of(top.kept[i])], 1);
-    __syncthreads();
-    if (tid < kWave) {
-      int c[kBins / kWave], sum = 0;  // this lane's bins, the highest values first
-#pragma unroll
-      for (int i = 0; i < kBins / kWave; ++i) sum += c[i] = top.bins[kBins - 1 - (lane * (kBins / kWave) + i)];
-      int front = sum;
-#pragma unroll
-      for (int d = 1; d < 64; d *= 2) {
-        const int o = __shfl_up(front, d);
-        front += lane >= d ? o : 0;
-      }
-      front -= sum;
-#pragma unroll
-      for (int i = 0; i < kBins / kWave; ++i) {
-        if (front < k && front + c[i] >= k) top.cut = kBins - 1 - (lane * (kBins / kWave) + i);
-        front += c[i];
-      }
-    }
-    __syncthreads();
-    const unsigned cut = (unsigned)top.cut;
+    const unsigned cut = cut_bins(n, [&](int i) { return (unsigned)(top.kept[i] >> 32); }, low);
     for (int i = tid; i < n; i += NT) {
       const uint64_t key = top.kept[i];
-      if (bin_of(key) >= cut) top.fewer[atomicAdd(&top.count_fewer, 1)] = key;
+      if (bin_of((unsigned)(key >> 32)) >= cut) top.fewer[atomicAdd(&top.count_fewer, 1)] = key;
     }
-    __syncthreads();
+    sync_row<NT>();
     n = top.count_fewer;
     list = top.fewer;
   }
@@ -566,21 +589,24 @@ __device__ __forceinline__ void row_top(Row<T, NT, CH>& row, int k, Tops tops, f
   }
 }
 
-template <typename T, bool TOP, int NT, int CH, int WAVES>
-__global__ __launch_bounds__(NT, WAVES) void token_log_probs_kernel(const T* __restrict__ x, int64_t ld, int vocab,
+template <typename T, bool TOP, int NT, int CH, bool OPEN, int WAVES>
+__global__ __launch_bounds__(NT * kRowsOf<NT>, WAVES) void token_log_probs_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int vocab,
                                                              const int64_t* __restrict__ tokens, float tau, int k,
                                                              float* __restrict__ log_probs, float* __restrict__ entropy,
                                                              float* __restrict__ top_log_probs,
                                                              int64_t* __restrict__ top_tokens) {
-  __shared__ Shared<NT> sh;
-  const int64_t r = blockIdx.x;
-  Row<T, NT, CH> row(x + r * ld, vocab);
+  __shared__ Shared<NT> sh_of[kRowsOf<NT>];
+  const int in_group = row_in_group<NT>();
+  const int64_t r = (int64_t)blockIdx.x * kRowsOf<NT> + in_group;
+  if (r >= rows) return;
+  Shared<NT>& sh = sh_of[in_group];
+  Row<T, NT, CH, OPEN> row(x + r * ld, vocab);
   row.load();
   TopShared<NT>* top_shared = nullptr;
   if constexpr (TOP) {
-    __shared__ TopShared<NT> top;
-    top_shared = &top;
-    top.clear();
+    __shared__ TopShared<NT> top[kRowsOf<NT>];
+    top_shared = top + in_group;
+    top_shared->clear();
   }
   Tops tops;
   const Stats<T> st = row_stats<true, TOP>(row, tau, sh, &tops);
@@ -608,8 +634,8 @@ struct Special {
 
 // The entries lane, lane + 64, .. of a row, by the first wavefront and for all behind the next barrier: f(i, token, part, logit)
 // gives entry i, token -1 for none.
-template <typename T, int NT, int CH, typename F>
-__device__ __forceinline__ void set_special(const Row<T, NT, CH>& row, Special<NT>& sp, int count, F f) {
+template <typename T, int NT, int CH, bool OPEN, typename F>
+__device__ __forceinline__ void set_special(const Row<T, NT, CH, OPEN>& row, Special<NT>& sp, int count, F f) {
   const int lane = threadIdx.x;
   for (int t = lane; t < NT; t += kWave) sp.first[t] = -1;
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -642,8 +668,8 @@ __device__ __forceinline__ void set_special(const Row<T, NT, CH>& row, Special<N
 
 // Writes f(x_j) of every logit of the row, and of the special ones' f(x) + scale total: over what was written, by the thread
 // that wrote it, so that nothing has to be waited for.  Entries of one token write one number.
-template <typename T, int NT, int CH, typename F>
-__device__ __forceinline__ void write_gradient(Row<T, NT, CH>& row, T* __restrict__ out, const Special<NT>& sp,
+template <typename T, int NT, int CH, bool OPEN, typename F>
+__device__ __forceinline__ void write_gradient(Row<T, NT, CH, OPEN>& row, T* __restrict__ out, const Special<NT>& sp,
                                                bool special, float scale, F f) {
   typedef typename RowVec<T>::V V;
   const bool whole = ((uintptr_t)out & 15) == ((uintptr_t)row.x & 15);
@@ -671,7 +697,7 @@ __device__ __forceinline__ void write_gradient(Row<T, NT, CH>& row, T* __restric
 
 template <typename T, int NT>
 __device__ __forceinline__ void write_zeros(T* __restrict__ out, int vocab) {
-  const Row<T, NT, 0> row(out, vocab);
+  const Row<T, NT, 0, true> row(out, vocab);
   typedef typename RowVec<T>::V V;
   for (int c = threadIdx.x; c < row.chunks; c += NT) reinterpret_cast<V*>(out + row.lead)[c] = V(0);
   if (row.loose >= 0) out[row.loose] = (T)0;
@@ -679,16 +705,20 @@ __device__ __forceinline__ void write_zeros(T* __restrict__ out, int vocab) {
 
 // dx_j = ([j = token] g + sum_i u_i [j = id_i] - p_j (g + sum_i u_i + h (log p_j + H))) / tau for the gradients g of
 // log p(token), h of the entropy and u_i of the top tokens' log probabilities.
-template <typename T, int NT, int CH, int WAVES>
-__global__ __launch_bounds__(NT, WAVES) void token_log_probs_backward_kernel(
-    const T* __restrict__ x, int64_t ld, int vocab, const int64_t* __restrict__ tokens, float tau,
+template <typename T, int NT, int CH, bool OPEN, int WAVES>
+__global__ __launch_bounds__(NT * kRowsOf<NT>, WAVES) void token_log_probs_backward_kernel(
+    const T* __restrict__ x, int64_t ld, int64_t rows, int vocab, const int64_t* __restrict__ tokens, float tau,
     const float* __restrict__ d_log_probs, const float* __restrict__ d_entropy, int k,
     const int64_t* __restrict__ top_tokens, const float* __restrict__ d_top, T* __restrict__ out, int64_t ld_out) {
-  __shared__ Shared<NT> sh;
-  __shared__ Special<NT> sp;
-  const int64_t r = blockIdx.x;
+  __shared__ Shared<NT> sh_of[kRowsOf<NT>];
+  __shared__ Special<NT> sp_of[kRowsOf<NT>];
+  const int in_group = row_in_group<NT>();
+  const int64_t r = (int64_t)blockIdx.x * kRowsOf<NT> + in_group;
+  if (r >= rows) return;
+  Shared<NT>& sh = sh_of[in_group];
+  Special<NT>& sp = sp_of[in_group];
   const int count = k + 1;
-  Row<T, NT, CH> row(x + r * ld, vocab);
+  Row<T, NT, CH, OPEN> row(x + r * ld, vocab);
   // Where the condition is the same for all threads, and not in a thread's branch below: a load from one address is
   // a scalar one, which a wavefront executes in a branch that none of its lanes takes.
   int64_t token = -1;
@@ -708,7 +738,7 @@ __global__ __launch_bounds__(NT, WAVES) void token_log_probs_backward_kernel(
       }
       if (t >= 0 && t < vocab) logit = row.at(t);
     });
-  __syncthreads();
+  sync_row<NT>();
   float g = 0.f;
   bool none = true;
 #pragma unroll 8
@@ -731,18 +761,28 @@ __global__ __launch_bounds__(NT, WAVES) void token_log_probs_backward_kernel(
   });
 }
 
+// A row's entries: a register each of all wavefronts otherwise.  total: 1, or 0 where there are none.
+struct Entries {
+  float q[kMaxTop], log_q[kMaxTop], x[kMaxTop], total;
+};
+
 // q = softmax(teacher / tau) over the row's entries (an id outside the vocabulary is no entry), loss = w sum q (log q -
 // log p); gradient w / tau (p_j - sum of q over the entries of token j).
-template <typename T, bool GRAD, int NT, int CH, int WAVES>
-__global__ __launch_bounds__(NT, WAVES) void distillation_kernel(const T* __restrict__ x, int64_t ld, int vocab,
+template <typename T, bool GRAD, int NT, int CH, bool OPEN, int WAVES>
+__global__ __launch_bounds__(NT * kRowsOf<NT>, WAVES) void distillation_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int vocab,
                                                           const int64_t* __restrict__ teacher_tokens,
                                                           const void* __restrict__ teacher, int teacher_f16, int k, float tau,
                                                           const float* __restrict__ weights, float* __restrict__ losses,
                                                           T* __restrict__ out, int64_t ld_out) {
-  __shared__ Shared<NT> sh;
-  __shared__ Special<NT> sp;
-  __shared__ float total;
-  const int64_t r = blockIdx.x;
+  __shared__ Shared<NT> sh_of[kRowsOf<NT>];
+  __shared__ Special<NT> sp_of[kRowsOf<NT>];
+  __shared__ Entries entries_of[kRowsOf<NT>];
+  const int in_group = row_in_group<NT>();
+  const int64_t r = (int64_t)blockIdx.x * kRowsOf<NT> + in_group;
+  if (r >= rows) return;
+  Shared<NT>& sh = sh_of[in_group];
+  Special<NT>& sp = sp_of[in_group];
+  Entries& entries = entries_of[in_group];
   const int tid = threadIdx.x;
   const float w = weights != nullptr ? weights[r] : 1.f;
   if (w == 0.f) {  // padding: whatever its logits are
@@ -750,9 +790,8 @@ __global__ __launch_bounds__(NT, WAVES) void distillation_kernel(const T* __rest
     if constexpr (GRAD) write_zeros<T, NT>(out + r * ld_out, vocab);
     return;
   }
-  Row<T, NT, CH> row(x + r * ld, vocab);
+  Row<T, NT, CH, OPEN> row(x + r * ld, vocab);
   constexpr int E = kMaxTop / kWave;  // a lane's entries, for the first wavefront
-  __shared__ float entry_q[kMaxTop], entry_log_q[kMaxTop], entry_x[kMaxTop];  // not a register each of all wavefronts
   float q[E], log_q[E], student[E];
   // the entries and their logits are requested first, and worked on while the row is on its way
   int64_t entry[E];
@@ -795,11 +834,11 @@ __global__ __launch_bounds__(NT, WAVES) void distillation_kernel(const T* __rest
 #pragma unroll
     for (int i = 0; i < E; ++i) {
       q[i] *= inv;
-      entry_q[tid + i * kWave] = q[i];
-      entry_log_q[tid + i * kWave] = log_q[i] - log_sum;
-      entry_x[tid + i * kWave] = student[i];
+      entries.q[tid + i * kWave] = q[i];
+      entries.log_q[tid + i * kWave] = log_q[i] - log_sum;
+      entries.x[tid + i * kWave] = student[i];
     }
-    if (tid == 0) total = sum == 0.f ? 0.f : 1.f;
+    if (tid == 0) entries.total = sum == 0.f ? 0.f : 1.f;
     if constexpr (GRAD)
       set_special(row, sp, k, [&](int e, int, int64_t& token, float& part, float& logit) {
         if (e >= E) return;
@@ -814,13 +853,13 @@ __global__ __launch_bounds__(NT, WAVES) void distillation_kernel(const T* __rest
 #pragma unroll
     for (int i = 0; i < E; ++i) {
       const int at = tid + i * kWave;
-      loss += entry_q[at] == 0.f ? 0.f : entry_q[at] * (entry_log_q[at] - st.log_p(entry_x[at]));
+      loss += entries.q[at] == 0.f ? 0.f : entries.q[at] * (entries.log_q[at] - st.log_p(entries.x[at]));
     }
     loss = wave_sum(loss);
-    if (tid == 0) losses[r] = total == 0.f ? 0.f : w * loss;
+    if (tid == 0) losses[r] = entries.total == 0.f ? 0.f : w * loss;
   }
   if constexpr (GRAD) {
-    const float scale = uniform(total == 0.f ? 0.f : w * st.inv * st.inv_tau);
+    const float scale = uniform(entries.total == 0.f ? 0.f : w * st.inv * st.inv_tau);
     write_gradient(row, out + r * ld_out, sp, st.S != 0.f, w * st.inv_tau,
                    [&](float y) { return __builtin_amdgcn_exp2f(st.t(y)) * scale; });
   }
@@ -830,64 +869,71 @@ __global__ __launch_bounds__(NT, WAVES) void distillation_kernel(const T* __rest
 // registers a thread and some 26 more, so few threads with long parts keep the most rows on a CU: of 50257 fp16 logits (6283
 // chunks) 3 with 512 threads, 4 with 256, 2 with 1024; 1477 rows scored 44 / 49 / 45 us, 2048 rows' loss and gradient 100 /
 // 105 / 104.  50304 fp32 logits (12576 chunks), forward and backward of 2048 rows: 512 threads 255 us, 1024 310.
+// Rows of up to 256 chunks have a wavefront each, four a workgroup; the longest, beyond 20480 chunks, are read again behind
+// those.  min_threads: what the call needs.
 template <typename F>
-void pick(int chunks, F f) {
-  auto go = [&](auto nt, auto ch, auto waves) { f(nt, ch, waves); };
-#define GPTMI_ROW(NT, CH, WAVES)                                                                             \
-  if (chunks <= NT * CH)                                                                                     \
-    return go(std::integral_constant<int, NT>(), std::integral_constant<int, CH>(), std::integral_constant<int, WAVES>())
-  GPTMI_ROW(64, 4, 4);
-  GPTMI_ROW(256, 4, 4);
-  GPTMI_ROW(256, 8, 4);
-  GPTMI_ROW(512, 8, 4);
-  GPTMI_ROW(512, 13, 6);
-  GPTMI_ROW(512, 16, 4);
-  GPTMI_ROW(512, 25, 4);
-  GPTMI_ROW(1024, 16, 4);
-  GPTMI_ROW(1024, 20, 4);
+void pick(int chunks, int min_threads, F f) {
+#define GPTMI_ROW(NT, CH, OPEN, WAVES)                                                                        \
+  if (NT >= min_threads && (OPEN || chunks <= NT * CH))                                                       \
+    return f(std::integral_constant<int, NT>(), std::integral_constant<int, CH>(), std::integral_constant<bool, OPEN>(), \
+             std::integral_constant<int, WAVES>())
+  GPTMI_ROW(64, 4, false, 4);
+  GPTMI_ROW(256, 4, false, 4);
+  GPTMI_ROW(256, 8, false, 4);
+  GPTMI_ROW(512, 8, false, 4);
+  GPTMI_ROW(512, 13, false, 6);
+  GPTMI_ROW(512, 16, false, 4);
+  GPTMI_ROW(512, 25, false, 4);
+  GPTMI_ROW(1024, 16, false, 4);
+  GPTMI_ROW(1024, 20, true, 4);
 #undef GPTMI_ROW
-  go(std::integral_constant<int, 1024>(), std::integral_constant<int, 0>(), std::integral_constant<int, 4>());
 }
 
 template <typename F>
-void pick_row(const LogitRows& a, F f) {
+void pick_row(const LogitRows& a, int min_threads, F f) {
   if (a.f16)
-    pick(a.vocab / 8, [&](auto nt, auto ch, auto waves) { f(_Float16(), nt, ch, waves); });
+    pick(a.vocab / 8, min_threads, [&](auto nt, auto ch, auto open, auto waves) { f(_Float16(), nt, ch, open, waves); });
   else
-    pick(a.vocab / 4, [&](auto nt, auto ch, auto waves) { f(float(), nt, ch, waves); });
+    pick(a.vocab / 4, min_threads, [&](auto nt, auto ch, auto open, auto waves) { f(float(), nt, ch, open, waves); });
 }
+
+template <int NT>
+dim3 grid_of(const LogitRows& a) { return dim3((unsigned)((a.rows + kRowsOf<NT> - 1) / kRowsOf<NT>)); }
+template <int NT>
+dim3 block_of() { return dim3(NT, kRowsOf<NT>); }
 
 }  // namespace
 
 void launch_token_log_probs(const LogitRows& a, const int64_t* tokens, int top, float* log_probs, float* entropy,
                             float* top_log_probs, int64_t* top_tokens, hipStream_t st) {
-  pick_row(a, [&](auto type, auto nt, auto ch, auto waves) {
+  // a wavefront has 64 groups to bound the top tokens with: no more than 32 of them
+  pick_row(a, top > 32 ? 256 : 0, [&](auto type, auto nt, auto ch, auto open, auto waves) {
     typedef decltype(type) T;
-    auto kernel = top > 0 ? token_log_probs_kernel<T, true, nt.value, ch.value, waves.value>
-                          : token_log_probs_kernel<T, false, nt.value, ch.value, waves.value>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)a.rows), dim3(nt.value), 0, st, (const T*)a.x, a.ld, a.vocab, tokens,
-                       a.temperature, top, log_probs, entropy, top_log_probs, top_tokens);
+    auto kernel = top > 0 ? token_log_probs_kernel<T, true, nt.value, ch.value, open.value, waves.value>
+                          : token_log_probs_kernel<T, false, nt.value, ch.value, open.value, waves.value>;
+    hipLaunchKernelGGL(kernel, grid_of<nt.value>(a), block_of<nt.value>(), 0, st, (const T*)a.x, a.ld, a.rows, a.vocab,
+                       tokens, a.temperature, top, log_probs, entropy, top_log_probs, top_tokens);
   });
 }
 
 void launch_token_log_probs_backward(const LogitRows& a, const int64_t* tokens, const float* d_log_probs,
                                      const float* d_entropy, int top, const int64_t* top_tokens, const float* d_top,
                                      void* grad, int64_t ld_grad, hipStream_t st) {
-  pick_row(a, [&](auto type, auto nt, auto ch, auto waves) {
+  pick_row(a, 0, [&](auto type, auto nt, auto ch, auto open, auto waves) {
     typedef decltype(type) T;
-    hipLaunchKernelGGL((token_log_probs_backward_kernel<T, nt.value, ch.value, waves.value>), dim3((unsigned)a.rows),
-                       dim3(nt.value), 0, st, (const T*)a.x, a.ld, a.vocab, tokens, a.temperature, d_log_probs,
-                       d_entropy, top, top_tokens, d_top, (T*)grad, ld_grad);
+    hipLaunchKernelGGL((token_log_probs_backward_kernel<T, nt.value, ch.value, open.value, waves.value>),
+                       grid_of<nt.value>(a), block_of<nt.value>(), 0, st, (const T*)a.x, a.ld, a.rows, a.vocab, tokens,
+                       a.temperature, d_log_probs, d_entropy, top, top_tokens, d_top, (T*)grad, ld_grad);
   });
 }
 
 void launch_distillation(const LogitRows& a, const int64_t* teacher_tokens, const void* teacher, bool teacher_f16,
                          int k, const float* weights, float* losses, void* grad, int64_t ld_grad, hipStream_t st) {
-  pick_row(a, [&](auto type, auto nt, auto ch, auto waves) {
+  pick_row(a, 0, [&](auto type, auto nt, auto ch, auto open, auto waves) {
     typedef decltype(type) T;
-    auto kernel = grad != nullptr ? distillation_kernel<T, true, nt.value, ch.value, waves.value>
-                                  : distillation_kernel<T, false, nt.value, ch.value, waves.value>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)a.rows), dim3(nt.value), 0, st, (const T*)a.x, a.ld, a.vocab,
+    auto kernel = grad != nullptr ? distillation_kernel<T, true, nt.value, ch.value, open.value, waves.value>
+                                  : distillation_kernel<T, false, nt.value, ch.value, open.value, waves.value>;
+    hipLaunchKernelGGL(kernel, grid_of<nt.value>(a), block_of<nt.value>(), 0, st, (const T*)a.x, a.ld, a.rows, a.vocab,
                        teacher_tokens, teacher, (int)teacher_f16, k, a.temperature, weights, losses, (T*)grad, ld_grad);
   });
 }
