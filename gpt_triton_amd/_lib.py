@@ -24,10 +24,10 @@ SIGNATURES = {
     "gptmi_layernorm": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _f32, _int, _vp]),
     "gptmi_softmax": (_int, [_vp, _vp, _i64, _i64, _int, _vp]),
     "gptmi_token_log_probs": (_int, [_vp, _i64, _vp, _f32, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _int, _vp]),
-    "gptmi_token_log_probs_backward": (_int, [_vp, _i64, _vp, _f32, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64,
-                                              _i64, _int, _vp]),
-    "gptmi_distillation_loss": (_int, [_vp, _i64, _vp, _vp, _i64, _f32, _vp, _vp, _vp, _i64, _i64, _i64, _int,
-                                       _int, _vp]),
+    "gptmi_token_log_probs_backward": (_int, [_vp, _i64, _vp, _f32, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp,
+                                              _i64, _i64, _i64, _int, _vp]),
+    "gptmi_distillation_loss": (_int, [_vp, _i64, _vp, _vp, _i64, _f32, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _i64,
+                                       _int, _int, _vp]),
     "gptmi_linear_workspace_bytes": (_sz, [_i64, _i64, _i64, _int, _int]),
     "gptmi_packed_weight_bytes": (_sz, [_i64, _i64]),
     "gptmi_pack_weight": (_int, [_vp, _vp, _i64, _i64, _int, _int, _vp]),

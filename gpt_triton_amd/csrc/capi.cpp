@@ -516,13 +516,14 @@ int gptmi_token_log_probs(const void* logits, int64_t ld, const int64_t* tokens,
 }
 
 int gptmi_token_log_probs_backward(const void* logits, int64_t ld, const int64_t* tokens, float temperature,
-                                   const float* d_log_probs, const float* d_entropy, int64_t top,
-                                   const int64_t* top_tokens, const float* d_top_log_probs, void* grad,
+                                   const float* d_log_probs, int64_t d_pitch, const float* d_entropy,
+                                   int64_t d_entropy_pitch, int64_t top, const int64_t* top_tokens, const float* d_top_log_probs, void* grad,
                                    int64_t ld_grad, int64_t M, int64_t V, int dtype, void* stream) {
   int rc = check_logits("token_log_probs_backward", logits, ld, temperature, M, V, dtype);
   if (!rc) rc = check_logits_gradient("token_log_probs_backward", grad, ld_grad, M, V, dtype);
   if (rc) return rc;
-  if ((d_log_probs && !tokens) || top < 0 || (top > 0 && (!top_tokens || !d_top_log_probs))) {
+  if ((d_log_probs && !tokens) || top < 0 || (top > 0 && (!top_tokens || !d_top_log_probs)) || (d_pitch & ~1ll) != 0 ||
+      (d_entropy_pitch & ~1ll) != 0) {
     set_error("token_log_probs_backward: invalid argument");
     return GPTMI_ERR_INVALID;
   }
@@ -530,19 +531,19 @@ int gptmi_token_log_probs_backward(const void* logits, int64_t ld, const int64_t
     set_error("token_log_probs_backward: %lld top tokens are beyond the supported %d", (long long)top, GPTMI_MAX_TOP);
     return GPTMI_ERR_UNSUPPORTED;
   }
-  launch_token_log_probs_backward(logit_rows(logits, ld, temperature, M, V, dtype), tokens, d_log_probs, d_entropy,
-                                  (int)top, top_tokens, d_top_log_probs, grad, ld_grad, (hipStream_t)stream);
+  launch_token_log_probs_backward(logit_rows(logits, ld, temperature, M, V, dtype), tokens,
+                                  RowGradient{d_log_probs, (int)d_pitch}, RowGradient{d_entropy, (int)d_entropy_pitch}, (int)top, top_tokens, d_top_log_probs, grad, ld_grad, (hipStream_t)stream);
   return check_launch("token_log_probs_backward");
 }
 
 int gptmi_distillation_loss(const void* logits, int64_t ld, const int64_t* teacher_tokens, const void* teacher_logits,
-                            int64_t k, float temperature, const float* weights, float* losses, void* grad,
-                            int64_t ld_grad, int64_t M, int64_t V, int dtype, int teacher_dtype, void* stream) {
+                            int64_t k, float temperature, const float* weights, const float* d_losses, int64_t d_pitch,
+                            float* losses, void* grad, int64_t ld_grad, int64_t M, int64_t V, int dtype, int teacher_dtype, void* stream) {
   int rc = check_logits("distillation_loss", logits, ld, temperature, M, V, dtype);
   if (!rc && grad) rc = check_logits_gradient("distillation_loss", grad, ld_grad, M, V, dtype);
   if (rc) return rc;
   if (!teacher_tokens || !teacher_logits || k <= 0 || (!losses && !grad) || !dtype_ok(teacher_dtype) ||
-      ((uintptr_t)teacher_logits & (teacher_dtype == GPTMI_F16 ? 1 : 3)) != 0) {
+      (d_pitch & ~1ll) != 0 || ((uintptr_t)teacher_logits & (teacher_dtype == GPTMI_F16 ? 1 : 3)) != 0) {
     set_error("distillation_loss: invalid argument");
     return GPTMI_ERR_INVALID;
   }
@@ -551,7 +552,7 @@ int gptmi_distillation_loss(const void* logits, int64_t ld, const int64_t* teach
     return GPTMI_ERR_UNSUPPORTED;
   }
   launch_distillation(logit_rows(logits, ld, temperature, M, V, dtype), teacher_tokens, teacher_logits,
-                      teacher_dtype == GPTMI_F16, (int)k, weights, losses, grad, ld_grad, (hipStream_t)stream);
+                      teacher_dtype == GPTMI_F16, (int)k, weights, RowGradient{d_losses, (int)d_pitch}, losses, grad, ld_grad, (hipStream_t)stream);
   return check_launch("distillation_loss");
 }
 

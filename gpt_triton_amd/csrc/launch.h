@@ -105,13 +105,18 @@ struct LogitRows {
 // log_probs (of tokens), entropy: one of them or both may be nullptr; top tokens: 0 to 128 a row
 void launch_token_log_probs(const LogitRows& a, const int64_t* tokens, int top, float* log_probs, float* entropy,
                             float* top_log_probs, int64_t* top_tokens, hipStream_t st);
-// d_log_probs, d_entropy may be nullptr, top 0
-void launch_token_log_probs_backward(const LogitRows& a, const int64_t* tokens, const float* d_log_probs,
-                                     const float* d_entropy, int top, const int64_t* top_tokens, const float* d_top,
+// d_log_probs, d_entropy may be nullptr, top 0; an element each for the rows, or one for all of them
+struct RowGradient {
+  const float* d;
+  int pitch;  // 1 or 0
+};
+void launch_token_log_probs_backward(const LogitRows& a, const int64_t* tokens, RowGradient d_log_probs,
+                                     RowGradient d_entropy, int top, const int64_t* top_tokens, const float* d_top,
                                      void* grad, int64_t ld_grad, hipStream_t st);
-// weights, losses, grad may be nullptr; k: 1 to 128 entries a row
+// weights, d_losses, losses, grad may be nullptr; k: 1 to 128 entries a row
 void launch_distillation(const LogitRows& a, const int64_t* teacher_tokens, const void* teacher, bool teacher_f16,
-                         int k, const float* weights, float* losses, void* grad, int64_t ld_grad, hipStream_t st);
+                         int k, const float* weights, RowGradient d_losses, float* losses, void* grad, int64_t ld_grad,
+                         hipStream_t st);
 
 // LayerNorm (unless x is normed), q, k, v product (packed weight image Bt [3h][h]) and causal attention of short
 // sequences in one launch: fp16, head size 64, out [B][L][heads][64], the bits of the launches it stands for.  All

@@ -708,8 +708,7 @@ __device__ __forceinline__ void write_zeros(T* __restrict__ out, int vocab) {
 template <typename T, int NT, int CH, bool OPEN, int WAVES>
 __global__ __launch_bounds__(NT * kRowsOf<NT>, WAVES) void token_log_probs_backward_kernel(
     const T* __restrict__ x, int64_t ld, int64_t rows, int vocab, const int64_t* __restrict__ tokens, float tau,
-    const float* __restrict__ d_log_probs, const float* __restrict__ d_entropy, int k,
-    const int64_t* __restrict__ top_tokens, const float* __restrict__ d_top, T* __restrict__ out, int64_t ld_out) {
+    RowGradient d_log_probs, RowGradient d_entropy, int k, const int64_t* __restrict__ top_tokens, const float* __restrict__ d_top, T* __restrict__ out, int64_t ld_out) {
   __shared__ Shared<NT> sh_of[kRowsOf<NT>];
   __shared__ Special<NT> sp_of[kRowsOf<NT>];
   const int in_group = row_in_group<NT>();
@@ -723,11 +722,11 @@ __global__ __launch_bounds__(NT * kRowsOf<NT>, WAVES) void token_log_probs_backw
   // a scalar one, which a wavefront executes in a branch that none of its lanes takes.
   int64_t token = -1;
   float d_token = 0.f, h = 0.f;
-  if (d_log_probs != nullptr) {
+  if (d_log_probs.d != nullptr) {
     token = tokens[r];
-    d_token = d_log_probs[r];
+    d_token = d_log_probs.d[r * d_log_probs.pitch];
   }
-  if (d_entropy != nullptr) h = d_entropy[r];
+  if (d_entropy.d != nullptr) h = d_entropy.d[r * d_entropy.pitch];
   if (threadIdx.x < kWave)
     set_special(row, sp, count, [&](int, int i, int64_t& t, float& part, float& logit) {
       t = token;
@@ -772,7 +771,7 @@ template <typename T, bool GRAD, int NT, int CH, bool OPEN, int WAVES>
 __global__ __launch_bounds__(NT * kRowsOf<NT>, WAVES) void distillation_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int vocab,
                                                           const int64_t* __restrict__ teacher_tokens,
                                                           const void* __restrict__ teacher, int teacher_f16, int k, float tau,
-                                                          const float* __restrict__ weights, float* __restrict__ losses,
+                                                          const float* __restrict__ weights, RowGradient d_losses, float* __restrict__ losses,
                                                           T* __restrict__ out, int64_t ld_out) {
   __shared__ Shared<NT> sh_of[kRowsOf<NT>];
   __shared__ Special<NT> sp_of[kRowsOf<NT>];
@@ -785,6 +784,8 @@ __global__ __launch_bounds__(NT * kRowsOf<NT>, WAVES) void distillation_kernel(c
   Entries& entries = entries_of[in_group];
   const int tid = threadIdx.x;
   const float w = weights != nullptr ? weights[r] : 1.f;
+  float w_grad = w;
+  if (d_losses.d != nullptr) w_grad *= d_losses.d[r * d_losses.pitch];
   if (w == 0.f) {  // padding: whatever its logits are
     if (tid == 0 && losses != nullptr) losses[r] = 0.f;
     if constexpr (GRAD) write_zeros<T, NT>(out + r * ld_out, vocab);
@@ -859,8 +860,8 @@ __global__ __launch_bounds__(NT * kRowsOf<NT>, WAVES) void distillation_kernel(c
     if (tid == 0) losses[r] = entries.total == 0.f ? 0.f : w * loss;
   }
   if constexpr (GRAD) {
-    const float scale = uniform(entries.total == 0.f ? 0.f : w * st.inv * st.inv_tau);
-    write_gradient(row, out + r * ld_out, sp, st.S != 0.f, w * st.inv_tau,
+    const float scale = uniform(entries.total == 0.f ? 0.f : w_grad * st.inv * st.inv_tau);
+    write_gradient(row, out + r * ld_out, sp, st.S != 0.f, w_grad * st.inv_tau,
                    [&](float y) { return __builtin_amdgcn_exp2f(st.t(y)) * scale; });
   }
 }
@@ -916,8 +917,8 @@ void launch_token_log_probs(const LogitRows& a, const int64_t* tokens, int top, 
   });
 }
 
-void launch_token_log_probs_backward(const LogitRows& a, const int64_t* tokens, const float* d_log_probs,
-                                     const float* d_entropy, int top, const int64_t* top_tokens, const float* d_top,
+void launch_token_log_probs_backward(const LogitRows& a, const int64_t* tokens, RowGradient d_log_probs,
+                                     RowGradient d_entropy, int top, const int64_t* top_tokens, const float* d_top,
                                      void* grad, int64_t ld_grad, hipStream_t st) {
   pick_row(a, 0, [&](auto type, auto nt, auto ch, auto open, auto waves) {
     typedef decltype(type) T;
@@ -928,13 +929,15 @@ void launch_token_log_probs_backward(const LogitRows& a, const int64_t* tokens, 
 }
 
 void launch_distillation(const LogitRows& a, const int64_t* teacher_tokens, const void* teacher, bool teacher_f16,
-                         int k, const float* weights, float* losses, void* grad, int64_t ld_grad, hipStream_t st) {
+                         int k, const float* weights, RowGradient d_losses, float* losses, void* grad, int64_t ld_grad,
+                         hipStream_t st) {
   pick_row(a, 0, [&](auto type, auto nt, auto ch, auto open, auto waves) {
     typedef decltype(type) T;
     auto kernel = grad != nullptr ? distillation_kernel<T, true, nt.value, ch.value, open.value, waves.value>
                                   : distillation_kernel<T, false, nt.value, ch.value, open.value, waves.value>;
     hipLaunchKernelGGL(kernel, grid_of<nt.value>(a), block_of<nt.value>(), 0, st, (const T*)a.x, a.ld, a.rows, a.vocab,
-                       teacher_tokens, teacher, (int)teacher_f16, k, a.temperature, weights, losses, (T*)grad, ld_grad);
+                       teacher_tokens, teacher, (int)teacher_f16, k, a.temperature, weights, d_losses, losses, (T*)grad,
+                       ld_grad);
   });
 }
 

@@ -26,7 +26,6 @@ import math
 import os
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -370,6 +369,23 @@ def _token_log_probs(logits, tokens, top, temperature):
     return log_probs, entropy, top_log_probs, top_tokens
 
 
+def _first_derivative(what):
+    # in a backward pass autograd is on where the pass is itself to be differentiated
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{what} has a first derivative only")
+
+
+def _row_gradient(g):
+    """(address, pitch in rows, what to keep until the call) of a gradient with an element a row; autograd hands one
+    number for all rows on as a view of pitch 0."""
+    if g is None:
+        return None, 0, None
+    if not any(g.stride()):
+        return g.data_ptr(), 0, g
+    g = g.contiguous()
+    return g.data_ptr(), 1, g
+
+
 class _TokenLogProbsFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, top, temperature):
@@ -382,19 +398,22 @@ class _TokenLogProbsFunction(torch.autograd.Function):
         return log_probs, entropy, top_log_probs, top_tokens
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, d_log_probs, d_entropy, d_top, _):
+        _first_derivative("token_log_probs")
         logits, tokens, top_tokens = ctx.saved_tensors
         if d_log_probs is None and d_entropy is None and d_top is None:
             return None, None, None, None
         dev, code, rows, V, ld = _logit_rows(logits, "token_log_probs")
-        d_log_probs, d_entropy, d_top = (None if g is None else g.contiguous() for g in (d_log_probs, d_entropy, d_top))
+        token_at, token_pitch, d_log_probs = _row_gradient(d_log_probs)
+        entropy_at, entropy_pitch, d_entropy = _row_gradient(d_entropy)
+        top = 0
+        if d_top is not None:
+            top, d_top = top_tokens.shape[-1], d_top.contiguous()
         grad, pitch = _logit_gradient(logits, rows, V, ld)
         if rows > 0:
             _call(dev, "token_log_probs_backward", _lib.load().gptmi_token_log_probs_backward, logits.data_ptr(), ld,
-                  _ptr(tokens), ctx.temperature, _ptr(d_log_probs), _ptr(d_entropy),
-                  0 if d_top is None else top_tokens.shape[-1], _ptr(top_tokens), _ptr(d_top), grad.data_ptr(), pitch,
-                  rows, V, code)
+                  _ptr(tokens), ctx.temperature, token_at, token_pitch, entropy_at, entropy_pitch, top, _ptr(top_tokens),
+                  _ptr(d_top), grad.data_ptr(), pitch, rows, V, code)
         return grad, None, None, None
 
 
@@ -415,7 +434,7 @@ def token_log_probs(logits, tokens=None, top=0, temperature=1.0):
     return TokenLogProbs(*_token_log_probs(logits, tokens, top, temperature))
 
 
-def _distillation(logits, teacher_tokens, teacher_logits, temperature, weights, losses, gradient):
+def _distillation(logits, teacher_tokens, teacher_logits, temperature, weights, losses, gradient, d_losses=None):
     """(losses or None, gradient or None)."""
     what = "distillation_loss"
     dev, code, rows, V, ld = _logit_rows(logits, what)
@@ -437,10 +456,11 @@ def _distillation(logits, teacher_tokens, teacher_logits, temperature, weights, 
     _check_temperature(temperature, what)
     out = logits.new_empty(lead, dtype=torch.float32) if losses else None
     grad, pitch = _logit_gradient(logits, rows, V, ld) if gradient else (None, V)
+    d_at, d_pitch, d_losses = _row_gradient(d_losses)
     if rows > 0:
         _call(dev, what, _lib.load().gptmi_distillation_loss, logits.data_ptr(), ld, teacher_tokens.data_ptr(),
-              teacher_logits.data_ptr(), k, temperature, _ptr(weights), _ptr(out), _ptr(grad), pitch, rows, V, code,
-              teacher_code)
+              teacher_logits.data_ptr(), k, temperature, _ptr(weights), d_at, d_pitch, _ptr(out), _ptr(grad), pitch, rows,
+              V, code, teacher_code)
     return out, grad
 
 
@@ -452,15 +472,10 @@ class _DistillationFunction(torch.autograd.Function):
         return _distillation(logits, teacher_tokens, teacher_logits, temperature, weights, True, False)[0]
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, d_losses):
+        _first_derivative("distillation_loss")
         logits, teacher_tokens, teacher_logits, weights = ctx.saved_tensors
-        # the gradient of the sum of the losses under other weights; where a weight is 0, so is its product with
-        # whatever comes back
-        if weights is not None:
-            d_losses = torch.where(weights == 0, weights, d_losses * weights)
-        grad = _distillation(logits, teacher_tokens, teacher_logits, ctx.temperature, d_losses.contiguous(), False,
-                             True)[1]
+        grad = _distillation(logits, teacher_tokens, teacher_logits, ctx.temperature, weights, False, True, d_losses)[1]
         return grad, None, None, None, None
 
 

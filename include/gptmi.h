@@ -153,15 +153,16 @@ int gptmi_token_log_probs(const void* logits, int64_t ld, const int64_t* tokens,
                           int64_t* top_tokens, int64_t M, int64_t V, int dtype, void* stream);
 
 /*
- * The gradient of the logits for the gradients of log_probs, entropy and top_log_probs (NULL, or top 0: of nothing):
+ * The gradient of the logits for the gradients of log_probs, entropy and top_log_probs (NULL, or top 0: of nothing); row
+ * m's of the former two are elements m * d_pitch, d_entropy_pitch (1, or 0 for one number for all rows):
  *   grad_j = ([j = token] g + sum_i [j = top_i] u_i - p_j (g + sum_i u_i + h (log p_j + H))) / temperature
  * in the logits' type at a pitch of ld_grad >= V elements; it may not overlap the logits.  Rows of zero gradients are
  * zeros whatever their logits are, rows without any probability too.  Fastest where grad and logits, and their pitches, are
  * equal modulo 16 bytes.
  */
 int gptmi_token_log_probs_backward(const void* logits, int64_t ld, const int64_t* tokens,
-                                   float temperature, const float* d_log_probs, const float* d_entropy,
-                                   int64_t top, const int64_t* top_tokens, const float* d_top_log_probs,
+                                   float temperature, const float* d_log_probs, int64_t d_pitch,
+                                   const float* d_entropy, int64_t d_entropy_pitch, int64_t top, const int64_t* top_tokens, const float* d_top_log_probs,
                                    void* grad, int64_t ld_grad, int64_t M, int64_t V, int dtype,
                                    void* stream);
 
@@ -169,8 +170,8 @@ int gptmi_token_log_probs_backward(const void* logits, int64_t ld, const int64_t
  * Distillation from a teacher's k top logits a row (1 <= k <= GPTMI_MAX_TOP), teacher_tokens, teacher_logits [M][k]:
  *   q = softmax(teacher_logits / temperature) over the row's entries, p = softmax(logits / temperature) over V
  *   losses[m] = weights[m] sum_i q_i (log q_i - log p[token_i])
- *   grad_j    = weights[m] / temperature (p_j - sum_i [j = token_i] q_i)   of the sum of the losses
- * in one pass over the logits.  Log probabilities serve as teacher_logits too (the softmax takes a constant out).  An
+ *   grad_j    = d_losses[m * d_pitch] weights[m] / temperature (p_j - sum_i [j = token_i] q_i)
+ * in one pass over the logits; d_losses NULL: 1, the gradient of the losses' sum; d_pitch 0: one number for all rows.  Log probabilities serve as teacher_logits too (the softmax takes a constant out).  An
  * entry whose token is outside [0, V) or whose logit is -infinity counts for nothing; a token that is there twice
  * counts twice.  A row without entries, or of weight 0 (padding), has loss 0 and gradient 0 whatever its logits are; a student
  * that gives the teacher's tokens no probability at all has loss +infinity.
@@ -179,7 +180,7 @@ int gptmi_token_log_probs_backward(const void* logits, int64_t ld, const int64_t
  */
 int gptmi_distillation_loss(const void* logits, int64_t ld, const int64_t* teacher_tokens,
                             const void* teacher_logits, int64_t k, float temperature, const float* weights,
-                            float* losses, void* grad, int64_t ld_grad, int64_t M, int64_t V, int dtype,
+                            const float* d_losses, int64_t d_pitch, float* losses, void* grad, int64_t ld_grad, int64_t M, int64_t V, int dtype,
                             int teacher_dtype, void* stream);
 
 /*

@@ -387,6 +387,37 @@ def test_gradients_against_differences(K, gpu_device):
         assert np.max(np.abs(host(grad)[0] - differences[:, i])) <= 8 / 6 * 2.0**-10 + 50 * U * 2**4
 
 
+def test_gradients_that_come_back(K, gpu_device):
+    """One number for all rows, one a row, every other one; weights of 0 whatever comes back; no second derivative."""
+    r = np.random.default_rng(21)
+    x = on_gpu(crowd(r, 4, 900), torch.float32, gpu_device).requires_grad_()
+    ids = torch.from_numpy(r.integers(0, 900, size=(4, 6))).to(gpu_device)
+    teacher = torch.from_numpy(r.standard_normal((4, 6))).float().to(gpu_device)
+    w = torch.tensor([1.0, 0.0, 2.0, 0.5], device=gpu_device)
+    t = ids[:, 0].contiguous()
+    each = torch.tensor([3.0, math.inf, -2.0, 0.25], device=gpu_device)
+    wide = torch.stack((each, each), 1)
+    _, one_pass = K.distillation_loss_and_grad(x.detach(), ids, teacher, 1.0, w)
+    for d in (each, wide[:, 0]):
+        loss = K.distillation_loss(x, ids, teacher, 1.0, w)
+        grad, = torch.autograd.grad(loss, x, d)
+        assert torch.all(grad[1] == 0)
+        # two products of fp32 numbers in another order: two roundings each
+        want = one_pass * torch.where(w == 0, w, each)[:, None]
+        assert torch.all((grad - want).abs() <= 8 * U * want.abs())
+        s = K.token_log_probs(x, t)
+        a, = torch.autograd.grad((s.log_probs, s.entropy), x, (d[:1].expand(4), w))
+        b, = torch.autograd.grad(K.token_log_probs(x, t).log_probs, x, d[:1].expand(4).contiguous())
+        c, = torch.autograd.grad(K.token_log_probs(x, t).entropy, x, w)
+        assert torch.all((a - b - c).abs() <= 200 * U * (b.abs() + c.abs() + 1e-3))
+    loss = K.distillation_loss(x, ids, teacher)
+    grad, = torch.autograd.grad(loss.sum(), x)
+    assert torch.equal(grad, K.distillation_loss_and_grad(x.detach(), ids, teacher)[1])
+    for out in (K.distillation_loss(x, ids, teacher), K.token_log_probs(x, t).log_probs):
+        with pytest.raises(RuntimeError, match="first derivative"):
+            torch.autograd.grad(out.sum(), x, create_graph=True)
+
+
 def test_shapes_and_views(K, gpu_device):
     """Leading dimensions, rows of one pitch, one row many times, no rows."""
     r = np.random.default_rng(8)
@@ -430,7 +461,7 @@ def test_what_lies_between_rows_stays(K, gpu_device):
         out = torch.full((3, pitch), 7.0, dtype=dtype, device=gpu_device)
         losses = torch.empty(3, device=gpu_device)
         K._call(0, "test", _lib.load().gptmi_distillation_loss, x.data_ptr(), x.stride(0), ids.data_ptr(), t.data_ptr(), 1,
-                1.0, None, losses.data_ptr(), out.data_ptr(), pitch, 3, V, K._dtype_code(x, "test"), _lib.GPTMI_F32)
+                1.0, None, None, 0, losses.data_ptr(), out.data_ptr(), pitch, 3, V, K._dtype_code(x, "test"), _lib.GPTMI_F32)
         _, want = K.distillation_loss_and_grad(x, ids, t)
         assert torch.equal(out[:, :V], want) and torch.all(out[:, V:] == 7.0)
 

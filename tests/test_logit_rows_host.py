@@ -41,26 +41,26 @@ def test_scores_refusals(lib):
 
 
 def test_gradient_refusals(lib):
-    def call(x=FAKE, ld=64, tokens=FAKE, tau=1.0, g=FAKE, h=None, top=0, ids=None, u=None, grad=FAKE, ld_grad=64, M=4,
+    def call(x=FAKE, ld=64, tokens=FAKE, tau=1.0, g=FAKE, g_pitch=1, h=None, h_pitch=1, top=0, ids=None, u=None, grad=FAKE, ld_grad=64, M=4,
              V=64, dtype=1):
-        return lib.gptmi_token_log_probs_backward(x, ld, tokens, tau, g, h, top, ids, u, grad, ld_grad, M, V, dtype,
+        return lib.gptmi_token_log_probs_backward(x, ld, tokens, tau, g, g_pitch, h, h_pitch, top, ids, u, grad, ld_grad, M, V, dtype,
                                                   None)
 
     for args in (dict(x=None), dict(grad=None), dict(ld_grad=63), dict(tokens=None), dict(top=3), dict(top=3, ids=FAKE),
-                 dict(grad=ctypes.c_void_p(257)), dict(tau=0.0), dict(top=-1)):
+                 dict(grad=ctypes.c_void_p(257)), dict(tau=0.0), dict(top=-1), dict(g_pitch=2), dict(h_pitch=-1)):
         assert call(**args) == -1, args
     assert call(top=129, ids=FAKE, u=FAKE) == -2
     assert call(ld_grad=(1 << 40) + 1) == -2
 
 
 def test_distillation_refusals(lib):
-    def call(x=FAKE, ld=64, ids=FAKE, t=FAKE, k=4, tau=1.0, losses=FAKE, grad=None, ld_grad=64, M=4, V=64, dtype=1,
+    def call(x=FAKE, ld=64, ids=FAKE, t=FAKE, k=4, tau=1.0, d=None, d_pitch=1, losses=FAKE, grad=None, ld_grad=64, M=4, V=64, dtype=1,
              t_dtype=0):
-        return lib.gptmi_distillation_loss(x, ld, ids, t, k, tau, None, losses, grad, ld_grad, M, V, dtype, t_dtype,
+        return lib.gptmi_distillation_loss(x, ld, ids, t, k, tau, None, d, d_pitch, losses, grad, ld_grad, M, V, dtype, t_dtype,
                                            None)
 
     for args in (dict(x=None), dict(ids=None), dict(t=None), dict(k=0), dict(losses=None), dict(t_dtype=2),
-                 dict(t=ctypes.c_void_p(258)), dict(grad=FAKE, ld_grad=63), dict(tau=-1.0), dict(dtype=-1)):
+                 dict(t=ctypes.c_void_p(258)), dict(grad=FAKE, ld_grad=63), dict(tau=-1.0), dict(dtype=-1), dict(d_pitch=4)):
         assert call(**args) == -1, args
     assert call(k=129) == -2
 
