@@ -786,7 +786,7 @@ __global__ __launch_bounds__(NT * kRowsOf<NT>, WAVES) void distillation_kernel(c
   const float w = weights != nullptr ? weights[r] : 1.f;
   float w_grad = w;
   if (d_losses.d != nullptr) w_grad *= d_losses.d[r * d_losses.pitch];
-  if (w == 0.f) {  // padding: whatever its logits are
+  if (w == 0.f || (losses == nullptr && w_grad == 0.f)) {  // padding: whatever its logits are
     if (tid == 0 && losses != nullptr) losses[r] = 0.f;
     if constexpr (GRAD) write_zeros<T, NT>(out + r * ld_out, vocab);
     return;

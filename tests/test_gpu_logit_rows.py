@@ -410,6 +410,13 @@ def test_gradients_that_come_back(K, gpu_device):
         b, = torch.autograd.grad(K.token_log_probs(x, t).log_probs, x, d[:1].expand(4).contiguous())
         c, = torch.autograd.grad(K.token_log_probs(x, t).entropy, x, w)
         assert torch.all((a - b - c).abs() <= 200 * U * (b.abs() + c.abs() + 1e-3))
+    nothing = x.detach().clone()
+    nothing[2] = math.nan
+    nothing.requires_grad_()
+    keep = torch.tensor([True, True, False, True], device=gpu_device)
+    loss = torch.where(keep, K.distillation_loss(nothing, ids, teacher), 0.0)
+    grad, = torch.autograd.grad(loss.sum(), nothing)
+    assert torch.all(torch.isfinite(loss)) and torch.all(torch.isfinite(grad)) and torch.all(grad[2] == 0)
     loss = K.distillation_loss(x, ids, teacher)
     grad, = torch.autograd.grad(loss.sum(), x)
     assert torch.equal(grad, K.distillation_loss_and_grad(x.detach(), ids, teacher)[1])
