@@ -760,7 +760,7 @@ int gptmi_flash_attn_packed(const void* q, const void* k, const void* v, void* o
                             int64_t q_head, int64_t k_row, int64_t k_head, int64_t v_row, int64_t v_head, float scale,
                             int dtype, void* stream) {
   if (!q || !k || !v || !out || !starts || sequences <= 0 || T <= 0 || N <= 0 || G <= 0 || N % G != 0 || d <= 0 ||
-      !dtype_ok(dtype) || !(scale > 0.0f) || isinf(scale) || ((uintptr_t)starts & 7) != 0) {
+      !dtype_ok(dtype) || !(scale >= 1e-20f && scale <= 1e20f) || ((uintptr_t)starts & 7) != 0) {
     set_error("flash_attn_packed: invalid argument");
     return GPTMI_ERR_INVALID;
   }

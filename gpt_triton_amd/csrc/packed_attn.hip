@@ -226,13 +226,17 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
   for (int n = 0; n < QB; ++n)
 #pragma unroll
     for (int i = 0; i < DB; ++i) oacc[n][i] = f4(0.f);
-  // The weights are 2^(t s - base), t = scale log2(e), base = t ref - 6, for a reference that the running maximum may pass by
-  // 2^8 before it follows: the accumulator is rescaled in few tiles, a weight is at most 2^14, and one is a subnormal fp16
-  // number, which has fewer bits, below 2^-20 of the reference.  The denominator adds the weights as rounded for the
-  // product with V.
+  // The weights are 2^(t s - base), t = scale log2(e), base = t ref - 6 as rounded, for a reference that the running maximum
+  // may pass by 2^8 before it follows: the accumulator is rescaled in few tiles (by what the bases as rounded differ by, so
+  // that tiles of different references agree), a weight is at most 2^14, and one is a subnormal fp16 number, which has fewer
+  // bits, below 2^-20 of the reference.  The denominator adds the weights in fp32, in the four lanes of a query and across
+  // them at the end.  (us, this / dot products of the rounded pairs with ones, which flush subnormal weights / a column of ones
+  // in the matrix product, which costs registers: 48 of up to 1024 rows 23.2 / 23.1 / 26.0, 1 x 16384 995 / 988 / 1003.)
+  // The key that set the reference weighs 2^6, so a denominator below 2^5 is one whose base was rounded by more than the weights
+  // reach, which the end looks for.
   float ref[QB], limit[QB], base[QB], den[QB];
 #pragma unroll
-  for (int n = 0; n < QB; ++n) ref[n] = limit[n] = -INFINITY, base[n] = den[n] = 0.f;
+  for (int n = 0; n < QB; ++n) ref[n] = limit[n] = base[n] = -INFINITY, den[n] = 0.f;
   const float room = 8.0f / to_exp2;
 
   // One 64-key tile.  MASK: the one that the diagonal cuts, in which query x of the wavefront sees keys 0 .. edge + x;
@@ -279,10 +283,11 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
     if (D > 128 || __any(higher)) {  // a branch there costs registers that there are none of
 #pragma unroll
       for (int n = 0; n < QB; ++n) {
-        const float to = larger(most[n], ref[n]), mult = __builtin_amdgcn_exp2f((ref[n] - to) * to_exp2);
+        const float to = larger(most[n], ref[n]), next = fmaf(to, to_exp2, -6.0f);
+        const float mult = __builtin_amdgcn_exp2f(base[n] - next);
         ref[n] = to;
         limit[n] = to + room;
-        base[n] = fmaf(to, to_exp2, -6.0f);
+        base[n] = next;
         den[n] *= mult;
 #pragma unroll
         for (int i = 0; i < DB; ++i) oacc[n][i] *= mult;
@@ -293,13 +298,10 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
 #pragma unroll
       for (int kb = 0; kb < 2 * KG; ++kb)
 #pragma unroll
-        for (int r = 0; r < 4; r += 2) {
-          h2 p;
-          p[0] = (_Float16)__builtin_amdgcn_exp2f(fmaf(s[n][kb][r], to_exp2, -base[n]));
-          p[1] = (_Float16)__builtin_amdgcn_exp2f(fmaf(s[n][kb][r + 1], to_exp2, -base[n]));
-          pf[n][kb >> 1][4 * (kb & 1) + r] = p[0];
-          pf[n][kb >> 1][4 * (kb & 1) + r + 1] = p[1];
-          den[n] = __builtin_amdgcn_fdot2(p, h2{1, 1}, den[n], false);
+        for (int r = 0; r < 4; ++r) {
+          const float p = __builtin_amdgcn_exp2f(fmaf(s[n][kb][r], to_exp2, -base[n]));
+          pf[n][kb >> 1][4 * (kb & 1) + r] = (_Float16)p;
+          den[n] += p;
         }
 #pragma unroll
     for (int n = 0; n < QB; ++n) asm volatile("" : "+v"(den[n]));  // here, not with copies of the weights behind the barrier
@@ -367,14 +369,14 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
   if (!wave_active) return;
 
   // ---- an infinity or a NaN among the results: one of the inputs is none, and a hidden key's value, times its weight
-  // of 0, may have spoilt queries in front of it.  Once more, key by key, for these 16 queries.  Then the output, 8 bytes
-  // a lane and 32 for the four of a query.
+  // of 0, may have spoilt queries in front of it; or scores are beyond what fp32 has of an exponent (some 2^25).  Once
+  // more, key by key, for these 16 queries.  Then the output, 8 bytes a lane and 32 for the four of a query.
 #pragma unroll
   for (int n = 0; n < QB; ++n) {
     const int q = qw0 + 16 * n + c;
     const LanePair pair = row_swap(half_sum(den[n]));
-    const float inv = 1.0f / (pair.a + pair.b);
-    float none = 0.f;
+    const float sum = pair.a + pair.b, inv = 1.0f / sum;
+    float none = sum >= 32.0f ? 0.f : 1.f;
 #pragma unroll
     for (int i = 0; i < DB; ++i) {
       oacc[n][i] *= inv;
@@ -382,25 +384,27 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
       for (int r = 0; r < 4; ++r) none = fmaf(oacc[n][i][r], 0.f, none);
     }
     if (__any(none != 0.f && q < L)) {
+#pragma clang fp contract(off)  // a score is one rounded number wherever it is used
       const int last = min(qw0 + 16 * n + 15, L - 1), mine = min(q, L - 1);
       const _Float16* p = qp + (int64_t)mine * a.q_row;
       auto score = [&](int j) {
+#pragma clang fp contract(off)
         const _Float16* kj = kp + (int64_t)j * a.k_row;
         float s = 0.f;
 #pragma unroll 1
         for (int d = 0; d < D; ++d) s = fmaf((float)p[d], (float)kj[d], s);
         return j <= mine ? s * a.scale : -INFINITY;
       };
-      float m = -INFINITY, sum = 0.f;
+      float m = -INFINITY, total = 0.f;
 #pragma unroll 1
       for (int j = 0; j <= last; ++j) m = fmaxf(m, score(j));
 #pragma unroll 1
-      for (int j = 0; j <= last; ++j) sum += j <= mine ? __expf(score(j) - m) : 0.f;
+      for (int j = 0; j <= last; ++j) total += j <= mine ? __expf(score(j) - m) : 0.f;
 #pragma unroll
       for (int i = 0; i < DB; ++i) oacc[n][i] = f4(0.f);
 #pragma unroll 1
       for (int j = 0; j <= last; ++j) {
-        const float w = __expf(score(j) - m) / sum;
+        const float w = __expf(score(j) - m) / total;
         const _Float16* vj = vp + (int64_t)j * a.v_row + 4 * g;
 #pragma unroll
         for (int i = 0; i < DB; ++i)
@@ -424,6 +428,12 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
 
 template <int D, int QB>
 int launch_as(PackedArgs a, int64_t slots, hipStream_t st) {
+  const int64_t blocks = slots * a.heads;
+  if (blocks >= 1ll << 31) {
+    set_error("flash_attn_packed: %lld rows in %d sequences of %d heads exceed the grid", (long long)a.rows, a.sequences,
+              a.heads);
+    return -2;
+  }
   constexpr int lds = 2 * 2 * kKeys * D * 2;
   static bool attr_done = false;  // idempotent; a race only repeats the call
   if (!attr_done) {
@@ -434,12 +444,6 @@ int launch_as(PackedArgs a, int64_t slots, hipStream_t st) {
       return -4;
     }
     attr_done = true;
-  }
-  const int64_t blocks = slots * a.heads;
-  if (blocks >= 1ll << 31) {
-    set_error("flash_attn_packed: %lld rows in %d sequences of %d heads exceed the grid", (long long)a.rows, a.sequences,
-              a.heads);
-    return -2;
   }
   a.slots = (int)slots;
   // Up to 10 workgroups a CU the heaviest first: whichever starts last ends the launch.  Beyond, a head's blocks one behind

@@ -341,7 +341,7 @@ def _maybe_check_row_tokens(t, V, what):
 
 
 def _check_temperature(temperature, what):
-    if not 1e-30 <= temperature < 1e30:
+    if not 1e-30 <= temperature <= 1e30:
         raise ValueError(f"{what}: temperature {temperature} is not between 1e-30 and 1e30")
 
 
@@ -656,7 +656,8 @@ def flash_attention_packed(q, k, v, starts, scale=None, out=None):
 
     fp16 (fp32 storage would round q, k and v to it).  A head's d elements lie side by side; rows and heads may be
     views of something larger at 16-byte aligned pitches, such as the columns of a q, k, v product.  Rows that belong to no
-    sequence are not read, and of `out` (dense; allocated if None) not written."""
+    sequence are not read, and of `out` (dense, apart from k and v; allocated if None) not written.  A forward pass only,
+    like `flash_attention_v1`."""
     assert q.dim() == k.dim() == 3 and k.shape == v.shape, (q.shape, k.shape, v.shape)
     T, N, d = q.shape
     G = k.shape[1]
@@ -681,8 +682,8 @@ def flash_attention_packed(q, k, v, starts, scale=None, out=None):
         pitches += (row, head)
     if scale is None:
         scale = d ** -0.5
-    if not 0.0 < scale < math.inf:
-        raise ValueError(f"flash_attention_packed: scale {scale} is not above 0 and finite")
+    if not 1e-20 <= scale <= 1e20:
+        raise ValueError(f"flash_attention_packed: scale {scale} is not between 1e-20 and 1e20")
     if out is None:
         out = q.new_empty((T, N, d))
     else:

@@ -137,7 +137,8 @@ int gptmi_softmax(const void* x, void* out, int64_t M, int64_t H, int dtype,
 
 /*
  * Scores of M rows of logits [V] at a pitch of ld elements (the padded rows of an LM head, a dense matrix, any
- * alignment that the element type allows), z = logits / temperature, p = softmax(z) with fp32 maximum and sums:
+ * alignment that the element type allows), z = logits / temperature (from 1e-30
+ * on), p = softmax(z) with fp32 maximum and sums:
  *   log_probs[m] = log p[tokens[m]]        a token outside [0, V) (padding) reads no memory and scores 0
  *   entropy[m]   = -sum p log p
  *   top_tokens[m][0 .. top): the tokens with the largest logits, largest first, equal ones in the order of their ids
@@ -173,7 +174,8 @@ int gptmi_token_log_probs_backward(const void* logits, int64_t ld, const int64_t
  *   grad_j    = d_losses[m * d_pitch] weights[m] / temperature (p_j - sum_i [j = token_i] q_i)
  * in one pass over the logits; d_losses NULL: 1, the gradient of the losses' sum; d_pitch 0: one number for all rows.  Log probabilities serve as teacher_logits too (the softmax takes a constant out).  An
  * entry whose token is outside [0, V) or whose logit is -infinity counts for nothing; a token that is there twice
- * counts twice.  A row without entries, or of weight 0 (padding), has loss 0 and gradient 0 whatever its logits are; a student
+ * counts twice.  A row without entries, or of weight 0 (padding), has loss 0 and gradient 0 whatever its logits are, and
+ * without losses one of d_losses 0 too; a student
  * that gives the teacher's tokens no probability at all has loss +infinity.
  * weights may be NULL (all 1), losses or grad may be NULL; grad as in gptmi_token_log_probs_backward.  teacher_dtype:
  * the type of teacher_logits.
@@ -341,7 +343,8 @@ int gptmi_flash_attn(const void* q, const void* k, const void* v, void* out,
  *   starts: sequences + 1 int64 on the device, not decreasing, from 0 to T.  Rows in front of the first and behind the
  *   last sequence are not read and not written.  (Starts that break these rules reach no row outside [0, T).)
  * fp16 storage; scores, softmax and sums are fp32, the weights are rounded to fp16 for the product with v (they lie in a
- * result of that type).  What hidden keys and values hold, infinities and NaN included, plays no part.  scale > 0.
+ * result of that type).  What hidden keys and values hold, infinities and NaN included, plays no part.  scale from 1e-20
+ * to 1e20; out may not overlap k or v.
  * Extends flash_attention_v1 -> kernels.py:477-525, which takes one length and as many key heads as heads.
  */
 int gptmi_flash_attn_packed(const void* q, const void* k, const void* v, void* out,

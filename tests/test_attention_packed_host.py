@@ -30,7 +30,7 @@ def test_refusals(lib):
     odd = ctypes.c_void_p(264)
     for args in (dict(q=None), dict(k=None), dict(v=None), dict(out=None), dict(starts=None), dict(S=0), dict(T=0),
                  dict(N=0), dict(G=0), dict(N=5), dict(d=0), dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan),
-                 dict(scale=math.inf), dict(dtype=3), dict(q=odd), dict(k=odd), dict(v=odd), dict(out=odd),
+                 dict(scale=math.inf), dict(scale=1e21), dict(scale=1e-21), dict(dtype=3), dict(q=odd), dict(k=odd), dict(v=odd), dict(out=odd),
                  dict(starts=ctypes.c_void_p(260)), dict(q_row=257), dict(k_head=4), dict(v_row=129)):
         assert call(lib, **args) == -1, args
         assert b"flash_attn_packed" in lib.gptmi_last_error()

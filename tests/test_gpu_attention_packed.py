@@ -146,6 +146,29 @@ def test_scores_that_rise_and_fall(K, gpu_device, d):
         check(K, q, k, v, [L], scale=1.0)
 
 
+@pytest.mark.parametrize("d", [16, 64, 128, 256])
+def test_scores_beyond_the_exponent(K, gpu_device, d):
+    """Scores so large that fp32 exponents are off by more than weights reach, and the largest fp16 inputs."""
+    r = np.random.default_rng(20)
+    L = 200
+    q, k, v = make(r, L, 2, 2, d, False, gpu_device)
+    for scale, size in ((1e4, 100.0), (1e15, 1.0), (1.0, 65504.0), (1e-20, 1.0)):
+        a, b = (q.sign() * size, k.sign() * size) if size > 1e3 else (q * size, k * size)
+        out = K.flash_attention_packed(a, b, v, starts_of([L], gpu_device), scale=scale)
+        s = torch.matmul(a[:, 0].double(), b[:, 0].double().t().contiguous()) * scale
+        s = torch.where(torch.ones_like(s, dtype=torch.bool).tril_(), s, -math.inf)
+        w = torch.softmax(s, 1)
+        # rows whose weights do not hang on the rounding of a score: (d + 16) u of its size either way
+        e = (d + 16) * U * torch.matmul(a[:, 0].double().abs(), b[:, 0].double().abs().t().contiguous()).amax(1) * scale
+        top = torch.topk(s, 2, dim=1).values if L > 1 else s
+        clear = (top[:, 0] - top[:, 1] > 2 * e + 40) | (e < 1e-3)
+        clear[0] = True  # a key alone
+        assert clear.sum() > 1 or size == 65504.0
+        want_ = torch.matmul(w, v[:, 0].double())
+        err = (out[:, 0].double() - want_).abs().amax(1)
+        assert torch.all(torch.isfinite(out)) and torch.all(err[clear] <= 8 * H * float(v.abs().max()))
+
+
 @pytest.mark.parametrize("count", [63, 64, 65, 130, 1000, 5000])
 def test_many_sequences(K, gpu_device, count):
     r = np.random.default_rng(count)
