@@ -384,35 +384,49 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
       for (int r = 0; r < 4; ++r) none = fmaf(oacc[n][i][r], 0.f, none);
     }
     if (__any(none != 0.f && q < L)) {
-#pragma clang fp contract(off)  // a score is one rounded number wherever it is used
-      const int last = min(qw0 + 16 * n + 15, L - 1), mine = min(q, L - 1);
-      const _Float16* p = qp + (int64_t)mine * a.q_row;
+      const int last = min(qw0 + 16 * n + 15, L - 1);
+      // of query c with key j, from this lane's elements of both and the other three lanes': one rounded number
       auto score = [&](int j) {
 #pragma clang fp contract(off)
-        const _Float16* kj = kp + (int64_t)j * a.k_row;
-        float s = 0.f;
-#pragma unroll 1
-        for (int d = 0; d < D; ++d) s = fmaf((float)p[d], (float)kj[d], s);
-        return j <= mine ? s * a.scale : -INFINITY;
+        const _Float16* kj = kp + (int64_t)j * a.k_row + g * 8;
+        float x = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          if (D < 32 && g >= 2) continue;
+          const h8 kf = *reinterpret_cast<const h8*>(kj + ks * 32);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x = fmaf((float)qf[n][ks][i], (float)kf[i], x);
+        }
+        const LanePair pair = row_swap(half_sum(x));
+        return (pair.a + pair.b) * a.scale;
       };
       float m = -INFINITY, total = 0.f;
-#pragma unroll 1
-      for (int j = 0; j <= last; ++j) m = fmaxf(m, score(j));
-#pragma unroll 1
-      for (int j = 0; j <= last; ++j) total += j <= mine ? __expf(score(j) - m) : 0.f;
-#pragma unroll
-      for (int i = 0; i < DB; ++i) oacc[n][i] = f4(0.f);
-#pragma unroll 1
+#pragma unroll 4
       for (int j = 0; j <= last; ++j) {
-        const float w = __expf(score(j) - m) / total;
-        const _Float16* vj = vp + (int64_t)j * a.v_row + 4 * g;
+        const float x = score(j), to = fmaxf(m, x), by = to == -INFINITY ? 0.f : to;
+        const float more = fmaf(total, __expf(m - by), __expf(x - by));
+        total = j <= q ? more : total;
+        m = j <= q ? to : m;
+      }
+      const bool number = total == total && fabsf(m) < INFINITY;  // else there is no softmax
+      const float inv_total = number ? 1.0f / total : NAN;
 #pragma unroll
-        for (int i = 0; i < DB; ++i)
+      for (int i = 0; i < DB; ++i) oacc[n][i] = f4(number ? 0.f : NAN);
+      if (__any(number && q < L)) {
+#pragma unroll 2
+        for (int j = 0; j <= last; ++j) {
+          const float w = __expf(score(j) - m) * inv_total;
+          const _Float16* vj = vp + (int64_t)j * a.v_row + 4 * g;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float more = fmaf(w, (float)vj[16 * i + r], oacc[n][i][r]);
-            oacc[n][i][r] = j <= mine ? more : oacc[n][i][r];
+          for (int i = 0; i < DB; ++i) {
+            const h4 vf = *reinterpret_cast<const h4*>(vj + 16 * i);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const float more = fmaf(w, (float)vf[r], oacc[n][i][r]);
+              oacc[n][i][r] = j <= q ? more : oacc[n][i][r];
+            }
           }
+        }
       }
     }
     _Float16* o = a.out + ((block.first + q) * a.heads + head) * D + 4 * g;

@@ -227,6 +227,33 @@ def test_hidden_keys_play_no_part(K, gpu_device, d, heads):
                     assert torch.all(torch.isnan(got[behind]))
 
 
+def test_many_numbers_that_are_none(K, gpu_device):
+    """Long prompts in which every query meets one, or the last alone."""
+    r = np.random.default_rng(22)
+    L = 20000
+    q, k, v = (t.clone() for t in make(r, L, 8, 2, 128, False, gpu_device))
+    starts = starts_of([L], gpu_device)
+    clean = K.flash_attention_packed(q, k, v, starts)
+    for which in (0, 1, 2):
+        x = [q.clone(), k.clone(), v.clone()]
+        x[which][L - 1] = math.nan
+        got = K.flash_attention_packed(*x, starts)
+        assert torch.all(torch.isnan(got[L - 1])) and torch.equal(got[:L - 64], clean[:L - 64])
+        x[which][:] = math.nan
+        assert torch.all(torch.isnan(K.flash_attention_packed(*x, starts)))
+    k[0] = math.nan
+    assert torch.all(torch.isnan(K.flash_attention_packed(q, k, v, starts)))
+
+
+def test_out_in_the_place_of_q(K, gpu_device):
+    r = np.random.default_rng(23)
+    for lengths in ([300, 1, 77], [2000, 3000]):
+        q, k, v = make(r, sum(lengths), 12, 4, 64, False, gpu_device)
+        starts = starts_of(lengths, gpu_device)
+        apart = K.flash_attention_packed(q, k, v, starts)
+        assert torch.equal(K.flash_attention_packed(q, k, v, starts, out=q), apart)
+
+
 def test_rows_of_no_sequence_stay(K, gpu_device):
     r = np.random.default_rng(11)
     for d in (16, 64, 128, 256):
