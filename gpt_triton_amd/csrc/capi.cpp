@@ -467,7 +467,7 @@ int gptmi_softmax(const void* x, void* out, int64_t M, int64_t H, int dtype, voi
 // What the operators on rows of logits ask of them.
 static int check_logits(const char* what, const void* x, int64_t ld, float temperature, int64_t M, int64_t V,
                         int dtype) {
-  if (!x || M <= 0 || V <= 0 || ld < 0 || !dtype_ok(dtype) || !(temperature >= 1e-30f) || isinf(temperature) ||
+  if (!x || M <= 0 || V <= 0 || ld < 0 || !dtype_ok(dtype) || !(temperature >= (dtype == GPTMI_F16 ? 1e-4f : 1e-30f) && temperature <= 1e30f) ||
       ((uintptr_t)x & (dtype == GPTMI_F16 ? 1 : 3)) != 0) {
     set_error("%s: invalid argument", what);
     return GPTMI_ERR_INVALID;
@@ -777,7 +777,7 @@ int gptmi_flash_attn_packed(const void* q, const void* k, const void* v, void* o
   const auto pitch_ok = [](int64_t row) { return row >= 0 && row <= 1 << 24; };
   const auto head_ok = [](int64_t head) { return head >= 0 && head <= 1ll << 40; };
   if (!pitch_ok(q_row) || !pitch_ok(k_row) || !pitch_ok(v_row) || !head_ok(q_head) || !head_ok(k_head) ||
-      !head_ok(v_head) || T >= 1ll << 31 || sequences >= 1ll << 31 || N > 1 << 20) {
+      !head_ok(v_head) || T >= 1ll << 31 || sequences > 1ll << 30 || N > 1 << 20) {
     set_error("flash_attn_packed: sizes or pitches beyond the supported");
     return GPTMI_ERR_UNSUPPORTED;
   }

@@ -150,8 +150,9 @@ __device__ __forceinline__ float join(float v, Op op) {
   return v;
 }
 
-// t = x c - b.  fp16: one operation from the logit as it is, b rounded once for all of a row (65504 c is finite for
-// any temperature above 1e-30).  fp32, whose m c may overflow: the difference, which is 0 for m, and its multiple.
+// t = x c - b.  fp16: one operation from the logit as it is, b rounded once for all of a row (by up to 32 for logits of 65504
+// and a temperature of 1e-4, the least that the host lets through, where 2^32 is the largest exponential).  fp32, whose m c
+// may overflow: the difference, which is 0 for m, and its multiple.
 template <typename T>
 struct Exponent {
   float c, ref, b;
@@ -819,14 +820,14 @@ __global__ __launch_bounds__(NT * kRowsOf<NT>, WAVES) void distillation_kernel(c
     float most = -INFINITY, sum = 0.f;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      log_q[i] = entry[i] >= 0 && entry[i] < vocab ? log_q[i] * inv_tau : -INFINITY;
+      if (entry[i] < 0 || entry[i] >= vocab) log_q[i] = -INFINITY;
       most = fmaxf(most, log_q[i]);
     }
     most = wave_max(most);
     if (most == -INFINITY) most = 0.f;  // no entry: q = 0
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      log_q[i] -= most;
+      log_q[i] = (log_q[i] - most) * inv_tau;  // in this order: finite, however small tau is
       q[i] = expf(log_q[i]);
       sum += q[i];
     }

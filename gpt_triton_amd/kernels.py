@@ -307,10 +307,10 @@ def _logit_rows(logits, what):
     V = logits.shape[-1]
     assert V > 0 and (V == 1 or logits.stride(-1) == 1), "the logits of a row must lie side by side"
     rows = logits.numel() // V
+    if rows <= 1:  # whatever its pitch is
+        return dev, code, rows, V, V
     if logits.dim() == 2:
         return dev, code, rows, V, logits.stride(0)
-    if logits.dim() == 1 or rows <= 1:
-        return dev, code, rows, V, V
     try:
         return dev, code, rows, V, logits.view(-1, V).stride(0)
     except RuntimeError:
@@ -340,9 +340,11 @@ def _maybe_check_row_tokens(t, V, what):
         raise IndexError(f"{what}: token id {int(t.max())}, but a row has {V} logits")
 
 
-def _check_temperature(temperature, what):
-    if not 1e-30 <= temperature <= 1e30:
-        raise ValueError(f"{what}: temperature {temperature} is not between 1e-30 and 1e30")
+def _check_temperature(temperature, code, what):
+    # the kernels' fp16 exponents are off by what fp32 rounds off the largest logit over the temperature
+    least = 1e-4 if code == _lib.GPTMI_F16 else 1e-30
+    if not least <= temperature <= 1e30:
+        raise ValueError(f"{what}: temperature {temperature} is not between {least} and 1e30")
 
 
 def _token_log_probs(logits, tokens, top, temperature):
@@ -355,7 +357,7 @@ def _token_log_probs(logits, tokens, top, temperature):
     assert 0 <= top <= V, (top, V)
     if top > MAX_TOP:
         raise NotImplementedError(f"token_log_probs: at most {MAX_TOP} top tokens, got {top}")
-    _check_temperature(temperature, "token_log_probs")
+    _check_temperature(temperature, code, "token_log_probs")
     entropy = logits.new_empty(lead, dtype=torch.float32)
     log_probs = None if tokens is None else torch.empty_like(entropy)
     top_log_probs = top_tokens = None
@@ -427,7 +429,7 @@ def token_log_probs(logits, tokens=None, top=0, temperature=1.0):
         top_tokens     [.., top]  ids, at most MAX_TOP; None for top = 0
 
     fp32 (the tokens int64) whatever the logits' type.  Logits of -infinity mark tokens that cannot occur.  Gradients flow
-    to the logits from all but top_tokens."""
+    to the logits from all but top_tokens.  temperature from 1e-4 on (fp32 logits: 1e-30) to 1e30."""
     temperature = float(temperature)
     if logits.requires_grad and torch.is_grad_enabled():
         return TokenLogProbs(*_TokenLogProbsFunction.apply(logits, tokens, top, temperature))
@@ -453,7 +455,7 @@ def _distillation(logits, teacher_tokens, teacher_logits, temperature, weights, 
             raise TypeError(f"{what}: weights must be float32, got {weights.dtype}")
         assert weights.shape == lead, (weights.shape, lead)
         assert weights.is_contiguous()
-    _check_temperature(temperature, what)
+    _check_temperature(temperature, code, what)
     out = logits.new_empty(lead, dtype=torch.float32) if losses else None
     grad, pitch = _logit_gradient(logits, rows, V, ld) if gradient else (None, V)
     d_at, d_pitch, d_losses = _row_gradient(d_losses)
@@ -492,7 +494,7 @@ def distillation_loss(logits, teacher_tokens, teacher_logits, temperature=1.0, w
 
     k up to MAX_TOP.  An entry whose token is outside [0, V) or whose logit is -infinity counts for nothing.  weights [..]
     (float32, all 1 if None): 0 marks padding, whose logits may be anything.  Gradients flow to the logits alone, which
-    are read again for them; `distillation_loss_and_grad` has both in one pass."""
+    are read again for them; `distillation_loss_and_grad` has both in one pass.  temperature as in `token_log_probs`."""
     _constants(teacher_logits, weights)
     temperature = float(temperature)
     if logits.requires_grad and torch.is_grad_enabled():
@@ -656,8 +658,8 @@ def flash_attention_packed(q, k, v, starts, scale=None, out=None):
 
     fp16 (fp32 storage would round q, k and v to it).  A head's d elements lie side by side; rows and heads may be
     views of something larger at 16-byte aligned pitches, such as the columns of a q, k, v product.  Rows that belong to no
-    sequence are not read, and of `out` (dense, apart from k and v; allocated if None) not written.  A forward pass only,
-    like `flash_attention_v1`."""
+    sequence are not read, and of `out` not written (dense, allocated if None; a dense q itself may be it, and it may overlap
+    nothing else).  A forward pass only, like `flash_attention_v1`."""
     assert q.dim() == k.dim() == 3 and k.shape == v.shape, (q.shape, k.shape, v.shape)
     T, N, d = q.shape
     G = k.shape[1]

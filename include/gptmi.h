@@ -137,8 +137,8 @@ int gptmi_softmax(const void* x, void* out, int64_t M, int64_t H, int dtype,
 
 /*
  * Scores of M rows of logits [V] at a pitch of ld elements (the padded rows of an LM head, a dense matrix, any
- * alignment that the element type allows), z = logits / temperature (from 1e-30
- * on), p = softmax(z) with fp32 maximum and sums:
+ * alignment that the element type allows), z = logits / temperature (from 1e-4 on
+ * for fp16 logits, 1e-30 for fp32, to 1e30), p = softmax(z) with fp32 maximum and sums:
  *   log_probs[m] = log p[tokens[m]]        a token outside [0, V) (padding) reads no memory and scores 0
  *   entropy[m]   = -sum p log p
  *   top_tokens[m][0 .. top): the tokens with the largest logits, largest first, equal ones in the order of their ids
@@ -344,7 +344,7 @@ int gptmi_flash_attn(const void* q, const void* k, const void* v, void* out,
  *   last sequence are not read and not written.  (Starts that break these rules reach no row outside [0, T).)
  * fp16 storage; scores, softmax and sums are fp32, the weights are rounded to fp16 for the product with v (they lie in a
  * result of that type).  What hidden keys and values hold, infinities and NaN included, plays no part.  scale from 1e-20
- * to 1e20; out may not overlap k or v.
+ * to 1e20; out may be q itself where that is dense, and overlap nothing else that is read.
  * Extends flash_attention_v1 -> kernels.py:477-525, which takes one length and as many key heads as heads.
  */
 int gptmi_flash_attn_packed(const void* q, const void* k, const void* v, void* out,

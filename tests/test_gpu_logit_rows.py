@@ -348,6 +348,26 @@ def test_distillation_entries_that_count_for_nothing(K, gpu_device):
         assert loss[2] == 0 and loss[3] == 0 and torch.all(grad[2:] == 0)
 
 
+def test_the_least_temperature(K, gpu_device):
+    """Differences of logits that are infinite when divided: all probability on the largest, and nothing that is no number.
+    fp16 logits, whose exponents are off by a rounding of 60000 log2(e) / tau, have a larger least: the one probability is
+    e / (e + 0) there, a quotient of two roundings, 1 / tau of it a gradient."""
+    for dtype, tau in ((torch.float32, 1e-30), (torch.float16, 1e-4)):
+        x = torch.zeros(2, 600, dtype=dtype, device=gpu_device)
+        x[:, 7], x[:, 9] = 60000.0, -60000.0
+        ids = torch.tensor([[9, 7, 11]] * 2, device=gpu_device)
+        teacher = torch.tensor([[0.0, 1e30, -1e30], [-3e38, 3e38, 0.0]], device=gpu_device)
+        loss, grad = K.distillation_loss_and_grad(x, ids, teacher, tau)
+        assert torch.all(loss == 0) and torch.all(grad.abs() <= (0 if dtype == torch.float32 else 4 * U / tau))
+        s = K.token_log_probs(x, torch.tensor([7, 7], device=gpu_device), top=1, temperature=tau)
+        assert torch.all(s.log_probs == 0) and torch.all(s.entropy == 0) and torch.all(s.top_tokens == 7)
+        for call in (lambda t: K.token_log_probs(x, temperature=t), lambda t: K.distillation_loss(x, ids, teacher, t)):
+            with pytest.raises(ValueError):
+                call(0.99 * tau)
+            with pytest.raises(ValueError):
+                call(1.1e30)
+
+
 def test_a_teacher_that_is_the_student(K, gpu_device):
     """Scores of the whole vocabulary as the teacher: the divergence is 0 and so is the gradient, up to roundings."""
     V = 128
@@ -451,6 +471,8 @@ def test_shapes_and_views(K, gpu_device):
         assert s.log_probs.shape == empty.shape[:-1] and s.top_tokens.shape == (*empty.shape[:-1], 2)
         loss, grad = K.distillation_loss_and_grad(empty, s.top_tokens, s.top_log_probs)
         assert loss.shape == empty.shape[:-1] and grad.shape == empty.shape
+    column = wide[3, :V].clone().view(V, 1).t()  # a single row, whose pitch says nothing
+    assert torch.equal(K.token_log_probs(column, torch.tensor([3], device=gpu_device)).log_probs[0], flat.log_probs[3])
     with pytest.raises(AssertionError):
         K.token_log_probs(wide.view(4, 6, 768)[:, :3, :V])  # rows at two pitches
     with pytest.raises(AssertionError):
