@@ -155,7 +155,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
     slot = at - nth * a.slots;
     head = ((id & 7) + 8 * (nth / rep)) * rep + nth % rep;
   }
-  const Block block = a.longest_first ? nth_longest<R>(a, slot) : find_block<R>(a, a.slots - 1 - slot);
+  const Block block = a.longest_first && a.sequences > 1 ? nth_longest<R>(a, slot) : find_block<R>(a, a.slots - 1 - slot);
   if (block.length == 0) return;
   const int L = block.length, q0 = block.block * R;
   const int qw0 = q0 + wave * 16 * QB;
@@ -460,11 +460,13 @@ int launch_as(PackedArgs a, int64_t slots, hipStream_t st) {
     attr_done = true;
   }
   a.slots = (int)slots;
-  // Up to 10 workgroups a CU the heaviest first: whichever starts last ends the launch.  Beyond, a head's blocks one behind
-  // the other, whose K and V then come from one XCD's L2.  us, by slots / heaviest first: 2 x 8192 rows of 12 heads (1560
-  // workgroups) 252 / 230, 16 x 1024 (1728) 48.7 / 40.8, 40 x 512 (2400) 39.3 / 38.4, 200 x 64 (3600) 21.1 / 23.4, 8 x
-  // 4096 of 16 (4224) 329 / 338; d = 256, 4 x 1024 of 12 (432) 108 / 69.
-  a.longest_first = a.sequences > 1 && a.sequences <= kMany * kWave && slots <= 512 && blocks <= 2560;
+  // Up to 20 workgroups a CU the heaviest of all heads first: whichever starts last ends the launch.  Beyond, and where there
+  // is hardly more than a block a sequence, a head's blocks one behind the other, whose K and V then come from one XCD's L2.
+  // us, by slots / heaviest first: 2 x 8192 rows of 12 heads (1560 workgroups) 268 / 236, 16 x 1024 (1728) 51.4 / 42.3, 8 x 4096 of
+  // 16 (4224) 349 / 336, 100 of up to 2048 (6064) 151 / 158, 64 x 1024 of 25 (14400) 337 / 441, 200 x 64 of 12 (3600) 22.0 /
+  // 23.6, 1 x 4096 (780) 62.6 / 58.3, 1 x 16384 of 25 (3225) 992 / 999; d = 128, 32 heads over 8, 6 of up to 4096 (3360) 394 /
+  // 375, 32 of up to 2048 (3680) 169 / 153, 16 x 1024 (4608) 211 / 202; d = 256, 4 x 1024 of 12 (432) 108 / 69.
+  a.longest_first = a.sequences <= kMany * kWave && slots <= 512 && blocks <= 5120 && a.rows >= 128ll * a.sequences;
   hipLaunchKernelGGL((packed_attn_kernel<D, QB>), dim3((unsigned)blocks), dim3(256), lds, st, a);
   return 0;
 }
