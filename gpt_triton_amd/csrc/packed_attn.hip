@@ -139,21 +139,32 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
   const unsigned smem_base = (unsigned)(uintptr_t)smem;
 
   // ids that are equal modulo 8 run on one XCD, whose L2 then holds the K and V of its heads; the heads of up to 7 key
-  // heads beyond a multiple of 8 are dealt to all, first, for they have no such order.  Late blocks, which have the most keys,
-  // come first.
+  // heads beyond a multiple of 8, untied, are dealt to all.  Either an XCD's heads one behind the other (the untied ones first), late
+  // blocks, which have the most keys, in front, or the late blocks of all its heads in front, eight slots at a time.
   const int id = (int)blockIdx.x, rep = a.heads / a.kv_heads, untied = (a.kv_heads & 7) * rep;
   int head, slot;
-  if (a.longest_first) {  // a key head's heads 8 ids apart where that can be
-    slot = id / a.heads;
-    const int at = id - slot * a.heads, nth = at / a.kv_heads;
-    head = (at - nth * a.kv_heads) * rep + nth;
+  const auto tied_head = [&](int nth) { return ((id & 7) + 8 * (nth / rep)) * rep + nth % rep; };
+  if (a.longest_first) {
+    // eight slots are a.heads rows of 8 ids, in the order of their slots: `untied` of them, spread among the others, for the untied heads
+    const int eight = id / (8 * a.heads), row = (id - eight * 8 * a.heads) >> 3, tied = a.heads - untied;
+    const int u = row * untied / a.heads, t = row - u;  // rows of either kind in front
+    if ((row + 1) * untied / a.heads > u) {
+      slot = (8 * u + (id & 7)) / untied;
+      const int at = 8 * u + (id & 7) - slot * untied, few = a.kv_heads & 7, nth = at / few;
+      head = tied + (at - nth * few) * rep + nth;  // 1, 2 or 4 key heads each have XCDs of their own
+    } else {
+      slot = t / (tied >> 3);
+      head = tied_head(t - slot * (tied >> 3));
+    }
+    slot += 8 * eight;
+    if (slot >= a.slots) return;
   } else if (id < a.slots * untied) {
     slot = id / untied;
     head = a.heads - untied + (id - slot * untied);
   } else {
     const int at = (id - a.slots * untied) >> 3, nth = at / a.slots;
     slot = at - nth * a.slots;
-    head = ((id & 7) + 8 * (nth / rep)) * rep + nth % rep;
+    head = tied_head(nth);
   }
   const Block block = a.longest_first && a.sequences > 1 ? nth_longest<R>(a, slot) : find_block<R>(a, a.slots - 1 - slot);
   if (block.length == 0) return;
@@ -464,10 +475,12 @@ int launch_as(PackedArgs a, int64_t slots, hipStream_t st) {
   // is hardly more than a block a sequence, a head's blocks one behind the other, whose K and V then come from one XCD's L2.
   // us, by slots / heaviest first: 2 x 8192 rows of 12 heads (1560 workgroups) 268 / 236, 16 x 1024 (1728) 51.4 / 42.3, 8 x 4096 of
   // 16 (4224) 349 / 336, 100 of up to 2048 (6064) 151 / 158, 64 x 1024 of 25 (14400) 337 / 441, 200 x 64 of 12 (3600) 22.0 /
-  // 23.6, 1 x 4096 (780) 62.6 / 58.3, 1 x 16384 of 25 (3225) 992 / 999; d = 128, 32 heads over 8, 6 of up to 4096 (3360) 394 /
+  // 23.6, 1 x 4096 (780) 62.6 / 58.3, 1 x 16384 of 25 (3225)
+  // 992 / 926 (980 with the heads dealt to all XCDs, from where 3.0 GB a launch then came to their L2s, ten times K and V); d = 128, 32 heads over 8, 6 of up to 4096 (3360) 394 /
   // 375, 32 of up to 2048 (3680) 169 / 153, 16 x 1024 (4608) 211 / 202; d = 256, 4 x 1024 of 12 (432) 108 / 69.
   a.longest_first = a.sequences <= kMany * kWave && slots <= 512 && blocks <= 5120 && a.rows >= 128ll * a.sequences;
-  hipLaunchKernelGGL((packed_attn_kernel<D, QB>), dim3((unsigned)blocks), dim3(256), lds, st, a);
+  const int64_t grid = a.longest_first ? (slots + 7) / 8 * 8 * a.heads : blocks;
+  hipLaunchKernelGGL((packed_attn_kernel<D, QB>), dim3((unsigned)grid), dim3(256), lds, st, a);
   return 0;
 }
 
