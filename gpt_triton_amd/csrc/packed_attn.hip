@@ -476,7 +476,7 @@ int launch_as(PackedArgs a, int64_t slots, hipStream_t st) {
   // us, by slots / heaviest first: 2 x 8192 rows of 12 heads (1560 workgroups) 268 / 236, 16 x 1024 (1728) 51.4 / 42.3, 8 x 4096 of
   // 16 (4224) 349 / 336, 100 of up to 2048 (6064) 151 / 158, 64 x 1024 of 25 (14400) 337 / 441, 200 x 64 of 12 (3600) 22.0 /
   // 23.6, 1 x 4096 (780) 62.6 / 58.3, 1 x 16384 of 25 (3225)
-  // 992 / 926 (980 with the heads dealt to all XCDs, from where 3.0 GB a launch then came to their L2s, ten times K and V); d = 128, 32 heads over 8, 6 of up to 4096 (3360) 394 /
+  // 992 / 926 (980 with the heads dealt to all XCDs, whose L2s then ask for seven times as much); d = 128, 32 heads over 8, 6 of up to 4096 (3360) 394 /
   // 375, 32 of up to 2048 (3680) 169 / 153, 16 x 1024 (4608) 211 / 202; d = 256, 4 x 1024 of 12 (432) 108 / 69.
   a.longest_first = a.sequences <= kMany * kWave && slots <= 512 && blocks <= 5120 && a.rows >= 128ll * a.sequences;
   const int64_t grid = a.longest_first ? (slots + 7) / 8 * 8 * a.heads : blocks;

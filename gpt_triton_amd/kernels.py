@@ -14,7 +14,10 @@ kernel, the fusion the reference's author notes as a TODO, kernels.py:132-133), 
 `lm_head(x, wte)` (the transposed-weight product the reference leaves as a TODO,
 gpt.py:159-161) and `pack_weight(weight)`: the GEMM reads its weight as an fp16,
 K-contiguous image, which `fused_ffn` / `matmul_and_split_qkv` otherwise rebuild on every call
-where the kernels cannot read the weight in place (fp16, K a multiple of 64); a `PackedWeight` may be passed wherever they take `weight`.  Tensors must live on the
+where the kernels cannot read the weight in place (fp16, K a multiple of 64); a `PackedWeight` may be passed wherever they take `weight`.
+For scoring texts and learning from the scores, which the reference has nothing for: `flash_attention_packed` (prompts of different
+lengths without padding, grouped heads), `token_log_probs` (of rows of logits, with entropy, alternatives and gradient) and
+`distillation_loss` / `distillation_loss_and_grad` (against a teacher's top logits).  Tensors must live on the
 GPU: there is no CPU path.  dropout_prob > 0 reproduces the reference's masks: Philox-4x32-10
 (Triton's tl.rand) with the kernels' default seed 1337 and the reference's offsets -- the column
 for the embedding, the flat index m*N + n for fused_ffn, query*Lk + key for the attention
