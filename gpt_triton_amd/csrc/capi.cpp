@@ -467,7 +467,8 @@ int gptmi_softmax(const void* x, void* out, int64_t M, int64_t H, int dtype, voi
 // What the operators on rows of logits ask of them.
 static int check_logits(const char* what, const void* x, int64_t ld, float temperature, int64_t M, int64_t V,
                         int dtype) {
-  if (!x || M <= 0 || V <= 0 || ld < 0 || !dtype_ok(dtype) || !(temperature >= (dtype == GPTMI_F16 ? 1e-4f : 1e-30f) && temperature <= 1e30f) ||
+  const float least = dtype == GPTMI_F16 ? 1e-4f : 1e-30f;
+  if (!x || M <= 0 || V <= 0 || ld < 0 || !dtype_ok(dtype) || !(temperature >= least && temperature <= 1e30f) ||
       ((uintptr_t)x & (dtype == GPTMI_F16 ? 1 : 3)) != 0) {
     set_error("%s: invalid argument", what);
     return GPTMI_ERR_INVALID;
@@ -517,8 +518,9 @@ int gptmi_token_log_probs(const void* logits, int64_t ld, const int64_t* tokens,
 
 int gptmi_token_log_probs_backward(const void* logits, int64_t ld, const int64_t* tokens, float temperature,
                                    const float* d_log_probs, int64_t d_pitch, const float* d_entropy,
-                                   int64_t d_entropy_pitch, int64_t top, const int64_t* top_tokens, const float* d_top_log_probs, void* grad,
-                                   int64_t ld_grad, int64_t M, int64_t V, int dtype, void* stream) {
+                                   int64_t d_entropy_pitch, int64_t top, const int64_t* top_tokens,
+                                   const float* d_top_log_probs, void* grad, int64_t ld_grad, int64_t M, int64_t V,
+                                   int dtype, void* stream) {
   int rc = check_logits("token_log_probs_backward", logits, ld, temperature, M, V, dtype);
   if (!rc) rc = check_logits_gradient("token_log_probs_backward", grad, ld_grad, M, V, dtype);
   if (rc) return rc;
@@ -532,13 +534,15 @@ int gptmi_token_log_probs_backward(const void* logits, int64_t ld, const int64_t
     return GPTMI_ERR_UNSUPPORTED;
   }
   launch_token_log_probs_backward(logit_rows(logits, ld, temperature, M, V, dtype), tokens,
-                                  RowGradient{d_log_probs, (int)d_pitch}, RowGradient{d_entropy, (int)d_entropy_pitch}, (int)top, top_tokens, d_top_log_probs, grad, ld_grad, (hipStream_t)stream);
+                                  RowGradient{d_log_probs, (int)d_pitch}, RowGradient{d_entropy, (int)d_entropy_pitch},
+                                  (int)top, top_tokens, d_top_log_probs, grad, ld_grad, (hipStream_t)stream);
   return check_launch("token_log_probs_backward");
 }
 
 int gptmi_distillation_loss(const void* logits, int64_t ld, const int64_t* teacher_tokens, const void* teacher_logits,
                             int64_t k, float temperature, const float* weights, const float* d_losses, int64_t d_pitch,
-                            float* losses, void* grad, int64_t ld_grad, int64_t M, int64_t V, int dtype, int teacher_dtype, void* stream) {
+                            float* losses, void* grad, int64_t ld_grad, int64_t M, int64_t V, int dtype,
+                            int teacher_dtype, void* stream) {
   int rc = check_logits("distillation_loss", logits, ld, temperature, M, V, dtype);
   if (!rc && grad) rc = check_logits_gradient("distillation_loss", grad, ld_grad, M, V, dtype);
   if (rc) return rc;
@@ -552,7 +556,8 @@ int gptmi_distillation_loss(const void* logits, int64_t ld, const int64_t* teach
     return GPTMI_ERR_UNSUPPORTED;
   }
   launch_distillation(logit_rows(logits, ld, temperature, M, V, dtype), teacher_tokens, teacher_logits,
-                      teacher_dtype == GPTMI_F16, (int)k, weights, RowGradient{d_losses, (int)d_pitch}, losses, grad, ld_grad, (hipStream_t)stream);
+                      teacher_dtype == GPTMI_F16, (int)k, weights, RowGradient{d_losses, (int)d_pitch}, losses, grad,
+                      ld_grad, (hipStream_t)stream);
   return check_launch("distillation_loss");
 }
 

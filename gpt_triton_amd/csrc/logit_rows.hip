@@ -132,6 +132,13 @@ __device__ __forceinline__ int row_in_group() {
   return NT == kWave ? __builtin_amdgcn_readfirstlane((int)threadIdx.y) : 0;
 }
 
+// 2^20 workgroups a row of the grid: threads of one dimension have to stay below 2^32.
+constexpr int kGridRow = 1 << 20;
+template <int NT>
+__device__ __forceinline__ int64_t row_of_group(int in_group) {
+  return ((int64_t)blockIdx.y * kGridRow + blockIdx.x) * kRowsOf<NT> + in_group;
+}
+
 template <int NT>
 struct Shared {
   static constexpr int W = NT / kWave;
@@ -591,14 +598,13 @@ __device__ __forceinline__ void row_top(const Row<T, NT, CH, OPEN>& row, int k, 
 }
 
 template <typename T, bool TOP, int NT, int CH, bool OPEN, int WAVES>
-__global__ __launch_bounds__(NT * kRowsOf<NT>, WAVES) void token_log_probs_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int vocab,
-                                                             const int64_t* __restrict__ tokens, float tau, int k,
-                                                             float* __restrict__ log_probs, float* __restrict__ entropy,
-                                                             float* __restrict__ top_log_probs,
-                                                             int64_t* __restrict__ top_tokens) {
+__global__ __launch_bounds__(NT * kRowsOf<NT>, WAVES) void token_log_probs_kernel(
+    const T* __restrict__ x, int64_t ld, int64_t rows, int vocab, const int64_t* __restrict__ tokens, float tau, int k,
+    float* __restrict__ log_probs, float* __restrict__ entropy, float* __restrict__ top_log_probs,
+    int64_t* __restrict__ top_tokens) {
   __shared__ Shared<NT> sh_of[kRowsOf<NT>];
   const int in_group = row_in_group<NT>();
-  const int64_t r = (int64_t)blockIdx.x * kRowsOf<NT> + in_group;
+  const int64_t r = row_of_group<NT>(in_group);
   if (r >= rows) return;
   Shared<NT>& sh = sh_of[in_group];
   Row<T, NT, CH, OPEN> row(x + r * ld, vocab);
@@ -709,11 +715,12 @@ __device__ __forceinline__ void write_zeros(T* __restrict__ out, int vocab) {
 template <typename T, int NT, int CH, bool OPEN, int WAVES>
 __global__ __launch_bounds__(NT * kRowsOf<NT>, WAVES) void token_log_probs_backward_kernel(
     const T* __restrict__ x, int64_t ld, int64_t rows, int vocab, const int64_t* __restrict__ tokens, float tau,
-    RowGradient d_log_probs, RowGradient d_entropy, int k, const int64_t* __restrict__ top_tokens, const float* __restrict__ d_top, T* __restrict__ out, int64_t ld_out) {
+    RowGradient d_log_probs, RowGradient d_entropy, int k, const int64_t* __restrict__ top_tokens,
+    const float* __restrict__ d_top, T* __restrict__ out, int64_t ld_out) {
   __shared__ Shared<NT> sh_of[kRowsOf<NT>];
   __shared__ Special<NT> sp_of[kRowsOf<NT>];
   const int in_group = row_in_group<NT>();
-  const int64_t r = (int64_t)blockIdx.x * kRowsOf<NT> + in_group;
+  const int64_t r = row_of_group<NT>(in_group);
   if (r >= rows) return;
   Shared<NT>& sh = sh_of[in_group];
   Special<NT>& sp = sp_of[in_group];
@@ -769,16 +776,15 @@ struct Entries {
 // q = softmax(teacher / tau) over the row's entries (an id outside the vocabulary is no entry), loss = w sum q (log q -
 // log p); gradient w / tau (p_j - sum of q over the entries of token j).
 template <typename T, bool GRAD, int NT, int CH, bool OPEN, int WAVES>
-__global__ __launch_bounds__(NT * kRowsOf<NT>, WAVES) void distillation_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int vocab,
-                                                          const int64_t* __restrict__ teacher_tokens,
-                                                          const void* __restrict__ teacher, int teacher_f16, int k, float tau,
-                                                          const float* __restrict__ weights, RowGradient d_losses, float* __restrict__ losses,
-                                                          T* __restrict__ out, int64_t ld_out) {
+__global__ __launch_bounds__(NT * kRowsOf<NT>, WAVES) void distillation_kernel(
+    const T* __restrict__ x, int64_t ld, int64_t rows, int vocab, const int64_t* __restrict__ teacher_tokens,
+    const void* __restrict__ teacher, int teacher_f16, int k, float tau, const float* __restrict__ weights,
+    RowGradient d_losses, float* __restrict__ losses, T* __restrict__ out, int64_t ld_out) {
   __shared__ Shared<NT> sh_of[kRowsOf<NT>];
   __shared__ Special<NT> sp_of[kRowsOf<NT>];
   __shared__ Entries entries_of[kRowsOf<NT>];
   const int in_group = row_in_group<NT>();
-  const int64_t r = (int64_t)blockIdx.x * kRowsOf<NT> + in_group;
+  const int64_t r = row_of_group<NT>(in_group);
   if (r >= rows) return;
   Shared<NT>& sh = sh_of[in_group];
   Special<NT>& sp = sp_of[in_group];
@@ -900,7 +906,10 @@ void pick_row(const LogitRows& a, int min_threads, F f) {
 }
 
 template <int NT>
-dim3 grid_of(const LogitRows& a) { return dim3((unsigned)((a.rows + kRowsOf<NT> - 1) / kRowsOf<NT>)); }
+dim3 grid_of(const LogitRows& a) {
+  const int64_t n = (a.rows + kRowsOf<NT> - 1) / kRowsOf<NT>;
+  return dim3((unsigned)(n < kGridRow ? n : kGridRow), (unsigned)((n + kGridRow - 1) / kGridRow));
+}
 template <int NT>
 dim3 block_of() { return dim3(NT, kRowsOf<NT>); }
 

@@ -17,6 +17,7 @@ namespace gptmi {
 namespace {
 
 constexpr int kKeys = 64;  // keys a tile
+constexpr int kGridRow = 1 << 20;  // workgroups a row of the grid: threads of one dimension have to stay below 2^32
 
 struct PackedArgs {
   const _Float16 *q, *k, *v;
@@ -123,9 +124,10 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
   constexpr int RPI = 1024 / ROWB;     // rows that a load instruction covers
   constexpr int TILE = kKeys * ROWB;   // bytes of a K (or V) tile
   constexpr int NDMA = D / 16;         // load instructions a wavefront and tile
-  // Unit u of K's row r lies at u ^ k_key(r), of V's at u ^ v_key(r).  A read of K takes one unit of rows 8 i + 0..3 (+ 4 b), i =
-  // 0..3, a transposing read of V two units of rows 8 g + 0..3, two g at a time: the keys put these into different banks.
-  // Neither depends on bit 2 or 5 of the row, and both are made of its bits by or, so a sum of rows has the keys' xor.
+  // Unit u of K's row r lies at u ^ k_key(r), of V's at u ^ v_key(r).  A read of K takes one unit of rows 8 i + 0..3
+  // (+ 4 b), i = 0..3, a transposing read of V two units of rows 8 g + 0..3, two g at a time: the keys put these into
+  // different banks. Neither depends on bit 2 or 5 of the row, and both are made of its bits by or, so a sum of rows
+  // has the keys' xor.
   const auto k_key = [](int r) {
     return CH >= 16 ? (r & 3) | (r >> 3 & 3) << 2 : CH == 8 ? (r >> 1 & 1) | (r >> 3 & 3) << 1 : (r >> 3 & 3) & (CH - 1);
   };
@@ -138,14 +140,16 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
   const int c = lane & 15, g = lane >> 4;
   const unsigned smem_base = (unsigned)(uintptr_t)smem;
 
-  // ids that are equal modulo 8 run on one XCD, whose L2 then holds the K and V of its heads; the heads of up to 7 key
-  // heads beyond a multiple of 8, untied, are dealt to all.  Either an XCD's heads one behind the other (the untied ones first), late
-  // blocks, which have the most keys, in front, or the late blocks of all its heads in front, eight slots at a time.
-  const int id = (int)blockIdx.x, rep = a.heads / a.kv_heads, untied = (a.kv_heads & 7) * rep;
+  // ids that are equal modulo 8 run on one XCD, whose L2 then holds the K and V of its heads; the heads of up to 7
+  // key heads beyond a multiple of 8, untied, are dealt to all.  Either an XCD's heads one behind the other (the
+  // untied ones first), late blocks, which have the most keys, in front, or the late blocks of all its heads in
+  // front, eight slots at a time.
+  const int id = (int)(blockIdx.y * kGridRow + blockIdx.x), rep = a.heads / a.kv_heads, untied = (a.kv_heads & 7) * rep;
   int head, slot;
   const auto tied_head = [&](int nth) { return ((id & 7) + 8 * (nth / rep)) * rep + nth % rep; };
   if (a.longest_first) {
-    // eight slots are a.heads rows of 8 ids, in the order of their slots: `untied` of them, spread among the others, for the untied heads
+    // eight slots are a.heads rows of 8 ids, in the order of their slots: `untied` of them, spread among the others,
+    // for the untied heads
     const int eight = id / (8 * a.heads), row = (id - eight * 8 * a.heads) >> 3, tied = a.heads - untied;
     const int u = row * untied / a.heads, t = row - u;  // rows of either kind in front
     if ((row + 1) * untied / a.heads > u) {
@@ -158,6 +162,8 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
     }
     slot += 8 * eight;
     if (slot >= a.slots) return;
+  } else if (id >= a.slots * a.heads) {
+    return;
   } else if (id < a.slots * untied) {
     slot = id / untied;
     head = a.heads - untied + (id - slot * untied);
@@ -237,14 +243,14 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
   for (int n = 0; n < QB; ++n)
 #pragma unroll
     for (int i = 0; i < DB; ++i) oacc[n][i] = f4(0.f);
-  // The weights are 2^(t s - base), t = scale log2(e), base = t ref - 6 as rounded, for a reference that the running maximum
-  // may pass by 2^8 before it follows: the accumulator is rescaled in few tiles (by what the bases as rounded differ by, so
-  // that tiles of different references agree), a weight is at most 2^14, and one is a subnormal fp16 number, which has fewer
-  // bits, below 2^-20 of the reference.  The denominator adds the weights in fp32, in the four lanes of a query and across
-  // them at the end.  (us, this / dot products of the rounded pairs with ones, which flush subnormal weights / a column of ones
-  // in the matrix product, which costs registers: 48 of up to 1024 rows 23.2 / 23.1 / 26.0, 1 x 16384 995 / 988 / 1003.)
-  // The key that set the reference weighs 2^6, so a denominator below 2^5 is one whose base was rounded by more than the weights
-  // reach, which the end looks for.
+  // The weights are 2^(t s - base), t = scale log2(e), base = t ref - 6 as rounded, for a reference that the running
+  // maximum may pass by 2^8 before it follows: the accumulator is rescaled in few tiles (by what the bases as rounded
+  // differ by, so that tiles of different references agree), a weight is at most 2^14, and one is a subnormal fp16
+  // number, which has fewer bits, below 2^-20 of the reference.  The denominator adds the weights in fp32, in the
+  // four lanes of a query and across them at the end.  (us, this / dot products of the rounded pairs with ones, which
+  // flush subnormal weights / a column of ones in the matrix product, which costs registers: 48 of up to 1024 rows
+  // 23.2 / 23.1 / 26.0, 1 x 16384 995 / 988 / 1003.) The key that set the reference weighs 2^6, so a denominator
+  // below 2^5 is one whose base was rounded by more than the weights reach, which the end looks for.
   float ref[QB], limit[QB], base[QB], den[QB];
 #pragma unroll
   for (int n = 0; n < QB; ++n) ref[n] = limit[n] = base[n] = -INFINITY, den[n] = 0.f;
@@ -259,7 +265,8 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
     for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        h8 kf = *reinterpret_cast<const h8*>(buf + (kb >> 1) * 32 * ROWB + (kb & 1) * 4 * ROWB + k_off[ks % KV] + (ks / KV) * 256);
+        const int at = (kb >> 1) * 32 * ROWB + (kb & 1) * 4 * ROWB + k_off[ks % KV] + (ks / KV) * 256;
+        h8 kf = *reinterpret_cast<const h8*>(buf + at);
         if (D < 32 && g >= 2) kf = h8(0);
 #pragma unroll
         for (int n = 0; n < QB; ++n)
@@ -454,7 +461,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
 template <int D, int QB>
 int launch_as(PackedArgs a, int64_t slots, hipStream_t st) {
   const int64_t blocks = slots * a.heads;
-  if (blocks >= 1ll << 31) {
+  if (blocks > (1ll << 31) - kGridRow) {
     set_error("flash_attn_packed: %lld rows in %d sequences of %d heads exceed the grid", (long long)a.rows, a.sequences,
               a.heads);
     return -2;
@@ -471,25 +478,28 @@ int launch_as(PackedArgs a, int64_t slots, hipStream_t st) {
     attr_done = true;
   }
   a.slots = (int)slots;
-  // Up to 20 workgroups a CU the heaviest of all heads first: whichever starts last ends the launch.  Beyond, and where there
-  // is hardly more than a block a sequence, a head's blocks one behind the other, whose K and V then come from one XCD's L2.
-  // us, by slots / heaviest first: 2 x 8192 rows of 12 heads (1560 workgroups) 268 / 236, 16 x 1024 (1728) 51.4 / 42.3, 8 x 4096 of
-  // 16 (4224) 349 / 336, 100 of up to 2048 (6064) 151 / 158, 64 x 1024 of 25 (14400) 337 / 441, 200 x 64 of 12 (3600) 22.0 /
-  // 23.6, 1 x 4096 (780) 62.6 / 58.3, 1 x 16384 of 25 (3225)
-  // 992 / 926 (980 with the heads dealt to all XCDs, whose L2s then ask for seven times as much); d = 128, 32 heads over 8, 6 of up to 4096 (3360) 394 /
-  // 375, 32 of up to 2048 (3680) 169 / 153, 16 x 1024 (4608) 211 / 202; d = 256, 4 x 1024 of 12 (432) 108 / 69.
+  // Up to 20 workgroups a CU the heaviest of all heads first: whichever starts last ends the launch.  Beyond, and
+  // where there is hardly more than a block a sequence, a head's blocks one behind the other, whose K and V then come
+  // from one XCD's L2. us, by slots / heaviest first: 2 x 8192 rows of 12 heads (1560 workgroups) 268 / 236, 16 x
+  // 1024 (1728) 51.4 / 42.3, 8 x 4096 of 16 (4224) 349 / 336, 100 of up to 2048 (6064) 151 / 158, 64 x 1024 of 25
+  // (14400) 337 / 441, 200 x 64 of 12 (3600) 22.0 / 23.6, 1 x 4096 (780) 62.6 / 58.3, 1 x 16384 of 25 (3225) 992 /
+  // 926 (980 with the heads dealt to all XCDs, whose L2s then ask for seven times as much); d = 128, 32 heads over 8,
+  // 6 of up to 4096 (3360) 394 / 375, 32 of up to 2048 (3680) 169 / 153, 16 x 1024 (4608) 211 / 202; d = 256, 4 x
+  // 1024 of 12 (432) 108 / 69.
   a.longest_first = a.sequences <= kMany * kWave && slots <= 512 && blocks <= 5120 && a.rows >= 128ll * a.sequences;
   const int64_t grid = a.longest_first ? (slots + 7) / 8 * 8 * a.heads : blocks;
-  hipLaunchKernelGGL((packed_attn_kernel<D, QB>), dim3((unsigned)grid), dim3(256), lds, st, a);
+  const dim3 dims((unsigned)(grid < kGridRow ? grid : kGridRow), (unsigned)((grid + kGridRow - 1) / kGridRow));
+  hipLaunchKernelGGL((packed_attn_kernel<D, QB>), dims, dim3(256), lds, st, a);
   return 0;
 }
 
-// 16 queries a wavefront while the workgroups number at most 5 a CU: they all run at once, and a wavefront's chain through
-// its key tiles, which is then what the launch takes, is shorter (0.5 us a tile for 16 queries, 0.8 for 32).  32 beyond: K and V
-// are read from LDS for more queries at a time.  us, 16 / 32: 1 x 1024 rows of 12 heads (204 workgroups of 64 queries) 14.0 /
-// 18.0, 4 x 1024 (816) 17.3 / 20.1, 16 x 300 (1092) 10.6 / 12.5, 3 x 2048 (1188) 35.1 / 35.7, 48 of up to 1024 (1992) 21.6 /
-// 21.2, 2 x 8192 (3096) 263 / 230; d = 128, 32 heads over 8, 1 x 1024 (544) 24.4 / 28.7, 1 x 8192 (4128) 653 / 520.  64 queries
-// were slower: 1 x 16384 of 25 heads 997, 32 969, 16 1046.  d = 256 has one workgroup a CU either way.
+// 16 queries a wavefront while the workgroups number at most 5 a CU: they all run at once, and a wavefront's chain
+// through its key tiles, which is then what the launch takes, is shorter (0.5 us a tile for 16 queries, 0.8 for 32).
+// 32 beyond: K and V are read from LDS for more queries at a time.  us, 16 / 32, the heaviest first: 1 x 1024 rows of
+// 12 heads (204 workgroups of 64 queries) 16.5 / 18.8, 4 x 1024 (816) 19.3 / 21.4, 16 x 300 (1092) 11.2 / 13.0, 3 x
+// 2048 (1188) 34.0 / 36.6, 48 of up to 1024 (1992) 22.9 / 21.9, 2 x 8192 (3096) 283 / 236; d = 128, 32 heads over 8,
+// 1 x 1024 (544) 22.8 / 28.3, 1 x 8192 (4128) 698 / 535.  64 queries were slower yet: 1 x 16384 of 25 heads 16 / 32 /
+// 64 1046 / 969 / 997 in an earlier state.  d = 256 has one workgroup a CU either way.
 template <int D>
 int launch_d(const PackedArgs& a, hipStream_t st) {
   const int64_t slots = a.rows / 64 + a.sequences;

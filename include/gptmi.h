@@ -137,8 +137,8 @@ int gptmi_softmax(const void* x, void* out, int64_t M, int64_t H, int dtype,
 
 /*
  * Scores of M rows of logits [V] at a pitch of ld elements (the padded rows of an LM head, a dense matrix, any
- * alignment that the element type allows), z = logits / temperature (from 1e-4 on
- * for fp16 logits, 1e-30 for fp32, to 1e30), p = softmax(z) with fp32 maximum and sums:
+ * alignment that the element type allows), z = logits / temperature (from 1e-4 on for fp16 logits, 1e-30 for fp32, to
+ * 1e30), p = softmax(z) with fp32 maximum and sums:
  *   log_probs[m] = log p[tokens[m]]        a token outside [0, V) (padding) reads no memory and scores 0
  *   entropy[m]   = -sum p log p
  *   top_tokens[m][0 .. top): the tokens with the largest logits, largest first, equal ones in the order of their ids
@@ -163,27 +163,27 @@ int gptmi_token_log_probs(const void* logits, int64_t ld, const int64_t* tokens,
  */
 int gptmi_token_log_probs_backward(const void* logits, int64_t ld, const int64_t* tokens,
                                    float temperature, const float* d_log_probs, int64_t d_pitch,
-                                   const float* d_entropy, int64_t d_entropy_pitch, int64_t top, const int64_t* top_tokens, const float* d_top_log_probs,
-                                   void* grad, int64_t ld_grad, int64_t M, int64_t V, int dtype,
-                                   void* stream);
+                                   const float* d_entropy, int64_t d_entropy_pitch, int64_t top,
+                                   const int64_t* top_tokens, const float* d_top_log_probs, void* grad,
+                                   int64_t ld_grad, int64_t M, int64_t V, int dtype, void* stream);
 
 /*
  * Distillation from a teacher's k top logits a row (1 <= k <= GPTMI_MAX_TOP), teacher_tokens, teacher_logits [M][k]:
  *   q = softmax(teacher_logits / temperature) over the row's entries, p = softmax(logits / temperature) over V
  *   losses[m] = weights[m] sum_i q_i (log q_i - log p[token_i])
  *   grad_j    = d_losses[m * d_pitch] weights[m] / temperature (p_j - sum_i [j = token_i] q_i)
- * in one pass over the logits; d_losses NULL: 1, the gradient of the losses' sum; d_pitch 0: one number for all rows.  Log probabilities serve as teacher_logits too (the softmax takes a constant out).  An
- * entry whose token is outside [0, V) or whose logit is -infinity counts for nothing; a token that is there twice
- * counts twice.  A row without entries, or of weight 0 (padding), has loss 0 and gradient 0 whatever its logits are, and
- * without losses one of d_losses 0 too; a student
- * that gives the teacher's tokens no probability at all has loss +infinity.
+ * in one pass over the logits; d_losses NULL: 1, the gradient of the losses' sum; d_pitch 0: one number for all rows.
+ * Log probabilities serve as teacher_logits too (the softmax takes a constant out).  An entry whose token is outside
+ * [0, V) or whose logit is -infinity counts for nothing; a token that is there twice counts twice.  A row without
+ * entries, or of weight 0 (padding), has loss 0 and gradient 0 whatever its logits are, and where no losses are asked for
+ * a row of d_losses 0 gradient 0 too; a student that gives the teacher's tokens no probability at all has loss +infinity.
  * weights may be NULL (all 1), losses or grad may be NULL; grad as in gptmi_token_log_probs_backward.  teacher_dtype:
  * the type of teacher_logits.
  */
 int gptmi_distillation_loss(const void* logits, int64_t ld, const int64_t* teacher_tokens,
                             const void* teacher_logits, int64_t k, float temperature, const float* weights,
-                            const float* d_losses, int64_t d_pitch, float* losses, void* grad, int64_t ld_grad, int64_t M, int64_t V, int dtype,
-                            int teacher_dtype, void* stream);
+                            const float* d_losses, int64_t d_pitch, float* losses, void* grad, int64_t ld_grad,
+                            int64_t M, int64_t V, int dtype, int teacher_dtype, void* stream);
 
 /*
  * Bytes of workspace gptmi_linear / gptmi_linear_qkv need for these sizes

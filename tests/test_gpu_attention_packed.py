@@ -188,6 +188,13 @@ def test_many_sequences(K, gpu_device, count):
     assert torch.equal(out[rows], v[rows].expand(-1, 2, -1))  # a key alone has all the weight
 
 
+def test_a_million_blocks(K, gpu_device):
+    """More workgroups than a row of the grid has: every token a sequence, which gives its value."""
+    count = 100000
+    q, k, v = make(np.random.default_rng(25), count, 12, 12, 16, False, gpu_device)
+    assert torch.equal(K.flash_attention_packed(q, k, v, torch.arange(count + 1, device=gpu_device)), v)
+
+
 @pytest.mark.parametrize("heads", [3, 200])
 @pytest.mark.parametrize("d", [16, 32, 64, 128, 256])
 def test_hidden_keys_play_no_part(K, gpu_device, d, heads):

@@ -505,6 +505,26 @@ def test_rows_beyond_32_bits(K, gpu_device):
     check_distillation(K, x, np.array([[1, 2], [3, 4], [5, 6]]), torch.zeros(3, 2, device=gpu_device), 1.0, np.ones(3))
 
 
+def test_millions_of_rows(K, gpu_device):
+    """More workgroups than a row of the grid has: one row of logits for all of them, and rows of their own, whose chunks
+    begin elsewhere: sums of another order."""
+    rows, V = 2**22 + 5, 9  # four rows a workgroup
+    x = torch.from_numpy(crowd(np.random.default_rng(24), 1, V)).float().to(gpu_device).expand(rows, V)
+    tokens = torch.arange(rows, device=gpu_device) % V
+    few = x[:V].detach().clone().requires_grad_()
+    one = K.token_log_probs(few, tokens[:V])
+    want, = torch.autograd.grad(one.log_probs.sum(), few, retain_graph=True)
+    tol, d_tol = 2 * sum_error(V) + 40 * U, 100 * U + 2 * sum_error(V)
+    s = K.token_log_probs(x, tokens)
+    assert torch.all((s.log_probs - one.log_probs[tokens]).abs() <= tol)
+    assert torch.all((s.entropy - one.entropy[0]).abs() <= tol + 64 * U * one.entropy[0])
+    loss, grad = K.distillation_loss_and_grad(x, tokens[:, None], torch.zeros(rows, 1, device=gpu_device))
+    assert torch.all((loss + s.log_probs).abs() <= tol) and torch.all((grad + want[tokens]).abs() <= d_tol)
+    leaf = x.contiguous().requires_grad_()
+    back, = torch.autograd.grad(K.token_log_probs(leaf, tokens).log_probs.sum(), leaf)
+    assert torch.all((back - want[tokens]).abs() <= d_tol)
+
+
 def test_streams_and_graphs(K, gpu_device):
     """On a stream of its own and captured: the bits of the eager calls, replay after replay."""
     r = np.random.default_rng(11)
