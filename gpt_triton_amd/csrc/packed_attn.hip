@@ -3,11 +3,12 @@
 // q [T][N][D], k, v [T][G][D] at row and head pitches of their own (the q, k, v product's rows as they are), out [T][N][D],
 // sequence s the rows starts[s] .. starts[s + 1] - 1.
 //
-// One workgroup = 4 wavefronts = 64 QB queries of one sequence and head, QB blocks of 16 for each wavefront.  The
-// products are the transposed ones, S^T = K . Q^T and O^T += V^T . P^T with v_mfma_f32_16x16x32_f16, so that a query's scores
-// and sums are in the four lanes (c, g), c = lane % 16 its number in the block, g = lane / 16.  Rows 4 g + r of K's 16-row
-// blocks b = 0, 1 are keys 8 g + 4 b + r of a group of 32, which makes a lane's weights the second operand of the next
-// product as they stand: keys 8 g .. 8 g + 7.
+// One workgroup = 4 wavefronts = 64 QB queries of one sequence and head, QB blocks of 16 for each wavefront; or, in P = 2
+// parts, half as many, two wavefronts for the key tiles of even number and two for the others, whose sums are joined at the
+// end.  The products are the transposed ones, S^T = K . Q^T and O^T += V^T . P^T with v_mfma_f32_16x16x32_f16, so that a
+// query's scores and sums are in the four lanes (c, g), c = lane % 16 its number in the block, g = lane / 16.  Rows 4 g +
+// r of K's 16-row blocks b = 0, 1 are keys 8 g + 4 b + r of a group of 32, which makes a lane's weights the second operand
+// of the next product as they stand: keys 8 g .. 8 g + 7.
 #include <type_traits>
 
 #include "common.h"
@@ -115,15 +116,16 @@ __device__ __forceinline__ Block nth_longest(const PackedArgs& a, int nth) {
   return {0, 0, 0};
 }
 
-template <int D, int QB>
+template <int D, int QB, int P>
 __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(PackedArgs a) {
-  constexpr int R = 64 * QB;           // queries a workgroup
+  constexpr int R = 64 * QB / P;       // queries a workgroup
   constexpr int KS = (D + 31) / 32, DB = D / 16;
   constexpr int ROWB = D * 2;          // bytes of a row in LDS
   constexpr int CH = D / 8;            // 16-byte units of it
   constexpr int RPI = 1024 / ROWB;     // rows that a load instruction covers
   constexpr int TILE = kKeys * ROWB;   // bytes of a K (or V) tile
-  constexpr int NDMA = D / 16;         // load instructions a wavefront and tile
+  constexpr int ROWS = 32 * P;         // rows of a tile that a wavefront brings
+  constexpr int NDMA = ROWS / RPI;     // in so many load instructions
   // Unit u of K's row r lies at u ^ k_key(r), of V's at u ^ v_key(r).  A read of K takes one unit of rows 8 i + 0..3
   // (+ 4 b), i = 0..3, a transposing read of V two units of rows 8 g + 0..3, two g at a time: the keys put these into
   // different banks. Neither depends on bit 2 or 5 of the row, and both are made of its bits by or, so a sum of rows
@@ -134,7 +136,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
   const auto v_key = [](int r) {
     return 2 * (CH >= 16 ? (r & 3) | (r >> 3 & 1) << 2 : CH == 8 ? (r >> 1 & 1) | (r >> 3 & 1) << 1 : CH == 4 ? r >> 3 & 1 : 0);
   };
-  extern __shared__ __attribute__((aligned(1024))) char smem[];  // K tiles of even and odd number, V tiles
+  extern __shared__ __attribute__((aligned(1024))) char smem[];  // of each part: two places for K tiles, two for V
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, g = lane >> 4;
@@ -175,10 +177,13 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
   const Block block = a.longest_first && a.sequences > 1 ? nth_longest<R>(a, slot) : find_block<R>(a, a.slots - 1 - slot);
   if (block.length == 0) return;
   const int L = block.length, q0 = block.block * R;
-  const int qw0 = q0 + wave * 16 * QB;
+  // part p of P has the key tiles p, p + P, .., perhaps none
+  const int part = P == 1 ? 0 : wave >> 1, in_part = P == 1 ? wave : wave & 1;
+  const int qw0 = q0 + in_part * 16 * QB;
   const bool wave_active = qw0 < L;
   const int last_q = min(q0 + R, L) - 1;
   const int nt = last_q / kKeys + 1;  // key tiles
+  const int own = (nt - part + P - 1) / P;  // of this part
   const int kv_head = head / rep;
   const _Float16* qp = a.q + (block.first * a.q_row + head * a.q_head);
   const _Float16* kp = a.k + (block.first * a.k_row + kv_head * a.k_head);
@@ -197,19 +202,21 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
     }
   }
 
-  // ---- tile loads: wavefronts 0-1 bring K, 2-3 V, 32 rows each.  Load j's rows are RPI j further on, which the scalar
+  // ---- tile loads: wavefronts 0-1 bring K, 2-3 V, 32 rows each; with two parts one wavefront of each K and one V.  Load j's rows are RPI j further on, which the scalar
   // base takes, and their keys differ by bits that are the same for all lanes; a sequence's last tile repeats its last row.
-  const bool brings_v = wave >= 2;
+  const bool brings_v = P == 1 ? wave >= 2 : wave & 1;
+  const int first_row = P == 1 ? (wave & 1) * 32 : 0;
   const int64_t pitch = (brings_v ? a.v_row : a.k_row) * 2;
-  const char* src = (const char*)(brings_v ? vp : kp) + (wave & 1) * 32 * pitch;
+  const char* src = (const char*)(brings_v ? vp : kp) + first_row * pitch;
   const int lrow = lane / CH;
   const unsigned lane_unit = (unsigned)((lane % CH) ^ (brings_v ? v_key(lrow) : k_key(lrow))) << 4;
   const unsigned lane_row = (unsigned)lrow * (unsigned)pitch;
-  auto issue_tile = [&](int t) {
-    const unsigned dst = smem_base + (unsigned)(((brings_v ? 2 : 0) + (t & 1)) * TILE) + (unsigned)((wave & 1) * NDMA) * 1024u;
+  auto issue_tile = [&](int nth) {  // of this part's tiles
+    const int t = nth * P + part;
+    const unsigned dst = smem_base + (unsigned)((part * 4 + (brings_v ? 2 : 0) + (nth & 1)) * TILE) + (unsigned)(first_row * ROWB);
     const char* base = src + (int64_t)t * kKeys * pitch;
-    const int rest = L - 1 - t * kKeys - (wave & 1) * 32;  // the last row of this wavefront's 32
-    if (rest >= 31) {
+    const int rest = L - 1 - t * kKeys - first_row;  // the last row of this wavefront's
+    if (rest >= ROWS - 1) {
 #pragma unroll
       for (int j = 0; j < NDMA; ++j) {
         const unsigned key = (unsigned)(brings_v ? v_key(j * RPI) : k_key(j * RPI));
@@ -217,7 +224,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
         base += RPI * pitch;
       }
     } else {
-      base += (int64_t)min(rest, 0) * pitch;  // of 32 rows behind the end, row 0 is the sequence's last
+      base += (int64_t)min(rest, 0) * pitch;  // of rows behind the end, row 0 is the sequence's last
       const int last = max(rest, 0);
 #pragma unroll
       for (int j = 0; j < NDMA; ++j) {
@@ -346,11 +353,11 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
   auto arrive = [&] { asm volatile("s_waitcnt vmcnt(0)\n\ts_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
   auto request = [&](int k_tile) {  // and the V tile in front of it
     const int t = brings_v ? k_tile - 1 : k_tile;
-    if (t < nt) issue_tile(t);
+    if (t < own) issue_tile(t);
   };
-  auto tile = [&](int t) { return (const char*)smem + (t & 1) * TILE; };
-  issue_tile(0);
-  if (!brings_v && nt > 1) issue_tile(1);
+  auto tile = [&](int t) { return (const char*)smem + part * 4 * TILE + (t & 1) * TILE; };
+  if (own > 0) issue_tile(0);
+  if (!brings_v && own > 1) issue_tile(1);
   arrive();
 #pragma unroll
   for (int n = 0; n < QB; ++n)  // they have landed too: no wait at their uses
@@ -358,13 +365,16 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
     for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[n][ks]));
   constexpr std::integral_constant<int, 1> one{};
   constexpr std::integral_constant<int, 2> two{};
-  if (wave_active) scores(tile(0));
-  if (nt > 1) {
+  const bool has = wave_active && (P == 1 || nfull >= part);
+  const int full = P == 1 ? nfull : (nfull - part) >> 1;  // tiles of this part in front of its last one
+  const int steps = (nt + P - 1) / P - 1;                 // for all wavefronts
+  if (has) scores(tile(0));
+  if (steps > 0) {
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // everyone is done with K of tile 0
     request(2);
   }
-  if (wave_active) {
-    for (int t = 0; t < nfull; ++t) {
+  if (has) {
+    for (int t = 0; t < full; ++t) {
       softmax(std::false_type{}, two);
       __builtin_amdgcn_sched_barrier(0);
       scores(tile(t + 1));
@@ -372,17 +382,44 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
       arrive();
       request(t + 3);
     }
-    if (D <= 64 && QB <= 2 && edge + 16 * QB <= 32) {
+    if (P > 1 && (nfull - part) % P != 0) {
+      softmax(std::false_type{}, two);
+      weighted(two, tile(full));
+    } else if (D <= 64 && QB <= 2 && edge + 16 * QB <= 32) {
       softmax(std::true_type{}, one);
-      weighted(one, tile(nfull));
+      weighted(one, tile(full));
     } else {
       softmax(std::true_type{}, two);
-      weighted(two, tile(nfull));
+      weighted(two, tile(full));
     }
   }
-  for (int t = wave_active ? nfull : 0; t < nt - 1; ++t) {
+  for (int t = has ? full : 0; t < steps; ++t) {
     arrive();
     request(t + 3);
+  }
+  if constexpr (P > 1) {
+    // The second part's sums, scaled to the larger of both references, to the first's: by LDS, whose tiles are done with.
+    f4* sums = reinterpret_cast<f4*>(smem) + in_part * QB * (DB + 1) * kWave + lane;
+    __syncthreads();
+    if (part == 1 && wave_active) {
+#pragma unroll
+      for (int n = 0; n < QB; ++n) {
+#pragma unroll
+        for (int i = 0; i < DB; ++i) sums[(n * (DB + 1) + i) * kWave] = oacc[n][i];
+        sums[(n * (DB + 1) + DB) * kWave] = f4{base[n], den[n], 0.f, 0.f};
+      }
+    }
+    __syncthreads();
+    if (part == 1 || !wave_active) return;
+#pragma unroll
+    for (int n = 0; n < QB; ++n) {
+      const f4 other = sums[(n * (DB + 1) + DB) * kWave];
+      const float to = larger(base[n], other[0]);
+      const float mine = __builtin_amdgcn_exp2f(base[n] - to), its = __builtin_amdgcn_exp2f(other[0] - to);
+      den[n] = fmaf(den[n], mine, other[1] * its);
+#pragma unroll
+      for (int i = 0; i < DB; ++i) oacc[n][i] = oacc[n][i] * mine + sums[(n * (DB + 1) + i) * kWave] * its;
+    }
   }
   if (!wave_active) return;
 
@@ -458,7 +495,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
   }
 }
 
-template <int D, int QB>
+template <int D, int QB, int P>
 int launch_as(PackedArgs a, int64_t slots, hipStream_t st) {
   const int64_t blocks = slots * a.heads;
   if (blocks > (1ll << 31) - kGridRow) {
@@ -466,10 +503,10 @@ int launch_as(PackedArgs a, int64_t slots, hipStream_t st) {
               a.heads);
     return -2;
   }
-  constexpr int lds = 2 * 2 * kKeys * D * 2;
+  constexpr int lds = P * 2 * 2 * kKeys * D * 2;
   static bool attr_done = false;  // idempotent; a race only repeats the call
   if (!attr_done) {
-    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(packed_attn_kernel<D, QB>),
+    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(packed_attn_kernel<D, QB, P>),
                                        hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) {
       set_error("hipFuncSetAttribute(%d bytes LDS): %s", lds, hipGetErrorString(e));
@@ -489,23 +526,32 @@ int launch_as(PackedArgs a, int64_t slots, hipStream_t st) {
   a.longest_first = a.sequences <= kMany * kWave && slots <= 512 && blocks <= 5120 && a.rows >= 128ll * a.sequences;
   const int64_t grid = a.longest_first ? (slots + 7) / 8 * 8 * a.heads : blocks;
   const dim3 dims((unsigned)(grid < kGridRow ? grid : kGridRow), (unsigned)((grid + kGridRow - 1) / kGridRow));
-  hipLaunchKernelGGL((packed_attn_kernel<D, QB>), dims, dim3(256), lds, st, a);
+  hipLaunchKernelGGL((packed_attn_kernel<D, QB, P>), dims, dim3(256), lds, st, a);
   return 0;
 }
 
-// 16 queries a wavefront while the workgroups number at most 5 a CU: they all run at once, and a wavefront's chain
-// through its key tiles, which is then what the launch takes, is shorter (0.5 us a tile for 16 queries, 0.8 for 32).
-// 32 beyond: K and V are read from LDS for more queries at a time.  us, 16 / 32, the heaviest first: 1 x 1024 rows of
-// 12 heads (204 workgroups of 64 queries) 16.5 / 18.8, 4 x 1024 (816) 19.3 / 21.4, 16 x 300 (1092) 11.2 / 13.0, 3 x
-// 2048 (1188) 34.0 / 36.6, 48 of up to 1024 (1992) 22.9 / 21.9, 2 x 8192 (3096) 283 / 236; d = 128, 32 heads over 8,
-// 1 x 1024 (544) 22.8 / 28.3, 1 x 8192 (4128) 698 / 535.  64 queries were slower yet: 1 x 16384 of 25 heads 16 / 32 /
-// 64 1046 / 969 / 997 in an earlier state.  d = 256 has one workgroup a CU either way.
+// While the workgroups run at once, the launch takes what a wavefront's chain through its key tiles takes: 0.5 us a tile
+// for 16 queries, 0.8 for 32.  So up to 2.5 workgroups a CU of 32 queries, in two parts of the key tiles; up to 2 of 64
+// in two parts, 3 or 4 the longer the sequences are, which then hide what a workgroup begins and ends with; up to 5 of 64
+// queries, 16 a wavefront; and 32 a wavefront beyond: K and V are read from LDS for more queries at a time.  us, 16 / 32 / 16 in two parts / 32 in two parts: 1 x 1024 rows of
+// 12 heads 15.8 / 18.7 / 10.4 / 12.7 (396 workgroups in two parts, 204 of 64 queries), 1 x 2500 34.1 / 39.5 / 25.3 / 27.5
+// (948, 480), 1 x 4096 56.3 / 64.6 / 57.5 / 44.0 (1548, 780), 1 x 1024 of 25 heads 16.4 / 19.1 / 15.1 / 13.9 (825, 425), 1 x
+// 2048 32.1 / 35.1 / 35.7 / 29.0 (1625, 825), 8 x 150 9.9 / 9.9 / 11.5 / 12.5 (1125, 650), 4 x 1024 of 12 19.8 / 22.6 /
+// 32.3 / 23.3 (1584, 816), 16 x 300 11.3 / 13.0 / 23.7 / 16.3 (2184, 1092), 48 of up to 1024 24.0 / 22.3 / 53.8 / 34.1
+// (3408, 1992), 2 x 8192 293 / 245 / 361 / 320.  d = 128: two parts fill a CU's LDS, 1 x 1024 of 12 heads 20.5 / 27.1 / 19.4 /
+// 19.7, 1 x 1024 of 32 over 8 23.1 / 28.2 / 42.1 / 27.1: not taken.  64 queries a wavefront were slower yet: 1 x 16384 of 25
+// heads 16 / 32 / 64 1046 / 969 / 997 in an earlier state.  d = 256 has one workgroup a CU either way.
 template <int D>
 int launch_d(const PackedArgs& a, hipStream_t st) {
-  const int64_t slots = a.rows / 64 + a.sequences;
+  const int64_t slots32 = a.rows / 32 + a.sequences, slots = a.rows / 64 + a.sequences;
+  if constexpr (D <= 64) {
+    if (slots32 * a.heads <= 640) return launch_as<D, 1, 2>(a, slots32, st);
+    const int64_t average = a.rows / a.sequences;
+    if (slots * a.heads <= (average >= 2048 ? 1024 : average >= 256 ? 768 : 512)) return launch_as<D, 2, 2>(a, slots, st);
+  }
   if constexpr (D <= 128)
-    if (slots * a.heads <= 1280) return launch_as<D, 1>(a, slots, st);
-  return launch_as<D, 2>(a, a.rows / 128 + a.sequences, st);
+    if (slots * a.heads <= 1280) return launch_as<D, 1, 1>(a, slots, st);
+  return launch_as<D, 2, 1>(a, a.rows / 128 + a.sequences, st);
 }
 
 }  // namespace

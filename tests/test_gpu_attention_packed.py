@@ -116,6 +116,22 @@ def test_many_blocks(K, gpu_device, d):
         assert torch.all(torch.isfinite(out))
 
 
+@pytest.mark.parametrize("d", [16, 32, 64, 128])
+@pytest.mark.parametrize("heads", [12, 25, 40, 64])
+@pytest.mark.parametrize("lengths", [[191, 320, 640, 7], [1000, 1, 383], [64, 128, 1024, 192]])
+def test_every_deal(K, gpu_device, d, heads, lengths):
+    """By the number of heads: 16 and 32 queries a wavefront with the key tiles in two parts, 16 and 32 in one."""
+    q, k, v = make(np.random.default_rng(26), sum(lengths), heads, heads, d, True, gpu_device)
+    out = K.flash_attention_packed(q, k, v, starts_of(lengths, gpu_device))
+    ends = np.cumsum(lengths)
+    for end, L in zip(ends, lengths):
+        rows = slice(int(end) - L, int(end))
+        for h in (0, heads // 2, heads - 1):
+            w, tol = want(q[rows, h:h + 1], k[rows, h:h + 1], v[rows, h:h + 1], d ** -0.5)
+            assert torch.all((out[rows, h:h + 1].double() - w).abs() <= tol), (L, h)
+    assert torch.all(torch.isfinite(out))
+
+
 @pytest.mark.parametrize("d", [16, 32, 64, 128, 256])
 def test_long(K, gpu_device, d):
     r = np.random.default_rng(7)
@@ -232,6 +248,12 @@ def test_hidden_keys_play_no_part(K, gpu_device, d, heads):
                     assert not torch.any(torch.isfinite(got[behind]))
                 elif math.isnan(bad):
                     assert torch.all(torch.isnan(got[behind]))
+
+
+@pytest.mark.parametrize("heads", [45, 100])
+@pytest.mark.parametrize("d", [16, 32, 64])
+def test_hidden_keys_in_every_deal(K, gpu_device, d, heads):
+    test_hidden_keys_play_no_part(K, gpu_device, d, heads)
 
 
 def test_many_numbers_that_are_none(K, gpu_device):
