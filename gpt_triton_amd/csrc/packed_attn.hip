@@ -79,35 +79,33 @@ constexpr int kMany = 4;
 template <int R>
 __device__ __forceinline__ Block nth_longest(const PackedArgs& a, int nth) {
   const int lane = threadIdx.x & 63;
-  int blocks[kMany], most = 0;  // of sequence lane + 64 i
+  int first[kMany], length[kMany], most = 0;  // of sequence lane + 64 i; rows are below 2^31
 #pragma unroll
   for (int i = 0; i < kMany; ++i) {
     const int s = lane + i * kWave;
-    blocks[i] = 0;
+    first[i] = length[i] = 0;
     if (i * kWave >= a.sequences) break;
     if (s < a.sequences) {
       const int64_t begin = a.starts[s], end = a.starts[s + 1];
-      const int64_t first = begin < 0 ? 0 : begin < a.rows ? begin : a.rows;
-      const int64_t last = end < first ? first : end < a.rows ? end : a.rows;
-      blocks[i] = (int)((last - first + R - 1) / R);
+      const int64_t from = begin < 0 ? 0 : begin < a.rows ? begin : a.rows;
+      const int64_t to = end < from ? from : end < a.rows ? end : a.rows;
+      first[i] = (int)from;
+      length[i] = (int)(to - from);
     }
-    most = max(most, blocks[i]);
+    most = max(most, length[i]);
   }
-  most = __builtin_amdgcn_readfirstlane((int)wave_max((float)most));  // below 2^24: the host sees to it
+  most = __builtin_amdgcn_readfirstlane((int)wave_max((float)((most + R - 1) / R)));  // below 2^24: the host sees to it
   for (int block = most - 1; block >= 0; --block) {
     int all = 0;
 #pragma unroll
     for (int i = 0; i < kMany; ++i) {
       if (i * kWave >= a.sequences) break;
-      const uint64_t have = __ballot(blocks[i] > block);
+      const uint64_t have = __ballot(length[i] > block * R);
       const int n = __popcll(have);
       if (nth >= all && nth < all + n) {  // the (nth - all)th of these
         const bool me = (have >> lane & 1) && __popcll(have & ((1ull << lane) - 1)) == nth - all;
-        const int s = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(me)) - 1 + i * kWave);
-        const int64_t begin = a.starts[s], end = a.starts[s + 1];
-        const int64_t first = begin < 0 ? 0 : begin < a.rows ? begin : a.rows;
-        const int64_t last = end < first ? first : end < a.rows ? end : a.rows;
-        return {first, (int)(last - first), block};
+        const int s = __ffsll((unsigned long long)__ballot(me)) - 1;
+        return {__builtin_amdgcn_readlane(first[i], s), __builtin_amdgcn_readlane(length[i], s), block};
       }
       all += n;
     }
