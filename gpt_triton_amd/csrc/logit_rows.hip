@@ -673,40 +673,56 @@ __device__ __forceinline__ void set_special(const Row<T, NT, CH, OPEN>& row, Spe
   }
 }
 
+// STREAM: past the caches.  (Not as a condition at the store, which the compiler makes one plain store of.)
+template <bool STREAM, typename V>
+__device__ __forceinline__ void store_chunk(V* at, V v) {
+  if constexpr (STREAM) __builtin_nontemporal_store(v, at);
+  else *at = v;
+}
+
 // Writes f(x_j) of every logit of the row, and of the special ones' f(x) + scale total: over what was written, by the thread
 // that wrote it, so that nothing has to be waited for.  Entries of one token write one number.
 template <typename T, int NT, int CH, bool OPEN, typename F>
 __device__ __forceinline__ void write_gradient(Row<T, NT, CH, OPEN>& row, T* __restrict__ out, const Special<NT>& sp,
-                                               bool special, float scale, F f) {
+                                               bool special, float scale, bool stream, F f) {
   typedef typename RowVec<T>::V V;
   const bool whole = ((uintptr_t)out & 15) == ((uintptr_t)row.x & 15);
   row.renew();
-  row.each([&](const auto& y, int first, auto n) {
-    if constexpr (n.value > 1) {
-      if (first >= row.lead + row.chunks * n.value) return;
-      V v;
+  auto write = [&](auto past) {
+    row.each([&](const auto& y, int first, auto n) {
+      if constexpr (n.value > 1) {
+        if (first >= row.lead + row.chunks * n.value) return;
+        V v;
 #pragma unroll
-      for (int j = 0; j < n.value; ++j) v[j] = (T)f(y[j]);
-      if (whole) {
-        *reinterpret_cast<V*>(out + first) = v;
-      } else {
+        for (int j = 0; j < n.value; ++j) v[j] = (T)f(y[j]);
+        if (whole) {
+          store_chunk<decltype(past)::value>(reinterpret_cast<V*>(out + first), v);
+        } else {
 #pragma unroll
-        for (int j = 0; j < n.value; ++j) out[first + j] = v[j];
+          for (int j = 0; j < n.value; ++j) out[first + j] = v[j];
+        }
+      } else if (first >= 0) {
+        out[first] = (T)f(y[0]);
       }
-    } else if (first >= 0) {
-      out[first] = (T)f(y[0]);
-    }
-  });
+    });
+  };
+  if (OPEN || stream) write(std::true_type{});  // what is read again here stays in the L2
+  else write(std::false_type{});
   asm volatile("" ::: "memory");
   if (special)
     for (int i = sp.first[threadIdx.x]; i >= 0; i = sp.next[i]) out[sp.id[i]] = (T)fmaf(scale, sp.total[i], f(sp.x[i]));
 }
 
 template <typename T, int NT>
-__device__ __forceinline__ void write_zeros(T* __restrict__ out, int vocab) {
+__device__ __forceinline__ void write_zeros(T* __restrict__ out, int vocab, bool stream) {
   const Row<T, NT, 0, true> row(out, vocab);
   typedef typename RowVec<T>::V V;
-  for (int c = threadIdx.x; c < row.chunks; c += NT) reinterpret_cast<V*>(out + row.lead)[c] = V(0);
+  auto write = [&](auto past) {
+    for (int c = threadIdx.x; c < row.chunks; c += NT)
+      store_chunk<decltype(past)::value>(reinterpret_cast<V*>(out + row.lead) + c, V(0));
+  };
+  if (stream) write(std::true_type{});
+  else write(std::false_type{});
   if (row.loose >= 0) out[row.loose] = (T)0;
 }
 
@@ -716,12 +732,12 @@ template <typename T, int NT, int CH, bool OPEN, int WAVES>
 __global__ __launch_bounds__(NT * kRowsOf<NT>, WAVES) void token_log_probs_backward_kernel(
     const T* __restrict__ x, int64_t ld, int64_t rows, int vocab, const int64_t* __restrict__ tokens, float tau,
     RowGradient d_log_probs, RowGradient d_entropy, int k, const int64_t* __restrict__ top_tokens,
-    const float* __restrict__ d_top, T* __restrict__ out, int64_t ld_out) {
+    const float* __restrict__ d_top, T* __restrict__ out, int64_t ld_out, bool stream) {
   __shared__ Shared<NT> sh_of[kRowsOf<NT>];
   __shared__ Special<NT> sp_of[kRowsOf<NT>];
   const int in_group = row_in_group<NT>();
-  const int64_t r = row_of_group<NT>(in_group);
-  if (r >= rows) return;
+  const int64_t r = rows - 1 - row_of_group<NT>(in_group);  // the last first: the forward pass read them last
+  if (r < 0) return;
   Shared<NT>& sh = sh_of[in_group];
   Special<NT>& sp = sp_of[in_group];
   const int count = k + 1;
@@ -756,13 +772,13 @@ __global__ __launch_bounds__(NT * kRowsOf<NT>, WAVES) void token_log_probs_backw
   g = uniform(g);
   T* o = out + r * ld_out;
   if (none && h == 0.f) {  // padding: whatever its logits are
-    write_zeros<T, NT>(o, vocab);
+    write_zeros<T, NT>(o, vocab, stream);
     return;
   }
   row.load();
   const Stats<T> st = row_stats<true, false>(row, tau, sh);
   const float scale = uniform(st.inv * st.inv_tau), lift = uniform(st.entropy - st.log_s - kLn2 * st.t.rest());
-  write_gradient(row, o, sp, st.S != 0.f, st.inv_tau, [&](float y) {
+  write_gradient(row, o, sp, st.S != 0.f, st.inv_tau, stream, [&](float y) {
     const float t = st.t(y), p = __builtin_amdgcn_exp2f(t) * scale;
     return -p * fmaf(h, fmaf(kLn2, fmaxf(t, -1e30f), lift), g);
   });
@@ -779,13 +795,14 @@ template <typename T, bool GRAD, int NT, int CH, bool OPEN, int WAVES>
 __global__ __launch_bounds__(NT * kRowsOf<NT>, WAVES) void distillation_kernel(
     const T* __restrict__ x, int64_t ld, int64_t rows, int vocab, const int64_t* __restrict__ teacher_tokens,
     const void* __restrict__ teacher, int teacher_f16, int k, float tau, const float* __restrict__ weights,
-    RowGradient d_losses, float* __restrict__ losses, T* __restrict__ out, int64_t ld_out) {
+    RowGradient d_losses, float* __restrict__ losses, T* __restrict__ out, int64_t ld_out, bool stream) {
   __shared__ Shared<NT> sh_of[kRowsOf<NT>];
   __shared__ Special<NT> sp_of[kRowsOf<NT>];
   __shared__ Entries entries_of[kRowsOf<NT>];
   const int in_group = row_in_group<NT>();
-  const int64_t r = row_of_group<NT>(in_group);
-  if (r >= rows) return;
+  int64_t r = row_of_group<NT>(in_group);
+  if (GRAD && losses == nullptr) r = rows - 1 - r;  // as in the gradient above
+  if (r < 0 || r >= rows) return;
   Shared<NT>& sh = sh_of[in_group];
   Special<NT>& sp = sp_of[in_group];
   Entries& entries = entries_of[in_group];
@@ -795,7 +812,7 @@ __global__ __launch_bounds__(NT * kRowsOf<NT>, WAVES) void distillation_kernel(
   if (d_losses.d != nullptr) w_grad *= d_losses.d[r * d_losses.pitch];
   if (w == 0.f || (losses == nullptr && w_grad == 0.f)) {  // padding: whatever its logits are
     if (tid == 0 && losses != nullptr) losses[r] = 0.f;
-    if constexpr (GRAD) write_zeros<T, NT>(out + r * ld_out, vocab);
+    if constexpr (GRAD) write_zeros<T, NT>(out + r * ld_out, vocab, stream);
     return;
   }
   Row<T, NT, CH, OPEN> row(x + r * ld, vocab);
@@ -868,7 +885,7 @@ __global__ __launch_bounds__(NT * kRowsOf<NT>, WAVES) void distillation_kernel(
   }
   if constexpr (GRAD) {
     const float scale = uniform(entries.total == 0.f ? 0.f : w_grad * st.inv * st.inv_tau);
-    write_gradient(row, out + r * ld_out, sp, st.S != 0.f, w_grad * st.inv_tau,
+    write_gradient(row, out + r * ld_out, sp, st.S != 0.f, w_grad * st.inv_tau, stream,
                    [&](float y) { return __builtin_amdgcn_exp2f(st.t(y)) * scale; });
   }
 }
@@ -910,6 +927,15 @@ dim3 grid_of(const LogitRows& a) {
   const int64_t n = (a.rows + kRowsOf<NT> - 1) / kRowsOf<NT>;
   return dim3((unsigned)(n < kGridRow ? n : kGridRow), (unsigned)((n + kGridRow - 1) / kGridRow));
 }
+// A gradient goes past the caches where it would push out the logits that the forward pass left in the memory-side cache of
+// 256 MB, whose last rows a backward pass therefore takes first, and a one-pass gradient where it would not stay there
+// itself; always where rows are so long that they are read again.  us, without / with, 50304 logits: forward and backward of
+// 1024 fp32 rows (206 MB) 129 / 115, with a sum that reads the gradient 171 / 167, of 2048 246 / 216 and 329 / 326 (the
+// first rows first 250 and 342), of 768 rows (155 MB) with the sum 126 / 131; one pass of 2048 fp16 rows (206 MB) 89 / 84,
+// but with the sum 139 / 149, of 1536 fp32 rows (309 MB) 129 / 121 and 210 / 207; of 512 rows of 128256 fp32 logits 129 / 108.
+constexpr int64_t kStreamBehindForward = 192 << 20, kStreamOnePass = 256 << 20;
+int64_t gradient_bytes(const LogitRows& a) { return a.rows * a.vocab * (a.f16 ? 2 : 4); }
+
 template <int NT>
 dim3 block_of() { return dim3(NT, kRowsOf<NT>); }
 
@@ -930,24 +956,26 @@ void launch_token_log_probs(const LogitRows& a, const int64_t* tokens, int top, 
 void launch_token_log_probs_backward(const LogitRows& a, const int64_t* tokens, RowGradient d_log_probs,
                                      RowGradient d_entropy, int top, const int64_t* top_tokens, const float* d_top,
                                      void* grad, int64_t ld_grad, hipStream_t st) {
+  const bool stream = gradient_bytes(a) > kStreamBehindForward;
   pick_row(a, 0, [&](auto type, auto nt, auto ch, auto open, auto waves) {
     typedef decltype(type) T;
     hipLaunchKernelGGL((token_log_probs_backward_kernel<T, nt.value, ch.value, open.value, waves.value>),
                        grid_of<nt.value>(a), block_of<nt.value>(), 0, st, (const T*)a.x, a.ld, a.rows, a.vocab, tokens,
-                       a.temperature, d_log_probs, d_entropy, top, top_tokens, d_top, (T*)grad, ld_grad);
+                       a.temperature, d_log_probs, d_entropy, top, top_tokens, d_top, (T*)grad, ld_grad, stream);
   });
 }
 
 void launch_distillation(const LogitRows& a, const int64_t* teacher_tokens, const void* teacher, bool teacher_f16,
                          int k, const float* weights, RowGradient d_losses, float* losses, void* grad, int64_t ld_grad,
                          hipStream_t st) {
+  const bool stream = gradient_bytes(a) > (losses == nullptr ? kStreamBehindForward : kStreamOnePass);
   pick_row(a, 0, [&](auto type, auto nt, auto ch, auto open, auto waves) {
     typedef decltype(type) T;
     auto kernel = grad != nullptr ? distillation_kernel<T, true, nt.value, ch.value, open.value, waves.value>
                                   : distillation_kernel<T, false, nt.value, ch.value, open.value, waves.value>;
     hipLaunchKernelGGL(kernel, grid_of<nt.value>(a), block_of<nt.value>(), 0, st, (const T*)a.x, a.ld, a.rows, a.vocab,
                        teacher_tokens, teacher, (int)teacher_f16, k, a.temperature, weights, d_losses, losses, (T*)grad,
-                       ld_grad);
+                       ld_grad, stream);
   });
 }
 
