@@ -505,6 +505,33 @@ def test_rows_beyond_32_bits(K, gpu_device):
     check_distillation(K, x, np.array([[1, 2], [3, 4], [5, 6]]), torch.zeros(3, 2, device=gpu_device), 1.0, np.ones(3))
 
 
+@pytest.mark.parametrize("dtype,rows", [(torch.float16, 2900), (torch.float32, 1450)])
+def test_large_gradients(K, gpu_device, dtype, rows):
+    """Gradients that go past the caches, from the last row on: the bits of the same rows by themselves."""
+    V = 50257
+    x = torch.randn(rows, 50304, device=gpu_device).mul_(2).to(dtype)[:, :V]
+    ids = torch.randint(0, V, (rows, 9), device=gpu_device)
+    teacher = torch.randn(rows, 9, device=gpu_device)
+    w = torch.ones(rows, device=gpu_device)
+    w[5] = w[-1] = 0
+    d = torch.randn(rows, device=gpu_device)
+    t = ids[:, 0].contiguous()
+
+    def gradients(part):
+        leaf = x[part].detach().requires_grad_()
+        one, = torch.autograd.grad(K.token_log_probs(leaf, t[part]).log_probs, leaf, d[part])
+        two, = torch.autograd.grad(K.distillation_loss(leaf, ids[part], teacher[part], 2.0, w[part]), leaf, d[part])
+        return one, two, K.distillation_loss_and_grad(leaf, ids[part], teacher[part], 2.0, w[part])[1]
+
+    whole = gradients(slice(0, rows))
+    assert whole[0].numel() * whole[0].element_size() > 256 << 20
+    for part in (slice(0, 8), slice(rows // 2, rows // 2 + 3), slice(rows - 5, rows)):
+        for a, b in zip(whole, gradients(part)):
+            assert torch.equal(a[part], b)
+    for a in whole[1:]:
+        assert torch.all(a[5] == 0) and torch.all(a[-1] == 0) and torch.all(torch.isfinite(a))
+
+
 def test_millions_of_rows(K, gpu_device):
     """More workgroups than a row of the grid has: one row of logits for all of them, and rows of their own, whose chunks
     begin elsewhere: sums of another order."""
