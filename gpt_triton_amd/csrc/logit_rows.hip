@@ -147,6 +147,14 @@ struct Shared {
   int scan[W];
 };
 
+// The value of the lane that differs by D = 1, 2, 4 or 8; for 4 and 8 of one with the same bits above, which is as good
+// where the lanes that differ by less have one value: a group's sum or maximum is formed with D = 1, 2, ..
+template <int D, typename A>
+__device__ __forceinline__ A from_lane(A v) {
+  constexpr int control = D == 1 ? 0xb1 : D == 2 ? 0x4e : D == 4 ? 0x141 : 0x140;  // quad_perm, row_half_mirror, row_mirror
+  return __builtin_bit_cast(A, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), control, 0xf, 0xf, true));
+}
+
 // op over the W values (a power of two up to 16) that lane l has the l % W-th of, for every lane.
 template <int W, typename Op>
 __device__ __forceinline__ float join(float v, Op op) {
@@ -320,13 +328,15 @@ __device__ __forceinline__ Stats<T> row_stats(Row<T, NT, CH, OPEN>& row, float t
     tops->mine = fmaxf(mine, -INFINITY);
     float g = tops->mine;
     constexpr int SMALL = NT >= 256 ? NT / 256 : 1, LANES = NT / 64;
-#pragma unroll
-    for (int d = 1; d < SMALL; d *= 2) g = fmaxf(g, __shfl_xor(g, d));
+    if constexpr (SMALL > 1) g = fmaxf(g, from_lane<1>(g));
+    if constexpr (SMALL > 2) g = fmaxf(g, from_lane<2>(g));
     const float least = group_reduce<kWave>(g > -INFINITY ? g : INFINITY, [](float a, float b) { return fminf(a, b); });
     if (lane == 0) sh.low[wave] = least;
     if (NT >= 256 && lane % SMALL == 0) sh.many[threadIdx.x / SMALL] = g;
-#pragma unroll
-    for (int d = SMALL; d < LANES; d *= 2) g = fmaxf(g, __shfl_xor(g, d));
+    if constexpr (SMALL == 1 && LANES > 1) g = fmaxf(g, from_lane<1>(g));
+    if constexpr (SMALL <= 2 && LANES > 2) g = fmaxf(g, from_lane<2>(g));
+    if constexpr (LANES > 4) g = fmaxf(g, from_lane<4>(g));
+    if constexpr (LANES > 8) g = fmaxf(g, from_lane<8>(g));
     if (lane % LANES == 0) sh.groups[threadIdx.x / LANES] = g;
   }
   const float m_wave = group_reduce<kWave>(mine, [](float a, float b) { return most_of(a, b); });
@@ -394,26 +404,25 @@ struct TopShared {
   }
 };
 
-// The k-th largest of the numbers that lanes 0 .. G - 1 have, or a little below it: ranks of numbers that differ, a number
-// without its last 6 bits and the lane in their place.
+// The k-th largest of the numbers that lanes 0 .. G - 1 have, or a little below it: its upper 18 bits, one by one from the top.
 template <int G>
 __device__ __forceinline__ float kth_of_lanes(float v, int k) {
-  const int lane = threadIdx.x & 63;
-  const unsigned key = (unsigned)(top_key(v, 0) >> 32) & ~63u | (63 - lane);
-  int rank = 0;
+  const unsigned key = (threadIdx.x & 63) < G ? (unsigned)(top_key(v, 0) >> 32) : 0;
+  unsigned kth = 0;
 #pragma unroll
-  for (int j = 0; j < G; ++j) rank += (unsigned)__builtin_amdgcn_readlane((int)key, j) > key;
-  const uint64_t kth = __ballot(rank == k - 1 && lane < G);
-  const unsigned down = (unsigned)__builtin_amdgcn_readlane((int)key, __ffsll((unsigned long long)kth) - 1) & ~63u;
-  return down < 0x007fffffu ? -INFINITY : uniform(key_value((uint64_t)down << 32));  // below -infinity's there are NaNs
+  for (int bit = 31; bit >= 14; --bit) {
+    const unsigned trial = kth | 1u << bit;
+    if (__popcll(__ballot(key >= trial)) >= k) kth = trial;
+  }
+  return kth < 0x007fffffu ? -INFINITY : key_value((uint64_t)kth << 32);  // below -infinity's there are NaNs
 }
 
 // found(r, key) of the k largest logits, r = 0 .. k - 1 in any order, by one thread each.  A bound that at least k of them
 // reach is the k-th largest of the maxima of some groups of threads: of the wavefronts for the least k, of 64 groups up to
 // k = 32, of 256, by a histogram, beyond.  The logits that reach it are gathered, little more than k (some 24 for k = 20, 180 for
-// 128), from memory, since a row's registers held any longer are too many: those of the few threads whose maximum reaches
-// it, or the whole row.  A histogram leaves of more than 256 those from the k-th's bin on, and the rest is ranked by
-// counting.  2048 rows of 50257 fp16 logits, us: no top tokens 42, 1 54, 20 60, 64 77, 128 113.
+// 128), from memory, since a row's registers held any longer are too many: the chunks of the few threads whose maximum
+// reaches it, one a thread, or the whole row.  A histogram leaves of more than 256 those from the k-th's bin on, and the rest is
+// ranked by counting.  2048 rows of 50257 fp16 logits, us: no top tokens 40, 1 53, 20 49, 64 58, 128 84.
 template <typename T, int NT, int CH, bool OPEN, typename F>
 __device__ __forceinline__ void row_top(const Row<T, NT, CH, OPEN>& row, int k, Tops tops, float high, TopShared<NT>& top,
                                         Shared<NT>& sh, F found) {
@@ -502,26 +511,23 @@ __device__ __forceinline__ void row_top(const Row<T, NT, CH, OPEN>& row, int k, 
     }
     sync_row<NT>();
     const int threads = top.threads;
-    const int part = (row.chunks + NT - 1) / NT * N + 1;  // logits of a thread, the last one single
-    if (threads * part <= 32 * NT) {
-      const float per = 1.0f / (float)part;
-      for (int f = tid; f < threads * part; f += 4 * NT) {
-        float y[4];
-        int index[4];
+    const int units = (row.chunks + NT - 1) / NT + 1;  // of a thread: its chunks and its single element
+    if (threads * units * N <= 32 * NT) {
+      const float per = 1.0f / (float)units;
+      for (int f = tid; f < threads * units; f += NT) {
+        const int nth = (int)(((float)f + 0.5f) * per), e = f - nth * units, t = top.thread[nth], chunk = t + e * NT;
+        if (e < units - 1) {
+          const auto v = row.chunk(chunk);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int at = f + i * NT, nth = (int)(((float)at + 0.5f) * per), e = at - nth * part;
-          y[i] = -INFINITY;
-          if (at < threads * part) {
-            const int t = top.thread[nth], chunk = t + e / N * NT;
-            const bool single = e == part - 1;
-            index[i] = !single ? row.lead + chunk * N + e % N : t < row.lead ? t : t + row.chunks * N;
-            if (single ? t < row.vocab - row.chunks * N : chunk < row.chunks) y[i] = row.at(index[i]);
+          for (int j = 0; j < N; ++j) {
+            const float y = (float)v[j];
+            if (y >= low) put(atomicAdd(&top.count, 1), y, row.lead + chunk * N + j);
           }
+        } else if (t < row.vocab - row.chunks * N) {
+          const int index = t < row.lead ? t : t + row.chunks * N;
+          const float y = row.at(index);
+          if (y >= low) put(atomicAdd(&top.count, 1), y, index);
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (y[i] >= low) put(atomicAdd(&top.count, 1), y[i], index[i]);
       }
       sync_row<NT>();
       n = top.count;
@@ -592,7 +598,10 @@ __device__ __forceinline__ void row_top(const Row<T, NT, CH, OPEN>& row, int k, 
     int rank = 0;
 #pragma unroll 8
     for (int j = part; j < n; j += parts) rank += list[j] > key;
-    for (int d = 1; d < parts; d *= 2) rank += __shfl_xor(rank, d);
+    if (parts > 1) rank += from_lane<1>(rank);
+    if (parts > 2) rank += from_lane<2>(rank);
+    if (parts > 4) rank += from_lane<4>(rank);
+    if (parts > 8) rank += from_lane<8>(rank);
     if (i < n && part == 0 && rank < k) found(rank, key);
   }
 }
