@@ -404,10 +404,9 @@ struct TopShared {
   }
 };
 
-// The k-th largest of the numbers that lanes 0 .. G - 1 have, or a little below it: its upper 18 bits, one by one from the top.
-template <int G>
+// The k-th largest of the lanes' numbers, or a little below it: its upper 18 bits, one by one from the top.
 __device__ __forceinline__ float kth_of_lanes(float v, int k) {
-  const unsigned key = (threadIdx.x & 63) < G ? (unsigned)(top_key(v, 0) >> 32) : 0;
+  const unsigned key = (unsigned)(top_key(v, 0) >> 32);
   unsigned kth = 0;
 #pragma unroll
   for (int bit = 31; bit >= 14; --bit) {
@@ -418,7 +417,7 @@ __device__ __forceinline__ float kth_of_lanes(float v, int k) {
 }
 
 // found(r, key) of the k largest logits, r = 0 .. k - 1 in any order, by one thread each.  A bound that at least k of them
-// reach is the k-th largest of the maxima of some groups of threads: of the wavefronts for the least k, of 64 groups up to
+// reach is the k-th largest of the maxima of some groups of threads: of 64 groups up to
 // k = 32, of 256, by a histogram, beyond.  The logits that reach it are gathered, little more than k (some 24 for k = 20, 180 for
 // 128), from memory, since a row's registers held any longer are too many: the chunks of the few threads whose maximum
 // reaches it, one a thread, or the whole row.  A histogram leaves of more than 256 those from the k-th's bin on, and the rest is
@@ -426,7 +425,7 @@ __device__ __forceinline__ float kth_of_lanes(float v, int k) {
 template <typename T, int NT, int CH, bool OPEN, typename F>
 __device__ __forceinline__ void row_top(const Row<T, NT, CH, OPEN>& row, int k, Tops tops, float high, TopShared<NT>& top,
                                         Shared<NT>& sh, F found) {
-  constexpr int kKeep = TopShared<NT>::kKeep, kBins = TopShared<NT>::kBins, N = RowVec<T>::N, W = Shared<NT>::W;
+  constexpr int kKeep = TopShared<NT>::kKeep, kBins = TopShared<NT>::kBins, N = RowVec<T>::N;
   const int tid = threadIdx.x, lane = tid & 63;
   // Bins of n keys between those of `from` and `high`, lower ones in the first: the lowest bin in which one of the k
   // largest is.
@@ -464,10 +463,8 @@ __device__ __forceinline__ void row_top(const Row<T, NT, CH, OPEN>& row, int k, 
     return (unsigned)top.cut;
   };
   float low = -INFINITY;
-  if (W >= 4 && 4 * k <= 3 * W) {
-    low = kth_of_lanes<W>(fmaxf(sh.top[lane % W], -INFINITY), k);
-  } else if (k <= 32 || (NT < 256 && k <= 64)) {
-    low = kth_of_lanes<64>(sh.groups[lane], k);
+  if (k <= 32 || (NT < 256 && k <= 64)) {
+    low = kth_of_lanes(sh.groups[lane], k);
   } else if (NT >= 256 && tops.low < INFINITY) {
     const unsigned cut = cut_bins(256, [&](int i) { return (unsigned)(top_key(sh.many[i], 0) >> 32); }, tops.low);
     if (cut > 0) low = key_value((uint64_t)(base + (cut << shift)) << 32);  // some in the first bin may be below its edge
