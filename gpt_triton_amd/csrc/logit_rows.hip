@@ -463,7 +463,7 @@ __device__ __forceinline__ void row_top(const Row<T, NT, CH, OPEN>& row, int k, 
     return (unsigned)top.cut;
   };
   float low = -INFINITY;
-  if (k <= 32 || (NT < 256 && k <= 64)) {
+  if (NT < 256 || k <= 32) {  // a wavefront's row has no more
     low = kth_of_lanes(sh.groups[lane], k);
   } else if (NT >= 256 && tops.low < INFINITY) {
     const unsigned cut = cut_bins(256, [&](int i) { return (unsigned)(top_key(sh.many[i], 0) >> 32); }, tops.low);
