@@ -326,7 +326,7 @@ def _logit_gradient(logits, rows, V, ld):
     pitch = V + (ld - V) % 64
     offset = logits.data_ptr() % 16 // logits.element_size()
     if offset == 0 and (pitch == V or rows <= 1):
-        return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device), pitch
+        return torch.empty_like(logits) if ld == V else logits.new_empty(logits.shape), pitch
     buf = logits.new_empty(offset + max(rows - 1, 0) * pitch + V)
     return buf.as_strided((rows, V), (pitch, 1), offset).view(logits.shape), pitch
 
@@ -365,8 +365,8 @@ def _token_log_probs(logits, tokens, top, temperature):
     log_probs = None if tokens is None else torch.empty_like(entropy)
     top_log_probs = top_tokens = None
     if top > 0:
-        top_log_probs = logits.new_empty((*lead, top), dtype=torch.float32)
-        top_tokens = logits.new_empty((*lead, top), dtype=torch.int64)
+        top_log_probs = entropy.new_empty((*lead, top))
+        top_tokens = torch.empty_like(top_log_probs, dtype=torch.int64)
     if rows > 0:
         _call(dev, "token_log_probs", _lib.load().gptmi_token_log_probs, logits.data_ptr(), ld, _ptr(tokens),
               temperature, _ptr(log_probs), entropy.data_ptr(), top, _ptr(top_log_probs), _ptr(top_tokens), rows, V,
@@ -459,7 +459,9 @@ def _distillation(logits, teacher_tokens, teacher_logits, temperature, weights, 
         assert weights.shape == lead, (weights.shape, lead)
         assert weights.is_contiguous()
     _check_temperature(temperature, code, what)
-    out = logits.new_empty(lead, dtype=torch.float32) if losses else None
+    out = None
+    if losses:
+        out = logits.new_empty(lead, dtype=torch.float32) if weights is None else torch.empty_like(weights)
     grad, pitch = _logit_gradient(logits, rows, V, ld) if gradient else (None, V)
     d_at, d_pitch, d_losses = _row_gradient(d_losses)
     if rows > 0:
@@ -505,7 +507,6 @@ def distillation_loss(logits, teacher_tokens, teacher_logits, temperature=1.0, w
     return _distillation(logits, teacher_tokens, teacher_logits, temperature, weights, True, False)[0]
 
 
-@torch.no_grad()
 def distillation_loss_and_grad(logits, teacher_tokens, teacher_logits, temperature=1.0, weights=None):
     """(losses, gradient of their sum with respect to the logits) of `distillation_loss` from one pass over the logits, for
     steps that know the weights of their rows beforehand: `logits.backward(gradient)` goes on from there.  The
