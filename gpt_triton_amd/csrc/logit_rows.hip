@@ -935,10 +935,11 @@ dim3 grid_of(const LogitRows& a) {
 }
 // A gradient goes past the caches where it would push out the logits that the forward pass left in the memory-side cache of
 // 256 MB, whose last rows a backward pass therefore takes first, and a one-pass gradient where it would not stay there
-// itself; always where rows are so long that they are read again.  us, without / with, 50304 logits: forward and backward of
-// 1024 fp32 rows (206 MB) 129 / 115, with a sum that reads the gradient 171 / 167, of 2048 246 / 216 and 329 / 326 (the
-// first rows first 250 and 342), of 768 rows (155 MB) with the sum 126 / 131; one pass of 2048 fp16 rows (206 MB) 89 / 84,
-// but with the sum 139 / 149, of 1536 fp32 rows (309 MB) 129 / 121 and 210 / 207; of 512 rows of 128256 fp32 logits 129 / 108.
+// itself (what waits there for its way to memory is written while the next kernel reads); always where rows are so long
+// that they are read again.  us, without / with, 50304 logits: forward and backward of 1024 fp32 rows (206 MB) 129 / 115,
+// with a sum that reads the gradient 171 / 167, of 2048 246 / 216 and 329 / 326 (the first rows first 250 and 342), of 768
+// rows (155 MB) with the sum 126 / 131; one pass of 2048 fp16 rows (206 MB) 89 / 84, but with the sum 139 / 149, of 1536
+// fp32 rows (309 MB) 129 / 121 and 210 / 207; of 512 rows of 128256 fp32 logits 129 / 108.
 constexpr int64_t kStreamBehindForward = 192 << 20, kStreamOnePass = 256 << 20;
 int64_t gradient_bytes(const LogitRows& a) { return a.rows * a.vocab * (a.f16 ? 2 : 4); }
 
