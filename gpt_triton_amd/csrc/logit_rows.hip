@@ -898,11 +898,13 @@ __global__ __launch_bounds__(NT * kRowsOf<NT>, WAVES) void distillation_kernel(
 
 // f(threads, chunks a thread, wavefronts a SIMD) as integral constants for rows of this many chunks.  A row takes 4 CH
 // registers a thread and some 26 more, so few threads with long parts keep the most rows on a CU: of 50257 fp16 logits (6283
-// chunks) 3 with 512 threads, 4 with 256, 2 with 1024; 1477 rows scored 44 / 49 / 45 us, 2048 rows' loss and gradient 100 /
-// 105 / 104.  50304 fp32 logits (12576 chunks), forward and backward of 2048 rows: 512 threads 255 us, 1024 310.
-// Rows of up to 256 chunks have a wavefront each, four a workgroup; the longest, beyond 20480 chunks, are read again behind
-// those.  min_threads: what the call needs.
-template <typename F>
+// chunks) 3 with 512 threads, 4 with 256, 2 with 1024; 1477 rows scored 31 / 32 / 38 us, with their top 20 37 / 41 / 43; of 50304
+// fp32 logits (12576 chunks), forward and backward of 2048 rows 216 with 512 threads, 225 with 1024, loss and gradient of 4096
+// 324 and 427.  WIDE, for a loss' gradient, whose stores are what it waits for: 1024 threads where a thread then has up to 8
+// chunks; 2048 rows of 50257 fp16 logits 512 / 1024 threads 85 / 78, with the loss 90 / 83, of 65024 102 / 99 and 108 / 105, of 32000
+// fp32 99 / 97 and 105 / 102, but the gradient of log probabilities 86 / 90.  Rows of up to 256 chunks have a wavefront each,
+// four a workgroup; the longest, beyond 20480 chunks, are read again behind those.  min_threads: what the call needs.
+template <bool WIDE, typename F>
 void pick(int chunks, int min_threads, F f) {
 #define GPTMI_ROW(NT, CH, OPEN, WAVES)                                                                        \
   if (NT >= min_threads && (OPEN || chunks <= NT * CH))                                                       \
@@ -912,20 +914,24 @@ void pick(int chunks, int min_threads, F f) {
   GPTMI_ROW(256, 4, false, 4);
   GPTMI_ROW(256, 8, false, 4);
   GPTMI_ROW(512, 8, false, 4);
-  GPTMI_ROW(512, 13, false, 6);
-  GPTMI_ROW(512, 16, false, 4);
+  if constexpr (WIDE) {
+    GPTMI_ROW(1024, 8, false, 8);
+  } else {
+    GPTMI_ROW(512, 13, false, 6);
+    GPTMI_ROW(512, 16, false, 4);
+  }
   GPTMI_ROW(512, 25, false, 4);
   GPTMI_ROW(1024, 16, false, 4);
   GPTMI_ROW(1024, 20, true, 4);
 #undef GPTMI_ROW
 }
 
-template <typename F>
+template <bool WIDE, typename F>
 void pick_row(const LogitRows& a, int min_threads, F f) {
   if (a.f16)
-    pick(a.vocab / 8, min_threads, [&](auto nt, auto ch, auto open, auto waves) { f(_Float16(), nt, ch, open, waves); });
+    pick<WIDE>(a.vocab / 8, min_threads, [&](auto nt, auto ch, auto open, auto waves) { f(_Float16(), nt, ch, open, waves); });
   else
-    pick(a.vocab / 4, min_threads, [&](auto nt, auto ch, auto open, auto waves) { f(float(), nt, ch, open, waves); });
+    pick<WIDE>(a.vocab / 4, min_threads, [&](auto nt, auto ch, auto open, auto waves) { f(float(), nt, ch, open, waves); });
 }
 
 template <int NT>
@@ -951,7 +957,7 @@ dim3 block_of() { return dim3(NT, kRowsOf<NT>); }
 void launch_token_log_probs(const LogitRows& a, const int64_t* tokens, int top, float* log_probs, float* entropy,
                             float* top_log_probs, int64_t* top_tokens, hipStream_t st) {
   // a wavefront has 64 groups to bound the top tokens with: no more than 32 of them
-  pick_row(a, top > 32 ? 256 : 0, [&](auto type, auto nt, auto ch, auto open, auto waves) {
+  pick_row<false>(a, top > 32 ? 256 : 0, [&](auto type, auto nt, auto ch, auto open, auto waves) {
     typedef decltype(type) T;
     auto kernel = top > 0 ? token_log_probs_kernel<T, true, nt.value, ch.value, open.value, waves.value>
                           : token_log_probs_kernel<T, false, nt.value, ch.value, open.value, waves.value>;
@@ -964,7 +970,7 @@ void launch_token_log_probs_backward(const LogitRows& a, const int64_t* tokens, 
                                      RowGradient d_entropy, int top, const int64_t* top_tokens, const float* d_top,
                                      void* grad, int64_t ld_grad, hipStream_t st) {
   const bool stream = gradient_bytes(a) > kStreamBehindForward;
-  pick_row(a, 0, [&](auto type, auto nt, auto ch, auto open, auto waves) {
+  pick_row<false>(a, 0, [&](auto type, auto nt, auto ch, auto open, auto waves) {
     typedef decltype(type) T;
     hipLaunchKernelGGL((token_log_probs_backward_kernel<T, nt.value, ch.value, open.value, waves.value>),
                        grid_of<nt.value>(a), block_of<nt.value>(), 0, st, (const T*)a.x, a.ld, a.rows, a.vocab, tokens,
@@ -976,14 +982,17 @@ void launch_distillation(const LogitRows& a, const int64_t* teacher_tokens, cons
                          int k, const float* weights, RowGradient d_losses, float* losses, void* grad, int64_t ld_grad,
                          hipStream_t st) {
   const bool stream = gradient_bytes(a) > (losses == nullptr ? kStreamBehindForward : kStreamOnePass);
-  pick_row(a, 0, [&](auto type, auto nt, auto ch, auto open, auto waves) {
-    typedef decltype(type) T;
-    auto kernel = grad != nullptr ? distillation_kernel<T, true, nt.value, ch.value, open.value, waves.value>
-                                  : distillation_kernel<T, false, nt.value, ch.value, open.value, waves.value>;
-    hipLaunchKernelGGL(kernel, grid_of<nt.value>(a), block_of<nt.value>(), 0, st, (const T*)a.x, a.ld, a.rows, a.vocab,
-                       teacher_tokens, teacher, (int)teacher_f16, k, a.temperature, weights, d_losses, losses, (T*)grad,
-                       ld_grad, stream);
-  });
+  const auto launch = [&](auto gradient) {
+    pick_row<gradient.value>(a, 0, [&](auto type, auto nt, auto ch, auto open, auto waves) {
+      typedef decltype(type) T;
+      hipLaunchKernelGGL((distillation_kernel<T, gradient.value, nt.value, ch.value, open.value, waves.value>),
+                         grid_of<nt.value>(a), block_of<nt.value>(), 0, st, (const T*)a.x, a.ld, a.rows, a.vocab,
+                         teacher_tokens, teacher, (int)teacher_f16, k, a.temperature, weights, d_losses, losses, (T*)grad,
+                         ld_grad, stream);
+    });
+  };
+  if (grad != nullptr) launch(std::true_type{});
+  else launch(std::false_type{});
 }
 
 }  // namespace gptmi
