@@ -443,22 +443,24 @@ def _distillation(logits, teacher_tokens, teacher_logits, temperature, weights, 
     """(losses or None, gradient or None)."""
     what = "distillation_loss"
     dev, code, rows, V, ld = _logit_rows(logits, what)
-    _on_gpu(logits, teacher_tokens, teacher_logits, weights)
-    lead, k = logits.shape[:-1], teacher_tokens.shape[-1]
-    _check_row_tokens(teacher_tokens, (*lead, k), what)
-    _maybe_check_row_tokens(teacher_tokens, V, what)
-    assert teacher_logits.shape == teacher_tokens.shape, (teacher_logits.shape, teacher_tokens.shape)
-    assert teacher_logits.is_contiguous()
+    k = teacher_tokens.shape[-1]
     teacher_code = _dtype_code(teacher_logits, what)
-    assert k > 0
-    if k > MAX_TOP:
-        raise NotImplementedError(f"{what}: at most {MAX_TOP} of the teacher's logits a row, got {k}")
-    if weights is not None:
-        if weights.dtype != torch.float32:
-            raise TypeError(f"{what}: weights must be float32, got {weights.dtype}")
-        assert weights.shape == lead, (weights.shape, lead)
-        assert weights.is_contiguous()
-    _check_temperature(temperature, code, what)
+    if d_losses is None:  # the forward pass of a gradient has checked these
+        lead = logits.shape[:-1]
+        _on_gpu(logits, teacher_tokens, teacher_logits, weights)
+        _check_row_tokens(teacher_tokens, (*lead, k), what)
+        _maybe_check_row_tokens(teacher_tokens, V, what)
+        assert teacher_logits.shape == teacher_tokens.shape, (teacher_logits.shape, teacher_tokens.shape)
+        assert teacher_logits.is_contiguous()
+        assert k > 0
+        if k > MAX_TOP:
+            raise NotImplementedError(f"{what}: at most {MAX_TOP} of the teacher's logits a row, got {k}")
+        if weights is not None:
+            if weights.dtype != torch.float32:
+                raise TypeError(f"{what}: weights must be float32, got {weights.dtype}")
+            assert weights.shape == lead, (weights.shape, lead)
+            assert weights.is_contiguous()
+        _check_temperature(temperature, code, what)
     out = None
     if losses:
         out = logits.new_empty(lead, dtype=torch.float32) if weights is None else torch.empty_like(weights)
