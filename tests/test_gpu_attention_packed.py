@@ -97,7 +97,7 @@ def test_heads(K, gpu_device, d, heads):
 @pytest.mark.parametrize("d", [16, 32, 64, 128, 256])
 def test_many_blocks(K, gpu_device, d):
     """More blocks than run at once: 32 queries a wavefront, the heaviest blocks first (few sequences, few blocks) or in
-    the order of the slots (more than 256 sequences, more than 2560 blocks), with and without heads that one XCD has."""
+    the order of the slots (more than 256 sequences, or hardly a block each), with and without heads that one XCD has."""
     r = np.random.default_rng(19)
     for heads, lengths in (((64, 16), [700, 33, 0, 512, 255, 1]), ((20, 20), [65, 1000, 129, 0, 640, 2000]),
                            ((48, 12), r.integers(0, 30, 300).tolist()), ((72, 9), [1500, 31, 900, 2100]), ((64, 64), [1600]),
@@ -114,6 +114,22 @@ def test_many_blocks(K, gpu_device, d):
                     w, tol = want(q[rows, h:h + 1], k[rows, h // rep:h // rep + 1], v[rows, h // rep:h // rep + 1], d ** -0.5)
                     assert torch.all((out[rows, h:h + 1].double() - w).abs() <= tol), (heads, s, h)
         assert torch.all(torch.isfinite(out))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("heads", [(72, 9), (80, 16)])
+def test_long_in_the_order_of_slots(K, gpu_device, d, heads):
+    """Too many blocks for the heaviest of all heads to come first."""
+    lengths = [3000, 5100, 0, 2500]
+    q, k, v = make(np.random.default_rng(27), sum(lengths), *heads, d, True, gpu_device)
+    out = K.flash_attention_packed(q, k, v, starts_of(lengths, gpu_device))
+    rep = heads[0] // heads[1]
+    for first, L in ((0, 3000), (8100, 2500)):
+        rows = slice(first, first + L)
+        for h in (0, 35, heads[0] - 1):
+            w, tol = want(q[rows, h:h + 1], k[rows, h // rep:h // rep + 1], v[rows, h // rep:h // rep + 1], d ** -0.5)
+            assert torch.all((out[rows, h:h + 1].double() - w).abs() <= tol), (L, h)
+    assert torch.all(torch.isfinite(out))
 
 
 @pytest.mark.parametrize("d", [16, 32, 64, 128])
