@@ -416,11 +416,11 @@ __device__ __forceinline__ float kth_of_lanes(float v, int k) {
   return kth < 0x007fffffu ? -INFINITY : key_value((uint64_t)kth << 32);  // below -infinity's there are NaNs
 }
 
-// found(r, key) of the k largest logits, r = 0 .. k - 1 in any order, by one thread each.  A bound that at least k of them
-// reach is the k-th largest of the maxima of some groups of threads: of 64 groups up to
-// k = 32, of 256, by a histogram, beyond.  The logits that reach it are gathered, little more than k (some 24 for k = 20, 180 for
-// 128), from memory, since a row's registers held any longer are too many: the chunks of the few threads whose maximum
-// reaches it, one a thread, or the whole row.  A histogram leaves of more than 256 those from the k-th's bin on, and the rest is
+// found(r, key) of the k largest logits, r = 0 .. k - 1 in any order, by one thread each.  A bound that at least k of
+// them reach is the k-th largest of the maxima of some groups of threads: of 64 groups up to k = 32, of 256, by a
+// histogram, beyond.  The logits that reach it are gathered, little more than k (some 24 for k = 20, 180 for 128), from
+// memory, since a row's registers held any longer are too many: the chunks of the few threads whose maximum reaches it,
+// one a thread, or the whole row.  A histogram leaves of more than 256 those from the k-th's bin on, and the rest is
 // ranked by counting.  2048 rows of 50257 fp16 logits, us: no top tokens 40, 1 53, 20 49, 64 58, 128 84.
 template <typename T, int NT, int CH, bool OPEN, typename F>
 __device__ __forceinline__ void row_top(const Row<T, NT, CH, OPEN>& row, int k, Tops tops, float high, TopShared<NT>& top,
@@ -645,8 +645,8 @@ struct Special {
   float x[kMaxTop + 1], add[kMaxTop + 1], total[kMaxTop + 1];
 };
 
-// The entries lane, lane + 64, .. of a row, by the first wavefront and for all behind the next barrier: f(i, token, part, logit)
-// gives entry i, token -1 for none.
+// The entries lane, lane + 64, .. of a row, by the first wavefront and for all behind the next barrier: f(i, token,
+// part, logit) gives entry i, token -1 for none.
 template <typename T, int NT, int CH, bool OPEN, typename F>
 __device__ __forceinline__ void set_special(const Row<T, NT, CH, OPEN>& row, Special<NT>& sp, int count, F f) {
   const int lane = threadIdx.x;
@@ -897,13 +897,14 @@ __global__ __launch_bounds__(NT * kRowsOf<NT>, WAVES) void distillation_kernel(
 }
 
 // f(threads, chunks a thread, wavefronts a SIMD) as integral constants for rows of this many chunks.  A row takes 4 CH
-// registers a thread and some 26 more, so few threads with long parts keep the most rows on a CU: of 50257 fp16 logits (6283
-// chunks) 3 with 512 threads, 4 with 256, 2 with 1024; 1477 rows scored 31 / 32 / 38 us, with their top 20 37 / 41 / 43; of 50304
-// fp32 logits (12576 chunks), forward and backward of 2048 rows 216 with 512 threads, 225 with 1024, loss and gradient of 4096
-// 324 and 427.  WIDE, for a loss' gradient, whose stores are what it waits for: 1024 threads where a thread then has up to 8
-// chunks; 2048 rows of 50257 fp16 logits 512 / 1024 threads 85 / 78, with the loss 90 / 83, of 65024 102 / 99 and 108 / 105, of 32000
-// fp32 99 / 97 and 105 / 102, but the gradient of log probabilities 86 / 90.  Rows of up to 256 chunks have a wavefront each,
-// four a workgroup; the longest, beyond 20480 chunks, are read again behind those.  min_threads: what the call needs.
+// registers a thread and some 26 more, so few threads with long parts keep the most rows on a CU: of 50257 fp16 logits
+// (6283 chunks) 3 with 512 threads, 4 with 256, 2 with 1024; 1477 rows scored 31 / 32 / 38 us, with their top 20 37 /
+// 41 / 43; of 50304 fp32 logits (12576 chunks), forward and backward of 2048 rows 216 with 512 threads, 225 with 1024,
+// loss and gradient of 4096 324 and 427.  WIDE, for a loss' gradient, whose stores are what it waits for: 1024 threads
+// where a thread then has up to 8 chunks; 2048 rows of 50257 fp16 logits 512 / 1024 threads 85 / 78, with the loss 90 /
+// 83, of 65024 102 / 99 and 108 / 105, of 32000 fp32 99 / 97 and 105 / 102, but the gradient of log probabilities 86 /
+// 90.  Rows of up to 256 chunks have a wavefront each, four a workgroup; the longest, beyond 20480 chunks, are read
+// again behind those.  min_threads: what the call needs.
 template <bool WIDE, typename F>
 void pick(int chunks, int min_threads, F f) {
 #define GPTMI_ROW(NT, CH, OPEN, WAVES)                                                                        \
@@ -939,13 +940,13 @@ dim3 grid_of(const LogitRows& a) {
   const int64_t n = (a.rows + kRowsOf<NT> - 1) / kRowsOf<NT>;
   return dim3((unsigned)(n < kGridRow ? n : kGridRow), (unsigned)((n + kGridRow - 1) / kGridRow));
 }
-// A gradient goes past the caches where it would push out the logits that the forward pass left in the memory-side cache of
-// 256 MB, whose last rows a backward pass therefore takes first, and a one-pass gradient where it would not stay there
-// itself (what waits there for its way to memory is written while the next kernel reads); always where rows are so long
-// that they are read again.  us, without / with, 50304 logits: forward and backward of 1024 fp32 rows (206 MB) 129 / 115,
-// with a sum that reads the gradient 171 / 167, of 2048 246 / 216 and 329 / 326 (the first rows first 250 and 342), of 768
-// rows (155 MB) with the sum 126 / 131; one pass of 2048 fp16 rows (206 MB) 89 / 84, but with the sum 139 / 149, of 1536
-// fp32 rows (309 MB) 129 / 121 and 210 / 207; of 512 rows of 128256 fp32 logits 129 / 108.
+// A gradient goes past the caches where it would push out the logits that the forward pass left in the memory-side
+// cache of 256 MB, whose last rows a backward pass therefore takes first, and a one-pass gradient where it would not
+// stay there itself (what waits there for its way to memory is written while the next kernel reads); always where rows
+// are so long that they are read again.  us, without / with, 50304 logits: forward and backward of 1024 fp32 rows (206
+// MB) 129 / 115, with a sum that reads the gradient 171 / 167, of 2048 246 / 216 and 329 / 326 (the first rows first
+// 250 and 342), of 768 rows (155 MB) with the sum 126 / 131; one pass of 2048 fp16 rows (206 MB) 89 / 84, but with the
+// sum 139 / 149, of 1536 fp32 rows (309 MB) 129 / 121 and 210 / 207; of 512 rows of 128256 fp32 logits 129 / 108.
 constexpr int64_t kStreamBehindForward = 192 << 20, kStreamOnePass = 256 << 20;
 int64_t gradient_bytes(const LogitRows& a) { return a.rows * a.vocab * (a.f16 ? 2 : 4); }
 

@@ -200,8 +200,9 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
     }
   }
 
-  // ---- tile loads: wavefronts 0-1 bring K, 2-3 V, 32 rows each; with two parts one wavefront of each K and one V.  Load j's rows are RPI j further on, which the scalar
-  // base takes, and their keys differ by bits that are the same for all lanes; a sequence's last tile repeats its last row.
+  // ---- tile loads: wavefronts 0-1 bring K, 2-3 V, 32 rows each; with two parts one wavefront of each K and one V.
+  // Load j's rows are RPI j further on, which the scalar base takes, and their keys differ by bits that are the same
+  // for all lanes; a sequence's last tile repeats its last row.
   const bool brings_v = P == 1 ? wave >= 2 : wave & 1;
   const int first_row = P == 1 ? (wave & 1) * 32 : 0;
   const int64_t pitch = (brings_v ? a.v_row : a.k_row) * 2;
@@ -211,7 +212,8 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
   const unsigned lane_row = (unsigned)lrow * (unsigned)pitch;
   auto issue_tile = [&](int nth) {  // of this part's tiles
     const int t = nth * P + part;
-    const unsigned dst = smem_base + (unsigned)((part * 4 + (brings_v ? 2 : 0) + (nth & 1)) * TILE) + (unsigned)(first_row * ROWB);
+    const int place = part * 4 + (brings_v ? 2 : 0) + (nth & 1);
+    const unsigned dst = smem_base + (unsigned)(place * TILE + first_row * ROWB);
     const char* base = src + (int64_t)t * kKeys * pitch;
     const int rest = L - 1 - t * kKeys - first_row;  // the last row of this wavefront's
     if (rest >= ROWS - 1) {
@@ -528,17 +530,18 @@ int launch_as(PackedArgs a, int64_t slots, hipStream_t st) {
   return 0;
 }
 
-// While the workgroups run at once, the launch takes what a wavefront's chain through its key tiles takes: 0.5 us a tile
-// for 16 queries, 0.8 for 32.  So up to 2.5 workgroups a CU of 32 queries, in two parts of the key tiles; up to 2 of 64
-// in two parts, 3 or 4 the longer the sequences are, which then hide what a workgroup begins and ends with; up to 5 of 64
-// queries, 16 a wavefront; and 32 a wavefront beyond: K and V are read from LDS for more queries at a time.  us, 16 / 32 / 16 in two parts / 32 in two parts: 1 x 1024 rows of
-// 12 heads 15.8 / 18.7 / 10.4 / 12.7 (396 workgroups in two parts, 204 of 64 queries), 1 x 2500 34.1 / 39.5 / 25.3 / 27.5
-// (948, 480), 1 x 4096 56.3 / 64.6 / 57.5 / 44.0 (1548, 780), 1 x 1024 of 25 heads 16.4 / 19.1 / 15.1 / 13.9 (825, 425), 1 x
-// 2048 32.1 / 35.1 / 35.7 / 29.0 (1625, 825), 8 x 150 9.9 / 9.9 / 11.5 / 12.5 (1125, 650), 4 x 1024 of 12 19.8 / 22.6 /
-// 32.3 / 23.3 (1584, 816), 16 x 300 11.3 / 13.0 / 23.7 / 16.3 (2184, 1092), 48 of up to 1024 24.0 / 22.3 / 53.8 / 34.1
-// (3408, 1992), 2 x 8192 293 / 245 / 361 / 320.  d = 128: two parts fill a CU's LDS, 1 x 1024 of 12 heads 20.5 / 27.1 / 19.4 /
-// 19.7, 1 x 1024 of 32 over 8 23.1 / 28.2 / 42.1 / 27.1: not taken.  64 queries a wavefront were slower yet: 1 x 16384 of 25
-// heads 16 / 32 / 64 1046 / 969 / 997 in an earlier state.  d = 256 has one workgroup a CU either way.
+// While the workgroups run at once, the launch takes what a wavefront's chain through its key tiles takes: 0.5 us a
+// tile for 16 queries, 0.8 for 32.  So up to 2.5 workgroups a CU of 32 queries, in two parts of the key tiles; up to 2
+// of 64 in two parts, 3 or 4 the longer the sequences are, which then hide what a workgroup begins and ends with; up to
+// 5 of 64 queries, 16 a wavefront; and 32 a wavefront beyond: K and V are read from LDS for more queries at a time.
+// us, 16 / 32 / 16 in two parts / 32 in two parts: 1 x 1024 rows of 12 heads 15.8 / 18.7 / 10.4 / 12.7 (396 workgroups
+// in two parts, 204 of 64 queries), 1 x 2500 34.1 / 39.5 / 25.3 / 27.5 (948, 480), 1 x 4096 56.3 / 64.6 / 57.5 / 44.0
+// (1548, 780), 1 x 1024 of 25 heads 16.4 / 19.1 / 15.1 / 13.9 (825, 425), 1 x 2048 32.1 / 35.1 / 35.7 / 29.0 (1625,
+// 825), 8 x 150 9.9 / 9.9 / 11.5 / 12.5 (1125, 650), 4 x 1024 of 12 19.8 / 22.6 / 32.3 / 23.3 (1584, 816), 16 x 300
+// 11.3 / 13.0 / 23.7 / 16.3 (2184, 1092), 48 of up to 1024 24.0 / 22.3 / 53.8 / 34.1 (3408, 1992), 2 x 8192 293 / 245 /
+// 361 / 320.  d = 128: two parts fill a CU's LDS, 1 x 1024 of 12 heads 20.5 / 27.1 / 19.4 / 19.7, 1 x 1024 of 32 over 8
+// 23.1 / 28.2 / 42.1 / 27.1: not taken.  64 queries a wavefront were slower yet: 1 x 16384 of 25 heads 16 / 32 / 64
+// 1046 / 969 / 997 in an earlier state.  d = 256 has one workgroup a CU either way.
 template <int D>
 int launch_d(const PackedArgs& a, hipStream_t st) {
   const int64_t slots32 = a.rows / 32 + a.sequences, slots = a.rows / 64 + a.sequences;

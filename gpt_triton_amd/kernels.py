@@ -681,13 +681,17 @@ def flash_attention_packed(q, k, v, starts, scale=None, out=None):
     if starts.dtype != torch.int64:
         raise TypeError(f"flash_attention_packed: starts must be int64, got {starts.dtype}")
     dev = _on_gpu(q, k, v, starts, out)
-    pitches = []
-    for t in (q, k, v):
-        row, head, one = t.stride()
-        assert one == 1, "the elements of a head must lie side by side"
-        if (row | head) & 7 or t.data_ptr() & 15:
-            raise NotImplementedError("flash_attention_packed: heads must start at multiples of 16 bytes")
-        pitches += (row, head)
+    (q_row, q_head, q_one), (k_row, k_head, k_one), (v_row, v_head, v_one) = q.stride(), k.stride(), v.stride()
+    assert q_one == k_one == v_one == 1, "the elements of a head must lie side by side"
+    if T == 1:  # whatever the pitch of one is
+        q_row = k_row = v_row = 0
+    if N == 1:
+        q_head = 0
+    if G == 1:
+        k_head = v_head = 0
+    q_at, k_at, v_at = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    if (q_row | q_head | k_row | k_head | v_row | v_head) & 7 or (q_at | k_at | v_at) & 15:
+        raise NotImplementedError("flash_attention_packed: heads must start at multiples of 16 bytes")
     if scale is None:
         scale = d ** -0.5
     if not 1e-20 <= scale <= 1e20:
@@ -696,11 +700,16 @@ def flash_attention_packed(q, k, v, starts, scale=None, out=None):
         out = q.new_empty((T, N, d))
     else:
         assert out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous()
-        if out.data_ptr() & 15:
+        at = out.data_ptr()
+        if at & 15:
             raise NotImplementedError("flash_attention_packed: out must start at a multiple of 16 bytes")
+        for x, start, last in ((q, q_at, (T - 1) * q_row + (N - 1) * q_head), (k, k_at, (T - 1) * k_row + (G - 1) * k_head),
+                               (v, v_at, (T - 1) * v_row + (G - 1) * v_head)):
+            apart = start + 2 * (last + d) <= at or at + 2 * T * N * d <= start
+            assert apart or T == 0 or (x is q and start == at and q.is_contiguous()), "out may be a dense q alone"
     if T > 0:
-        _call(dev, "flash_attention_packed", _lib.load().gptmi_flash_attn_packed, q.data_ptr(), k.data_ptr(),
-              v.data_ptr(), out.data_ptr(), starts.data_ptr(), starts.shape[0] - 1, T, N, G, d, *pitches, scale,
+        _call(dev, "flash_attention_packed", _lib.load().gptmi_flash_attn_packed, q_at, k_at, v_at, out.data_ptr(),
+              starts.data_ptr(), starts.shape[0] - 1, T, N, G, d, q_row, q_head, k_row, k_head, v_row, v_head, scale,
               _lib.GPTMI_F16)
     return out
 

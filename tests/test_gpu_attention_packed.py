@@ -338,6 +338,10 @@ def test_views_and_pitches(K, gpu_device):
     assert torch.equal(K.flash_attention_packed(spaced(q), spaced(k), spaced(v), starts_of(lengths, gpu_device)), base)
     one_key_head = k[:, :1].expand(-1, 2, -1)  # a pitch of 0
     check(K, q, one_key_head, v, lengths)
+    # one row, one head: no pitch at all
+    odd = torch.randn(3, 1, 67, dtype=torch.float16, device=gpu_device)
+    token = odd[:1, :, :64]
+    check(K, token.expand(1, 4, 64), token, token, [1])
 
 
 def test_rows_beyond_32_bits(K, gpu_device):

@@ -25,3 +25,20 @@ def test_refusals(gpu_device):
             call(*args, **more)
     empty = call(q[:0], k[:0], v[:0], torch.tensor([0, 0], device=gpu_device))
     assert empty.shape == (0, 4, 64)
+
+
+def test_out_that_overlaps(gpu_device):
+    from gpt_triton_amd import kernels as K
+
+    buf = torch.randn(4, 40, 4, 64, device=gpu_device).half()
+    q, k, v, out = buf
+    starts = torch.tensor([0, 40], device=gpu_device)
+    want = K.flash_attention_packed(q, k, v, starts)
+    for bad in (k, v, buf.view(-1, 4, 64)[1:41], buf.view(-1, 4, 64)[79:119], buf.view(-1, 4, 64)[81:121]):
+        with pytest.raises(AssertionError):
+            K.flash_attention_packed(q, k, v, starts, out=bad)
+    with pytest.raises(AssertionError):  # q's columns of a product, whose rows are not dense
+        wide = torch.randn(40, 12, 64, device=gpu_device).half()
+        K.flash_attention_packed(*wide.split(4, dim=1), starts, out=wide.view(-1, 4, 64)[:40])
+    assert torch.equal(K.flash_attention_packed(q, k, v, starts, out=out), want)
+    assert torch.equal(K.flash_attention_packed(q, k, v, starts, out=q), want)
