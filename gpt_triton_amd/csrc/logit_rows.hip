@@ -236,8 +236,9 @@ __device__ __forceinline__ int scan_exclusive(int c, Shared<NT>& sh, int& total)
 // a thread takes its logits in groups of G chunks, of each first the maximum, which is then the reference of what it has
 // summed (so that no exponent is above 0 and u never changes sign), and keeps the largest logit so far out of the sums:
 // where a larger one comes, the old one goes in.  The groups' sums start while later groups are on their way.
-// TOP: the maxima of 64 and of 256 groups of threads go to sh.groups and sh.many; low: the least of the latter above
-// -infinity; mine: this thread's maximum; a NaN counts as -infinity.
+// TOP: the maxima of 64 and of 256 groups of threads go to sh.groups and sh.many, a thread with a NaN as -infinity there
+// (its other logits may reach what the groups' bound is, which holds without them); low: the least of the latter above
+// -infinity; mine: this thread's maximum, NaN where it has met one.
 struct Tops {
   float low, mine;
 };
@@ -325,8 +326,8 @@ __device__ __forceinline__ Stats<T> row_stats(Row<T, NT, CH, OPEN>& row, float t
     }
   };
   if constexpr (TOP) {
-    tops->mine = fmaxf(mine, -INFINITY);
-    float g = tops->mine;
+    tops->mine = mine;
+    float g = fmaxf(mine, -INFINITY);
     constexpr int SMALL = NT >= 256 ? NT / 256 : 1, LANES = NT / 64;
     if constexpr (SMALL > 1) g = fmaxf(g, from_lane<1>(g));
     if constexpr (SMALL > 2) g = fmaxf(g, from_lane<2>(g));
@@ -419,8 +420,8 @@ __device__ __forceinline__ float kth_of_lanes(float v, int k) {
 // found(r, key) of the k largest logits, r = 0 .. k - 1 in any order, by one thread each.  A bound that at least k of
 // them reach is the k-th largest of the maxima of some groups of threads: of 64 groups up to k = 32, of 256, by a
 // histogram, beyond.  The logits that reach it are gathered, little more than k (some 24 for k = 20, 180 for 128), from
-// memory, since a row's registers held any longer are too many: the chunks of the few threads whose maximum reaches it,
-// one a thread, or the whole row.  A histogram leaves of more than 256 those from the k-th's bin on, and the rest is
+// memory, since a row's registers held any longer are too many: the chunks of the few threads whose maximum reaches it
+// or is NaN, one a thread, or the whole row.  A histogram leaves of more than 256 those from the k-th's bin on, and the rest is
 // ranked by counting.  2048 rows of 50257 fp16 logits, us: no top tokens 40, 1 53, 20 49, 64 58, 128 84.
 template <typename T, int NT, int CH, bool OPEN, typename F>
 __device__ __forceinline__ void row_top(const Row<T, NT, CH, OPEN>& row, int k, Tops tops, float high, TopShared<NT>& top,
@@ -499,7 +500,7 @@ __device__ __forceinline__ void row_top(const Row<T, NT, CH, OPEN>& row, int k, 
   auto above = [&](float y) { return y > low; };
   int n = kKeep + 1;  // all logits reach -infinity: not gathered
   if (low > -INFINITY) {
-    const uint64_t in = __ballot(tops.mine >= low);
+    const uint64_t in = __ballot(!(tops.mine < low));  // NaN: others of the thread may reach it
     if (in) {
       int at = 0;
       if (lane == 0) at = atomicAdd(&top.threads, __popcll(in));
