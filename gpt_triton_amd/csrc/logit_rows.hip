@@ -794,7 +794,8 @@ __global__ __launch_bounds__(NT * kRowsOf<NT>, WAVES) void token_log_probs_backw
   const float scale = uniform(st.inv * st.inv_tau), lift = uniform(st.entropy - st.log_s - kLn2 * st.t.rest());
   write_gradient(row, o, sp, st.S != 0.f, st.inv_tau, stream, [&](float y) {
     const float t = st.t(y), p = __builtin_amdgcn_exp2f(t) * scale;
-    return -p * fmaf(h, fmaf(kLn2, fmaxf(t, -1e30f), lift), g);
+    // an exponent below -200 is as good as -200, where p is 0: h times an infinite one would make a NaN of that 0
+    return -p * fmaf(h, fmaf(kLn2, fmaxf(t, -200.f), lift), g);
   });
 }
 
