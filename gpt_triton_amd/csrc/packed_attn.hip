@@ -42,6 +42,12 @@ __device__ __forceinline__ void load_lds16(const void* base, unsigned lane_off, 
 // Without the compiler's quieting of NaNs in front; one makes a NaN of the row, which is looked for at the end.
 __device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
+// A mean of finite fp16 values is at most the largest of them, 65504, but its weights as rounded may make up to 2^-11 more
+// than 1, and what is above 65519 would be an infinity.
+__device__ __forceinline__ float bounded(float x) {
+  return fabsf(x) < INFINITY ? __builtin_amdgcn_fmed3f(x, -65504.f, 65504.f) : x;
+}
+
 // Slots: sequence s, which starts at row a, has its blocks of R queries from slot a / R + s on, which leaves room for
 // every sequence whatever the lengths are (floor(a / R) + floor(len / R) <= floor((a + len) / R)), needs no
 // lengths on the host and no pass over them on the GPU.  Slots that are left over hold nothing.
@@ -489,7 +495,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
     for (int i = 0; i < DB; ++i) {
       h4 x;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) x[r] = (_Float16)oacc[n][i][r];
+      for (int r = 0; r < 4; ++r) x[r] = (_Float16)bounded(oacc[n][i][r]);
       if (q < L) *reinterpret_cast<h4*>(o + 16 * i) = x;
     }
   }
