@@ -703,10 +703,12 @@ def flash_attention_packed(q, k, v, starts, scale=None, out=None):
         at = out.data_ptr()
         if at & 15:
             raise NotImplementedError("flash_attention_packed: out must start at a multiple of 16 bytes")
-        for x, start, last in ((q, q_at, (T - 1) * q_row + (N - 1) * q_head), (k, k_at, (T - 1) * k_row + (G - 1) * k_head),
-                               (v, v_at, (T - 1) * v_row + (G - 1) * v_head)):
-            apart = start + 2 * (last + d) <= at or at + 2 * T * N * d <= start
-            assert apart or T == 0 or (x is q and start == at and q.is_contiguous()), "out may be a dense q alone"
+        end = at + 2 * T * N * d
+        for start, last, may in ((q_at, (T - 1) * q_row + (N - 1) * q_head, q.is_contiguous()),
+                                 (k_at, (T - 1) * k_row + (G - 1) * k_head, False),
+                                 (v_at, (T - 1) * v_row + (G - 1) * v_head, False)):
+            apart = start + 2 * (last + d) <= at or end <= start
+            assert apart or T == 0 or (may and start == at), "out may be a dense q alone"
     if T > 0:
         _call(dev, "flash_attention_packed", _lib.load().gptmi_flash_attn_packed, q_at, k_at, v_at, out.data_ptr(),
               starts.data_ptr(), starts.shape[0] - 1, T, N, G, d, q_row, q_head, k_row, k_head, v_row, v_head, scale,
