@@ -704,10 +704,11 @@ def flash_attention_packed(q, k, v, starts, scale=None, out=None):
         if at & 15:
             raise NotImplementedError("flash_attention_packed: out must start at a multiple of 16 bytes")
         end = at + 2 * T * N * d
-        for start, last, may in ((q_at, (T - 1) * q_row + (N - 1) * q_head, q.is_contiguous()),
-                                 (k_at, (T - 1) * k_row + (G - 1) * k_head, False),
-                                 (v_at, (T - 1) * v_row + (G - 1) * v_head, False)):
-            apart = start + 2 * (last + d) <= at or end <= start
+        for start, size, may in ((q_at, 2 * ((T - 1) * q_row + (N - 1) * q_head + d), q.is_contiguous()),
+                                 (k_at, 2 * ((T - 1) * k_row + (G - 1) * k_head + d), False),
+                                 (v_at, 2 * ((T - 1) * v_row + (G - 1) * v_head + d), False),
+                                 (starts.data_ptr(), 8 * starts.shape[0], False)):
+            apart = start + size <= at or end <= start
             assert apart or T == 0 or (may and start == at), "out may be a dense q alone"
     if T > 0:
         _call(dev, "flash_attention_packed", _lib.load().gptmi_flash_attn_packed, q_at, k_at, v_at, out.data_ptr(),

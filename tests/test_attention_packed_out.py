@@ -38,3 +38,16 @@ def test_one_tensor_in_several_places(calls):
     assert kernels.flash_attention_packed(x, y, y, starts, out=x.view(5, 4, 64)).data_ptr() == x.data_ptr()
     assert kernels.flash_attention_packed(x[:0], x[:0], x[:0], starts, out=x[:0]).shape == (0, 4, 64)
     assert len(calls) == 3
+
+
+def test_starts_inside_out(calls):
+    buf = aligned(8, 4, 64)
+    x, y = aligned(7, 4, 64), aligned(7, 4, 64)
+    for first, last in ((0, 2), (100, 103), (446, 448)):  # of 7 * 4 * 64 / 4 = 448 int64, the last two of them out's
+        starts = buf.view(-1).view(torch.int64)[first:last]
+        with pytest.raises(AssertionError, match="out"):
+            kernels.flash_attention_packed(x, y, y, starts, out=buf[:7])
+    assert not calls
+    kernels.flash_attention_packed(x, y, y, buf.view(-1).view(torch.int64)[448:451], out=buf[:7])
+    kernels.flash_attention_packed(x, y, y, buf.view(-1).view(torch.int64)[0:3], out=buf[1:])
+    assert len(calls) == 2
