@@ -29,6 +29,7 @@ import math
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -380,6 +381,14 @@ def _first_derivative(what):
         raise RuntimeError(f"{what} has a first derivative only")
 
 
+def _no_tangents(what, *tensors):
+    # the calls that leave torch's graph alone would drop them; a level of dual tensors is rarely open
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{what} has no forward-mode derivative")
+
+
 def _row_gradient(g):
     """(address, pitch in rows, what to keep until the call) of a gradient with an element a row; autograd hands one
     number for all rows on as a view of pitch 0."""
@@ -433,6 +442,7 @@ def token_log_probs(logits, tokens=None, top=0, temperature=1.0):
 
     fp32 (the tokens int64) whatever the logits' type.  Logits of -infinity mark tokens that cannot occur.  Gradients flow
     to the logits from all but top_tokens.  temperature from 1e-4 on (fp32 logits: 1e-30) to 1e30."""
+    _no_tangents("token_log_probs", logits)
     temperature = float(temperature)
     if logits.requires_grad and torch.is_grad_enabled():
         return TokenLogProbs(*_TokenLogProbsFunction.apply(logits, tokens, top, temperature))
@@ -488,8 +498,9 @@ class _DistillationFunction(torch.autograd.Function):
         return grad, None, None, None, None
 
 
-def _constants(*tensors):
-    assert not any(t is not None and t.requires_grad for t in tensors), "only the logits have a gradient"
+def _check_derivatives(logits, *constants):
+    assert not any(t is not None and t.requires_grad for t in constants), "only the logits have a gradient"
+    _no_tangents("distillation_loss", logits, *constants)
 
 
 def distillation_loss(logits, teacher_tokens, teacher_logits, temperature=1.0, weights=None):
@@ -502,7 +513,7 @@ def distillation_loss(logits, teacher_tokens, teacher_logits, temperature=1.0, w
     k up to MAX_TOP.  An entry whose token is outside [0, V) or whose logit is -infinity counts for nothing.  weights [..]
     (float32, all 1 if None): 0 marks padding, whose logits may be anything.  Gradients flow to the logits alone, which
     are read again for them; `distillation_loss_and_grad` has both in one pass.  temperature as in `token_log_probs`."""
-    _constants(teacher_logits, weights)
+    _check_derivatives(logits, teacher_logits, weights)
     temperature = float(temperature)
     if logits.requires_grad and torch.is_grad_enabled():
         return _DistillationFunction.apply(logits, teacher_tokens, teacher_logits, temperature, weights)
@@ -513,7 +524,7 @@ def distillation_loss_and_grad(logits, teacher_tokens, teacher_logits, temperatu
     """(losses, gradient of their sum with respect to the logits) of `distillation_loss` from one pass over the logits, for
     steps that know the weights of their rows beforehand: `logits.backward(gradient)` goes on from there.  The
     gradient has the logits' shape and type; the rows of padded logits' gradient are padded too."""
-    _constants(teacher_logits, weights)
+    _check_derivatives(logits, teacher_logits, weights)
     return _distillation(logits, teacher_tokens, teacher_logits, float(temperature), weights, True, True)
 
 
