@@ -428,8 +428,9 @@ __device__ __forceinline__ float kth_of_lanes(float v, int k) {
 // them reach is the k-th largest of the maxima of some groups of threads: of 64 groups up to k = 32, of 256, by a
 // histogram, beyond.  The logits that reach it are gathered, little more than k (some 24 for k = 20, 180 for 128), from
 // memory, since a row's registers held any longer are too many: the chunks of the few threads whose maximum reaches it
-// or is NaN, one a thread, or the whole row.  A histogram leaves of more than 256 those from the k-th's bin on, and the rest is
-// ranked by counting.  2048 rows of 50257 fp16 logits, us: no top tokens 40, 1 53, 20 49, 64 58, 128 84.
+// or is NaN, one a thread, or the whole row.  A histogram leaves of more than 256 those from the k-th's bin on, and the
+// rest is ranked by counting.  2048 rows of 50257 fp16 logits, us: no top tokens 41, 1 41, 5 42, 20 46, 64 57, 128 80; 16384 of
+// 300: none 16, 20 33, 128, for which a row has 256 threads and most groups nothing, 123.
 template <typename T, int NT, int CH, bool OPEN, typename F>
 __device__ __forceinline__ void row_top(const Row<T, NT, CH, OPEN>& row, int k, Tops tops, float high, TopShared<NT>& top,
                                         Shared<NT>& sh, F found) {

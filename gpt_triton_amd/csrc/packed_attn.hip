@@ -544,10 +544,10 @@ int launch_as(PackedArgs a, int64_t slots, hipStream_t st) {
 // in two parts, 204 of 64 queries), 1 x 2500 34.1 / 39.5 / 25.3 / 27.5 (948, 480), 1 x 4096 56.3 / 64.6 / 57.5 / 44.0
 // (1548, 780), 1 x 1024 of 25 heads 16.4 / 19.1 / 15.1 / 13.9 (825, 425), 1 x 2048 32.1 / 35.1 / 35.7 / 29.0 (1625,
 // 825), 8 x 150 9.9 / 9.9 / 11.5 / 12.5 (1125, 650), 4 x 1024 of 12 19.8 / 22.6 / 32.3 / 23.3 (1584, 816), 16 x 300
-// 11.3 / 13.0 / 23.7 / 16.3 (2184, 1092), 48 of up to 1024 24.0 / 22.3 / 53.8 / 34.1 (3408, 1992), 2 x 8192 293 / 245 /
-// 361 / 320.  d = 128: two parts fill a CU's LDS, 1 x 1024 of 12 heads 20.5 / 27.1 / 19.4 / 19.7, 1 x 1024 of 32 over 8
-// 23.1 / 28.2 / 42.1 / 27.1: not taken.  64 queries a wavefront were slower yet: 1 x 16384 of 25 heads 16 / 32 / 64
-// 1046 / 969 / 997 in an earlier state.  d = 256 has one workgroup a CU either way.
+// 11.3 / 13.0 / 23.7 / 16.3 (2184, 1092), 48 of up to 1024 (7558 rows) 24.0 / 22.3 / 53.8 / 34.1 (3408, 1992), 2 x 8192
+// 293 / 245 / 361 / 320.  d = 128: two parts fill a CU's LDS, 1 x 1024 of 12 heads 20.5 / 27.1 / 19.4 / 19.7, 1 x 1024 of
+// 32 over 8 23.1 / 28.2 / 42.1 / 27.1: not taken.  64 queries a wavefront were slower yet: 1 x 16384 of 25 heads 16 / 32 /
+// 64 1046 / 969 / 997 in an earlier state.  d = 256 has one workgroup a CU either way.
 template <int D>
 int launch_d(const PackedArgs& a, hipStream_t st) {
   const int64_t slots32 = a.rows / 32 + a.sequences, slots = a.rows / 64 + a.sequences;

@@ -440,8 +440,9 @@ def token_log_probs(logits, tokens=None, top=0, temperature=1.0):
         top_log_probs  [.., top]  the `top` most likely tokens, the likeliest first, equal ones in the order of their
         top_tokens     [.., top]  ids, at most MAX_TOP; None for top = 0
 
-    fp32 (the tokens int64) whatever the logits' type.  Logits of -infinity mark tokens that cannot occur.  Gradients flow
-    to the logits from all but top_tokens.  temperature from 1e-4 on (fp32 logits: 1e-30) to 1e30."""
+    fp32 (the tokens int64, contiguous) whatever the logits' type.  Logits of -infinity mark tokens that cannot occur, and a
+    row with a NaN, which is -infinity among the top tokens, or +infinity scores NaN.  Gradients flow to the logits from
+    all but top_tokens, backward and once.  temperature from 1e-4 on (fp32 logits: 1e-30) to 1e30."""
     _no_tangents("token_log_probs", logits)
     temperature = float(temperature)
     if logits.requires_grad and torch.is_grad_enabled():
@@ -510,9 +511,11 @@ def distillation_loss(logits, teacher_tokens, teacher_logits, temperature=1.0, w
 
         weights * sum_i q_i (log q_i - log p[teacher_tokens_i])
 
-    k up to MAX_TOP.  An entry whose token is outside [0, V) or whose logit is -infinity counts for nothing.  weights [..]
-    (float32, all 1 if None): 0 marks padding, whose logits may be anything.  Gradients flow to the logits alone, which
-    are read again for them; `distillation_loss_and_grad` has both in one pass.  temperature as in `token_log_probs`."""
+    k up to MAX_TOP; all but the logits contiguous.  An entry whose token is outside [0, V) or whose logit is -infinity
+    counts for nothing; a row without entries has loss and gradient 0, whatever its logits are.  weights [..] (float32, all
+    1 if None): 0 marks padding, whose logits may be anything.  Gradients flow to the logits alone, which are read again
+    for them, backward and once; `distillation_loss_and_grad` has both in one pass.  temperature as in
+    `token_log_probs`."""
     _check_derivatives(logits, teacher_logits, weights)
     temperature = float(temperature)
     if logits.requires_grad and torch.is_grad_enabled():

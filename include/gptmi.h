@@ -177,6 +177,7 @@ int gptmi_token_log_probs_backward(const void* logits, int64_t ld, const int64_t
  * [0, V) or whose logit is -infinity counts for nothing; a token that is there twice counts twice.  A row without
  * entries, or of weight 0 (padding), has loss 0 and gradient 0 whatever its logits are, and where no losses are asked for
  * a row of d_losses 0 gradient 0 too; a student that gives the teacher's tokens no probability at all has loss +infinity.
+ * An entry whose q fp32 rounds to 0 counts for nothing in the loss, whatever the student gives its token.
  * weights may be NULL (all 1), losses or grad may be NULL; grad as in gptmi_token_log_probs_backward.  teacher_dtype:
  * the type of teacher_logits.
  */
