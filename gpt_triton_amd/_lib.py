@@ -58,6 +58,9 @@ SIGNATURES = {
     "gptmi_flash_attn": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _f32, _f32,
                                 _u64, _int, _int, _vp]),
     "gptmi_flash_attn_packed": (_int, [_vp] * 5 + [_i64] * 11 + [_f32, _int, _vp]),
+    "gptmi_flash_attn_packed_train": (_int, [_vp] * 6 + [_i64] * 11 + [_f32, _int, _vp]),
+    "gptmi_flash_attn_packed_backward_workspace_bytes": (_sz, [_i64, _i64]),
+    "gptmi_flash_attn_packed_backward": (_int, [_vp] * 10 + [_i64] * 11 + [_f32, _vp, _sz, _int, _vp]),
 }
 
 _lib = None

@@ -760,37 +760,94 @@ int gptmi_flash_attn(const void* q, const void* k, const void* v, void* out, int
   return check_launch("flash_attn");
 }
 
+// What the calls on packed sequences check alike: q, k, v, starts, sizes, pitches and types; `more` are the addresses of
+// the call's other matrices or'ed together.
+static int check_packed(const char* what, const PackedAttention& p, int64_t d, uintptr_t more, int dtype) {
+  if (!p.q || !p.k || !p.v || !p.starts || p.sequences <= 0 || p.rows <= 0 || p.heads <= 0 || p.kv_heads <= 0 ||
+      p.heads % p.kv_heads != 0 || d <= 0 || !dtype_ok(dtype) || !(p.scale >= 1e-20f && p.scale <= 1e20f) ||
+      ((uintptr_t)p.starts & 7) != 0) {
+    set_error("%s: invalid argument", what);
+    return GPTMI_ERR_INVALID;
+  }
+  if (dtype != GPTMI_F16) {
+    set_error("%s: fp16 only", what);
+    return GPTMI_ERR_UNSUPPORTED;
+  }
+  const uintptr_t all = (uintptr_t)p.q | (uintptr_t)p.k | (uintptr_t)p.v | more;
+  if ((all & 15) != 0 || ((p.q_row | p.q_head | p.k_row | p.k_head | p.v_row | p.v_head) & 7) != 0) {
+    set_error("%s: q, k, v and out must be 16-byte aligned, and their pitches multiples of 8", what);
+    return GPTMI_ERR_INVALID;
+  }
+  // the kernels' offsets of a tile's 64 rows are 32-bit numbers of bytes
+  const auto pitch_ok = [](int64_t row) { return row >= 0 && row <= 1 << 24; };
+  const auto head_ok = [](int64_t head) { return head >= 0 && head <= 1ll << 40; };
+  if (!pitch_ok(p.q_row) || !pitch_ok(p.k_row) || !pitch_ok(p.v_row) || !head_ok(p.q_head) || !head_ok(p.k_head) ||
+      !head_ok(p.v_head) || p.rows >= 1ll << 31 || p.sequences > 1ll << 30 || p.heads > 1 << 20) {
+    set_error("%s: sizes or pitches beyond the supported", what);
+    return GPTMI_ERR_UNSUPPORTED;
+  }
+  return GPTMI_OK;
+}
+
+static int flash_attn_packed(const char* what, const PackedAttention& p, int64_t d, int dtype, void* stream) {
+  if (!p.out) {
+    set_error("%s: invalid argument", what);
+    return GPTMI_ERR_INVALID;
+  }
+  int rc = check_packed(what, p, d, (uintptr_t)p.out, dtype);
+  if (!rc) rc = launch_flash_attn_packed(p, (int)d, (hipStream_t)stream);
+  return rc ? rc : check_launch(what);
+}
+
 int gptmi_flash_attn_packed(const void* q, const void* k, const void* v, void* out, const int64_t* starts,
                             int64_t sequences, int64_t T, int64_t N, int64_t G, int64_t d, int64_t q_row,
                             int64_t q_head, int64_t k_row, int64_t k_head, int64_t v_row, int64_t v_head, float scale,
                             int dtype, void* stream) {
-  if (!q || !k || !v || !out || !starts || sequences <= 0 || T <= 0 || N <= 0 || G <= 0 || N % G != 0 || d <= 0 ||
-      !dtype_ok(dtype) || !(scale >= 1e-20f && scale <= 1e20f) || ((uintptr_t)starts & 7) != 0) {
-    set_error("flash_attn_packed: invalid argument");
+  return flash_attn_packed("flash_attn_packed",
+                           PackedAttention{q, k, v, out, nullptr, starts, sequences, T, N, G, q_row, q_head, k_row, k_head,
+                                           v_row, v_head, scale},
+                           d, dtype, stream);
+}
+
+int gptmi_flash_attn_packed_train(const void* q, const void* k, const void* v, void* out, float* stats,
+                                  const int64_t* starts, int64_t sequences, int64_t T, int64_t N, int64_t G, int64_t d,
+                                  int64_t q_row, int64_t q_head, int64_t k_row, int64_t k_head, int64_t v_row,
+                                  int64_t v_head, float scale, int dtype, void* stream) {
+  if (!stats || ((uintptr_t)stats & 7) != 0) {
+    set_error("flash_attn_packed_train: invalid argument");
     return GPTMI_ERR_INVALID;
   }
-  if (dtype != GPTMI_F16) {
-    set_error("flash_attn_packed: fp16 only");
-    return GPTMI_ERR_UNSUPPORTED;
-  }
-  const uintptr_t all = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out;
-  if ((all & 15) != 0 || ((q_row | q_head | k_row | k_head | v_row | v_head) & 7) != 0) {
-    set_error("flash_attn_packed: q, k, v and out must be 16-byte aligned, and their pitches multiples of 8");
+  return flash_attn_packed("flash_attn_packed_train",
+                           PackedAttention{q, k, v, out, stats, starts, sequences, T, N, G, q_row, q_head, k_row, k_head,
+                                           v_row, v_head, scale},
+                           d, dtype, stream);
+}
+
+size_t gptmi_flash_attn_packed_backward_workspace_bytes(int64_t T, int64_t N) {
+  return T > 0 && N > 0 && T < 1ll << 31 && N <= 1 << 20 ? packed_attn_grad_bytes(T, N) : 0;
+}
+
+int gptmi_flash_attn_packed_backward(const void* q, const void* k, const void* v, const void* out, const float* stats,
+                                     const void* d_out, const int64_t* starts, void* dq, void* dk, void* dv,
+                                     int64_t sequences, int64_t T, int64_t N, int64_t G, int64_t d, int64_t q_row,
+                                     int64_t q_head, int64_t k_row, int64_t k_head, int64_t v_row, int64_t v_head,
+                                     float scale, void* workspace, size_t workspace_bytes, int dtype, void* stream) {
+  const char* what = "flash_attn_packed_backward";
+  if (!out || !stats || ((uintptr_t)stats & 7) != 0 || !d_out || (dk == nullptr) != (dv == nullptr) || (!dq && !dk)) {
+    set_error("%s: invalid argument", what);
     return GPTMI_ERR_INVALID;
   }
-  // the kernel's offsets of a tile's 64 rows are 32-bit numbers of bytes
-  const auto pitch_ok = [](int64_t row) { return row >= 0 && row <= 1 << 24; };
-  const auto head_ok = [](int64_t head) { return head >= 0 && head <= 1ll << 40; };
-  if (!pitch_ok(q_row) || !pitch_ok(k_row) || !pitch_ok(v_row) || !head_ok(q_head) || !head_ok(k_head) ||
-      !head_ok(v_head) || T >= 1ll << 31 || sequences > 1ll << 30 || N > 1 << 20) {
-    set_error("flash_attn_packed: sizes or pitches beyond the supported");
-    return GPTMI_ERR_UNSUPPORTED;
-  }
-  const int rc = launch_flash_attn_packed(
-      PackedAttention{q, k, v, out, starts, sequences, T, N, G, q_row, q_head, k_row, k_head, v_row, v_head, scale},
-      (int)d, (hipStream_t)stream);
+  const PackedAttention p{q, k, v, (void*)out, (void*)stats, starts, sequences, T, N, G, q_row, q_head, k_row, k_head, v_row,
+                          v_head, scale};
+  int rc = check_packed(what, p, d, (uintptr_t)out | (uintptr_t)d_out | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv, dtype);
   if (rc) return rc;
-  return check_launch("flash_attn_packed");
+  const size_t needed = packed_attn_grad_bytes(T, N);
+  if (!workspace || workspace_bytes < needed || ((uintptr_t)workspace & 255) != 0) {
+    set_error("%s: workspace of %zu bytes needed, 256-byte aligned, %zu given", what, needed, workspace ? workspace_bytes : (size_t)0);
+    return GPTMI_ERR_WORKSPACE;
+  }
+  rc = launch_flash_attn_packed_backward(p, PackedGradients{d_out, dq, dk, dv}, (int)d, workspace, (hipStream_t)stream);
+  return rc ? rc : check_launch(what);
 }
 
 size_t gptmi_dropout_mask_bytes(int64_t n) {

@@ -87,12 +87,22 @@ int launch_gemm_layernorm(const void* x, const void* ln_w, const void* ln_b, flo
 struct PackedAttention {
   const void *q, *k, *v;
   void* out;
+  void* stats;  // float2 [heads][rows], what the gradients need of each row, or nullptr
   const int64_t* starts;
   int64_t sequences, rows, heads, kv_heads;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;
   float scale;
 };
 int launch_flash_attn_packed(const PackedAttention& p, int d, hipStream_t st);
+// Its gradients (packed_attn_grad.hip), all dense: dq, or dk and dv, may be nullptr.  `out` and `stats` are the forward
+// pass's.  workspace: packed_attn_grad_bytes, 8-byte aligned.
+struct PackedGradients {
+  const void* d_out;
+  void *dq, *dk, *dv;
+};
+size_t packed_attn_grad_bytes(int64_t rows, int64_t heads);
+int launch_flash_attn_packed_backward(const PackedAttention& p, const PackedGradients& d, int head_size, void* workspace,
+                                      hipStream_t st);
 
 // Rows of logits: x [rows][vocab] at a pitch of ld elements, no alignment beyond the element's.
 struct LogitRows {

@@ -13,31 +13,23 @@
 
 #include "common.h"
 #include "launch.h"
+#include "packed_attn.h"
 
 namespace gptmi {
 namespace {
 
 constexpr int kKeys = 64;  // keys a tile
-constexpr int kGridRow = 1 << 20;  // workgroups a row of the grid: threads of one dimension have to stay below 2^32
 
 struct PackedArgs {
   const _Float16 *q, *k, *v;
   _Float16* out;
+  float2* stats;              // [heads][T], or nullptr: what the gradients need
   const int64_t* starts;
   int64_t rows;               // T
   int sequences, heads, kv_heads, slots, longest_first;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;  // pitches in elements
   float scale;
 };
-
-// 16 bytes a lane from base + lane_off into LDS at lds_off + 16 lane.  Assembly, so that the compiler does not wait
-// for these loads in front of each LDS read; the kernel waits by hand.
-__device__ __forceinline__ void load_lds16(const void* base, unsigned lane_off, unsigned lds_off) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2"
-               :
-               : "s"(lds_off), "v"(lane_off), "s"(base)
-               : "memory", "m0");
-}
 
 // Without the compiler's quieting of NaNs in front; one makes a NaN of the row, which is looked for at the end.
 __device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
@@ -46,78 +38,6 @@ __device__ __forceinline__ float larger(float a, float b) { return __builtin_ele
 // than 1, and what is above 65519 would be an infinity.
 __device__ __forceinline__ float bounded(float x) {
   return fabsf(x) < INFINITY ? __builtin_amdgcn_fmed3f(x, -65504.f, 65504.f) : x;
-}
-
-// Slots: sequence s, which starts at row a, has its blocks of R queries from slot a / R + s on, which leaves room for
-// every sequence whatever the lengths are (floor(a / R) + floor(len / R) <= floor((a + len) / R)), needs no
-// lengths on the host and no pass over them on the GPU.  Slots that are left over hold nothing.
-struct Block {
-  int64_t first;  // the sequence's first row
-  int length;     // rows of it, 0: nothing to do
-  int block;      // which R of them
-};
-template <int R>
-__device__ __forceinline__ Block find_block(const PackedArgs& a, int slot) {
-  // the last sequence whose first slot is not behind this one: 64 probes at a time
-  const int lane = threadIdx.x & 63;
-  int low = 0, left = a.sequences;
-  while (left > 1) {
-    const int step = (left + 63) >> 6, at = low + lane * step;
-    bool in = false;
-    if (lane * step < left) in = a.starts[at] / R + at <= slot;
-    const int n = __popcll(__ballot(in));
-    const int skip = (n > 1 ? n - 1 : 0) * step;
-    low += skip;
-    left = min(step, left - skip);
-  }
-  low = __builtin_amdgcn_readfirstlane(low);
-  // whatever the starts are, rows stay inside [0, T)
-  const int64_t begin = a.starts[low], end = a.starts[low + 1];
-  const int64_t first = begin < 0 ? 0 : begin < a.rows ? begin : a.rows;
-  const int64_t last = end < first ? first : end < a.rows ? end : a.rows;
-  const int64_t length = last - first, block = slot - (begin / R + low);
-  return {first, block >= 0 && block * R < length ? (int)length : 0, (int)block};
-}
-
-// The nth block of all sequences' blocks in the order of their keys, the most first, for up to 64 kMany sequences.
-// Where all workgroups run at once or nearly, the last one to start decides when the launch ends.
-constexpr int kMany = 4;
-template <int R>
-__device__ __forceinline__ Block nth_longest(const PackedArgs& a, int nth) {
-  const int lane = threadIdx.x & 63;
-  int first[kMany], length[kMany], most = 0;  // of sequence lane + 64 i; rows are below 2^31
-#pragma unroll
-  for (int i = 0; i < kMany; ++i) {
-    const int s = lane + i * kWave;
-    first[i] = length[i] = 0;
-    if (i * kWave >= a.sequences) break;
-    if (s < a.sequences) {
-      const int64_t begin = a.starts[s], end = a.starts[s + 1];
-      const int64_t from = begin < 0 ? 0 : begin < a.rows ? begin : a.rows;
-      const int64_t to = end < from ? from : end < a.rows ? end : a.rows;
-      first[i] = (int)from;
-      length[i] = (int)(to - from);
-    }
-    most = max(most, length[i]);
-  }
-  most = __builtin_amdgcn_readfirstlane((int)wave_max((float)((most + R - 1) / R)));  // below 2^24: the host sees to it
-  for (int block = most - 1; block >= 0; --block) {
-    int all = 0;
-#pragma unroll
-    for (int i = 0; i < kMany; ++i) {
-      if (i * kWave >= a.sequences) break;
-      const uint64_t have = __ballot(length[i] > block * R);
-      const int n = __popcll(have);
-      if (nth >= all && nth < all + n) {  // the (nth - all)th of these
-        const bool me = (have >> lane & 1) && __popcll(have & ((1ull << lane) - 1)) == nth - all;
-        const int s = __ffsll((unsigned long long)__ballot(me)) - 1;
-        return {__builtin_amdgcn_readlane(first[i], s), __builtin_amdgcn_readlane(length[i], s), block};
-      }
-      all += n;
-    }
-    nth -= all;
-  }
-  return {0, 0, 0};
 }
 
 template <int D, int QB, int P>
@@ -146,39 +66,12 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
   const int c = lane & 15, g = lane >> 4;
   const unsigned smem_base = (unsigned)(uintptr_t)smem;
 
-  // ids that are equal modulo 8 run on one XCD, whose L2 then holds the K and V of its heads; the heads of up to 7
-  // key heads beyond a multiple of 8, untied, are dealt to all.  Either an XCD's heads one behind the other (the
-  // untied ones first), late blocks, which have the most keys, in front, or the late blocks of all its heads in
-  // front, eight slots at a time.
-  const int id = (int)(blockIdx.y * kGridRow + blockIdx.x), rep = a.heads / a.kv_heads, untied = (a.kv_heads & 7) * rep;
-  int head, slot;
-  const auto tied_head = [&](int nth) { return ((id & 7) + 8 * (nth / rep)) * rep + nth % rep; };
-  if (a.longest_first) {
-    // eight slots are a.heads rows of 8 ids, in the order of their slots: `untied` of them, spread among the others,
-    // for the untied heads
-    const int eight = id / (8 * a.heads), row = (id - eight * 8 * a.heads) >> 3, tied = a.heads - untied;
-    const int u = row * untied / a.heads, t = row - u;  // rows of either kind in front
-    if ((row + 1) * untied / a.heads > u) {
-      slot = (8 * u + (id & 7)) / untied;
-      const int at = 8 * u + (id & 7) - slot * untied, few = a.kv_heads & 7, nth = at / few;
-      head = tied + (at - nth * few) * rep + nth;  // 1, 2 or 4 key heads each have XCDs of their own
-    } else {
-      slot = t / (tied >> 3);
-      head = tied_head(t - slot * (tied >> 3));
-    }
-    slot += 8 * eight;
-    if (slot >= a.slots) return;
-  } else if (id >= a.slots * a.heads) {
-    return;
-  } else if (id < a.slots * untied) {
-    slot = id / untied;
-    head = a.heads - untied + (id - slot * untied);
-  } else {
-    const int at = (id - a.slots * untied) >> 3, nth = at / a.slots;
-    slot = at - nth * a.slots;
-    head = tied_head(nth);
-  }
-  const Block block = a.longest_first && a.sequences > 1 ? nth_longest<R>(a, slot) : find_block<R>(a, a.slots - 1 - slot);
+  const int rep = a.heads / a.kv_heads;
+  Place place;
+  if (!find_place((int)(blockIdx.y * kGridRow + blockIdx.x), a.heads, a.kv_heads, a.slots, a.longest_first, &place)) return;
+  const int head = place.head, slot = place.slot;
+  const Sequences in{a.starts, a.rows, a.sequences};
+  const Block block = a.longest_first && a.sequences > 1 ? nth_longest<R>(in, slot) : find_block<R>(in, a.slots - 1 - slot);
   if (block.length == 0) return;
   const int L = block.length, q0 = block.block * R;
   // part p of P has the key tiles p, p + P, .., perhaps none
@@ -423,6 +316,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
       const float to = larger(base[n], other[0]);
       const float mine = __builtin_amdgcn_exp2f(base[n] - to), its = __builtin_amdgcn_exp2f(other[0] - to);
       den[n] = fmaf(den[n], mine, other[1] * its);
+      base[n] = to;
 #pragma unroll
       for (int i = 0; i < DB; ++i) oacc[n][i] = oacc[n][i] * mine + sums[(n * (DB + 1) + i) * kWave] * its;
     }
@@ -444,7 +338,11 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
 #pragma unroll
       for (int r = 0; r < 4; ++r) none = fmaf(oacc[n][i][r], 0.f, none);
     }
-    if (__any(none != 0.f && q < L)) {
+    // For the gradients: a weight is 2^(t s - x) y; or, y < 0, exp(score - x) -y of the scores key by key, where one rounded
+    // base is not as good as an fp16 number.
+    float2 stat = {base[n], inv};
+    const bool again = __any(none != 0.f && q < L);
+    if (again || (a.stats && __any(!(fabsf(base[n]) < 8192.f) && q < L))) {
       const int last = min(qw0 + 16 * n + 15, L - 1);
       // of query c with key j, from this lane's elements of both and the other three lanes': one rounded number
       auto score = [&](int j) {
@@ -471,9 +369,12 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
       }
       const bool number = total == total && fabsf(m) < INFINITY;  // else there is no softmax
       const float inv_total = number ? 1.0f / total : NAN;
+      stat = {m, -inv_total};
+      if (again) {
 #pragma unroll
-      for (int i = 0; i < DB; ++i) oacc[n][i] = f4(number ? 0.f : NAN);
-      if (__any(number && q < L)) {
+        for (int i = 0; i < DB; ++i) oacc[n][i] = f4(number ? 0.f : NAN);
+      }
+      if (again && __any(number && q < L)) {
 #pragma unroll 2
         for (int j = 0; j <= last; ++j) {
           const float w = __expf(score(j) - m) * inv_total;
@@ -490,6 +391,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
         }
       }
     }
+    if (a.stats && g == 0 && q < L) a.stats[head * a.rows + block.first + q] = stat;
     _Float16* o = a.out + ((block.first + q) * a.heads + head) * D + 4 * g;
 #pragma unroll
     for (int i = 0; i < DB; ++i) {
@@ -569,6 +471,7 @@ int launch_flash_attn_packed(const PackedAttention& p, int d, hipStream_t st) {
   a.k = (const _Float16*)p.k;
   a.v = (const _Float16*)p.v;
   a.out = (_Float16*)p.out;
+  a.stats = (float2*)p.stats;
   a.starts = p.starts;
   a.rows = p.rows;
   a.sequences = (int)p.sequences;

@@ -670,16 +670,25 @@ def flash_attention_v1(q, k, v, dropout_prob=0.0, *, merged_heads_layout=False):
     return buf.transpose(1, 2) if merged_heads_layout else buf
 
 
-def flash_attention_packed(q, k, v, starts, scale=None, out=None):
-    """Causal attention over whole prompts of different lengths, one behind the other without padding, with grouped
-    heads: q [T, N, d], k and v [T, G, d], N a multiple of G -> [T, N, d].  Sequence s is the rows starts[s] ..
-    starts[s + 1] - 1 (int64 on the GPU, S + 1 of them, not decreasing, from 0 to T; a sequence may be empty), scale
-    1 / sqrt(d) if None.
+def _packed_pitches(q, k, v):
+    """(q's, k's and v's row and head pitches, their addresses); NotImplementedError where a head does not start at a multiple
+    of 16 bytes."""
+    (q_row, q_head, q_one), (k_row, k_head, k_one), (v_row, v_head, v_one) = q.stride(), k.stride(), v.stride()
+    assert q_one == k_one == v_one == 1, "the elements of a head must lie side by side"
+    if q.shape[0] == 1:  # whatever the pitch of one is
+        q_row = k_row = v_row = 0
+    if q.shape[1] == 1:
+        q_head = 0
+    if k.shape[1] == 1:
+        k_head = v_head = 0
+    q_at, k_at, v_at = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    if (q_row | q_head | k_row | k_head | v_row | v_head) & 7 or (q_at | k_at | v_at) & 15:
+        raise NotImplementedError("flash_attention_packed: heads must start at multiples of 16 bytes")
+    return (q_row, q_head, k_row, k_head, v_row, v_head), (q_at, k_at, v_at)
 
-    fp16 (fp32 storage would round q, k and v to it).  A head's d elements lie side by side; rows and heads may be
-    views of something larger at 16-byte aligned pitches, such as the columns of a q, k, v product.  Rows that belong to no
-    sequence are not read, and of `out` not written (dense, allocated if None; a dense q itself may be it, and it may overlap
-    nothing else).  A forward pass only, like `flash_attention_v1`."""
+
+def _packed_attention(q, k, v, starts, scale, out, with_stats):
+    """(out, what the gradients need of each row or None, the scale)."""
     assert q.dim() == k.dim() == 3 and k.shape == v.shape, (q.shape, k.shape, v.shape)
     T, N, d = q.shape
     G = k.shape[1]
@@ -695,17 +704,7 @@ def flash_attention_packed(q, k, v, starts, scale=None, out=None):
     if starts.dtype != torch.int64:
         raise TypeError(f"flash_attention_packed: starts must be int64, got {starts.dtype}")
     dev = _on_gpu(q, k, v, starts, out)
-    (q_row, q_head, q_one), (k_row, k_head, k_one), (v_row, v_head, v_one) = q.stride(), k.stride(), v.stride()
-    assert q_one == k_one == v_one == 1, "the elements of a head must lie side by side"
-    if T == 1:  # whatever the pitch of one is
-        q_row = k_row = v_row = 0
-    if N == 1:
-        q_head = 0
-    if G == 1:
-        k_head = v_head = 0
-    q_at, k_at, v_at = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    if (q_row | q_head | k_row | k_head | v_row | v_head) & 7 or (q_at | k_at | v_at) & 15:
-        raise NotImplementedError("flash_attention_packed: heads must start at multiples of 16 bytes")
+    pitches, (q_at, k_at, v_at) = _packed_pitches(q, k, v)
     if scale is None:
         scale = d ** -0.5
     if not 1e-20 <= scale <= 1e20:
@@ -713,6 +712,7 @@ def flash_attention_packed(q, k, v, starts, scale=None, out=None):
     if out is None:
         out = q.new_empty((T, N, d))
     else:
+        q_row, q_head, k_row, k_head, v_row, v_head = pitches
         assert out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous()
         at = out.data_ptr()
         if at & 15:
@@ -724,11 +724,62 @@ def flash_attention_packed(q, k, v, starts, scale=None, out=None):
                                  (starts.data_ptr(), 8 * starts.shape[0], False)):
             apart = start + size <= at or end <= start
             assert apart or T == 0 or (may and start == at), "out may be a dense q alone"
+    stats = q.new_empty((N, T, 2), dtype=torch.float32) if with_stats else None
     if T > 0:
-        _call(dev, "flash_attention_packed", _lib.load().gptmi_flash_attn_packed, q_at, k_at, v_at, out.data_ptr(),
-              starts.data_ptr(), starts.shape[0] - 1, T, N, G, d, q_row, q_head, k_row, k_head, v_row, v_head, scale,
-              _lib.GPTMI_F16)
-    return out
+        lib, sizes = _lib.load(), (starts.data_ptr(), starts.shape[0] - 1, T, N, G, d, *pitches, scale, _lib.GPTMI_F16)
+        if with_stats:
+            _call(dev, "flash_attention_packed", lib.gptmi_flash_attn_packed_train, q_at, k_at, v_at, out.data_ptr(),
+                  stats.data_ptr(), *sizes)
+        else:
+            _call(dev, "flash_attention_packed", lib.gptmi_flash_attn_packed, q_at, k_at, v_at, out.data_ptr(), *sizes)
+    return out, stats, scale
+
+
+class _PackedAttentionFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, starts, scale):
+        out, stats, ctx.scale = _packed_attention(q, k, v, starts, scale, None, True)
+        ctx.save_for_backward(q, k, v, out, stats, starts)
+        return out
+
+    @staticmethod
+    def backward(ctx, d_out):
+        _first_derivative("flash_attention_packed")
+        q, k, v, out, stats, starts = ctx.saved_tensors
+        (T, N, d), G = q.shape, k.shape[1]
+        need_q, need_k, need_v = ctx.needs_input_grad[:3]
+        dq = q.new_empty((T, N, d)) if need_q else None
+        dk, dv = (k.new_empty((T, G, d)) for _ in range(2)) if need_k or need_v else (None, None)
+        if T > 0:
+            d_out = d_out.contiguous()
+            if d_out.data_ptr() & 15:
+                d_out = d_out.clone()
+            pitches, addresses = _packed_pitches(q, k, v)
+            lib = _lib.load()
+            nbytes = lib.gptmi_flash_attn_packed_backward_workspace_bytes(T, N)
+            workspace = _workspace(nbytes, q)
+            _call(q.get_device(), "flash_attention_packed", lib.gptmi_flash_attn_packed_backward, *addresses,
+                  out.data_ptr(), stats.data_ptr(), d_out.data_ptr(), starts.data_ptr(), _ptr(dq), _ptr(dk), _ptr(dv),
+                  starts.shape[0] - 1, T, N, G, d, *pitches, ctx.scale, workspace.data_ptr(), nbytes, _lib.GPTMI_F16)
+        return dq, dk if need_k else None, dv if need_v else None, None, None
+
+
+def flash_attention_packed(q, k, v, starts, scale=None, out=None):
+    """Causal attention over whole prompts of different lengths, one behind the other without padding, with grouped
+    heads: q [T, N, d], k and v [T, G, d], N a multiple of G -> [T, N, d].  Sequence s is the rows starts[s] ..
+    starts[s + 1] - 1 (int64 on the GPU, S + 1 of them, not decreasing, from 0 to T; a sequence may be empty), scale
+    1 / sqrt(d) if None.
+
+    fp16 (fp32 storage would round q, k and v to it).  A head's d elements lie side by side; rows and heads may be
+    views of something larger at 16-byte aligned pitches, such as the columns of a q, k, v product.  Rows that belong to no
+    sequence are not read, and of `out` not written (dense, allocated if None; a dense q itself may be it, and it may overlap
+    nothing else).
+
+    Gradients flow to q, k and v (dense ones, fp16), backward and once; of rows that belong to no sequence they are 0.  Each
+    is one sum in one order: the same step gives the same bits.  With `out` given the call is a forward pass only."""
+    if out is None and (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
+        return _PackedAttentionFunction.apply(q, k, v, starts, scale)
+    return _packed_attention(q, k, v, starts, scale, out, False)[0]
 
 
 class DropoutMask:

@@ -355,6 +355,38 @@ int gptmi_flash_attn_packed(const void* q, const void* k, const void* v, void* o
                             void* stream);
 
 /*
+ * gptmi_flash_attn_packed in a training step: the same output, and in stats [N][T][2] (8-byte aligned) what the gradients need
+ * of each row's softmax.
+ */
+int gptmi_flash_attn_packed_train(const void* q, const void* k, const void* v, void* out, float* stats,
+                                  const int64_t* starts, int64_t sequences, int64_t T, int64_t N,
+                                  int64_t G, int64_t d, int64_t q_row, int64_t q_head, int64_t k_row,
+                                  int64_t k_head, int64_t v_row, int64_t v_head, float scale, int dtype,
+                                  void* stream);
+
+/*
+ * The gradients of q, k and v for d_out [T][N][d], that of the output: with e_i = d_out[i][n], delta_i = e_i . out[i][n],
+ * u_ij = w_ij (e_i . v_j - delta_i):
+ *   dq[i][n] = scale sum_j u_ij k_j     dk[j][g] = scale sum_i u_ij q_i     dv[j][g] = sum_i w_ij e_i
+ * the latter over the queries of all heads that share the key head, in one order: the same call gives the same bits.
+ *   out, d_out, dq [T][N][d], dk, dv [T][G][d] dense; out, stats: gptmi_flash_attn_packed_train's for these q, k, v, starts
+ *   and scale.  dq, or dk and dv, may be NULL.  The gradients overlap nothing.  Rows that belong to no sequence are not read
+ *   and have gradients of 0.
+ * w and u are formed again in fp32 and rounded to fp16 for the products, scaled by powers of two so that they stay normal
+ * numbers.  What hidden rows hold, infinities and NaN included, plays no part.  workspace:
+ * gptmi_flash_attn_packed_backward_workspace_bytes(T, N), 256-byte aligned.
+ * No counterpart in the reference, which has no gradients.
+ */
+size_t gptmi_flash_attn_packed_backward_workspace_bytes(int64_t T, int64_t N);
+int gptmi_flash_attn_packed_backward(const void* q, const void* k, const void* v, const void* out,
+                                     const float* stats, const void* d_out, const int64_t* starts,
+                                     void* dq, void* dk, void* dv, int64_t sequences, int64_t T,
+                                     int64_t N, int64_t G, int64_t d, int64_t q_row, int64_t q_head,
+                                     int64_t k_row, int64_t k_head, int64_t v_row, int64_t v_head,
+                                     float scale, void* workspace, size_t workspace_bytes, int dtype,
+                                     void* stream);
+
+/*
  * The dropout mask of gptmi_linear and gptmi_flash_attn as bits: bit o % 32 of 32-bit word o / 32 is set
  * iff offset o < n is kept, rand(seed, o) > p.  Both count flat indices from 0, so one mask of the
  * largest matrix serves all the layers of a forward; 1 <= n <= 2^32.  gptmi_dropout_mask_bytes(n) is what
