@@ -19,6 +19,10 @@ SIGNATURES = {
     "gptmi_last_error": (ctypes.c_char_p, []),
     "gptmi_embed": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _f32, _u64, _int,
                            _vp]),
+    "gptmi_embed_backward_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "gptmi_embed_backward": (_int, [_vp] * 4 + [_i64] * 5 + [_f32, _u64, _vp, _sz, _int, _vp]),
+    "gptmi_clip_grad_norm_workspace_bytes": (_sz, [_i64]),
+    "gptmi_clip_grad_norm": (_int, [_vp] * 5 + [_i64, _f32, _f32, _vp, _vp, _sz, _vp]),
     "gptmi_embed_layernorm": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64,
                                      _i64, _f32, _int, _vp]),
     "gptmi_layernorm": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _f32, _int, _vp]),

@@ -5,6 +5,7 @@
 #include <math.h>
 #include <stdarg.h>
 #include <stdio.h>
+#include <stdlib.h>
 
 #include <mutex>
 
@@ -44,6 +45,10 @@ constexpr int kMaxN = 1 << 26;
 // Rows of logits: a thread counts a row's elements in an int, with some thousands to spare; a row's place in
 // 64 bits.
 constexpr int64_t kMaxVocab = 1ll << 30, kMaxPitch = 1ll << 40;
+
+// Sizes that the grids of the embedding's gradients take; tensors and elements of one clip_grad_norm.
+constexpr int64_t kMaxGradTokens = 1 << 30, kMaxGradVocab = 1 << 26, kMaxGradPositions = 1 << 21, kMaxGradWidth = 1 << 20;
+constexpr int64_t kMaxGradients = 1 << 20, kMaxGradElements = 1ll << 42;
 
 // Workspace plan of one GEMM: where the packed weight and (if needed) the
 // packed activations live.
@@ -406,6 +411,117 @@ int gptmi_embed(const int64_t* ids, const void* wte, const void* wpe, void* out,
   launch_embed(ids, wte, wpe, out, B * L, L, V, (int)H, Dropout{p, seed}, dtype == GPTMI_F16,
                (hipStream_t)stream);
   return check_launch("embed");
+}
+
+size_t gptmi_embed_backward_workspace_bytes(int64_t B, int64_t L, int64_t H) {
+  if (B <= 0 || L <= 0 || H <= 0 || B > kMaxGradTokens / L || H > kMaxGradWidth) return 0;
+  return embed_grad_bytes(B * L, H);
+}
+
+int gptmi_embed_backward(const int64_t* ids, const void* dz, void* d_wte, void* d_wpe, int64_t B, int64_t L, int64_t V,
+                         int64_t P, int64_t H, float p, uint64_t seed, void* workspace, size_t workspace_bytes, int dtype,
+                         void* stream) {
+  if (!ids || !dz || (!d_wte && !d_wpe) || B <= 0 || L <= 0 || V <= 0 || P <= 0 || H <= 0 || !dtype_ok(dtype) ||
+      !dropout_ok(p)) {
+    set_error("embed_backward: invalid argument");
+    return GPTMI_ERR_INVALID;
+  }
+  if (L > P) {
+    set_error("embed_backward: sequence length %lld exceeds the %lld position rows", (long long)L, (long long)P);
+    return GPTMI_ERR_INVALID;
+  }
+  if (B > kMaxGradTokens / L || V > kMaxGradVocab || P > kMaxGradPositions || H > kMaxGradWidth) {
+    set_error("embed_backward: sizes beyond the supported");
+    return GPTMI_ERR_UNSUPPORTED;
+  }
+  const uintptr_t element = dtype == GPTMI_F16 ? 1 : 3;
+  if ((((uintptr_t)dz | (uintptr_t)d_wte | (uintptr_t)d_wpe) & element) != 0 || ((uintptr_t)ids & 7) != 0) {
+    set_error("embed_backward: addresses must be multiples of the elements' size");
+    return GPTMI_ERR_INVALID;
+  }
+  const size_t needed = d_wte ? embed_grad_bytes(B * L, H) : 0;
+  if (needed > 0 && (!workspace || workspace_bytes < needed || ((uintptr_t)workspace & 255) != 0)) {
+    set_error("embed_backward: workspace of %zu bytes needed, 256-byte aligned, %zu given", needed,
+              workspace ? workspace_bytes : (size_t)0);
+    return GPTMI_ERR_WORKSPACE;
+  }
+  launch_embed_backward(ids, dz, d_wte, d_wpe, B * L, L, V, P, (int)H, Dropout{p, seed}, dtype == GPTMI_F16, workspace,
+                        (hipStream_t)stream);
+  return check_launch("embed_backward");
+}
+
+size_t gptmi_clip_grad_norm_workspace_bytes(int64_t n) { return n > 0 && n <= kMaxGradients ? clip_grad_bytes(n) : 0; }
+
+namespace {
+struct Range {
+  uintptr_t begin, end;
+  bool written;
+};
+int by_begin(const void* a, const void* b) {
+  const uintptr_t x = ((const Range*)a)->begin, y = ((const Range*)b)->begin;
+  return x < y ? -1 : x > y;
+}
+}  // namespace
+
+int gptmi_clip_grad_norm(const void* const* grads, void* const* out, const int64_t* sizes, const unsigned char* f16,
+                         const unsigned char* out_f16, int64_t n, float scale, float max_norm, float* norm, void* workspace,
+                         size_t workspace_bytes, void* stream) {
+  const char* what = "clip_grad_norm";
+  if (!grads || !out || !sizes || !f16 || !out_f16 || n <= 0 || !norm || ((uintptr_t)norm & 3) != 0 || !(scale > 0.f) ||
+      !(scale < INFINITY) || !(max_norm > 0.f)) {
+    set_error("%s: invalid argument", what);
+    return GPTMI_ERR_INVALID;
+  }
+  if (n > kMaxGradients) {
+    set_error("%s: %lld tensors are beyond the supported %lld", what, (long long)n, (long long)kMaxGradients);
+    return GPTMI_ERR_UNSUPPORTED;
+  }
+  const size_t needed = clip_grad_bytes(n);
+  if (!workspace || workspace_bytes < needed || ((uintptr_t)workspace & 7) != 0) {
+    set_error("%s: workspace of %zu bytes needed, 8-byte aligned, %zu given", what, needed, workspace ? workspace_bytes : (size_t)0);
+    return GPTMI_ERR_WORKSPACE;
+  }
+  // nothing that is written may be, or overlap, anything else
+  Range* ranges = (Range*)malloc(2 * (size_t)n * sizeof(Range));
+  if (!ranges) {
+    set_error("%s: no memory for %lld tensors' addresses", what, (long long)n);
+    return GPTMI_ERR_INVALID;
+  }
+  size_t count = 0;
+  bool in_place = true, ok = true;
+  int64_t elements = 0;
+  for (int64_t i = 0; i < n && ok; ++i) {
+    const uintptr_t size = f16[i] ? 2 : 4, out_size = out_f16[i] ? 2 : 4;
+    ok = sizes[i] >= 0 && sizes[i] <= kMaxGradElements - elements;
+    if (!ok || sizes[i] == 0) continue;
+    elements += sizes[i];
+    const uintptr_t at = (uintptr_t)grads[i], to = (uintptr_t)out[i];
+    ok = at != 0 && to != 0 && at % size == 0 && to % out_size == 0;
+    const bool same = at == to && size == out_size;
+    in_place &= same;
+    ranges[count++] = {at, at + size * (uintptr_t)sizes[i], same};
+    if (!same) ranges[count++] = {to, to + out_size * (uintptr_t)sizes[i], true};
+  }
+  if (!ok) {
+    free(ranges);
+    set_error("%s: invalid argument", what);
+    return GPTMI_ERR_INVALID;
+  }
+  qsort(ranges, count, sizeof(Range), by_begin);
+  uintptr_t end = 0, end_written = 0;
+  for (size_t i = 0; i < count && ok; ++i) {
+    ok = ranges[i].begin >= (ranges[i].written ? end : end_written);
+    if (ranges[i].end > end) end = ranges[i].end;
+    if (ranges[i].written && ranges[i].end > end_written) end_written = ranges[i].end;
+  }
+  free(ranges);
+  if (!ok) {
+    set_error("%s: a tensor that is written overlaps another one", what);
+    return GPTMI_ERR_INVALID;
+  }
+  launch_clip_grad_norm(Gradients{grads, out, sizes, f16, out_f16, n, in_place}, scale, max_norm, norm, workspace,
+                        (hipStream_t)stream);
+  return check_launch(what);
 }
 
 int gptmi_embed_layernorm(const int64_t* ids, const void* wte, const void* wpe,

@@ -1,0 +1,532 @@
+// Gradients of the embedding's tables: row v of the token table's is the sum of dz over the positions of token v, row l of the
+// position table's the sum over the batch, both dense, rows without a token zeros.
+//
+// The sums are formed in fp32, each in one order, in the order of the positions and without atomics, so the same call
+// gives the same bits.  That takes each token's positions one behind the other:
+//   up to 256 tokens, one launch: every workgroup has a range of the vocabulary and looks all tokens through;
+//   more, a stable radix sort of the tokens with their positions, a workgroup a tile of them, whose launches also write the zero rows and
+//   form the position table's sums; then runs of the sorted positions are summed, whoever has a token to itself writes its
+//   row, and what a token has in several runs is joined in a last launch.
+// Bound by memory: dz twice (once for each table), the tables' gradients once.
+#include "common.h"
+#include "launch.h"
+
+namespace gptmi {
+namespace {
+
+constexpr int kFew = 256;          // tokens of the single launch
+constexpr int kTile = 4096;        // tokens a workgroup sorts
+constexpr int kSortThreads = 1024;
+constexpr int kMaxBits = 9;        // of a digit
+
+// VN elements of a row: 16 bytes, or one element where a row or an address is no multiple of that.
+template <typename T, int VN>
+__device__ __forceinline__ void add_chunk(const T* p, float (&sum)[VN]) {
+  typedef T V __attribute__((ext_vector_type(VN)));
+  const V x = *reinterpret_cast<const V*>(p);
+#pragma unroll
+  for (int i = 0; i < VN; ++i) sum[i] += (float)x[i];
+}
+template <typename T>
+__device__ __forceinline__ void add_chunk(const T* p, float (&sum)[1]) {
+  sum[0] += (float)*p;
+}
+template <typename T, int VN>
+__device__ __forceinline__ void put_chunk(T* p, const float (&sum)[VN]) {
+  if constexpr (VN == 1) {
+    *p = (T)sum[0];
+  } else {
+    typedef T V __attribute__((ext_vector_type(VN)));
+    V x;
+#pragma unroll
+    for (int i = 0; i < VN; ++i) x[i] = (T)sum[i];
+    *reinterpret_cast<V*>(p) = x;
+  }
+}
+template <int VN>
+__device__ __forceinline__ void clear(float (&sum)[VN]) {
+#pragma unroll
+  for (int i = 0; i < VN; ++i) sum[i] = 0.f;
+}
+
+struct EmbedGradArgs {
+  const int64_t* ids;
+  const void* dz;
+  void *d_wte, *d_wpe;  // one of them may be nullptr
+  int64_t tokens, L, V, P;
+  int H;
+  DropoutArgs drop;
+  // the sort's
+  int tiles, bits;          // workgroups, bits of a digit
+  unsigned *keys[2], *at[2];  // tokens (V: none) and positions
+  unsigned* hist;           // [tiles][1 << bits]
+  // the sums'
+  const unsigned *sorted, *order;
+  float* parts;             // [runs][2][H]: what a run has of a token that began in front of it, and of one that goes on behind
+  int run;                  // tokens of a run
+  int sort_blocks, fill_blocks;
+};
+
+// A mask of dropout is one for all rows: it comes behind the sums.
+template <typename T, int VN>
+__device__ __forceinline__ void put_sum(const EmbedGradArgs& a, T* row, int chunk, float (&sum)[VN]) {
+  if (a.drop.p > 0.f) {
+    unsigned column[VN];
+#pragma unroll
+    for (int i = 0; i < VN; ++i) column[i] = (unsigned)(chunk * VN + i);
+    dropout_apply<VN>(a.drop, column, sum);
+  }
+  put_chunk<T, VN>(row + chunk * VN, sum);
+}
+
+// Adds rows place(first) .. place(last - 1) of chunk `chunk`, eight on their way at a time.
+template <typename T, int VN, typename F>
+__device__ __forceinline__ void add_rows(const T* dz, int H, int chunk, int64_t first, int64_t last, F place, float (&sum)[VN]) {
+  typedef T V __attribute__((ext_vector_type(VN)));
+  constexpr int U = 8;
+  int64_t i = first;
+  for (; i + U <= last; i += U) {
+    if constexpr (VN == 1) {
+      T x[U];
+#pragma unroll
+      for (int j = 0; j < U; ++j) x[j] = dz[place(i + j) * H + chunk];
+#pragma unroll
+      for (int j = 0; j < U; ++j) sum[0] += (float)x[j];
+    } else {
+      V x[U];
+#pragma unroll
+      for (int j = 0; j < U; ++j) x[j] = *reinterpret_cast<const V*>(dz + place(i + j) * H + chunk * VN);
+#pragma unroll
+      for (int j = 0; j < U; ++j)
+#pragma unroll
+        for (int n = 0; n < VN; ++n) sum[n] += (float)x[j][n];
+    }
+  }
+  for (; i < last; ++i) add_chunk(dz + place(i) * H + chunk * VN, sum);
+}
+
+// Row l of the position table's gradient, by a workgroup in groups of `lanes` threads that share the batch.
+template <typename T, int VN, int NT>
+__device__ __forceinline__ void position_row(const EmbedGradArgs& a, int64_t l, int lanes, float* lds) {
+  const T* dz = (const T*)a.dz;
+  T* row = (T*)a.d_wpe + l * a.H;
+  const int chunks = a.H / VN, tid = threadIdx.x;
+  const int groups = NT / lanes, group = tid / lanes, lane = tid - group * lanes;
+  const int64_t batch = l < a.L ? a.tokens / a.L : 0, share = (batch + groups - 1) / groups;
+  const int64_t first = min((int64_t)group * share, batch), last = group < groups ? min(first + share, batch) : first;
+  for (int c0 = 0; c0 < chunks; c0 += lanes) {
+    const int chunk = c0 + lane;
+    float sum[VN];
+    clear(sum);
+    if (chunk < chunks) add_rows<T, VN>(dz, a.H, chunk, first, last, [&](int64_t b) { return b * a.L + l; }, sum);
+    if (groups > 1) {
+      __syncthreads();
+      if (group < groups)
+#pragma unroll
+        for (int i = 0; i < VN; ++i) lds[(group * VN + i) * lanes + lane] = sum[i];
+      __syncthreads();
+      if (group == 0)
+        for (int n = 1; n < groups; ++n)
+#pragma unroll
+          for (int i = 0; i < VN; ++i) sum[i] += lds[(n * VN + i) * lanes + lane];
+    }
+    if (group == 0 && chunk < chunks) put_sum<T, VN>(a, row, chunk, sum);
+  }
+}
+
+// Threads that share a row's chunks: a power of two below a wavefront, whole wavefronts beyond.
+__device__ __forceinline__ int lanes_of(int chunks, int most) {
+  if (chunks >= most) return most;
+  if (chunks > 32) return (chunks + 63) & ~63;
+  int n = 1;
+  while (n < chunks) n *= 2;
+  return n;
+}
+
+// ---------------------------------------------------------------------------
+// Up to kFew tokens: workgroups of `rows_of` tokens of the vocabulary each, then one for each position.
+// ---------------------------------------------------------------------------
+template <typename T, int VN>
+__global__ __launch_bounds__(256) void embed_grad_few_kernel(EmbedGradArgs a, int rows_of, int vocab_blocks) {
+  __shared__ float lds[256 * VN];
+  __shared__ unsigned found[kFew], sorted[kFew];
+  __shared__ int counts[4], begin[64 + 1];
+  const int tid = threadIdx.x, chunks = a.H / VN, lanes = lanes_of(chunks, 256);
+  if ((int)blockIdx.x >= vocab_blocks) {
+    position_row<T, VN, 256>(a, blockIdx.x - vocab_blocks, lanes, lds);
+    return;
+  }
+  const int64_t v0 = (int64_t)blockIdx.x * rows_of;
+  const int rows = (int)min((int64_t)rows_of, a.V - v0);
+  const int64_t token = tid < a.tokens ? a.ids[tid] - v0 : -1;
+  const bool mine = token >= 0 && token < rows;
+  const uint64_t have = __ballot(mine);
+  if ((tid & 63) == 0) counts[tid >> 6] = __popcll(have);
+  __syncthreads();
+  int in_front = 0, all = 0;
+  for (int w = 0; w < 4; ++w) {
+    if (w == tid >> 6) in_front = all;
+    all += counts[w];
+  }
+  if (mine) found[in_front + __popcll(have & ((1ull << (tid & 63)) - 1))] = (unsigned)token << 8 | tid;
+  __syncthreads();
+  // by token, then position: a few of them, ranked by counting
+  if (tid < all) {
+    const unsigned me = found[tid];
+    int rank = 0;
+    for (int i = 0; i < all; ++i) rank += found[i] < me;
+    sorted[rank] = me;
+  }
+  if (tid <= rows) {
+    int n = 0;
+    for (int i = 0; i < all; ++i) n += (int)(found[i] >> 8) < tid;
+    begin[tid] = n;
+  }
+  __syncthreads();
+  const T* dz = (const T*)a.dz;
+  const int groups = 256 / lanes, group = tid / lanes, lane = tid - group * lanes;
+  if (group >= groups) return;
+  for (int r = group; r < rows; r += groups) {
+    T* row = (T*)a.d_wte + (v0 + r) * a.H;
+    const int first = begin[r], last = begin[r + 1];
+    for (int chunk = lane; chunk < chunks; chunk += lanes) {
+      float sum[VN];
+      clear(sum);
+      if (first < last) {
+        add_rows<T, VN>(dz, a.H, chunk, first, last, [&](int64_t i) { return (int64_t)(sorted[i] & 255); }, sum);
+        put_sum<T, VN>(a, row, chunk, sum);
+      } else {
+        put_chunk<T, VN>(row + chunk * VN, sum);
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// More: the sort.
+// ---------------------------------------------------------------------------
+// Lanes of the wavefront with the same digit.
+__device__ __forceinline__ uint64_t same_digit(unsigned digit, int bits, bool valid) {
+  uint64_t same = __ballot(valid);
+  for (int b = 0; b < bits; ++b) {
+    const uint64_t ones = __ballot(digit >> b & 1);
+    same &= digit >> b & 1 ? ones : ~ones;
+  }
+  return same;
+}
+
+__device__ __forceinline__ unsigned key_of(const EmbedGradArgs& a, int64_t i) {
+  const int64_t id = a.ids[i];
+  return (unsigned)((uint64_t)id < (uint64_t)a.V ? id : a.V);
+}
+
+// What fills the GPU beside the sort: zero rows of the token table's gradient (in blocks of 64 KB), rows of the position table's.
+template <typename T, int VN, int NT>
+__device__ __forceinline__ void fill_block(const EmbedGradArgs& a, int64_t block) {
+  const int64_t elements = a.V * (int64_t)a.H;
+  constexpr int64_t PER = 65536 / sizeof(T);
+  const int64_t first = block * PER, last = min(first + PER, elements);
+  float none[VN];
+  clear(none);
+  for (int64_t i = first + threadIdx.x * VN; i < last; i += NT * VN) put_chunk<T, VN>((T*)a.d_wte + i, none);
+}
+
+// How many tokens of each tile have each digit.  FIRST: from the ids themselves; blocks behind the sort's fill.
+template <typename T, int VN, bool FIRST>
+__global__ __launch_bounds__(kSortThreads) void embed_grad_count_kernel(EmbedGradArgs a, int shift, int from) {
+  if (FIRST && (int)blockIdx.x >= a.sort_blocks) {
+    fill_block<T, VN, kSortThreads>(a, (int64_t)blockIdx.x - a.sort_blocks);
+    return;
+  }
+  __shared__ unsigned counts[1 << kMaxBits];
+  const int tid = threadIdx.x, digits = 1 << a.bits;
+  if (tid < digits) counts[tid] = 0;
+  __syncthreads();
+  const int64_t base = (int64_t)blockIdx.x * kTile;
+  for (int i = tid; i < kTile && base + i < a.tokens; i += kSortThreads) {
+    const unsigned key = FIRST ? key_of(a, base + i) : a.keys[from][base + i];
+    atomicAdd(&counts[key >> shift & (digits - 1)], 1u);
+  }
+  __syncthreads();
+  if (tid < digits) a.hist[(int64_t)blockIdx.x * digits + tid] = counts[tid];
+}
+
+// Moves the tokens to their places by one digit.  FIRST: from the ids, with rows of the position table in blocks behind.
+template <typename T, int VN, bool FIRST>
+__global__ __launch_bounds__(kSortThreads) void embed_grad_move_kernel(EmbedGradArgs a, int shift, int from) {
+  constexpr int WAVES = kSortThreads / kWave, EACH = kTile / kSortThreads;
+  __shared__ union {
+    struct {
+      unsigned counts[WAVES][1 << kMaxBits];
+      unsigned base[1 << kMaxBits];
+      unsigned sums[WAVES];
+    } s;
+    float lds[kSortThreads * VN];
+  } sh;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, digits = 1 << a.bits;
+  if (FIRST && (int)blockIdx.x >= a.sort_blocks) {
+    position_row<T, VN, kSortThreads>(a, (int64_t)blockIdx.x - a.sort_blocks, lanes_of(a.H / VN, kSortThreads), sh.lds);
+    return;
+  }
+  for (int i = tid; i < WAVES << a.bits; i += kSortThreads) sh.s.counts[i >> a.bits][i & (digits - 1)] = 0;
+  // where this tile's tokens of each digit begin: behind all of smaller digits and the tiles in front
+  unsigned before = 0, total = 0;
+  if (tid < digits)
+    for (int t = 0; t < a.tiles; ++t) {
+      const unsigned n = a.hist[(int64_t)t * digits + tid];
+      before += t < (int)blockIdx.x ? n : 0;
+      total += n;
+    }
+  unsigned scan = total;
+#pragma unroll
+  for (int step = 1; step < 64; step *= 2) {
+    const unsigned other = __shfl_up(scan, step);
+    scan += lane >= step ? other : 0;
+  }
+  if (lane == 63) sh.s.sums[wave] = scan;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) scan += sh.s.sums[w];
+  if (tid < digits) sh.s.base[tid] = scan - total + before;
+  // each wavefront has 64 EACH tokens in a row, 64 at a time
+  const int64_t base = (int64_t)blockIdx.x * kTile + wave * (kWave * EACH);
+  unsigned key[EACH], at[EACH], rank[EACH];
+#pragma unroll
+  for (int j = 0; j < EACH; ++j) {
+    const int64_t i = base + j * kWave + lane;
+    key[j] = at[j] = 0;
+    if (i < a.tokens) {
+      key[j] = FIRST ? key_of(a, i) : a.keys[from][i];
+      at[j] = FIRST ? (unsigned)i : a.at[from][i];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < EACH; ++j) {
+    const bool valid = base + j * kWave + lane < a.tokens;
+    const unsigned digit = key[j] >> shift & (digits - 1);
+    const uint64_t same = same_digit(digit, a.bits, valid);
+    const int in_front = __popcll(same & ((1ull << lane) - 1));
+    volatile unsigned* count = &sh.s.counts[wave][digit];
+    rank[j] = *count + in_front;
+    __builtin_amdgcn_wave_barrier();
+    if (valid && in_front == 0) *count = rank[j] + __popcll(same);
+    __builtin_amdgcn_wave_barrier();
+  }
+  __syncthreads();
+  if (tid < digits) {
+    unsigned sum = sh.s.base[tid];
+    for (int w = 0; w < WAVES; ++w) {
+      const unsigned n = sh.s.counts[w][tid];
+      sh.s.counts[w][tid] = sum;
+      sum += n;
+    }
+  }
+  __syncthreads();
+  unsigned* keys = a.keys[1 - from];
+  unsigned* to = a.at[1 - from];
+#pragma unroll
+  for (int j = 0; j < EACH; ++j)
+    if (base + j * kWave + lane < a.tokens) {
+      const unsigned place = sh.s.counts[wave][key[j] >> shift & (digits - 1)] + rank[j];
+      keys[place] = key[j];
+      to[place] = at[j];
+    }
+}
+
+// ---------------------------------------------------------------------------
+// The sums of runs of a.run sorted tokens, a group of threads a run.
+// ---------------------------------------------------------------------------
+constexpr int kMaxRun = 128;
+
+template <typename T, int VN>
+__global__ __launch_bounds__(256) void embed_grad_sum_kernel(EmbedGradArgs a) {
+  typedef T V __attribute__((ext_vector_type(VN)));
+  const int chunks = a.H / VN, lanes = lanes_of(chunks, 256), groups = 256 / lanes;
+  const int group = threadIdx.x / lanes, lane = threadIdx.x - group * lanes;
+  const int64_t runs = (a.tokens + a.run - 1) / a.run, r = (int64_t)blockIdx.x * groups + group;
+  if (group >= groups || r >= runs) return;
+  const int64_t first = r * a.run, last = min(first + a.run, a.tokens);
+  const T* dz = (const T*)a.dz;
+  const unsigned none = (unsigned)a.V;
+  const unsigned before = first > 0 ? a.sorted[first - 1] : ~0u, behind = last < a.tokens ? a.sorted[last] : ~0u;
+  constexpr int U = 8;
+  for (int chunk = blockIdx.y * 256 + lane; chunk < min(chunks, (int)(blockIdx.y + 1) * 256); chunk += lanes) {
+    float sum[VN];
+    clear(sum);
+    bool began = a.sorted[first] != before;  // the token at hand began in this run
+    for (int64_t i0 = first; i0 < last; i0 += U) {
+      unsigned token[U + 1];
+      V x[U];
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const int64_t i = min(i0 + j, last - 1);
+        token[j] = a.sorted[i];
+        if (token[j] != none) {
+          const T* from = dz + (int64_t)a.order[i] * a.H + chunk * VN;
+          if constexpr (VN == 1) x[j][0] = *from;
+          else x[j] = *reinterpret_cast<const V*>(from);
+        }
+      }
+      token[U] = i0 + U < last ? a.sorted[i0 + U] : behind;
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        if (i0 + j >= last || token[j] == none) break;
+#pragma unroll
+        for (int n = 0; n < VN; ++n) sum[n] += (float)x[j][n];
+        const bool end = i0 + j == last - 1;
+        if ((end ? behind : token[j + 1]) != token[j]) {
+          if (began) {
+            put_sum<T, VN>(a, (T*)a.d_wte + (int64_t)token[j] * a.H, chunk, sum);
+          } else {
+            put_chunk<float, VN>(a.parts + (r * 2) * a.H + chunk * VN, sum);
+          }
+          clear(sum);
+          began = true;
+        } else if (end) {
+          put_chunk<float, VN>(a.parts + (r * 2 + (began ? 1 : 0)) * a.H + chunk * VN, sum);
+        }
+      }
+    }
+  }
+}
+
+// The tokens that go on behind the run in which they began: a workgroup each run, most of which have none.
+template <typename T, int VN>
+__global__ __launch_bounds__(256) void embed_grad_join_kernel(EmbedGradArgs a) {
+  __shared__ float lds[256 * VN];
+  const int64_t r = blockIdx.x, first = r * a.run, last = first + a.run;
+  const unsigned token = a.sorted[last - 1];  // no workgroup has the last run
+  if (a.sorted[last] != token || token == (unsigned)a.V) return;
+  if (a.sorted[first] == token && first > 0 && a.sorted[first - 1] == token) return;
+  // runs behind that begin with it
+  const int64_t runs = (a.tokens + a.run - 1) / a.run;
+  int64_t more = 0;
+  for (;;) {
+    const int64_t at = r + 1 + more + (threadIdx.x & 63);
+    const int n = __popcll(__ballot(at < runs && a.sorted[min(at, runs - 1) * a.run] == token));
+    more += n;
+    if (n < kWave) break;
+  }
+  const int chunks = a.H / VN, lanes = lanes_of(chunks, 256), groups = 256 / lanes;
+  const int group = threadIdx.x / lanes, lane = threadIdx.x - group * lanes;
+  const int64_t share = (more + groups - 1) / groups;
+  const int64_t from = min((int64_t)group * share, more), to = group < groups ? min(from + share, more) : from;
+  for (int c0 = blockIdx.y * 256; c0 < min(chunks, (int)(blockIdx.y + 1) * 256); c0 += lanes) {
+    const int chunk = c0 + lane;
+    float sum[VN];
+    clear(sum);
+    if (group < groups && chunk < chunks) {
+      if (group == 0) add_chunk(a.parts + (r * 2 + 1) * a.H + chunk * VN, sum);
+      add_rows<float, VN>(a.parts, a.H, chunk, from, to, [&](int64_t i) { return (r + 1 + i) * 2; }, sum);
+    }
+    if (groups > 1) {
+      __syncthreads();
+      if (group < groups)
+#pragma unroll
+        for (int i = 0; i < VN; ++i) lds[(group * VN + i) * lanes + lane] = sum[i];
+      __syncthreads();
+      if (group == 0)
+        for (int n = 1; n < groups; ++n)
+#pragma unroll
+          for (int i = 0; i < VN; ++i) sum[i] += lds[(n * VN + i) * lanes + lane];
+    }
+    if (group == 0 && chunk < chunks) put_sum<T, VN>(a, (T*)a.d_wte + (int64_t)token * a.H, chunk, sum);
+  }
+}
+
+// Only the position table's.
+template <typename T, int VN>
+__global__ __launch_bounds__(kSortThreads) void embed_grad_positions_kernel(EmbedGradArgs a) {
+  __shared__ float lds[kSortThreads * VN];
+  position_row<T, VN, kSortThreads>(a, blockIdx.x, lanes_of(a.H / VN, kSortThreads), lds);
+}
+
+int run_of(int64_t tokens) { return tokens >= 1 << 17 ? 128 : tokens >= 1 << 15 ? 64 : 32; }
+
+template <typename T, int VN>
+void launch_as(EmbedGradArgs a, hipStream_t st) {
+  if (!a.d_wte) {
+    hipLaunchKernelGGL((embed_grad_positions_kernel<T, VN>), dim3((unsigned)a.P), dim3(kSortThreads), 0, st, a);
+    return;
+  }
+  const int64_t positions = a.d_wpe ? a.P : 0;
+  if (a.tokens <= kFew) {
+    // up to 64 rows a workgroup, fewer where that leaves CUs without one
+    int rows = 64;
+    while (rows > 4 && (a.V + rows - 1) / rows < 512) rows /= 2;
+    const int64_t blocks = (a.V + rows - 1) / rows;
+    hipLaunchKernelGGL((embed_grad_few_kernel<T, VN>), dim3((unsigned)(blocks + positions)), dim3(256), 0, st, a, rows,
+                       (int)blocks);
+    return;
+  }
+  int width = 1;
+  while (a.V >> width) ++width;  // bits of V, the key of no token
+  const int passes = (width + kMaxBits - 1) / kMaxBits;
+  a.bits = (width + passes - 1) / passes;
+  a.tiles = a.sort_blocks = (int)((a.tokens + kTile - 1) / kTile);
+  const int64_t fill = (a.V * a.H * (int64_t)sizeof(T) + 65535) / 65536;
+  for (int pass = 0; pass < passes; ++pass) {
+    const int shift = pass * a.bits, from = pass & 1;
+    if (pass == 0) {
+      hipLaunchKernelGGL((embed_grad_count_kernel<T, VN, true>), dim3((unsigned)(a.tiles + fill)), dim3(kSortThreads), 0, st, a,
+                         shift, from);
+      hipLaunchKernelGGL((embed_grad_move_kernel<T, VN, true>), dim3((unsigned)(a.tiles + positions)), dim3(kSortThreads), 0,
+                         st, a, shift, from);
+    } else {
+      hipLaunchKernelGGL((embed_grad_count_kernel<T, VN, false>), dim3(a.tiles), dim3(kSortThreads), 0, st, a, shift, from);
+      hipLaunchKernelGGL((embed_grad_move_kernel<T, VN, false>), dim3(a.tiles), dim3(kSortThreads), 0, st, a, shift, from);
+    }
+  }
+  a.sorted = a.keys[passes & 1];
+  a.order = a.at[passes & 1];
+  const int chunks = a.H / VN;
+  int lanes = 1;  // lanes_of(chunks, 256)
+  if (chunks >= 256) lanes = 256;
+  else if (chunks > 32) lanes = (chunks + 63) & ~63;
+  else
+    while (lanes < chunks) lanes *= 2;
+  const int groups = 256 / lanes;
+  const int64_t runs = (a.tokens + a.run - 1) / a.run;
+  const unsigned across = (unsigned)((chunks + 255) / 256);
+  hipLaunchKernelGGL((embed_grad_sum_kernel<T, VN>), dim3((unsigned)((runs + groups - 1) / groups), across), dim3(256), 0, st, a);
+  if (runs > 1)
+    hipLaunchKernelGGL((embed_grad_join_kernel<T, VN>), dim3((unsigned)(runs - 1), across), dim3(256), 0, st, a);
+}
+
+int64_t up(int64_t bytes) { return (bytes + 255) & ~(int64_t)255; }
+
+}  // namespace
+
+size_t embed_grad_bytes(int64_t tokens, int64_t H) {
+  if (tokens <= kFew) return 0;
+  const int64_t run = run_of(tokens), runs = (tokens + run - 1) / run, tiles = (tokens + kTile - 1) / kTile;
+  return (size_t)(4 * up(tokens * 4) + up(tiles * (4 << kMaxBits)) + up(runs * 2 * H * 4));
+}
+
+void launch_embed_backward(const int64_t* ids, const void* dz, void* d_wte, void* d_wpe, int64_t tokens, int64_t L, int64_t V,
+                           int64_t P, int H, Dropout drop, bool f16, void* workspace, hipStream_t st) {
+  EmbedGradArgs a = {};
+  a.ids = ids;
+  a.dz = dz;
+  a.d_wte = d_wte;
+  a.d_wpe = d_wpe;
+  a.tokens = tokens, a.L = L, a.V = V, a.P = P, a.H = H;
+  a.drop = DropoutArgs{drop.p, (unsigned)drop.seed, (unsigned)(drop.seed >> 32)};
+  a.run = run_of(tokens);
+  char* ws = (char*)workspace;
+  for (int i = 0; i < 2; ++i) {
+    a.keys[i] = (unsigned*)(ws + (2 * i) * up(tokens * 4));
+    a.at[i] = (unsigned*)(ws + (2 * i + 1) * up(tokens * 4));
+  }
+  a.hist = (unsigned*)(ws + 4 * up(tokens * 4));
+  a.parts = (float*)((char*)a.hist + up((tokens + kTile - 1) / kTile * (4 << kMaxBits)));
+  const uintptr_t all = (uintptr_t)dz | (uintptr_t)d_wte | (uintptr_t)d_wpe;
+  if (f16) {
+    if (H % 8 == 0 && (all & 15) == 0) launch_as<_Float16, 8>(a, st);
+    else launch_as<_Float16, 1>(a, st);
+  } else {
+    if (H % 4 == 0 && (all & 15) == 0) launch_as<float, 4>(a, st);
+    else launch_as<float, 1>(a, st);
+  }
+}
+
+}  // namespace gptmi

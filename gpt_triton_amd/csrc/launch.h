@@ -20,6 +20,11 @@ void launch_dropout_mask(void* mask, int64_t words, Dropout drop, hipStream_t st
 
 int launch_embed(const int64_t* ids, const void* wte, const void* wpe, void* out,
                  int64_t rows, int64_t L, int64_t V, int H, Dropout drop, bool f16, hipStream_t st);
+// Gradients of the embedding's tables (embed_grad.hip); one of them may be nullptr.  workspace: embed_grad_bytes, 256-byte
+// aligned.
+size_t embed_grad_bytes(int64_t tokens, int64_t H);
+void launch_embed_backward(const int64_t* ids, const void* dz, void* d_wte, void* d_wpe, int64_t tokens, int64_t L, int64_t V,
+                           int64_t P, int H, Dropout drop, bool f16, void* workspace, hipStream_t st);
 bool launch_embed_layernorm(const int64_t* ids, const void* wte, const void* wpe, const void* w,
                             const void* b, void* emb, void* out, int64_t rows, int64_t L,
                             int64_t V, int H, float eps, bool f16, hipStream_t st);
@@ -127,6 +132,18 @@ void launch_token_log_probs_backward(const LogitRows& a, const int64_t* tokens, 
 void launch_distillation(const LogitRows& a, const int64_t* teacher_tokens, const void* teacher, bool teacher_f16,
                          int k, const float* weights, RowGradient d_losses, float* losses, void* grad, int64_t ld_grad,
                          hipStream_t st);
+
+// Many gradients (grad_norm.hip): arrays on the host.  workspace: clip_grad_bytes, 8-byte aligned.
+struct Gradients {
+  const void* const* in;
+  void* const* out;
+  const int64_t* sizes;
+  const unsigned char *in_f16, *out_f16;
+  int64_t tensors;
+  bool in_place;  // all of them
+};
+size_t clip_grad_bytes(int64_t tensors);
+void launch_clip_grad_norm(const Gradients& g, float scale, float limit, float* norm, void* workspace, hipStream_t st);
 
 // LayerNorm (unless x is normed), q, k, v product (packed weight image Bt [3h][h]) and causal attention of short
 // sequences in one launch: fp16, head size 64, out [B][L][heads][64], the bits of the launches it stands for.  All

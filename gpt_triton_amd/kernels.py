@@ -147,8 +147,7 @@ def _wlayout(weight, default):
     return _lib.GPTMI_W_PACKED if isinstance(weight, PackedWeight) else default
 
 
-def fused_embeddings(x, wte, wpe, dropout_prob=0.0):
-    """dropout(wte[x] + wpe[position]) for token ids x [B, L] -> [B, L, H] in wte's dtype."""
+def _embeddings(x, wte, wpe, dropout_prob):
     assert wte.shape[1] == wpe.shape[1]
     assert x.is_contiguous()
     assert wte.is_contiguous()
@@ -167,6 +166,97 @@ def fused_embeddings(x, wte, wpe, dropout_prob=0.0):
           wpe.data_ptr(), z.data_ptr(), B, L, V, P, H, float(dropout_prob), 1337,
           _dtype_code(wte, "fused_embeddings"))
     return z
+
+
+class _EmbeddingsFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, wte, wpe, dropout_prob):
+        ctx.save_for_backward(x)
+        ctx.tables, ctx.dropout_prob = (wte.shape[0], wpe.shape[0], wte.shape[1]), float(dropout_prob)
+        return _embeddings(x, wte, wpe, dropout_prob)
+
+    @staticmethod
+    def backward(ctx, dz):
+        _first_derivative("fused_embeddings")
+        x, = ctx.saved_tensors
+        (B, L), (V, P, H) = x.shape, ctx.tables
+        dz = dz.contiguous()
+        d_wte = dz.new_empty((V, H)) if ctx.needs_input_grad[1] else None
+        d_wpe = dz.new_empty((P, H)) if ctx.needs_input_grad[2] else None
+        lib = _lib.load()
+        nbytes = 0 if d_wte is None else lib.gptmi_embed_backward_workspace_bytes(B, L, H)
+        ws = _workspace(nbytes, dz)
+        _call(dz.get_device(), "fused_embeddings", lib.gptmi_embed_backward, x.data_ptr(), dz.data_ptr(), _ptr(d_wte),
+              _ptr(d_wpe), B, L, V, P, H, ctx.dropout_prob, 1337, _ptr(ws), nbytes, _dtype_code(dz, "fused_embeddings"))
+        return None, d_wte, d_wpe, None
+
+
+def fused_embeddings(x, wte, wpe, dropout_prob=0.0):
+    """dropout(wte[x] + wpe[position]) for token ids x [B, L] -> [B, L, H] in wte's dtype.
+
+    Gradients flow to wte and wpe, dense, backward and once: sums over a token's positions and over the batch, in fp32, each
+    in one order, so that the same step gives the same bits."""
+    if (wte.requires_grad or wpe.requires_grad) and torch.is_grad_enabled():
+        return _EmbeddingsFunction.apply(x, wte, wpe, dropout_prob)
+    return _embeddings(x, wte, wpe, dropout_prob)
+
+
+def _side_by_side(t):
+    """Whether a tensor's elements fill its memory without gaps, in whatever order of the dimensions."""
+    if t.is_contiguous():
+        return True
+    expected = 1
+    for stride, size in sorted((stride, size) for stride, size in zip(t.stride(), t.shape) if size != 1):
+        if stride != expected:
+            return False
+        expected *= size
+    return True
+
+
+def clip_grad_norm_(grads, max_norm, scale=1.0, out=None):
+    """norm = scale * sqrt(sum of the squares of all elements of all of `grads`), and min(1, max_norm / norm) * scale times each
+    gradient in its place, or in `out`'s tensor of the same shape (which leaves `grads` as they are).  Returns the norm, a
+    float32 number on the GPU; nothing waits for it.
+
+    grads: tensors, float32 or float16, on one GPU, dense in any order of dimensions, none twice; out: as many, each of
+    either type and of the order of its gradient, none of which overlaps anything else; a gradient itself may be in its place.
+    scale: the inverse of a loss scale; max_norm infinity: the norm, and the gradients times scale.  Squares are summed in 64
+    bits.  Gradients in place are written only where the factor is not 1.  An infinity among them makes the norm infinite and
+    the results 0 or NaN, a NaN makes all of them NaN: a step to skip."""
+    grads = list(grads)
+    outs = grads if out is None else list(out)
+    what = "clip_grad_norm_"
+    assert grads, "no gradients"
+    assert len(outs) == len(grads), (len(outs), len(grads))
+    dev = _on_gpu(grads[0], *grads[1:], *outs)
+    scale, max_norm = float(scale), float(max_norm)
+    if not 0.0 < scale < math.inf or not max_norm > 0.0:
+        raise ValueError(f"{what}: scale {scale} or max_norm {max_norm} is not positive")
+    half = torch.float16
+    for t in grads if out is None else grads + outs:
+        if t.dtype is not half and t.dtype is not torch.float32:
+            _dtype_code(t, what)
+        assert t.is_contiguous() or _side_by_side(t), "the elements of a gradient must fill its memory"
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{what} has no derivative")
+    if out is not None:
+        for g, o in zip(grads, outs):
+            assert o.shape == g.shape and (o.stride() == g.stride() or o.is_contiguous() and g.is_contiguous()), (
+                "out must have the gradients' shapes and orders")
+    n = len(grads)
+    at = array.array("Q", [t.data_ptr() for t in grads])
+    sizes = array.array("q", [t.numel() for t in grads])
+    types = bytes([t.dtype is half for t in grads])
+    to, out_types = (at, types) if out is None else (array.array("Q", [t.data_ptr() for t in outs]),
+                                                     bytes([t.dtype is half for t in outs]))
+    norm = grads[0].new_empty((), dtype=torch.float32)
+    lib = _lib.load()
+    nbytes = lib.gptmi_clip_grad_norm_workspace_bytes(n)
+    ws = _workspace(nbytes, grads[0])
+    _call(dev, what, lib.gptmi_clip_grad_norm, at.buffer_info()[0], to.buffer_info()[0], sizes.buffer_info()[0], types,
+          out_types, n, scale, max_norm, norm.data_ptr(), _ptr(ws), nbytes)
+    torch.autograd.graph.increment_version([t for t in outs if not t.is_inference()])
+    return norm
 
 
 def fused_embeddings_layer_norm(x, wte, wpe, weight, bias):

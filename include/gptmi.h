@@ -96,6 +96,23 @@ int gptmi_embed(const int64_t* ids, const void* wte, const void* wpe, void* out,
                 float p, uint64_t seed, int dtype, void* stream);
 
 /*
+ * The gradients of gptmi_embed's tables for dz [B*L][H], that of its output, dense:
+ *   d_wte[v,:] = sum of dz[b,l,:] over the positions with ids[b,l] = v     d_wpe[l,:] = sum_b dz[b,l,:]
+ * with dropout times the mask of the column over 1 - p.  Rows without a token, and positions from L on, are zeros; a token id
+ * outside [0, V) counts for its position alone.  Sums are fp32, each in the order of its positions, without atomics: the
+ * same call gives the same bits; one rounding to the storage dtype.
+ *   d_wte [V][H], d_wpe [P][H]: one of them may be NULL; they overlap nothing
+ *   workspace: gptmi_embed_backward_workspace_bytes(B, L, H) bytes, 256-byte aligned (may be NULL where that is 0, or d_wte is)
+ * Up to 2^30 tokens, 2^26 rows of wte, 2^21 of wpe, H up to 2^20; any alignment that the element type allows, fastest where rows
+ * and addresses are multiples of 16 bytes.
+ * No counterpart in the reference, which has no gradients.
+ */
+size_t gptmi_embed_backward_workspace_bytes(int64_t B, int64_t L, int64_t H);
+int gptmi_embed_backward(const int64_t* ids, const void* dz, void* d_wte, void* d_wpe, int64_t B, int64_t L,
+                         int64_t V, int64_t P, int64_t H, float p, uint64_t seed, void* workspace,
+                         size_t workspace_bytes, int dtype, void* stream);
+
+/*
  * gptmi_embed (without dropout) and gptmi_layernorm of its result in one pass over the rows:
  *   emb[b,l,:] = wte[ids[b,l],:] + wpe[l,:]          out[b,l,:] = LayerNorm(emb[b,l,:]; ln_w, ln_b)
  * Both outputs are bit-identical to the two calls made one after the other (the LayerNorm works
@@ -185,6 +202,22 @@ int gptmi_distillation_loss(const void* logits, int64_t ld, const int64_t* teach
                             const void* teacher_logits, int64_t k, float temperature, const float* weights,
                             const float* d_losses, int64_t d_pitch, float* losses, void* grad, int64_t ld_grad,
                             int64_t M, int64_t V, int dtype, int teacher_dtype, void* stream);
+
+/*
+ * The norm of n gradients together, and these at most at max_norm:
+ *   norm = scale sqrt(sum g^2) over all elements of all tensors        out = scale min(1, max_norm / norm) g
+ * Squares are summed in 64 bits.  An infinity among the gradients makes the norm infinite and out 0, and NaN in its place; a
+ * NaN makes all of them NaN.
+ *   grads, out, sizes, f16, out_f16: host arrays, read during the call: device addresses, elements (0 allowed), and whether the
+ *   tensor is of type GPTMI_F16 (else GPTMI_F32).  out[i] may be grads[i], of the same type, which is then written only where it
+ *   changes; what is written overlaps nothing else (GPTMI_ERR_INVALID)
+ *   norm: one float on the device     scale > 0     max_norm > 0, infinity for the norm alone
+ * workspace: gptmi_clip_grad_norm_workspace_bytes(n) bytes, 8-byte aligned.  n up to 2^20.  No counterpart in the reference.
+ */
+size_t gptmi_clip_grad_norm_workspace_bytes(int64_t n);
+int gptmi_clip_grad_norm(const void* const* grads, void* const* out, const int64_t* sizes,
+                         const unsigned char* f16, const unsigned char* out_f16, int64_t n, float scale,
+                         float max_norm, float* norm, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Bytes of workspace gptmi_linear / gptmi_linear_qkv need for these sizes
