@@ -939,8 +939,10 @@ int gptmi_flash_attn_packed_train(const void* q, const void* k, const void* v, v
                            d, dtype, stream);
 }
 
-size_t gptmi_flash_attn_packed_backward_workspace_bytes(int64_t T, int64_t N) {
-  return T > 0 && N > 0 && T < 1ll << 31 && N <= 1 << 20 ? packed_attn_grad_bytes(T, N) : 0;
+size_t gptmi_flash_attn_packed_backward_workspace_bytes(int64_t sequences, int64_t T, int64_t N, int64_t G, int64_t d) {
+  const bool ok = sequences > 0 && sequences <= 1ll << 30 && T > 0 && T < 1ll << 31 && N > 0 && N <= 1 << 20 && G > 0 &&
+                  N % G == 0 && d > 0 && d <= 256;
+  return ok ? packed_attn_grad_bytes(T, sequences, N, G, d) : 0;
 }
 
 int gptmi_flash_attn_packed_backward(const void* q, const void* k, const void* v, const void* out, const float* stats,
@@ -957,7 +959,7 @@ int gptmi_flash_attn_packed_backward(const void* q, const void* k, const void* v
                           v_head, scale};
   int rc = check_packed(what, p, d, (uintptr_t)out | (uintptr_t)d_out | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv, dtype);
   if (rc) return rc;
-  const size_t needed = packed_attn_grad_bytes(T, N);
+  const size_t needed = packed_attn_grad_bytes(T, sequences, N, G, d);
   if (!workspace || workspace_bytes < needed || ((uintptr_t)workspace & 255) != 0) {
     set_error("%s: workspace of %zu bytes needed, 256-byte aligned, %zu given", what, needed, workspace ? workspace_bytes : (size_t)0);
     return GPTMI_ERR_WORKSPACE;

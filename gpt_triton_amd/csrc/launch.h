@@ -100,12 +100,12 @@ struct PackedAttention {
 };
 int launch_flash_attn_packed(const PackedAttention& p, int d, hipStream_t st);
 // Its gradients (packed_attn_grad.hip), all dense: dq, or dk and dv, may be nullptr.  `out` and `stats` are the forward
-// pass's.  workspace: packed_attn_grad_bytes, 8-byte aligned.
+// pass's.  workspace: packed_attn_grad_bytes, 256-byte aligned.
 struct PackedGradients {
   const void* d_out;
   void *dq, *dk, *dv;
 };
-size_t packed_attn_grad_bytes(int64_t rows, int64_t heads);
+size_t packed_attn_grad_bytes(int64_t rows, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t d);
 int launch_flash_attn_packed_backward(const PackedAttention& p, const PackedGradients& d, int head_size, void* workspace,
                                       hipStream_t st);
 

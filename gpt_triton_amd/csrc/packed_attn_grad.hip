@@ -14,6 +14,7 @@
 // row c of x and four rows of y; rows 4 g + r of the two 16-row blocks b of a group of 32 are y's rows 8 g + 4 b + r, so
 // that w and u, rounded to fp16, are the second operand of the sums over y as they stand.
 #include <type_traits>
+#include <utility>
 
 #include "common.h"
 #include "launch.h"
@@ -25,18 +26,25 @@ namespace {
 // The weights are formed as 2^kUp w and u as 2^kUp f u, f a power of two: fp16 numbers of the size of one that stay
 // normal numbers down to 2^-28 of it.
 constexpr int kUp = 14;
-constexpr int kSums = 512;  // workgroups of the row sums at most
+constexpr int kSums = 1024;  // workgroups of the row sums at most
 
+struct SlotDeal {
+  int slots, grid;
+  bool longest_first;
+};
 struct GradArgs {
   const _Float16 *q, *k, *v, *out, *d_out;
   _Float16 *dq, *dk, *dv;  // dense; dq, or dk and dv, may be nullptr
   const float2* stats;     // [heads][T], the forward pass's
-  float *lse, *delta;      // [heads][T]: w = 2^(s t log2(e) - lse - kUp); a NaN: see packed_sums_kernel
+  float *lse, *minus_delta;  // [heads][T]: 2^kUp w = 2^(s t log2(e) - lse); a NaN: see packed_sums_kernel
   float2* most;            // the largest e . e and v . v of each workgroup of the row sums
   int mosts;
   const int64_t* starts;
   int64_t rows;  // T
-  int sequences, heads, kv_heads, slots, longest_first;
+  int sequences, heads, kv_heads;
+  SlotDeal deal[2];  // of the blocks of queries, and of keys
+  int shares;        // into which the heads that share a key head are divided
+  float* parts;      // more than one: their sums, [shares][2][T][kv_heads][d], dk and dv
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;  // pitches in elements
   float scale;
 };
@@ -50,7 +58,7 @@ template <int D>
 __global__ __launch_bounds__(256) void packed_sums_kernel(GradArgs a) {
   constexpr int LPR = D / 8;          // lanes a row
   constexpr int RPP = 256 / LPR;      // rows a pass
-  constexpr int BLOCK = RPP > 64 ? RPP : 64;
+  constexpr int BLOCK = RPP > 64 ? RPP : 64, PASSES = BLOCK / RPP;
   __shared__ float2 largest[4];
   const int tid = threadIdx.x, in_row = tid % LPR, row_of = tid / LPR;
   const int64_t from = a.starts[0], to = a.starts[a.sequences];
@@ -59,27 +67,35 @@ __global__ __launch_bounds__(256) void packed_sums_kernel(GradArgs a) {
   for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
     const int64_t block = item / a.heads;
     const int head = (int)(item - block * a.heads);
+    // all rows' loads first
+    h8 e[PASSES], o[PASSES], v[PASSES];
+    float2 stat[PASSES];
 #pragma unroll
-    for (int pass = 0; pass < BLOCK / RPP; ++pass) {
+    for (int pass = 0; pass < PASSES; ++pass) {
+      const int64_t row = block * BLOCK + pass * RPP + row_of, at = (row * a.heads + head) * D + in_row * 8;
+      e[pass] = o[pass] = v[pass] = h8(0);
+      if (row < from || row >= to || row >= a.rows) continue;
+      e[pass] = *reinterpret_cast<const h8*>(a.d_out + at);
+      o[pass] = *reinterpret_cast<const h8*>(a.out + at);
+      if (head < a.kv_heads) v[pass] = *reinterpret_cast<const h8*>(a.v + row * a.v_row + head * a.v_head + in_row * 8);
+      stat[pass] = a.stats[head * a.rows + row];
+    }
+#pragma unroll
+    for (int pass = 0; pass < PASSES; ++pass) {
       const int64_t row = block * BLOCK + pass * RPP + row_of;
       if (row >= a.rows) break;
-      const int64_t at = (row * a.heads + head) * D + in_row * 8, kv_at = (row * a.kv_heads + head) * D + in_row * 8;
       if (row < from || row >= to) {
+        const int64_t at = (row * a.heads + head) * D + in_row * 8, kv_at = (row * a.kv_heads + head) * D + in_row * 8;
         if (a.dq) *reinterpret_cast<h8*>(a.dq + at) = h8(0);
         if (a.dk && head < a.kv_heads) *reinterpret_cast<h8*>(a.dk + kv_at) = *reinterpret_cast<h8*>(a.dv + kv_at) = h8(0);
         continue;
       }
-      const h8 e = *reinterpret_cast<const h8*>(a.d_out + at), o = *reinterpret_cast<const h8*>(a.out + at);
       float dot = 0.f, ee = 0.f, vv = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        dot = fmaf((float)e[i], (float)o[i], dot);
-        ee = fmaf((float)e[i], (float)e[i], ee);
-      }
-      if (head < a.kv_heads) {
-        const h8 v = *reinterpret_cast<const h8*>(a.v + row * a.v_row + head * a.v_head + in_row * 8);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) vv = fmaf((float)v[i], (float)v[i], vv);
+        dot = fmaf((float)e[pass][i], (float)o[pass][i], dot);
+        ee = fmaf((float)e[pass][i], (float)e[pass][i], ee);
+        vv = fmaf((float)v[pass][i], (float)v[pass][i], vv);
       }
 #pragma unroll
       for (int step = 1; step < LPR; step *= 2) {
@@ -92,9 +108,8 @@ __global__ __launch_bounds__(256) void packed_sums_kernel(GradArgs a) {
       if (vv < INFINITY) most_v = fmaxf(most_v, vv);
       if (in_row == 0) {
         const int64_t place = head * a.rows + row;
-        const float2 stat = a.stats[place];
-        a.lse[place] = stat.x - __builtin_amdgcn_logf(stat.y) - kUp;  // to the base 2; NaN where stat.y < 0
-        a.delta[place] = dot;
+        a.lse[place] = stat[pass].x - __builtin_amdgcn_logf(stat[pass].y) - kUp;  // to the base 2; NaN where .y < 0
+        a.minus_delta[place] = -dot;
       }
     }
   }
@@ -112,6 +127,18 @@ __global__ __launch_bounds__(256) void packed_sums_kernel(GradArgs a) {
   }
 }
 
+// 4 bytes a lane, as load_lds16.
+__device__ __forceinline__ void load_lds4(const void* base, unsigned lane_off, unsigned lds_off) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dword %1, %2"
+               :
+               : "s"(lds_off), "v"(lane_off), "s"(base)
+               : "memory", "m0");
+}
+
+__device__ __forceinline__ h8 lds_read16(unsigned at) {
+  return *(const __attribute__((address_space(3))) h8*)(uintptr_t)at;
+}
+
 // 2^n with 4 < 2^n bound <= 8 for bound = sqrt(ee vv), which |e . v| does not pass: |u| is at most bound / 2, since what
 // w leaves of 1 is the others' part of delta, so 2^kUp 2^n |u| is at most 2^16, which 65519 rounds to.  (A u that is off
 // by more comes out as an infinity, and is done again.)
@@ -120,46 +147,63 @@ __device__ __forceinline__ float factor_of(float ee, float vv) {
   return bound > 0.f && bound < INFINITY ? ldexpf(1.f, min(ilogbf(7.99f / bound), 100)) : 1.f;
 }
 
-// KEYS: x = k, v and y = q, e of all the key head's heads; else x = q, e and y = k, v.  A workgroup has 64 NB rows of x.
+// f(0), .. f(N - 1), the numbers as types.
+template <typename F, int... I>
+__device__ __forceinline__ void for_each_of(F f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void for_each_of(F f) {
+  for_each_of(f, std::make_integer_sequence<int, N>{});
+}
+
+constexpr int tile_rows(int d) { return d <= 128 ? 64 : 32; }  // of y
+// Whether the steps of a walk overlap (see there): where the sums leave registers for one wavefront a SIMD, which has
+// nothing else to hide its waits behind.
+constexpr bool overlaps(int d, bool keys) { return keys && d >= 128; }
+// Places of tiles in LDS, for the order of the steps.
+constexpr int places_of(int d, bool keys) { return !overlaps(d, keys) ? 2 : tile_rows(d) == 64 ? 3 : 4; }
+constexpr int lds_of(int d, bool keys) { return places_of(d, keys) * 2 * tile_rows(d) * (d * 2 + 4); }
+// Wavefronts a SIMD that the registers are divided for.
+constexpr int waves_of(int d, bool keys) { return d <= 64 ? 3 : keys ? 1 : 2; }
+
+// One workgroup's rows of x against all its rows of y, 64 NB rows of x.  KEYS: x = k, v and y = q, e of all the key head's heads;
+// else x = q, e and y = k, v.
 template <int D, int NB, bool KEYS>
-__global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void packed_grad_kernel(GradArgs a) {
+__device__ __forceinline__ void walk(const GradArgs& a, int id, int slots, bool longest_first) {
   constexpr int R = 64 * NB;
-  constexpr int TY = D <= 128 ? 64 : 32;  // rows of y a tile
+  constexpr int TY = tile_rows(D);
   constexpr int KS = (D + 31) / 32, DB = D / 16;
   constexpr int ROWB = D * 2, CH = D / 8, RPI = 1024 / ROWB;
   constexpr int TILE = TY * ROWB;
+  constexpr bool OVERLAPS = overlaps(D, KEYS);
+  constexpr int GROUPS = TY / 32, PLACES = places_of(D, KEYS);
   constexpr int ROWS = TY / 2, NDMA = ROWS / RPI;  // rows of a tile that a wavefront brings, and its load instructions
-  // Unit u of row r of a tile lies at u ^ key(r).  Row reads take one unit of rows 8 i + 0..3 (+ 4 b), i = 0..3,
-  // transposing ones two units of rows 8 g + 0..3 (+ 4), two g at a time: in different banks both.
+  // Unit u of row r of a tile lies at u ^ key(r).  A row read takes unit g of rows 8 (c / 4) + c % 4 (+ 4 b), served lanes
+  // 0..3, 12..15, 20..27 first, a transposing one two units of rows 8 g + 0..3 (+ 4), two g at a time: in different banks both.
   const auto key = [](int r) {
-    return CH >= 16 ? (r >> 4 & 1) | (r & 3) << 1 | (r >> 3 & 1) << 3
-           : CH == 8 ? (r >> 4 & 1) | (r >> 1 & 1) << 1 | (r >> 3 & 1) << 2
-           : CH == 4 ? (r >> 4 & 1) | (r >> 3 & 1) << 1
-                     : r >> 3 & 1;
+    return 2 * (CH >= 16 ? (r & 3) | (r >> 3 & 1) << 2 : CH == 8 ? (r >> 1 & 1) | (r >> 3 & 1) << 1 : CH == 4 ? r >> 3 & 1 : 0);
   };
-  extern __shared__ __attribute__((aligned(1024))) char smem[];  // two places each for y's two tiles, and their rows' lse and delta
-  float* rows_of = reinterpret_cast<float*>(smem + 4 * TILE);
+  extern __shared__ __attribute__((aligned(1024))) char smem[];  // PLACES of y's two tiles each, and of their rows' lse and delta
+  float* rows_of = reinterpret_cast<float*>(smem + PLACES * 2 * TILE);
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, g = lane >> 4;
   const unsigned smem_base = (unsigned)(uintptr_t)smem;
 
-  const int rep = a.heads / a.kv_heads;
+  const int per_key = a.heads / a.kv_heads, rep = KEYS ? per_key / a.shares : 1;  // heads over a key head, and of this walk
   Place place;
-  if (!find_place((int)(blockIdx.y * kGridRow + blockIdx.x), KEYS ? a.kv_heads : a.heads, a.kv_heads, a.slots,
-                  a.longest_first, &place))
-    return;
+  if (!find_place(id, KEYS ? a.kv_heads * a.shares : a.heads, a.kv_heads, slots, longest_first, &place)) return;
   const Sequences in{a.starts, a.rows, a.sequences};
-  const Block block = a.longest_first && a.sequences > 1 ? nth_longest<R>(in, place.slot)
-                                                         : find_block<R>(in, a.slots - 1 - place.slot);
+  const Block block = longest_first && a.sequences > 1 ? nth_longest<R>(in, place.slot) : find_block<R>(in, slots - 1 - place.slot);
   if (block.length == 0) return;
   const int L = block.length;
   // early keys have the most queries, late queries the most keys
   const int x0 = (KEYS ? (L - 1) / R - block.block : block.block) * R;
   const int xw0 = x0 + wave * 16 * NB;
   const bool active = xw0 < L;
-  const int kv_head = KEYS ? place.head : place.head / rep;
-  const int head0 = KEYS ? place.head * rep : place.head;
+  const int kv_head = __builtin_amdgcn_readfirstlane(place.head / (KEYS ? a.shares : per_key));
+  const int head0 = __builtin_amdgcn_readfirstlane(place.head * rep);
   const int first_tile = KEYS ? x0 / TY : 0;
   const int tiles = (KEYS ? (L - 1) / TY : (min(x0 + R, L) - 1) / TY) + 1 - first_tile;
   const int all = KEYS ? tiles * rep : tiles;
@@ -169,7 +213,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void packed_grad_kernel(GradA
   const _Float16* ep = a.d_out + (block.first * a.heads + head0) * D;
   const int64_t e_row = (int64_t)a.heads * D;
   const float* lse = a.lse + (head0 * a.rows + block.first);
-  const float* delta = a.delta + (head0 * a.rows + block.first);
+  const float* minus_delta = a.minus_delta + (head0 * a.rows + block.first);
 
   // ---- x: lane (c, g) holds d = 32 ks + 8 g + 0..7; rows past the end repeat the last one and are not stored
   h8 xa[NB][KS], xb[NB][KS];
@@ -215,6 +259,11 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void packed_grad_kernel(GradA
         load_lds16(base, (unsigned)min(j * RPI + lrow, last) * (unsigned)pitch + (lane_unit ^ ((unsigned)key(j * RPI) << 4)),
                    dst + j * 1024);
     }
+    if (KEYS && (wave & 1) == 0 && lane < TY) {  // the rows' lse and -delta, too
+      const float* from = (second ? minus_delta : lse) + h * a.rows + (int64_t)t * TY;
+      load_lds4(from, (unsigned)min(lane, L - 1 - t * TY) * 4u,
+                smem_base + (unsigned)(PLACES * 2 * TILE + (place_of * 2 + (second ? 1 : 0)) * TY * 4));
+    }
   };
 
   // ---- the factor that keeps u in fp16's range: one for all rows where rows are summed over, each row's own otherwise
@@ -225,9 +274,9 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void packed_grad_kernel(GradA
     most_v = fmaxf(most_v, m.y);
   }
   most_v = wave_max(most_v);
-  float x_lse[NB], x_delta[NB], factor[NB];  // of row c of block n
+  float x_lse[NB], x_less[NB], factor[NB];  // of row c of block n: lse, less the factor's exponent, and -delta
   if constexpr (KEYS) {
-    factor[0] = factor_of(wave_max(most_e), most_v);
+    factor[0] = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, factor_of(wave_max(most_e), most_v))));
   } else {
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
@@ -239,30 +288,15 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void packed_grad_kernel(GradA
         for (int i = 0; i < 8; ++i) ee = fmaf((float)xb[n][ks][i], (float)xb[n][ks][i], ee);
       const LanePair pair = row_swap(half_sum(ee));
       factor[n] = factor_of(pair.a + pair.b, most_v);
-      x_lse[n] = lse[row];
-      x_delta[n] = delta[row] * factor[n];
+      x_lse[n] = lse[row] - (float)ilogbf(factor[n]);
+      x_less[n] = minus_delta[row];
     }
   }
-  // lse of the rows of y's tile in the first TY threads, delta times the factor in the next; rows behind the end weigh 0
-  auto stat_of = [&](int h, int t) {
-    float x = INFINITY;
-    if (KEYS && tid < 2 * TY) {
-      const int row = t * TY + tid % TY;
-      const float* from = (tid < TY ? lse : delta) + h * a.rows;
-      x = from[min(row, L - 1)];
-      x = tid >= TY ? x * factor[0] : row < L ? x : INFINITY;
-    }
-    return x;
-  };
-
-  // ---- LDS read offsets of this lane inside a tile
+  // ---- this lane's LDS addresses inside a tile: unit g of its row for the row reads, unit (c / 2) % 2 of its row for the
+  // transposing ones.  Another k-slice or 16-column block is another unit, whose bits an xor sets, since the keys are xor'ed too.
   const int k_row = 8 * (c >> 2) + (c & 3), v_row = 8 * g + (c >> 2);
-  constexpr int KV = KS < 4 ? KS : 4, VV = DB < 8 ? DB : 8;
-  int k_off[KV], v_off[VV];
-#pragma unroll
-  for (int ks = 0; ks < KV; ++ks) k_off[ks] = k_row * ROWB + (((4 * ks + (D >= 32 ? g : g & 1)) ^ key(k_row)) << 4);
-#pragma unroll
-  for (int i = 0; i < VV; ++i) v_off[i] = v_row * ROWB + (((2 * i + ((c & 3) >> 1)) ^ key(v_row)) << 4) + (c & 1) * 8;
+  const unsigned k_base = (unsigned)(k_row * ROWB + (((D >= 32 ? g : g & 1) ^ key(k_row)) << 4));
+  const unsigned v_base = (unsigned)(v_row * ROWB + ((((c & 3) >> 1) ^ key(v_row)) << 4) + (c & 1) * 8);
   const float to_exp2 = a.scale * 1.4426950408889634f;
 
   f4 sa[NB][DB], sb[KEYS ? NB : 1][KEYS ? DB : 1];  // sums of u times q or k, and of w times e: d = 16 i + 4 g + 0..3 of row c
@@ -274,89 +308,239 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void packed_grad_kernel(GradA
       if constexpr (KEYS) sb[n][i] = f4(0.f);
     }
 
-  // 32 rows of y, from row y0 of the sequence, at `at` in LDS.  MASK: the diagonal passes through.
-  auto group = [&](auto mask, int y0, const char* at, const float* stat) {
-    constexpr bool MASK = decltype(mask)::value;
-    f4 s[NB][2], p[NB][2];
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const char* from = at + b * 4 * ROWB + k_off[ks % KV] + (ks / KV) * 256;
-        h8 ya = *reinterpret_cast<const h8*>(from), yb = *reinterpret_cast<const h8*>(from + TILE);
-        if (D < 32 && g >= 2) ya = yb = h8(0);
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-          s[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ya, xa[n][ks], ks == 0 ? f4(0.f) : s[n][b], 0, 0, 0);
-          p[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(yb, xb[n][ks], ks == 0 ? f4(0.f) : p[n][b], 0, 0, 0);
-        }
-      }
+  // y goes by in groups of 32 rows.  Without overlap a step is the scores and e . v of a group, its w and u, and the sums over
+  // it; the SIMD's other wavefronts are at another of these.  With overlap it is w and u of one group, the scores and e . v of the
+  // next and the sums over the one in front, which do not wait for each other; the LDS reads of each chunk of some 8 matrix
+  // instructions are issued in front of the one before it, and a part of the vector instructions goes beside each.
+  constexpr int C = KS < 2 ? KS : 2, NQ = 2 * KS / C;                        // score chunks: C k-slices of a 16-row block
+  constexpr int CI = DB < (KEYS ? 1 : 2) ? DB : KEYS ? 1 : 2, NS = DB / CI;  // sum chunks: CI 16-column blocks
+  constexpr int UNITS = 2 * NB;                                              // of four rows' w and u each
+  struct Scores {
+    f4 s[NB][2], p[NB][2], lse[2];
+  };
+  struct Weights {
     h8 w[NB], u[NB];
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      f4 y_lse, y_delta;
-      if constexpr (KEYS) {
-        y_lse = *reinterpret_cast<const f4*>(stat + 8 * g + 4 * b);
-        y_delta = *reinterpret_cast<const f4*>(stat + TY + 8 * g + 4 * b);
-      }
-#pragma unroll
-      for (int n = 0; n < NB; ++n)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float e = fmaf(s[n][b][r], to_exp2, -(KEYS ? y_lse[r] : x_lse[n]));
-          if constexpr (MASK) {
-            const int y = y0 + 8 * g + 4 * b + r, x = xw0 + 16 * n + c;
-            e = (KEYS ? x <= y : y <= x) ? e : -INFINITY;
-          }
-          const float weight = __builtin_amdgcn_exp2f(e);
-          if constexpr (KEYS) w[n][4 * b + r] = (_Float16)weight;
-          u[n][4 * b + r] = (_Float16)(weight * fmaf(p[n][b][r], KEYS ? factor[0] : factor[n], -(KEYS ? y_delta[r] : x_delta[n])));
-        }
+  };
+  struct Rows {
+    h8 a[C], b[C];
+    f4 less;
+  };
+  struct Columns {
+    h8 a[CI], b[KEYS ? CI : 1];
+  };
+  auto read_tr = [](unsigned at) { return lds_read_tr16((const char*)(uintptr_t)at); };
+  auto read_rows = [&](auto chunk, Rows& to, Scores& next, unsigned at, const float* stat) {
+    constexpr int b = decltype(chunk)::value / (KS / C), first = decltype(chunk)::value % (KS / C) * C;
+    if constexpr (KEYS && first == 0) {
+      to.less = *reinterpret_cast<const f4*>(stat + TY + 8 * g + 4 * b);
+      if constexpr (OVERLAPS) next.lse[b] = *reinterpret_cast<const f4*>(stat + 8 * g + 4 * b);
     }
 #pragma unroll
-    for (int i = 0; i < DB; ++i) {
-      const char* from = at + v_off[i % VV] + (i / VV) * 256;
-      const h4 lo = lds_read_tr16(from), hi = lds_read_tr16(from + 4 * ROWB);
-      const h8 ya = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    for (int j = 0; j < C; ++j) {
+      const int ks = first + j;
+      const unsigned from = ((at + k_base) ^ (ks << 6)) + b * 4 * ROWB;
+      to.a[j] = lds_read16(from);
+      to.b[j] = lds_read16(from + TILE);
+      if (D < 32 && g >= 2) to.a[j] = to.b[j] = h8(0);
+    }
+  };
+  auto scores = [&](auto chunk, const Rows& y, Scores& to) {  // s: q . k, p: e . v - delta
+    constexpr int b = decltype(chunk)::value / (KS / C), first = decltype(chunk)::value % (KS / C) * C;
 #pragma unroll
-      for (int n = 0; n < NB; ++n) sa[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ya, u[n], sa[n][i], 0, 0, 0);
+    for (int j = 0; j < C; ++j)
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        const int ks = first + j;
+        to.s[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y.a[j], xa[n][ks], ks == 0 ? f4(0.f) : to.s[n][b], 0, 0, 0);
+        to.p[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y.b[j], xb[n][ks], ks > 0 ? to.p[n][b] : KEYS ? y.less : f4(x_less[n]), 0, 0, 0);
+      }
+  };
+  auto read_columns = [&](auto chunk, Columns& to, unsigned at) {
+#pragma unroll
+    for (int j = 0; j < CI; ++j) {
+      const int i = decltype(chunk)::value * CI + j;
+      const unsigned from = (at + v_base) ^ (i << 5);
+      const h4 lo = read_tr(from), hi = read_tr(from + 4 * ROWB);
+      to.a[j] = h8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
       if constexpr (KEYS) {
-        const h4 lo2 = lds_read_tr16(from + TILE), hi2 = lds_read_tr16(from + TILE + 4 * ROWB);
-        const h8 yb = {lo2[0], lo2[1], lo2[2], lo2[3], hi2[0], hi2[1], hi2[2], hi2[3]};
-#pragma unroll
-        for (int n = 0; n < NB; ++n) sb[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(yb, w[n], sb[n][i], 0, 0, 0);
+        const h4 lo2 = read_tr(from + TILE), hi2 = read_tr(from + TILE + 4 * ROWB);
+        to.b[j] = h8{lo2[0], lo2[1], lo2[2], lo2[3], hi2[0], hi2[1], hi2[2], hi2[3]};
       }
     }
   };
-
-  issue_tile(0, first_tile, 0);
-  float stat = stat_of(0, first_tile);
-  int h = 0, t = first_tile;  // of tile `it`
-  for (int it = 0; it < all; ++it) {
-    if (KEYS && tid < 2 * TY) rows_of[(it & 1) * 2 * TY + tid] = stat;
-    // what this wavefront requested has landed; behind the barrier that holds for everyone, and the last step's tiles are free
-    asm volatile("s_waitcnt vmcnt(0)\n\ts_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    int next_t = t + 1, next_h = h;
-    if (next_t == first_tile + tiles) next_t = first_tile, ++next_h;
-    if (it + 1 < all) {
-      issue_tile(next_h, next_t, (it + 1) & 1);
-      stat = stat_of(next_h, next_t);
-    }
-    if (active) {
-      const char* at = smem + (it & 1) * 2 * TILE;
-      const float* stats = rows_of + (it & 1) * 2 * TY;
-      const int x_last = xw0 + 16 * NB - 1;
+  auto sums = [&](auto chunk, const Columns& y, const Weights& by) {
 #pragma unroll
-      for (int half = 0; half < TY / 32; ++half) {
-        const int y0 = t * TY + half * 32;
-        const bool none = KEYS ? y0 + 31 < xw0 : y0 > x_last, full = KEYS ? y0 >= x_last : y0 + 31 <= xw0;
-        if (none) continue;
-        if (full) group(std::false_type{}, y0, at + half * 32 * ROWB, stats + half * 32);
-        else group(std::true_type{}, y0, at + half * 32 * ROWB, stats + half * 32);
+    for (int j = 0; j < CI; ++j)
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        const int i = decltype(chunk)::value * CI + j;
+        sa[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y.a[j], by.u[n], sa[n][i], 0, 0, 0);
+        if constexpr (KEYS) sb[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y.b[j], by.w[n], sb[n][i], 0, 0, 0);
       }
+  };
+  auto weights = [&](int unit, const Scores& from, Weights& to, const float* stat = nullptr) {
+    const int n = unit % NB, b = unit / NB;
+    f4 lse;
+    if constexpr (KEYS) lse = OVERLAPS ? from.lse[b] : *reinterpret_cast<const f4*>(stat + 8 * g + 4 * b);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float w = __builtin_amdgcn_exp2f(fmaf(from.s[n][b][r], to_exp2, -(KEYS ? lse[r] : x_lse[n])));
+      if constexpr (KEYS) to.w[n][4 * b + r] = (_Float16)w;
+      to.u[n][4 * b + r] = (_Float16)((KEYS ? w * factor[0] : w) * from.p[n][b][r]);
     }
-    t = next_t;
-    h = next_h;
+  };
+  auto some_scores = [&](auto block, Scores& to, unsigned at, const float* stat) {
+    for_each_of<NQ / 2>([&](auto q) {
+      constexpr std::integral_constant<int, decltype(block)::value * (NQ / 2) + decltype(q)::value> chunk{};
+      Rows rows;
+      read_rows(chunk, rows, to, at, stat);
+      if constexpr (decltype(q)::value > 0) rows.less = f4(0.f);
+      scores(chunk, rows, to);
+    });
+  };
+  auto all_sums = [&](const Weights& by, unsigned at) {
+    for_each_of<NS>([&](auto i) {
+      Columns columns;
+      read_columns(i, columns, at);
+      sums(i, columns, by);
+    });
+  };
+  auto hide = [&](Scores& now, int y0, int from, int to) {  // blocks from .. to - 1
+    const int x_last = xw0 + 16 * NB - 1;
+    if (KEYS ? y0 < x_last || y0 + 31 >= L : y0 + 31 > xw0) {  // the diagonal passes through, or the end, or nothing is seen
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int b = from; b < to; ++b)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int y = y0 + 8 * g + 4 * b + r, x = xw0 + 16 * n + c;
+            now.s[n][b][r] = (KEYS ? x <= y && y < L : y <= x) ? now.s[n][b][r] : -INFINITY;
+          }
+    }
+  };
+  auto step = [&](Scores& now, Weights& made, int y0, Scores& next, unsigned next_at, const float* next_stat,
+                  const Weights& last, unsigned last_at) {
+    Rows rows[2];
+    Columns columns[2];
+    read_rows(std::integral_constant<int, 0>{}, rows[0], next, next_at, next_stat);
+    hide(now, y0, 0, 2);
+    constexpr int NC = NQ + NS;
+    // unit u of the weights goes beside chunk u (NC + 1) / UNITS - 1, the first in front of all
+    const auto some_weights = [&](int chunk) {
+#pragma unroll
+      for (int u = 0; u < UNITS; ++u)
+        if (u * (NC + 1) / UNITS == chunk) weights(u, now, made);
+    };
+    some_weights(0);
+    for_each_of<NQ>([&](auto q) {
+      constexpr int i = decltype(q)::value;
+      if constexpr (i + 1 < NQ) read_rows(std::integral_constant<int, i + 1>{}, rows[(i + 1) & 1], next, next_at, next_stat);
+      else read_columns(std::integral_constant<int, 0>{}, columns[0], last_at);
+      scores(q, rows[i & 1], next);
+      some_weights(i + 1);
+    });
+    for_each_of<NS>([&](auto q) {
+      constexpr int i = decltype(q)::value;
+      if constexpr (i + 1 < NS) read_columns(std::integral_constant<int, i + 1>{}, columns[(i + 1) & 1], last_at);
+      sums(q, columns[i & 1], last);
+      some_weights(NQ + i + 1);
+    });
+  };
+
+  // Tile `it` is in place it % PLACES.  Without overlap the barrier in front of it says that it has landed, and that all are
+  // done with tile it - 1, whose place tile it + 1 takes.  With overlap the barrier of tile `it`, in front of its last step, says
+  // that tile it + 1 has landed, and that all are done with the tile whose place tile it + 2 takes (two groups a tile:
+  // it - 1, last read by the step of the first half; one: it - 2).
+  struct At {
+    int h, t, place;
+  };
+  auto following = [&](At at) {
+    At to = {at.h, at.t + 1, at.place + 1 == PLACES ? 0 : at.place + 1};
+    if (to.t == first_tile + tiles) to.t = first_tile, ++to.h;
+    return to;
+  };
+  auto tile_at = [&](const At& at) { return smem_base + (unsigned)(at.place * 2 * TILE); };
+  auto stat_at = [&](const At& at) { return rows_of + at.place * 2 * TY; };
+  auto arrive = [] { asm volatile("s_waitcnt vmcnt(0)\n\ts_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+  At now = {0, first_tile, 0}, next = following(now), last = now;
+  issue_tile(now.h, now.t, now.place);
+  if constexpr (OVERLAPS) arrive();
+  else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {  // they have landed too: no wait at their uses, which would be one for the tiles
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(xa[n][ks]), "+v"(xb[n][ks]));
+    if constexpr (!KEYS) asm volatile("" : "+v"(x_lse[n]), "+v"(x_less[n]));
+  }
+  if (OVERLAPS && all > 1) issue_tile(next.h, next.t, next.place);
+  Scores even, odd;
+  Weights front, back;  // of the group in front, by turns
+#pragma unroll
+  for (int n = 0; n < NB; ++n) front.w[n] = front.u[n] = back.w[n] = back.u[n] = h8(0);
+  if (OVERLAPS && active) {
+    some_scores(std::integral_constant<int, 0>{}, even, tile_at(now), stat_at(now));
+    some_scores(std::integral_constant<int, 1>{}, even, tile_at(now), stat_at(now));
+  }
+  auto barrier = [&](int it) {
+    if (it + 1 >= all) return;
+    arrive();
+    if (it + 2 < all) {
+      const At then = following(next);
+      issue_tile(then.h, then.t, then.place);
+    }
+  };
+  if constexpr (!OVERLAPS) {
+    for (int it = 0; it < all; ++it) {
+      arrive();
+      if (it + 1 < all) issue_tile(next.h, next.t, next.place);
+      // the groups that this wavefront's rows see something of; one body, for the sums stay in place then
+      const int seen = (KEYS ? xw0 : xw0 + 16 * NB - 1) - now.t * TY;
+      const int begin = KEYS && seen > 0 ? seen >> 5 : 0, end = KEYS ? GROUPS : seen < 0 ? 0 : min(GROUPS, (seen >> 5) + 1);
+#pragma unroll 1
+      for (int group = active ? begin : end; group < end; ++group) {
+        const unsigned at = tile_at(now) + group * 32 * ROWB;
+        const float* stat = stat_at(now) + group * 32;
+        for_each_of<2>([&](auto b) {  // 16 rows after the other: fewer registers at a time
+          some_scores(b, even, at, stat);
+          hide(even, now.t * TY + 32 * group, b, b + 1);
+#pragma unroll
+          for (int n = 0; n < NB; ++n) weights(b * NB + n, even, front, stat);
+        });
+        all_sums(front, at);
+      }
+      now = next;
+      next = following(next);
+    }
+  } else if constexpr (GROUPS == 2) {
+    for (int it = 0; it < all; ++it) {
+      const unsigned at = tile_at(now), half = at + 32 * ROWB;
+      if (active) step(even, front, now.t * TY, odd, half, stat_at(now) + 32, back, tile_at(last) + 32 * ROWB);
+      barrier(it);
+      if (active) step(odd, back, now.t * TY + 32, even, tile_at(next), stat_at(next), front, at);
+      last = now;
+      now = next;
+      next = following(next);
+    }
+    if (active) all_sums(back, tile_at(last) + 32 * ROWB);
+  } else {
+    for (int it = 0; it < all; it += 2) {
+      barrier(it);
+      if (active) step(even, front, now.t * TY, odd, tile_at(next), stat_at(next), back, tile_at(last));
+      last = now;
+      now = next;
+      next = following(next);
+      if (it + 1 == all) {
+        back = front;
+        break;
+      }
+      barrier(it + 1);
+      if (active) step(odd, back, now.t * TY, even, tile_at(next), stat_at(next), front, tile_at(last));
+      last = now;
+      now = next;
+      next = following(next);
+    }
+    if (active) all_sums(back, tile_at(last));
   }
   if (!active) return;
 
@@ -375,21 +559,24 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void packed_grad_kernel(GradA
         if constexpr (KEYS) none = fmaf(sb[n][i][r], 0.f, none);
       }
     const int64_t row = block.first + x;
-    _Float16* to_a = KEYS ? a.dk + (row * a.kv_heads + kv_head) * D : a.dq + (row * a.heads + head0) * D;
-    _Float16* to_b = KEYS ? a.dv + (row * a.kv_heads + kv_head) * D : nullptr;
+    const int64_t place_a = KEYS ? (row * a.kv_heads + kv_head) * D : (row * a.heads + head0) * D;
+    // four numbers of the results, or of this walk's part of them
+    const auto store = [&](int at, f4 ra, f4 rb) {
+      if (x >= L) return;
+      if (KEYS && a.shares > 1) {
+        float* to = a.parts + (int64_t)(place.head % a.shares) * 2 * a.rows * a.kv_heads * D + place_a + at;
+        *reinterpret_cast<f4*>(to) = ra;
+        *reinterpret_cast<f4*>(to + a.rows * a.kv_heads * D) = rb;
+        return;
+      }
+      *reinterpret_cast<h4*>((KEYS ? a.dk : a.dq) + place_a + at) = __builtin_convertvector(ra, h4);
+      if constexpr (KEYS) *reinterpret_cast<h4*>(a.dv + place_a + at) = __builtin_convertvector(rb, h4);
+    };
     if (!__any(none != 0.f && x < L)) {
 #pragma unroll
       for (int i = 0; i < DB; ++i) {
-        h4 ra, rb;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          ra[r] = (_Float16)(sa[n][i][r] * by_a);
-          if constexpr (KEYS) rb[r] = (_Float16)(sb[n][i][r] * by_b);
-        }
-        if (x < L) {
-          *reinterpret_cast<h4*>(to_a + 16 * i + 4 * g) = ra;
-          if constexpr (KEYS) *reinterpret_cast<h4*>(to_b + 16 * i + 4 * g) = rb;
-        }
+        if constexpr (KEYS) store(16 * i + 4 * g, sa[n][i] * by_a, sb[n][i] * by_b);
+        else store(16 * i + 4 * g, sa[n][i] * by_a, f4(0.f));
       }
       continue;
     }
@@ -409,7 +596,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void packed_grad_kernel(GradA
         const _Float16* yb = (KEYS ? ep + head * D + y * e_row : vp + y * a.v_row) + g * 8;
         const int query = KEYS ? y : min(x, L - 1);
         const float2 stat = a.stats[(int64_t)(head0 + head) * a.rows + block.first + query];
-        const float del = delta[head * a.rows + query];
+        const float less = minus_delta[head * a.rows + query];
         float s = 0.f, p = 0.f;  // the score as the forward pass forms it key by key
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
@@ -426,7 +613,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void packed_grad_kernel(GradA
         p = pp.a + pp.b;
         const float w = stat.y > 0.f ? __builtin_amdgcn_exp2f(fmaf(s, to_exp2, -stat.x)) * stat.y
                                      : __expf(s * a.scale - stat.x) * -stat.y;
-        const float u = w * (p - del);
+        const float u = w * (p + less);
         const bool seen = KEYS ? x <= y : y <= x;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
@@ -444,66 +631,125 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void packed_grad_kernel(GradA
         }
       }
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      h8 ra, rb;
+    for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        ra[i] = (_Float16)(va[ks][i] * a.scale);
-        if constexpr (KEYS) rb[i] = (_Float16)vb[ks][i];
+      for (int half = 0; half < 2; ++half) {
+        f4 ra, rb;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          ra[i] = va[ks][4 * half + i] * a.scale;
+          rb[i] = KEYS ? vb[KEYS ? ks : 0][4 * half + i] : 0.f;
+        }
+        if (D >= 32 || g < 2) store(ks * 32 + g * 8 + 4 * half, ra, rb);
       }
-      if (x < L && (D >= 32 || g < 2)) {
-        *reinterpret_cast<h8*>(to_a + ks * 32 + g * 8) = ra;
-        if constexpr (KEYS) *reinterpret_cast<h8*>(to_b + ks * 32 + g * 8) = rb;
-      }
-    }
+  }
+}
+
+// The parts of dk and dv, added in the order of the heads.
+template <int D>
+__global__ __launch_bounds__(256) void packed_join_kernel(GradArgs a) {
+  const int64_t all = a.rows * a.kv_heads * D, at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  const int64_t row = at / (a.kv_heads * D);
+  if (at >= all || row < a.starts[0] || row >= a.starts[a.sequences]) return;
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    f4 sum = *reinterpret_cast<const f4*>(a.parts + which * all + at);
+    for (int i = 1; i < a.shares; ++i) sum += *reinterpret_cast<const f4*>(a.parts + (2 * i + which) * all + at);
+    *reinterpret_cast<h4*>((which ? a.dv : a.dk) + at) = __builtin_convertvector(sum, h4);
   }
 }
 
 template <int D, int NB, bool KEYS>
-int launch_as(GradArgs a, hipStream_t st) {
-  constexpr int R = 64 * NB, TY = D <= 128 ? 64 : 32, lds = 4 * TY * D * 2 + 4 * TY * 4;
-  const int heads = KEYS ? a.kv_heads : a.heads;
-  const int64_t slots = a.rows / R + a.sequences, blocks = slots * heads;
-  if (blocks > (1ll << 31) - kGridRow) {
+__global__ __launch_bounds__(256, waves_of(D, KEYS)) void packed_grad_kernel(GradArgs a) {
+  walk<D, NB, KEYS>(a, (int)(blockIdx.y * kGridRow + blockIdx.x), a.deal[KEYS].slots, a.deal[KEYS].longest_first);
+}
+
+// Both walks in one launch: which workgroups start last decides when a launch ends, and one end is less than two.  Eight ids
+// of the one, then eight of the other, as far as both go: the ids' place modulo 8 says which XCD has them.
+template <int D, int NB>
+__global__ __launch_bounds__(256, waves_of(D, true)) void packed_grads_kernel(GradArgs a) {
+  const int id = (int)(blockIdx.y * kGridRow + blockIdx.x), keys = a.deal[1].grid, queries = a.deal[0].grid;
+  const int both = 2 * min(keys, queries);
+  const bool key = id < both ? (id >> 3 & 1) == 0 : keys > queries;
+  const int own = id < both ? (id >> 4) * 8 + (id & 7) : id - both / 2;
+  if (key) walk<D, NB, true>(a, own, a.deal[1].slots, a.deal[1].longest_first);
+  else walk<D, NB, false>(a, own, a.deal[0].slots, a.deal[0].longest_first);
+}
+
+// How many slots of 64 NB rows, in which order, and the workgroups, a multiple of 8.
+template <int NB>
+bool deal_slots(const GradArgs& a, int heads, SlotDeal* deal) {
+  const int64_t slots = a.rows / (64 * NB) + a.sequences, blocks = slots * heads;
+  if (blocks > (1ll << 30) - kGridRow) {
     set_error("flash_attn_packed_backward: %lld rows in %d sequences of %d heads exceed the grid", (long long)a.rows,
               a.sequences, heads);
-    return -2;
+    return false;
   }
-  static bool attr_done = false;  // idempotent; a race only repeats the call
-  if (!attr_done) {
-    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(packed_grad_kernel<D, NB, KEYS>),
-                                       hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  const bool longest_first = a.sequences <= kMany * kWave && slots <= 512 && blocks <= 5120 && a.rows >= 128ll * a.sequences;
+  const int64_t grid = longest_first ? (slots + 7) / 8 * 8 * heads : (blocks + 7) / 8 * 8;
+  *deal = {(int)slots, (int)grid, longest_first};
+  return true;
+}
+
+template <typename K>
+int launch(K kernel, const GradArgs& a, int64_t grid, int lds, bool* attr_done, hipStream_t st) {
+  if (!*attr_done) {  // idempotent; a race only repeats the call
+    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) {
       set_error("hipFuncSetAttribute(%d bytes LDS): %s", lds, hipGetErrorString(e));
       return -4;
     }
-    attr_done = true;
+    *attr_done = true;
   }
-  a.slots = (int)slots;
-  a.longest_first = a.sequences <= kMany * kWave && slots <= 512 && blocks <= 5120 && a.rows >= 128ll * a.sequences;
-  const int64_t grid = a.longest_first ? (slots + 7) / 8 * 8 * heads : blocks;
   const dim3 dims((unsigned)(grid < kGridRow ? grid : kGridRow), (unsigned)((grid + kGridRow - 1) / kGridRow));
-  hipLaunchKernelGGL((packed_grad_kernel<D, NB, KEYS>), dims, dim3(256), lds, st, a);
+  hipLaunchKernelGGL(kernel, dims, dim3(256), lds, st, a);
   return 0;
+}
+
+// Where the blocks of keys would not fill the GPU, the heads that share a key head are divided, into no more parts than needed.
+template <int NB>
+int shares_of(int64_t rows, int64_t sequences, int heads, int kv_heads) {
+  const int64_t blocks = (rows / (64 * NB) + sequences) * kv_heads;
+  const int rep = heads / kv_heads;
+  int shares = 1;
+  while (shares < rep && (rep % shares != 0 || blocks * shares < 512)) ++shares;
+  return shares;
+}
+template <int D>
+constexpr int blocks_of() {  // of 16 rows a wavefront
+  return D <= 128 ? 2 : 1;
 }
 
 template <int D>
 int launch_d(GradArgs a, hipStream_t st) {
+  constexpr int NB = blocks_of<D>();
   constexpr int BLOCK = 256 / (D / 8) > 64 ? 256 / (D / 8) : 64;
   const int64_t items = (a.rows + BLOCK - 1) / BLOCK * a.heads;
   a.mosts = (int)(items < kSums ? items : kSums);
+  if (!deal_slots<NB>(a, a.heads, &a.deal[0]) || !deal_slots<NB>(a, a.kv_heads * a.shares, &a.deal[1])) return -2;
   hipLaunchKernelGGL((packed_sums_kernel<D>), dim3(a.mosts), dim3(256), 0, st, a);
-  constexpr int NB = D <= 128 ? 2 : 1;
+  static bool done[3];
   int rc = 0;
-  if (a.dk) rc = launch_as<D, NB, true>(a, st);
-  if (a.dq && !rc) rc = launch_as<D, NB, false>(a, st);
+  if (D <= 64 && a.dk && a.dq) {
+    if constexpr (D <= 64)
+      rc = launch(packed_grads_kernel<D, NB>, a, (int64_t)a.deal[0].grid + a.deal[1].grid, lds_of(D, true), &done[2], st);
+  } else {
+    if (a.dk) rc = launch(packed_grad_kernel<D, NB, true>, a, a.deal[1].grid, lds_of(D, true), &done[1], st);
+    if (a.dq && !rc) rc = launch(packed_grad_kernel<D, NB, false>, a, a.deal[0].grid, lds_of(D, false), &done[0], st);
+  }
+  if (a.dk && a.shares > 1 && !rc)
+    hipLaunchKernelGGL((packed_join_kernel<D>), dim3((unsigned)((a.rows * a.kv_heads * D + 1023) / 1024)), dim3(256), 0, st, a);
   return rc;
 }
 
 }  // namespace
 
-size_t packed_attn_grad_bytes(int64_t rows, int64_t heads) {
-  return (size_t)(kSums * sizeof(float2)) + (size_t)rows * (size_t)heads * 2 * sizeof(float);
+// The largest rows' (kSums), lse and -delta, and the parts of dk and dv.
+size_t packed_attn_grad_bytes(int64_t rows, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t d) {
+  const int shares = d <= 128 ? shares_of<blocks_of<128>()>(rows, sequences, (int)heads, (int)kv_heads)
+                              : shares_of<blocks_of<256>()>(rows, sequences, (int)heads, (int)kv_heads);
+  const size_t stats = kSums * sizeof(float2) + (size_t)rows * (size_t)heads * 2 * sizeof(float);
+  return (stats + 255) / 256 * 256 + (shares > 1 ? (size_t)shares * 2 * (size_t)(rows * kv_heads * d) * sizeof(float) : 0);
 }
 
 int launch_flash_attn_packed_backward(const PackedAttention& p, const PackedGradients& d, int head_size, void* workspace,
@@ -520,7 +766,11 @@ int launch_flash_attn_packed_backward(const PackedAttention& p, const PackedGrad
   a.stats = (const float2*)p.stats;
   a.most = (float2*)workspace;
   a.lse = (float*)(a.most + kSums);
-  a.delta = a.lse + p.rows * p.heads;
+  a.minus_delta = a.lse + p.rows * p.heads;
+  const size_t stats = kSums * sizeof(float2) + (size_t)p.rows * (size_t)p.heads * 2 * sizeof(float);
+  a.parts = (float*)((char*)workspace + (stats + 255) / 256 * 256);
+  a.shares = head_size <= 128 ? shares_of<blocks_of<128>()>(p.rows, p.sequences, (int)p.heads, (int)p.kv_heads)
+                              : shares_of<blocks_of<256>()>(p.rows, p.sequences, (int)p.heads, (int)p.kv_heads);
   a.starts = p.starts;
   a.rows = p.rows;
   a.sequences = (int)p.sequences;

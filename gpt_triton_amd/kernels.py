@@ -846,7 +846,7 @@ class _PackedAttentionFunction(torch.autograd.Function):
                 d_out = d_out.clone()
             pitches, addresses = _packed_pitches(q, k, v)
             lib = _lib.load()
-            nbytes = lib.gptmi_flash_attn_packed_backward_workspace_bytes(T, N)
+            nbytes = lib.gptmi_flash_attn_packed_backward_workspace_bytes(starts.shape[0] - 1, T, N, G, d)
             workspace = _workspace(nbytes, q)
             _call(q.get_device(), "flash_attention_packed", lib.gptmi_flash_attn_packed_backward, *addresses,
                   out.data_ptr(), stats.data_ptr(), d_out.data_ptr(), starts.data_ptr(), _ptr(dq), _ptr(dk), _ptr(dv),

@@ -55,10 +55,11 @@ def test_refusals(lib):
         assert train(lib, **args) == -2, args
     for args in (*BEYOND[:4], dict(N=1 << 21, G=1)):
         assert backward(lib, **args) == -2, args
-    needed = lib.gptmi_flash_attn_packed_backward_workspace_bytes(8, 4)
+    needed = lib.gptmi_flash_attn_packed_backward_workspace_bytes(2, 8, 4, 2, 64)
     for args in (dict(ws=None), dict(ws_bytes=needed - 1), dict(ws=ctypes.c_void_p(264))):
         assert backward(lib, **args) == -3, args
-    for args in ((0, 4), (8, 0), (1 << 31, 4), (8, 1 << 21)):
+    for args in ((0, 8, 4, 2, 64), (2, 0, 4, 2, 64), (2, 8, 0, 2, 64), (2, 8, 4, 0, 64), (2, 8, 5, 2, 64), (2, 8, 4, 2, 0),
+                 (2, 1 << 31, 4, 2, 64), (2, 8, 1 << 21, 1, 64), (1 << 31, 8, 4, 2, 64)):
         assert lib.gptmi_flash_attn_packed_backward_workspace_bytes(*args) == 0
 
 
