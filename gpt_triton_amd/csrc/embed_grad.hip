@@ -58,23 +58,38 @@ struct EmbedGradArgs {
   DropoutArgs drop;
   // the sort's
   int tiles, bits;          // workgroups, bits of a digit
+  int64_t fill, fills;      // other work of a launch: from which 64 KB on, and how many of them; positions behind
   unsigned *keys[2], *at[2];  // tokens (V: none) and positions
   unsigned* hist;           // [tiles][1 << bits]
   // the sums'
   const unsigned *sorted, *order;
   float* parts;             // [runs][2][H]: what a run has of a token that began in front of it, and of one that goes on behind
   int run;                  // tokens of a run
-  int sort_blocks, fill_blocks;
 };
 
-// A mask of dropout is one for all rows: it comes behind the sums.
-template <typename T, int VN>
-__device__ __forceinline__ void put_sum(const EmbedGradArgs& a, T* row, int chunk, float (&sum)[VN]) {
+// A mask of dropout is one for all rows, so it comes behind the sums: which of a chunk's columns are kept, and the sums over
+// 1 - p, by a reciprocal with the remainder's correction (subnormal remainders aside, correctly rounded).
+template <int VN>
+__device__ __forceinline__ unsigned kept_columns(const EmbedGradArgs& a, int chunk) {
+  unsigned kept = ~0u;
   if (a.drop.p > 0.f) {
     unsigned column[VN];
+    float u[VN];
 #pragma unroll
     for (int i = 0; i < VN; ++i) column[i] = (unsigned)(chunk * VN + i);
-    dropout_apply<VN>(a.drop, column, sum);
+    philox_uniform<VN>(a.drop, column, u);
+    kept = 0;
+#pragma unroll
+    for (int i = 0; i < VN; ++i) kept |= u[i] > a.drop.p ? 1u << i : 0u;
+  }
+  return kept;
+}
+template <typename T, int VN>
+__device__ __forceinline__ void put_sum(const EmbedGradArgs& a, T* row, int chunk, unsigned kept, float (&sum)[VN]) {
+  if (a.drop.p > 0.f) {
+    const KeepScale scale(a.drop.p);
+#pragma unroll
+    for (int i = 0; i < VN; ++i) sum[i] = kept >> i & 1 ? scale.of_half(sum[i]) : 0.f;
   }
   put_chunk<T, VN>(row + chunk * VN, sum);
 }
@@ -130,7 +145,7 @@ __device__ __forceinline__ void position_row(const EmbedGradArgs& a, int64_t l, 
 #pragma unroll
           for (int i = 0; i < VN; ++i) sum[i] += lds[(n * VN + i) * lanes + lane];
     }
-    if (group == 0 && chunk < chunks) put_sum<T, VN>(a, row, chunk, sum);
+    if (group == 0 && chunk < chunks) put_sum<T, VN>(a, row, chunk, kept_columns<VN>(a, chunk), sum);
   }
 }
 
@@ -194,7 +209,7 @@ __global__ __launch_bounds__(256) void embed_grad_few_kernel(EmbedGradArgs a, in
       clear(sum);
       if (first < last) {
         add_rows<T, VN>(dz, a.H, chunk, first, last, [&](int64_t i) { return (int64_t)(sorted[i] & 255); }, sum);
-        put_sum<T, VN>(a, row, chunk, sum);
+        put_sum<T, VN>(a, row, chunk, kept_columns<VN>(a, chunk), sum);
       } else {
         put_chunk<T, VN>(row + chunk * VN, sum);
       }
@@ -205,6 +220,13 @@ __global__ __launch_bounds__(256) void embed_grad_few_kernel(EmbedGradArgs a, in
 // ---------------------------------------------------------------------------
 // More: the sort.
 // ---------------------------------------------------------------------------
+constexpr int kWaves = kSortThreads / kWave, kEach = kTile / kSortThreads;
+struct SortLds {
+  unsigned counts[kWaves][1 << kMaxBits];
+  unsigned base[1 << kMaxBits];
+  unsigned sums[kWaves];
+};
+
 // Lanes of the wavefront with the same digit.
 __device__ __forceinline__ uint64_t same_digit(unsigned digit, int bits, bool valid) {
   uint64_t same = __ballot(valid);
@@ -220,123 +242,199 @@ __device__ __forceinline__ unsigned key_of(const EmbedGradArgs& a, int64_t i) {
   return (unsigned)((uint64_t)id < (uint64_t)a.V ? id : a.V);
 }
 
-// What fills the GPU beside the sort: zero rows of the token table's gradient (in blocks of 64 KB), rows of the position table's.
-template <typename T, int VN, int NT>
-__device__ __forceinline__ void fill_block(const EmbedGradArgs& a, int64_t block) {
+// What fills the GPU beside the sort: zero rows of the token table's gradient in blocks of 64 KB, and rows of the position
+// table's.  Every launch of the sort has a part of each, in workgroups behind its own.
+template <typename T, int VN>
+__device__ __forceinline__ void other_work(const EmbedGradArgs& a, int64_t item, float* lds) {
+  if (item >= a.fills) {
+    position_row<T, VN, kSortThreads>(a, item - a.fills, lanes_of(a.H / VN, kSortThreads), lds);
+    return;
+  }
+  item += a.fill;
   const int64_t elements = a.V * (int64_t)a.H;
   constexpr int64_t PER = 65536 / sizeof(T);
-  const int64_t first = block * PER, last = min(first + PER, elements);
+  const int64_t first = item * PER, last = min(first + PER, elements);
   float none[VN];
   clear(none);
-  for (int64_t i = first + threadIdx.x * VN; i < last; i += NT * VN) put_chunk<T, VN>((T*)a.d_wte + i, none);
+  for (int64_t i = first + threadIdx.x * VN; i < last; i += kSortThreads * VN) put_chunk<T, VN>((T*)a.d_wte + i, none);
 }
 
-// How many tokens of each tile have each digit.  FIRST: from the ids themselves; blocks behind the sort's fill.
-template <typename T, int VN, bool FIRST>
-__global__ __launch_bounds__(kSortThreads) void embed_grad_count_kernel(EmbedGradArgs a, int shift, int from) {
-  if (FIRST && (int)blockIdx.x >= a.sort_blocks) {
-    fill_block<T, VN, kSortThreads>(a, (int64_t)blockIdx.x - a.sort_blocks);
-    return;
-  }
-  __shared__ unsigned counts[1 << kMaxBits];
-  const int tid = threadIdx.x, digits = 1 << a.bits;
-  if (tid < digits) counts[tid] = 0;
+// Where this thread's tokens go by one digit: wavefront w has tokens 64 kEach w .. of the tile, 64 at a time.  place_of: the
+// first place of each digit for this tile, by the threads of the digits.
+template <typename F>
+__device__ __forceinline__ void rank_tile(SortLds& lds, int count, int bits, int shift, const unsigned (&key)[kEach],
+                                          unsigned (&place)[kEach], F place_of) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, digits = 1 << bits, base = wave * (kWave * kEach);
+  for (int i = tid; i < kWaves << bits; i += kSortThreads) lds.counts[i >> bits][i & (digits - 1)] = 0;
   __syncthreads();
-  const int64_t base = (int64_t)blockIdx.x * kTile;
-  for (int i = tid; i < kTile && base + i < a.tokens; i += kSortThreads) {
-    const unsigned key = FIRST ? key_of(a, base + i) : a.keys[from][base + i];
-    atomicAdd(&counts[key >> shift & (digits - 1)], 1u);
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    const bool valid = base + j * kWave + lane < count;
+    const unsigned digit = key[j] >> shift & (digits - 1);
+    const uint64_t same = same_digit(digit, bits, valid);
+    const int in_front = __popcll(same & ((1ull << lane) - 1));
+    volatile unsigned* counted = &lds.counts[wave][digit];
+    place[j] = *counted + in_front;
+    __builtin_amdgcn_wave_barrier();
+    if (valid && in_front == 0) *counted = place[j] + __popcll(same);
+    __builtin_amdgcn_wave_barrier();
   }
   __syncthreads();
-  if (tid < digits) a.hist[(int64_t)blockIdx.x * digits + tid] = counts[tid];
-}
-
-// Moves the tokens to their places by one digit.  FIRST: from the ids, with rows of the position table in blocks behind.
-template <typename T, int VN, bool FIRST>
-__global__ __launch_bounds__(kSortThreads) void embed_grad_move_kernel(EmbedGradArgs a, int shift, int from) {
-  constexpr int WAVES = kSortThreads / kWave, EACH = kTile / kSortThreads;
-  __shared__ union {
-    struct {
-      unsigned counts[WAVES][1 << kMaxBits];
-      unsigned base[1 << kMaxBits];
-      unsigned sums[WAVES];
-    } s;
-    float lds[kSortThreads * VN];
-  } sh;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, digits = 1 << a.bits;
-  if (FIRST && (int)blockIdx.x >= a.sort_blocks) {
-    position_row<T, VN, kSortThreads>(a, (int64_t)blockIdx.x - a.sort_blocks, lanes_of(a.H / VN, kSortThreads), sh.lds);
-    return;
-  }
-  for (int i = tid; i < WAVES << a.bits; i += kSortThreads) sh.s.counts[i >> a.bits][i & (digits - 1)] = 0;
-  // where this tile's tokens of each digit begin: behind all of smaller digits and the tiles in front
-  unsigned before = 0, total = 0;
+  // behind all of smaller digits: the sum of what place_of counts of them
+  unsigned mine = 0, before = 0;
   if (tid < digits)
-    for (int t = 0; t < a.tiles; ++t) {
-      const unsigned n = a.hist[(int64_t)t * digits + tid];
-      before += t < (int)blockIdx.x ? n : 0;
-      total += n;
-    }
+    for (int w = 0; w < kWaves; ++w) mine += lds.counts[w][tid];
+  const unsigned total = place_of(mine, &before);
   unsigned scan = total;
 #pragma unroll
   for (int step = 1; step < 64; step *= 2) {
     const unsigned other = __shfl_up(scan, step);
     scan += lane >= step ? other : 0;
   }
-  if (lane == 63) sh.s.sums[wave] = scan;
+  if (lane == 63) lds.sums[wave] = scan;
   __syncthreads();
-  for (int w = 0; w < wave; ++w) scan += sh.s.sums[w];
-  if (tid < digits) sh.s.base[tid] = scan - total + before;
-  // each wavefront has 64 EACH tokens in a row, 64 at a time
-  const int64_t base = (int64_t)blockIdx.x * kTile + wave * (kWave * EACH);
-  unsigned key[EACH], at[EACH], rank[EACH];
-#pragma unroll
-  for (int j = 0; j < EACH; ++j) {
-    const int64_t i = base + j * kWave + lane;
-    key[j] = at[j] = 0;
-    if (i < a.tokens) {
-      key[j] = FIRST ? key_of(a, i) : a.keys[from][i];
-      at[j] = FIRST ? (unsigned)i : a.at[from][i];
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < EACH; ++j) {
-    const bool valid = base + j * kWave + lane < a.tokens;
-    const unsigned digit = key[j] >> shift & (digits - 1);
-    const uint64_t same = same_digit(digit, a.bits, valid);
-    const int in_front = __popcll(same & ((1ull << lane) - 1));
-    volatile unsigned* count = &sh.s.counts[wave][digit];
-    rank[j] = *count + in_front;
-    __builtin_amdgcn_wave_barrier();
-    if (valid && in_front == 0) *count = rank[j] + __popcll(same);
-    __builtin_amdgcn_wave_barrier();
-  }
-  __syncthreads();
+  for (int w = 0; w < wave; ++w) scan += lds.sums[w];
   if (tid < digits) {
-    unsigned sum = sh.s.base[tid];
-    for (int w = 0; w < WAVES; ++w) {
-      const unsigned n = sh.s.counts[w][tid];
-      sh.s.counts[w][tid] = sum;
+    unsigned sum = scan - total + before;
+    for (int w = 0; w < kWaves; ++w) {
+      const unsigned n = lds.counts[w][tid];
+      lds.counts[w][tid] = sum;
       sum += n;
     }
   }
   __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) place[j] += lds.counts[wave][key[j] >> shift & (digits - 1)];
+}
+
+// A single tile: all digits in one workgroup.
+template <typename T, int VN>
+__global__ __launch_bounds__(kSortThreads) void embed_grad_sort_kernel(EmbedGradArgs a, int passes) {
+  __shared__ union {
+    SortLds s;
+    float other[kSortThreads * VN];
+  } lds;
+  __shared__ unsigned keys[kTile], at[kTile];
+  if (blockIdx.x > 0) {
+    other_work<T, VN>(a, blockIdx.x - 1, lds.other);
+    return;
+  }
+  const int count = (int)a.tokens, base = (threadIdx.x >> 6) * (kWave * kEach) + (threadIdx.x & 63);
+  unsigned key[kEach], from[kEach], place[kEach];
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    const int i = base + j * kWave;
+    key[j] = i < count ? key_of(a, i) : 0;
+    from[j] = (unsigned)i;
+  }
+  for (int pass = 0; pass < passes; ++pass) {
+    rank_tile(lds.s, count, a.bits, pass * a.bits, key, place, [](unsigned mine, unsigned*) { return mine; });
+#pragma unroll
+    for (int j = 0; j < kEach; ++j)
+      if (base + j * kWave < count) {
+        keys[place[j]] = key[j];
+        at[place[j]] = from[j];
+      }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const int i = base + j * kWave;
+      key[j] = i < count ? keys[i] : 0;
+      from[j] = i < count ? at[i] : 0;
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    const int i = base + j * kWave;
+    if (i < count) {
+      a.keys[0][i] = key[j];
+      a.at[0][i] = from[j];
+    }
+  }
+}
+
+// More tiles, a launch to count and one to move for each digit.  How many tokens of each tile have each digit; FIRST: from the
+// ids themselves.
+template <typename T, int VN, bool FIRST>
+__global__ __launch_bounds__(kSortThreads) void embed_grad_count_kernel(EmbedGradArgs a, int shift, int from) {
+  __shared__ union {
+    unsigned counts[1 << kMaxBits];
+    float other[kSortThreads * VN];
+  } lds;
+  if ((int)blockIdx.x >= a.tiles) {
+    other_work<T, VN>(a, (int64_t)blockIdx.x - a.tiles, lds.other);
+    return;
+  }
+  const int tid = threadIdx.x, digits = 1 << a.bits;
+  const int64_t base = (int64_t)blockIdx.x * kTile;
+  unsigned key[kEach];
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    const int64_t i = base + j * kSortThreads + tid;
+    key[j] = 0;
+    if (i < a.tokens) key[j] = FIRST ? key_of(a, i) : a.keys[from][i];
+  }
+  if (tid < digits) lds.counts[tid] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kEach; ++j)
+    if (base + j * kSortThreads + tid < a.tokens) atomicAdd(&lds.counts[key[j] >> shift & (digits - 1)], 1u);
+  __syncthreads();
+  if (tid < digits) a.hist[(int64_t)blockIdx.x * digits + tid] = lds.counts[tid];
+}
+
+// Moves the tokens to their places by one digit.
+template <typename T, int VN, bool FIRST>
+__global__ __launch_bounds__(kSortThreads) void embed_grad_move_kernel(EmbedGradArgs a, int shift, int from) {
+  __shared__ union {
+    SortLds s;
+    float other[kSortThreads * VN];
+  } lds;
+  if ((int)blockIdx.x >= a.tiles) {
+    other_work<T, VN>(a, (int64_t)blockIdx.x - a.tiles, lds.other);
+    return;
+  }
+  const int tid = threadIdx.x, digits = 1 << a.bits;
+  const int64_t first = (int64_t)blockIdx.x * kTile;
+  const int count = (int)min((int64_t)kTile, a.tokens - first), base = (tid >> 6) * (kWave * kEach) + (tid & 63);
+  unsigned key[kEach], at[kEach], place[kEach];
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    const int i = base + j * kWave;
+    key[j] = at[j] = 0;
+    if (i < count) {
+      key[j] = FIRST ? key_of(a, first + i) : a.keys[from][first + i];
+      at[j] = FIRST ? (unsigned)(first + i) : a.at[from][first + i];
+    }
+  }
+  // of each digit, the tokens of all tiles, and of those in front of this one
+  unsigned total = 0, in_front = 0;
+  if (tid < digits) {
+#pragma unroll 16
+    for (int t = 0; t < a.tiles; ++t) {
+      const unsigned n = a.hist[(int64_t)t * digits + tid];
+      in_front += t < (int)blockIdx.x ? n : 0;
+      total += n;
+    }
+  }
+  rank_tile(lds.s, count, a.bits, shift, key, place, [&](unsigned, unsigned* before) {
+    *before = in_front;
+    return total;
+  });
   unsigned* keys = a.keys[1 - from];
   unsigned* to = a.at[1 - from];
 #pragma unroll
-  for (int j = 0; j < EACH; ++j)
-    if (base + j * kWave + lane < a.tokens) {
-      const unsigned place = sh.s.counts[wave][key[j] >> shift & (digits - 1)] + rank[j];
-      keys[place] = key[j];
-      to[place] = at[j];
+  for (int j = 0; j < kEach; ++j)
+    if (base + j * kWave < count) {
+      keys[place[j]] = key[j];
+      to[place[j]] = at[j];
     }
 }
 
 // ---------------------------------------------------------------------------
 // The sums of runs of a.run sorted tokens, a group of threads a run.
 // ---------------------------------------------------------------------------
-constexpr int kMaxRun = 128;
-
 template <typename T, int VN>
 __global__ __launch_bounds__(256) void embed_grad_sum_kernel(EmbedGradArgs a) {
   typedef T V __attribute__((ext_vector_type(VN)));
@@ -344,45 +442,54 @@ __global__ __launch_bounds__(256) void embed_grad_sum_kernel(EmbedGradArgs a) {
   const int group = threadIdx.x / lanes, lane = threadIdx.x - group * lanes;
   const int64_t runs = (a.tokens + a.run - 1) / a.run, r = (int64_t)blockIdx.x * groups + group;
   if (group >= groups || r >= runs) return;
-  const int64_t first = r * a.run, last = min(first + a.run, a.tokens);
+  const int64_t first = r * a.run;
+  const int count = (int)min((int64_t)a.run, a.tokens - first);
   const T* dz = (const T*)a.dz;
+  const unsigned *tokens = a.sorted + first, *rows = a.order + first;
   const unsigned none = (unsigned)a.V;
-  const unsigned before = first > 0 ? a.sorted[first - 1] : ~0u, behind = last < a.tokens ? a.sorted[last] : ~0u;
+  const unsigned before = first > 0 ? tokens[-1] : ~0u, behind = first + count < a.tokens ? tokens[count] : ~0u;
   constexpr int U = 8;
   for (int chunk = blockIdx.y * 256 + lane; chunk < min(chunks, (int)(blockIdx.y + 1) * 256); chunk += lanes) {
     float sum[VN];
     clear(sum);
-    bool began = a.sorted[first] != before;  // the token at hand began in this run
-    for (int64_t i0 = first; i0 < last; i0 += U) {
-      unsigned token[U + 1];
+    const unsigned kept = kept_columns<VN>(a, chunk);
+    bool began = tokens[0] != before;  // the token at hand began in this run
+    unsigned row[U], token[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      row[j] = rows[min(j, count - 1)];
+      token[j] = tokens[min(j, count - 1)];
+    }
+    for (int i0 = 0; i0 < count; i0 += U) {
       V x[U];
+      unsigned now[U];
 #pragma unroll
-      for (int j = 0; j < U; ++j) {
-        const int64_t i = min(i0 + j, last - 1);
-        token[j] = a.sorted[i];
-        if (token[j] != none) {
-          const T* from = dz + (int64_t)a.order[i] * a.H + chunk * VN;
-          if constexpr (VN == 1) x[j][0] = *from;
-          else x[j] = *reinterpret_cast<const V*>(from);
-        }
+      for (int j = 0; j < U; ++j) {  // rows behind the last token are rows all the same
+        const T* from = dz + (int64_t)row[j] * a.H + chunk * VN;
+        if constexpr (VN == 1) x[j][0] = *from;
+        else x[j] = *reinterpret_cast<const V*>(from);
+        now[j] = token[j];
       }
-      token[U] = i0 + U < last ? a.sorted[i0 + U] : behind;
 #pragma unroll
       for (int j = 0; j < U; ++j) {
-        if (i0 + j >= last || token[j] == none) break;
+        row[j] = rows[min(i0 + U + j, count - 1)];
+        token[j] = tokens[min(i0 + U + j, count - 1)];
+      }
 #pragma unroll
-        for (int n = 0; n < VN; ++n) sum[n] += (float)x[j][n];
-        const bool end = i0 + j == last - 1;
-        if ((end ? behind : token[j + 1]) != token[j]) {
-          if (began) {
-            put_sum<T, VN>(a, (T*)a.d_wte + (int64_t)token[j] * a.H, chunk, sum);
-          } else {
-            put_chunk<float, VN>(a.parts + (r * 2) * a.H + chunk * VN, sum);
+      for (int j = 0; j < U; ++j) {
+        const bool there = i0 + j < count && now[j] != none, end = i0 + j == count - 1;
+        const unsigned next = end ? behind : j + 1 < U ? now[j + 1 < U ? j + 1 : 0] : token[0];
+        if (there) {
+#pragma unroll
+          for (int n = 0; n < VN; ++n) sum[n] += (float)x[j][n];
+          if (next != now[j]) {
+            if (began) put_sum<T, VN>(a, (T*)a.d_wte + (int64_t)now[j] * a.H, chunk, kept, sum);
+            else put_chunk<float, VN>(a.parts + (r * 2) * a.H + chunk * VN, sum);
+            clear(sum);
+            began = true;
+          } else if (end) {
+            put_chunk<float, VN>(a.parts + (r * 2 + (began ? 1 : 0)) * a.H + chunk * VN, sum);
           }
-          clear(sum);
-          began = true;
-        } else if (end) {
-          put_chunk<float, VN>(a.parts + (r * 2 + (began ? 1 : 0)) * a.H + chunk * VN, sum);
         }
       }
     }
@@ -429,7 +536,7 @@ __global__ __launch_bounds__(256) void embed_grad_join_kernel(EmbedGradArgs a) {
 #pragma unroll
           for (int i = 0; i < VN; ++i) sum[i] += lds[(n * VN + i) * lanes + lane];
     }
-    if (group == 0 && chunk < chunks) put_sum<T, VN>(a, (T*)a.d_wte + (int64_t)token * a.H, chunk, sum);
+    if (group == 0 && chunk < chunks) put_sum<T, VN>(a, (T*)a.d_wte + (int64_t)token * a.H, chunk, kept_columns<VN>(a, chunk), sum);
   }
 }
 
@@ -462,22 +569,39 @@ void launch_as(EmbedGradArgs a, hipStream_t st) {
   while (a.V >> width) ++width;  // bits of V, the key of no token
   const int passes = (width + kMaxBits - 1) / kMaxBits;
   a.bits = (width + passes - 1) / passes;
-  a.tiles = a.sort_blocks = (int)((a.tokens + kTile - 1) / kTile);
-  const int64_t fill = (a.V * a.H * (int64_t)sizeof(T) + 65535) / 65536;
-  for (int pass = 0; pass < passes; ++pass) {
-    const int shift = pass * a.bits, from = pass & 1;
-    if (pass == 0) {
-      hipLaunchKernelGGL((embed_grad_count_kernel<T, VN, true>), dim3((unsigned)(a.tiles + fill)), dim3(kSortThreads), 0, st, a,
-                         shift, from);
-      hipLaunchKernelGGL((embed_grad_move_kernel<T, VN, true>), dim3((unsigned)(a.tiles + positions)), dim3(kSortThreads), 0,
-                         st, a, shift, from);
-    } else {
-      hipLaunchKernelGGL((embed_grad_count_kernel<T, VN, false>), dim3(a.tiles), dim3(kSortThreads), 0, st, a, shift, from);
-      hipLaunchKernelGGL((embed_grad_move_kernel<T, VN, false>), dim3(a.tiles), dim3(kSortThreads), 0, st, a, shift, from);
+  a.tiles = (int)((a.tokens + kTile - 1) / kTile);
+  const int64_t fills = (a.V * a.H * (int64_t)sizeof(T) + 65535) / 65536;
+  if (a.tiles == 1) {
+    a.fills = fills;
+    hipLaunchKernelGGL((embed_grad_sort_kernel<T, VN>), dim3((unsigned)(1 + fills + positions)), dim3(kSortThreads), 0, st, a, passes);
+    a.sorted = a.keys[0];
+    a.order = a.at[0];
+  } else {
+    // The last launch has the position table's rows, few and long ones; a launch that counts takes about half as long as one
+    // that moves, so the others divide the zero rows in thirds a pass.  us, 512 x 300 tokens fp16, the sort's launches with all
+    // zero rows in the first and the positions in the second / all divided / this: 91 / 102 / 84.
+    const auto part = [&](int third, int pass) {
+      const int64_t in = 3 * pass + third, of = 3 * passes - 2;
+      a.fill += a.fills;
+      a.fills = fills * (in < of ? in : of) / of - a.fill;
+      return dim3((unsigned)(a.tiles + a.fills + (in > of ? positions : 0)));
+    };
+    for (int pass = 0; pass < passes; ++pass) {
+      const int shift = pass * a.bits, from = pass & 1;
+      const dim3 count = part(1, pass);
+      if (pass == 0)
+        hipLaunchKernelGGL((embed_grad_count_kernel<T, VN, true>), count, dim3(kSortThreads), 0, st, a, shift, from);
+      else
+        hipLaunchKernelGGL((embed_grad_count_kernel<T, VN, false>), count, dim3(kSortThreads), 0, st, a, shift, from);
+      const dim3 move = part(3, pass);
+      if (pass == 0)
+        hipLaunchKernelGGL((embed_grad_move_kernel<T, VN, true>), move, dim3(kSortThreads), 0, st, a, shift, from);
+      else
+        hipLaunchKernelGGL((embed_grad_move_kernel<T, VN, false>), move, dim3(kSortThreads), 0, st, a, shift, from);
     }
+    a.sorted = a.keys[passes & 1];
+    a.order = a.at[passes & 1];
   }
-  a.sorted = a.keys[passes & 1];
-  a.order = a.at[passes & 1];
   const int chunks = a.H / VN;
   int lanes = 1;  // lanes_of(chunks, 256)
   if (chunks >= 256) lanes = 256;
