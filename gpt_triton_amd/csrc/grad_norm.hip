@@ -2,8 +2,8 @@
 // tensors, out = scale min(1, limit / norm) g.
 //
 // Squares are summed in 64 bits, which vector units do at the rate of 32: no square is too large or too small, and the norm does
-// not depend on how the tensors are divided but for its last bits.  Two launches for each kTensors tensors: chunks' sums, in an order
-// of their own each; then every workgroup adds all chunks' sums (some 2000 numbers from the L2) in one order and scales its chunk,
+// not depend on how the tensors are divided but for its last bits.  Two launches for each kTensors tensors: workgroups' sums over their
+// chunks, each in one order; then every workgroup adds all workgroups' sums (1024 numbers a launch, from the L2) in one order and scales its chunks,
 // the last first, which the memory-side cache still has.  Bound by memory.
 #include "common.h"
 #include "launch.h"
@@ -11,39 +11,64 @@
 namespace gptmi {
 namespace {
 
-constexpr int kTensors = 112;   // of one launch: what kernel arguments, 4 KB, have room for
-constexpr int kChunks = 2048;   // of all tensors, and one more each
+constexpr int kTensors = 152;    // of one launch: what kernel arguments, 4 KB, have room for (a model of 12 layers has 148)
+constexpr int kBlocks = 1024;    // workgroups of one launch at most
 constexpr int kThreads = 256;
+constexpr int kGroups = 8;       // of 8 elements a thread at a time
+constexpr int64_t kChunk = kThreads * 8 * kGroups;  // elements
 
 struct ClipArgs {
   const void* in[kTensors];
   void* out[kTensors];
-  int64_t size[kTensors];
-  unsigned first[kTensors];    // this launch's first chunk of each
-  unsigned char f16[kTensors];  // 1: in, 2: out
+  unsigned first[kTensors];     // this launch's first chunk of each
+  unsigned size_low[kTensors];
+  uint16_t size_high[kTensors];  // of the elements; and bit 14: in is fp16, bit 15: out is
   int tensors;
-  unsigned chunks, before;     // of this launch, of the launches in front
-  int64_t chunk;               // elements, a multiple of 8
-  double* sums;                // of all chunks
-  unsigned all;                // chunks of all launches
+  bool in_place;                // all of them
+  unsigned chunks, before;     // of this launch; sums of the launches in front
+  double* sums;                // of all launches' workgroups
+  unsigned all;                // of them
   float* norm;
   float scale, limit;
 };
-
-struct Piece {
-  int tensor;
-  int64_t begin, count;
-};
-__device__ __forceinline__ Piece piece_of(const ClipArgs& a, unsigned chunk) {
-  int low = 0, high = a.tensors;
-  while (high - low > 1) {
-    const int mid = (low + high) / 2;
-    if (a.first[mid] <= chunk) low = mid;
-    else high = mid;
-  }
-  const int64_t begin = (int64_t)(chunk - a.first[low]) * a.chunk;
-  return {low, begin, min(a.chunk, a.size[low] - begin)};
+static_assert(sizeof(ClipArgs) <= 4096, "kernel arguments");
+constexpr int kInHalf = 1, kOutHalf = 2;
+__device__ __forceinline__ int types_of(const ClipArgs& a, int tensor) { return a.size_high[tensor] >> 14; }
+__device__ __forceinline__ int64_t size_of(const ClipArgs& a, int tensor) {
+  return (int64_t)(a.size_high[tensor] & 0x3fff) << 32 | a.size_low[tensor];
 }
+
+// Elements in front of the first that lies at a multiple of 16 bytes.
+__host__ __device__ __forceinline__ int ragged(const void* p, bool f16, int64_t n) {
+  const int head = (int)((16 - ((uintptr_t)p & 15)) & 15) / (f16 ? 2 : 4);
+  return head < n ? head : (int)n;
+}
+
+// Chunk after chunk, in either direction: which tensor it is of, where its elements begin, at a multiple of 16 bytes, how many
+// they are, and how many of the tensor lie in front of its first chunk.
+struct Cursor {
+  int tensor, count, front;
+  int64_t begin;
+  __device__ __forceinline__ explicit Cursor(const ClipArgs& a, unsigned chunk) {
+    int low = 0, high = a.tensors;
+    while (high - low > 1) {
+      const int mid = (low + high) / 2;
+      if (a.first[mid] <= chunk) low = mid;
+      else high = mid;
+    }
+    tensor = low;
+    at(a, chunk);
+  }
+  __device__ __forceinline__ void at(const ClipArgs& a, unsigned chunk) {
+    while (tensor + 1 < a.tensors && a.first[tensor + 1] <= chunk) ++tensor;
+    while (a.first[tensor] > chunk) --tensor;
+    const int64_t size = size_of(a, tensor);
+    const int head = ragged(a.in[tensor], types_of(a, tensor) & kInHalf, size);
+    begin = (int64_t)(chunk - a.first[tensor]) * kChunk + head;
+    count = (int)min(kChunk, size - begin);
+    front = chunk == a.first[tensor] ? head : 0;
+  }
+};
 
 typedef float f8 __attribute__((ext_vector_type(8)));
 template <typename T>
@@ -57,13 +82,6 @@ __device__ __forceinline__ void store8(T* p, f8 x) {
   *reinterpret_cast<V*>(p) = __builtin_convertvector(x, V);
 }
 
-// Elements in front of the first that lies at a multiple of 16 bytes.
-template <typename T>
-__device__ __forceinline__ int64_t ragged(const T* p, int64_t n) {
-  const int64_t head = (int64_t)((16 - ((uintptr_t)p & 15)) & 15) / (int64_t)sizeof(T);
-  return min(head, n);
-}
-
 __device__ __forceinline__ double sum_of(double x, double* lds) {  // of the workgroup, in every thread
 #pragma unroll
   for (int step = 32; step > 0; step /= 2) x += __shfl_xor(x, step);
@@ -73,39 +91,39 @@ __device__ __forceinline__ double sum_of(double x, double* lds) {  // of the wor
 }
 
 template <typename T>
-__device__ __forceinline__ double squares(const T* p, int64_t n) {
-  const int tid = threadIdx.x;
-  const int64_t head = ragged(p, n), groups = (n - head) / 8, tail = head + groups * 8;
+__device__ __forceinline__ double squares(const T* p, int n, int front) {
+  const int tid = threadIdx.x, groups = n / 8;
   double sum = 0.0;
-  const auto add = [&](float x) { sum = fma((double)x, (double)x, sum); };
-  if (tid < head) add((float)p[tid]);
-  if (tid < n - tail) add((float)p[tail + tid]);
-  p += head;
-  constexpr int U = 4;
-  int64_t i = tid;
-  for (; i + (U - 1) * kThreads < groups; i += U * kThreads) {
-    f8 x[U];
+  const auto add = [&](f8 x) {
 #pragma unroll
-    for (int j = 0; j < U; ++j) x[j] = load8(p + (i + j * kThreads) * 8);
+    for (int k = 0; k < 8; ++k) sum = fma((double)x[k], (double)x[k], sum);
+  };
+  const auto add_one = [&](float x) { sum = fma((double)x, (double)x, sum); };
+  if (n == kChunk) {
+    f8 x[kGroups];
 #pragma unroll
-    for (int j = 0; j < U; ++j)
+    for (int j = 0; j < kGroups; ++j) x[j] = load8(p + (tid + j * kThreads) * 8);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) add(x[j][k]);
+    for (int j = 0; j < kGroups; ++j) add(x[j]);
+  } else {
+    for (int i = tid; i < groups; i += kThreads) add(load8(p + i * 8));
+    if (tid < n - groups * 8) add_one((float)p[groups * 8 + tid]);
   }
-  for (; i < groups; i += kThreads) {
-    const f8 x = load8(p + i * 8);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) add(x[k]);
-  }
+  if (tid < front) add_one((float)p[tid - front]);
   return sum;
 }
 
 __global__ __launch_bounds__(kThreads) void grad_squares_kernel(ClipArgs a) {
   __shared__ double lds[4];
-  const Piece piece = piece_of(a, blockIdx.x);
-  const void* in = a.in[piece.tensor];
-  const double sum = sum_of(a.f16[piece.tensor] & 1 ? squares((const _Float16*)in + piece.begin, piece.count)
-                                                    : squares((const float*)in + piece.begin, piece.count), lds);
+  double sum = 0.0;
+  Cursor cursor(a, blockIdx.x);
+  for (unsigned chunk = blockIdx.x; chunk < a.chunks; chunk += gridDim.x) {
+    cursor.at(a, chunk);
+    const void* in = a.in[cursor.tensor];
+    sum += types_of(a, cursor.tensor) & kInHalf ? squares((const _Float16*)in + cursor.begin, cursor.count, cursor.front)
+                                    : squares((const float*)in + cursor.begin, cursor.count, cursor.front);
+  }
+  sum = sum_of(sum, lds);
   if (threadIdx.x == 0) a.sums[a.before + blockIdx.x] = sum;
 }
 
@@ -119,33 +137,27 @@ struct Factor {
 };
 
 template <typename S, typename T>
-__device__ __forceinline__ void scaled(const S* in, T* out, int64_t n, Factor by) {
-  const int tid = threadIdx.x;
-  const int64_t head = ragged(in, n);
-  if (((uintptr_t)(out + head) & 15) != 0) {  // aligned differently
-    for (int64_t i = tid; i < n; i += kThreads) out[i] = (T)by((float)in[i]);
-    return;
-  }
-  const int64_t groups = (n - head) / 8, tail = head + groups * 8;
-  if (tid < head) out[tid] = (T)by((float)in[tid]);
-  if (tid < n - tail) out[tail + tid] = (T)by((float)in[tail + tid]);
-  in += head;
-  out += head;
-  constexpr int U = 4;
-  int64_t i = tid;
-  for (; i + (U - 1) * kThreads < groups; i += U * kThreads) {
-    f8 x[U];
+__device__ __forceinline__ void scaled(const S* in, T* out, int n, int front, Factor by) {
+  const int tid = threadIdx.x, groups = n / 8;
+  if (tid < front) out[tid - front] = (T)by((float)in[tid - front]);
+  if (((uintptr_t)out & 15) != 0) {  // aligned differently
+    for (int i = tid; i < n; i += kThreads) out[i] = (T)by((float)in[i]);
+  } else if (n == kChunk) {
+    f8 x[kGroups];
 #pragma unroll
-    for (int j = 0; j < U; ++j) x[j] = load8(in + (i + j * kThreads) * 8);
+    for (int j = 0; j < kGroups; ++j) x[j] = load8(in + (tid + j * kThreads) * 8);
 #pragma unroll
-    for (int j = 0; j < U; ++j) store8(out + (i + j * kThreads) * 8, by(x[j]));
+    for (int j = 0; j < kGroups; ++j) store8(out + (tid + j * kThreads) * 8, by(x[j]));
+  } else {
+    for (int i = tid; i < groups; i += kThreads) store8(out + i * 8, by(load8(in + i * 8)));
+    if (tid < n - groups * 8) out[groups * 8 + tid] = (T)by((float)in[groups * 8 + tid]);
   }
-  for (; i < groups; i += kThreads) store8(out + i * 8, by(load8(in + i * 8)));
 }
 
 __global__ __launch_bounds__(kThreads) void grad_scale_kernel(ClipArgs a) {
   __shared__ double lds[4];
   double sum = 0.0;
+#pragma unroll 8
   for (unsigned i = threadIdx.x; i < a.all; i += kThreads) sum += a.sums[i];
   sum = sum_of(sum, lds);
   const double norm = (double)a.scale * sqrt(sum);
@@ -153,39 +165,41 @@ __global__ __launch_bounds__(kThreads) void grad_scale_kernel(ClipArgs a) {
   if (a.chunks == 0) return;
   // a NaN is passed on
   const Factor by((double)a.scale * (norm <= (double)a.limit ? 1.0 : (double)a.limit / norm));
-  const Piece piece = piece_of(a, a.chunks - 1 - blockIdx.x);
-  const void* in = a.in[piece.tensor];
-  void* out = a.out[piece.tensor];
-  if (in == out && by.first == 1.f) return;
-  const int64_t at = piece.begin, n = piece.count;
-  switch (a.f16[piece.tensor]) {
-    case 0: return scaled((const float*)in + at, (float*)out + at, n, by);
-    case 1: return scaled((const _Float16*)in + at, (float*)out + at, n, by);
-    case 2: return scaled((const float*)in + at, (_Float16*)out + at, n, by);
-    default: return scaled((const _Float16*)in + at, (_Float16*)out + at, n, by);
+  const bool same = by.first == 1.f;
+  if (same && a.in_place) return;
+  Cursor cursor(a, a.chunks - 1 - blockIdx.x);
+  for (unsigned i = blockIdx.x; i < a.chunks; i += gridDim.x) {
+    cursor.at(a, a.chunks - 1 - i);
+    const void* in = a.in[cursor.tensor];
+    void* out = a.out[cursor.tensor];
+    if (in == out && same) continue;
+    const int64_t at = cursor.begin;
+    const int n = cursor.count, front = cursor.front;
+    switch (types_of(a, cursor.tensor)) {
+      case 0: scaled((const float*)in + at, (float*)out + at, n, front, by); break;
+      case kInHalf: scaled((const _Float16*)in + at, (float*)out + at, n, front, by); break;
+      case kOutHalf: scaled((const float*)in + at, (_Float16*)out + at, n, front, by); break;
+      default: scaled((const _Float16*)in + at, (_Float16*)out + at, n, front, by); break;
+    }
   }
 }
 
 }  // namespace
 
-size_t clip_grad_bytes(int64_t tensors) { return (size_t)(kChunks + tensors) * sizeof(double); }
+// The sums of the launches' workgroups: no more than a launch has, nor than there are chunks.
+size_t clip_grad_bytes(int64_t tensors) { return (size_t)((tensors + kTensors - 1) / kTensors) * kBlocks * sizeof(double); }
 
 void launch_clip_grad_norm(const Gradients& g, float scale, float limit, float* norm, void* workspace, hipStream_t st) {
-  int64_t elements = 0;
-  for (int64_t i = 0; i < g.tensors; ++i) elements += g.sizes[i];
   ClipArgs a;
-  a.chunk = ((elements + kChunks - 1) / kChunks + 4095) / 4096 * 4096;
-  if (a.chunk < 8192) a.chunk = 8192;
   a.sums = (double*)workspace;
+  a.all = 0;
+  a.in_place = g.in_place;
   a.norm = norm;
   a.scale = scale;
   a.limit = limit;
-  int64_t all = 0;
-  for (int64_t i = 0; i < g.tensors; ++i) all += (g.sizes[i] + a.chunk - 1) / a.chunk;
-  a.all = (unsigned)all;
   const bool nothing = g.in_place && scale == 1.f && limit == INFINITY;  // the norm alone
   for (int scale_them = 0; scale_them < 2; ++scale_them) {
-    if (scale_them && (nothing || all == 0)) {
+    if (scale_them && (nothing || a.all == 0)) {
       a.tensors = 0;
       a.chunks = a.before = 0;
       hipLaunchKernelGGL(grad_scale_kernel, dim3(1), dim3(kThreads), 0, st, a);
@@ -195,21 +209,29 @@ void launch_clip_grad_norm(const Gradients& g, float scale, float limit, float* 
     a.before = 0;
     while (next < g.tensors) {
       a.tensors = 0;
-      a.chunks = 0;
+      int64_t chunks = 0;
       for (; next < g.tensors && a.tensors < kTensors; ++next) {
         if (g.sizes[next] == 0) continue;
+        const int64_t aligned = g.sizes[next] - ragged(g.in[next], g.in_f16[next] != 0, g.sizes[next]);
+        const int64_t more = aligned <= kChunk ? 1 : (aligned + kChunk - 1) / kChunk;
         const int n = a.tensors++;
         a.in[n] = g.in[next];
         a.out[n] = g.out[next];
-        a.size[n] = g.sizes[next];
-        a.f16[n] = (unsigned char)((g.in_f16[next] ? 1 : 0) | (g.out_f16[next] ? 2 : 0));
-        a.first[n] = a.chunks;
-        a.chunks += (unsigned)((g.sizes[next] + a.chunk - 1) / a.chunk);
+        a.size_low[n] = (unsigned)g.sizes[next];
+        a.size_high[n] = (uint16_t)(g.sizes[next] >> 32 | (int64_t)((g.in_f16[next] ? kInHalf : 0) | (g.out_f16[next] ? kOutHalf : 0)) << 14);
+        a.first[n] = (unsigned)chunks;
+        chunks += more;
       }
-      if (a.chunks == 0) continue;
-      if (scale_them) hipLaunchKernelGGL(grad_scale_kernel, dim3(a.chunks), dim3(kThreads), 0, st, a);
-      else hipLaunchKernelGGL(grad_squares_kernel, dim3(a.chunks), dim3(kThreads), 0, st, a);
-      a.before += a.chunks;
+      if (chunks == 0) continue;
+      a.chunks = (unsigned)chunks;
+      const unsigned blocks = chunks < kBlocks ? (unsigned)chunks : kBlocks;
+      if (scale_them) {
+        hipLaunchKernelGGL(grad_scale_kernel, dim3(blocks), dim3(kThreads), 0, st, a);
+      } else {
+        hipLaunchKernelGGL(grad_squares_kernel, dim3(blocks), dim3(kThreads), 0, st, a);
+        a.all += blocks;
+      }
+      a.before += blocks;
     }
   }
 }

@@ -223,39 +223,40 @@ def clip_grad_norm_(grads, max_norm, scale=1.0, out=None):
     scale: the inverse of a loss scale; max_norm infinity: the norm, and the gradients times scale.  Squares are summed in 64
     bits.  Gradients in place are written only where the factor is not 1.  An infinity among them makes the norm infinite and
     the results 0 or NaN, a NaN makes all of them NaN: a step to skip."""
+    what = "clip_grad_norm_"
     grads = list(grads)
     outs = grads if out is None else list(out)
-    what = "clip_grad_norm_"
     assert grads, "no gradients"
     assert len(outs) == len(grads), (len(outs), len(grads))
-    dev = _on_gpu(grads[0], *grads[1:], *outs)
+    dev = _on_gpu(*grads) if out is None else _on_gpu(*grads, *outs)
     scale, max_norm = float(scale), float(max_norm)
     if not 0.0 < scale < math.inf or not max_norm > 0.0:
         raise ValueError(f"{what}: scale {scale} or max_norm {max_norm} is not positive")
-    half = torch.float16
-    for t in grads if out is None else grads + outs:
-        if t.dtype is not half and t.dtype is not torch.float32:
+    every = grads if out is None else grads + outs
+    types = [t.dtype for t in every]
+    if not _DTYPES.keys() >= set(types):
+        for t in every:
             _dtype_code(t, what)
+    for t in every:
         assert t.is_contiguous() or _side_by_side(t), "the elements of a gradient must fill its memory"
-        if t.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError(f"{what} has no derivative")
+    if torch.is_grad_enabled() and any([t.requires_grad for t in every]):
+        raise RuntimeError(f"{what} has no derivative")
     if out is not None:
         for g, o in zip(grads, outs):
             assert o.shape == g.shape and (o.stride() == g.stride() or o.is_contiguous() and g.is_contiguous()), (
                 "out must have the gradients' shapes and orders")
     n = len(grads)
-    at = array.array("Q", [t.data_ptr() for t in grads])
+    addresses = array.array("Q", [t.data_ptr() for t in every])
     sizes = array.array("q", [t.numel() for t in grads])
-    types = bytes([t.dtype is half for t in grads])
-    to, out_types = (at, types) if out is None else (array.array("Q", [t.data_ptr() for t in outs]),
-                                                     bytes([t.dtype is half for t in outs]))
+    halves = bytes([t is torch.float16 for t in types])
+    at = addresses.buffer_info()[0]
     norm = grads[0].new_empty((), dtype=torch.float32)
     lib = _lib.load()
     nbytes = lib.gptmi_clip_grad_norm_workspace_bytes(n)
-    ws = _workspace(nbytes, grads[0])
-    _call(dev, what, lib.gptmi_clip_grad_norm, at.buffer_info()[0], to.buffer_info()[0], sizes.buffer_info()[0], types,
-          out_types, n, scale, max_norm, norm.data_ptr(), _ptr(ws), nbytes)
-    torch.autograd.graph.increment_version([t for t in outs if not t.is_inference()])
+    ws = _workspace(nbytes, norm)
+    _call(dev, what, lib.gptmi_clip_grad_norm, at, at if out is None else at + 8 * n, sizes.buffer_info()[0], halves,
+          halves if out is None else halves[n:], n, scale, max_norm, norm.data_ptr(), ws.data_ptr(), nbytes)
+    torch.autograd.graph.increment_version(outs)
     return norm
 
 
