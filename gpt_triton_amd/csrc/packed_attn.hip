@@ -40,7 +40,8 @@ __device__ __forceinline__ float bounded(float x) {
   return fabsf(x) < INFINITY ? __builtin_amdgcn_fmed3f(x, -65504.f, 65504.f) : x;
 }
 
-template <int D, int QB, int P>
+// STATS: with what the gradients need of each row (as a branch, 1 % of the others' time).
+template <int D, int QB, int P, bool STATS>
 __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(PackedArgs a) {
   constexpr int R = 64 * QB / P;       // queries a workgroup
   constexpr int KS = (D + 31) / 32, DB = D / 16;
@@ -316,7 +317,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
       const float to = larger(base[n], other[0]);
       const float mine = __builtin_amdgcn_exp2f(base[n] - to), its = __builtin_amdgcn_exp2f(other[0] - to);
       den[n] = fmaf(den[n], mine, other[1] * its);
-      base[n] = to;
+      if constexpr (STATS) base[n] = to;
 #pragma unroll
       for (int i = 0; i < DB; ++i) oacc[n][i] = oacc[n][i] * mine + sums[(n * (DB + 1) + i) * kWave] * its;
     }
@@ -342,7 +343,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
     // base is not as good as an fp16 number.
     float2 stat = {base[n], inv};
     const bool again = __any(none != 0.f && q < L);
-    if (again || (a.stats && __any(!(fabsf(base[n]) < 8192.f) && q < L))) {
+    if (again || (STATS && __any(!(fabsf(base[n]) < 8192.f) && q < L))) {
       const int last = min(qw0 + 16 * n + 15, L - 1);
       // of query c with key j, from this lane's elements of both and the other three lanes': one rounded number
       auto score = [&](int j) {
@@ -370,7 +371,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
       const bool number = total == total && fabsf(m) < INFINITY;  // else there is no softmax
       const float inv_total = number ? 1.0f / total : NAN;
       stat = {m, -inv_total};
-      if (again) {
+      if (again) {  // the output, too
 #pragma unroll
         for (int i = 0; i < DB; ++i) oacc[n][i] = f4(number ? 0.f : NAN);
       }
@@ -391,7 +392,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
         }
       }
     }
-    if (a.stats && g == 0 && q < L) a.stats[head * a.rows + block.first + q] = stat;
+    if (STATS && g == 0 && q < L) a.stats[head * a.rows + block.first + q] = stat;
     _Float16* o = a.out + ((block.first + q) * a.heads + head) * D + 4 * g;
 #pragma unroll
     for (int i = 0; i < DB; ++i) {
@@ -403,8 +404,8 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
   }
 }
 
-template <int D, int QB, int P>
-int launch_as(PackedArgs a, int64_t slots, hipStream_t st) {
+template <int D, int QB, int P, bool STATS>
+int launch_with(PackedArgs a, int64_t slots, hipStream_t st) {
   const int64_t blocks = slots * a.heads;
   if (blocks > (1ll << 31) - kGridRow) {
     set_error("flash_attn_packed: %lld rows in %d sequences of %d heads exceed the grid", (long long)a.rows, a.sequences,
@@ -414,7 +415,7 @@ int launch_as(PackedArgs a, int64_t slots, hipStream_t st) {
   constexpr int lds = P * 2 * 2 * kKeys * D * 2;
   static bool attr_done = false;  // idempotent; a race only repeats the call
   if (!attr_done) {
-    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(packed_attn_kernel<D, QB, P>),
+    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(packed_attn_kernel<D, QB, P, STATS>),
                                        hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) {
       set_error("hipFuncSetAttribute(%d bytes LDS): %s", lds, hipGetErrorString(e));
@@ -434,8 +435,13 @@ int launch_as(PackedArgs a, int64_t slots, hipStream_t st) {
   a.longest_first = a.sequences <= kMany * kWave && slots <= 512 && blocks <= 5120 && a.rows >= 128ll * a.sequences;
   const int64_t grid = a.longest_first ? (slots + 7) / 8 * 8 * a.heads : blocks;
   const dim3 dims((unsigned)(grid < kGridRow ? grid : kGridRow), (unsigned)((grid + kGridRow - 1) / kGridRow));
-  hipLaunchKernelGGL((packed_attn_kernel<D, QB, P>), dims, dim3(256), lds, st, a);
+  hipLaunchKernelGGL((packed_attn_kernel<D, QB, P, STATS>), dims, dim3(256), lds, st, a);
   return 0;
+}
+
+template <int D, int QB, int P>
+int launch_as(const PackedArgs& a, int64_t slots, hipStream_t st) {
+  return a.stats ? launch_with<D, QB, P, true>(a, slots, st) : launch_with<D, QB, P, false>(a, slots, st);
 }
 
 // While the workgroups run at once, the launch takes what a wavefront's chain through its key tiles takes: 0.5 us a
