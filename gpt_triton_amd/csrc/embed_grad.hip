@@ -58,6 +58,7 @@ struct EmbedGradArgs {
   DropoutArgs drop;
   // the sort's
   int tiles, bits;          // workgroups, bits of a digit
+  int lanes, across, share;  // of the position table's parts: chunks each, parts a row, groups that share a batch
   int64_t fill, fills;      // other work of a launch: from which 64 KB on, and how many of them; positions behind
   unsigned *keys[2], *at[2];  // tokens (V: none) and positions
   unsigned* hist;           // [tiles][1 << bits]
@@ -120,37 +121,35 @@ __device__ __forceinline__ void add_rows(const T* dz, int H, int chunk, int64_t 
   for (; i < last; ++i) add_chunk(dz + place(i) * H + chunk * VN, sum);
 }
 
-// Row l of the position table's gradient, by a workgroup in groups of `lanes` threads that share the batch.
+// Parts of rows of the position table's gradient, a.lanes chunks of each, by a workgroup in groups of as many threads: a.share
+// of them share the batch of a row.
 template <typename T, int VN, int NT>
-__device__ __forceinline__ void position_row(const EmbedGradArgs& a, int64_t l, int lanes, float* lds) {
-  const T* dz = (const T*)a.dz;
-  T* row = (T*)a.d_wpe + l * a.H;
-  const int chunks = a.H / VN, tid = threadIdx.x;
-  const int groups = NT / lanes, group = tid / lanes, lane = tid - group * lanes;
-  const int64_t batch = l < a.L ? a.tokens / a.L : 0, share = (batch + groups - 1) / groups;
-  const int64_t first = min((int64_t)group * share, batch), last = group < groups ? min(first + share, batch) : first;
-  for (int c0 = 0; c0 < chunks; c0 += lanes) {
-    const int chunk = c0 + lane;
-    float sum[VN];
-    clear(sum);
-    if (chunk < chunks) add_rows<T, VN>(dz, a.H, chunk, first, last, [&](int64_t b) { return b * a.L + l; }, sum);
-    if (groups > 1) {
-      __syncthreads();
-      if (group < groups)
+__device__ __forceinline__ void position_parts(const EmbedGradArgs& a, int64_t item, float* lds) {
+  const int tid = threadIdx.x, lanes = a.lanes, group = tid / lanes, lane = tid - group * lanes;
+  const int rows = NT / lanes / a.share, in_block = group / a.share, part = group - in_block * a.share;
+  const int64_t block = item / a.across, l = block * rows + in_block;
+  const int chunk = (int)(item - block * a.across) * lanes + lane;
+  const bool there = in_block < rows && l < a.P && chunk < a.H / VN;
+  const int64_t batch = l < a.L ? a.tokens / a.L : 0, share = (batch + a.share - 1) / a.share;
+  const int64_t first = min((int64_t)part * share, batch), last = min(first + share, batch);
+  float sum[VN];
+  clear(sum);
+  if (there) add_rows<T, VN>((const T*)a.dz, a.H, chunk, first, last, [&](int64_t b) { return b * a.L + l; }, sum);
+  if (a.share > 1) {
+    if (in_block < rows)
 #pragma unroll
-        for (int i = 0; i < VN; ++i) lds[(group * VN + i) * lanes + lane] = sum[i];
-      __syncthreads();
-      if (group == 0)
-        for (int n = 1; n < groups; ++n)
+      for (int i = 0; i < VN; ++i) lds[(group * VN + i) * lanes + lane] = sum[i];
+    __syncthreads();
+    if (there && part == 0)
+      for (int n = 1; n < a.share; ++n)
 #pragma unroll
-          for (int i = 0; i < VN; ++i) sum[i] += lds[(n * VN + i) * lanes + lane];
-    }
-    if (group == 0 && chunk < chunks) put_sum<T, VN>(a, row, chunk, kept_columns<VN>(a, chunk), sum);
+        for (int i = 0; i < VN; ++i) sum[i] += lds[((group + n) * VN + i) * lanes + lane];
   }
+  if (there && part == 0) put_sum<T, VN>(a, (T*)a.d_wpe + l * a.H, chunk, kept_columns<VN>(a, chunk), sum);
 }
 
 // Threads that share a row's chunks: a power of two below a wavefront, whole wavefronts beyond.
-__device__ __forceinline__ int lanes_of(int chunks, int most) {
+__host__ __device__ __forceinline__ int lanes_of(int chunks, int most) {
   if (chunks >= most) return most;
   if (chunks > 32) return (chunks + 63) & ~63;
   int n = 1;
@@ -168,7 +167,7 @@ __global__ __launch_bounds__(256) void embed_grad_few_kernel(EmbedGradArgs a, in
   __shared__ int counts[4], begin[64 + 1];
   const int tid = threadIdx.x, chunks = a.H / VN, lanes = lanes_of(chunks, 256);
   if ((int)blockIdx.x >= vocab_blocks) {
-    position_row<T, VN, 256>(a, blockIdx.x - vocab_blocks, lanes, lds);
+    position_parts<T, VN, 256>(a, blockIdx.x - vocab_blocks, lds);
     return;
   }
   const int64_t v0 = (int64_t)blockIdx.x * rows_of;
@@ -247,7 +246,7 @@ __device__ __forceinline__ unsigned key_of(const EmbedGradArgs& a, int64_t i) {
 template <typename T, int VN>
 __device__ __forceinline__ void other_work(const EmbedGradArgs& a, int64_t item, float* lds) {
   if (item >= a.fills) {
-    position_row<T, VN, kSortThreads>(a, item - a.fills, lanes_of(a.H / VN, kSortThreads), lds);
+    position_parts<T, VN, kSortThreads>(a, item - a.fills, lds);
     return;
   }
   item += a.fill;
@@ -544,18 +543,33 @@ __global__ __launch_bounds__(256) void embed_grad_join_kernel(EmbedGradArgs a) {
 template <typename T, int VN>
 __global__ __launch_bounds__(kSortThreads) void embed_grad_positions_kernel(EmbedGradArgs a) {
   __shared__ float lds[kSortThreads * VN];
-  position_row<T, VN, kSortThreads>(a, blockIdx.x, lanes_of(a.H / VN, kSortThreads), lds);
+  position_parts<T, VN, kSortThreads>(a, blockIdx.x, lds);
 }
 
 int run_of(int64_t tokens) { return tokens >= 1 << 17 ? 128 : tokens >= 1 << 15 ? 64 : 32; }
 
 template <typename T, int VN>
 void launch_as(EmbedGradArgs a, hipStream_t st) {
+  const int chunks = a.H / VN;
+  // The batch of a row of the position table is shared, by groups that are narrower then, where the rows alone would be few threads
+  // (us, 583 x 11 tokens, 1280 wide, fp32: 126 as whole rows, 94 shared by 16 groups; 512 x 300 fp16, 768 wide, of which the
+  // launch with them: 57 by 8, 63 by 16).
+  const int threads = a.d_wte && a.tokens <= kFew ? 256 : kSortThreads;
+  int64_t positions = 0;  // workgroups
+  const auto share_by = [&](int share) {
+    a.share = share;
+    a.lanes = lanes_of(chunks, threads / share);
+    a.across = (chunks + a.lanes - 1) / a.lanes;
+    const int rows = threads / a.lanes / share;
+    positions = a.d_wpe ? (a.P + rows - 1) / rows * a.across : 0;
+  };
+  share_by(1);
+  while (a.share < threads / 64 && a.share < a.tokens / a.L && a.L * chunks * a.share < 1 << 17 && positions < 1 << 19)
+    share_by(2 * a.share);
   if (!a.d_wte) {
-    hipLaunchKernelGGL((embed_grad_positions_kernel<T, VN>), dim3((unsigned)a.P), dim3(kSortThreads), 0, st, a);
+    hipLaunchKernelGGL((embed_grad_positions_kernel<T, VN>), dim3((unsigned)positions), dim3(kSortThreads), 0, st, a);
     return;
   }
-  const int64_t positions = a.d_wpe ? a.P : 0;
   if (a.tokens <= kFew) {
     // up to 64 rows a workgroup, fewer where that leaves CUs without one
     int rows = 64;
@@ -602,13 +616,7 @@ void launch_as(EmbedGradArgs a, hipStream_t st) {
     a.sorted = a.keys[passes & 1];
     a.order = a.at[passes & 1];
   }
-  const int chunks = a.H / VN;
-  int lanes = 1;  // lanes_of(chunks, 256)
-  if (chunks >= 256) lanes = 256;
-  else if (chunks > 32) lanes = (chunks + 63) & ~63;
-  else
-    while (lanes < chunks) lanes *= 2;
-  const int groups = 256 / lanes;
+  const int groups = 256 / lanes_of(chunks, 256);
   const int64_t runs = (a.tokens + a.run - 1) / a.run;
   const unsigned across = (unsigned)((chunks + 255) / 256);
   hipLaunchKernelGGL((embed_grad_sum_kernel<T, VN>), dim3((unsigned)((runs + groups - 1) / groups), across), dim3(256), 0, st, a);

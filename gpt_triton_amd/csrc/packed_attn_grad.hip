@@ -416,6 +416,7 @@ __device__ __forceinline__ void walk(const GradArgs& a, int id, int slots, bool 
           for (int r = 0; r < 4; ++r) {
             const int y = y0 + 8 * g + 4 * b + r, x = xw0 + 16 * n + c;
             now.s[n][b][r] = (KEYS ? x <= y && y < L : y <= x) ? now.s[n][b][r] : -INFINITY;
+            if ((KEYS ? y : x) == 0) now.p[n][b][r] *= 0.f;  // a sequence's first query has one key, and no gradient
           }
     }
   };
@@ -613,7 +614,7 @@ __device__ __forceinline__ void walk(const GradArgs& a, int id, int slots, bool 
         p = pp.a + pp.b;
         const float w = stat.y > 0.f ? __builtin_amdgcn_exp2f(fmaf(s, to_exp2, -stat.x)) * stat.y
                                      : __expf(s * a.scale - stat.x) * -stat.y;
-        const float u = w * (p + less);
+        const float u = w * ((p + less) * (query == 0 ? 0.f : 1.f));
         const bool seen = KEYS ? x <= y : y <= x;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {

@@ -255,6 +255,19 @@ def test_large_gradients_are_finite(K, gpu_device):
     check(K, q, k, v, e, [100])
 
 
+@pytest.mark.parametrize("d", [16, 32, 64, 128, 256])
+def test_first_rows(K, gpu_device, d):
+    """A query with one key has weight 1 whatever its score is: its gradient is 0, and so is what it adds to the key's."""
+    r = np.random.default_rng(15)
+    lengths = [1] * 70
+    q, k, v, e = make(r, 70, 4, 2, d, True, gpu_device)
+    _, dq, dk, dv = grads(K, q, k, v, e, starts_of(lengths, gpu_device))
+    assert not dq.any() and not dk.any()
+    assert torch.equal(dv, (e[:, 0::2].float() + e[:, 1::2].float()).half())
+    _, dq, dk, dv = grads(K, q, k, v, e, starts_of([30, 40], gpu_device))
+    assert not dq[0].any() and not dq[30].any() and dq[1:30].any() and dq[31:].any()
+
+
 def test_same_bits(K, gpu_device):
     r = np.random.default_rng(9)
     lengths = [300, 1, 513]

@@ -32,7 +32,7 @@ def test_embed_backward(lib):
                  dict(dz=ctypes.c_void_p(257)), dict(d_wte=ctypes.c_void_p(258), dtype=0), dict(ids=ctypes.c_void_p(260))):
         assert embed(lib, **args) == -1, args
         assert b"embed_backward" in lib.gptmi_last_error()
-    for args in (dict(B=1 << 30), dict(V=(1 << 26) + 1), dict(P=(1 << 21) + 1), dict(H=(1 << 20) + 1), dict(B=1 << 62)):
+    for args in (dict(B=1 << 30), dict(V=(1 << 26) + 1), dict(P=(1 << 24) + 1), dict(H=(1 << 20) + 1), dict(B=1 << 62)):
         assert embed(lib, **args) == -2, args
     needed = lib.gptmi_embed_backward_workspace_bytes(2, 300, 64)
     assert needed > 0 and lib.gptmi_embed_backward_workspace_bytes(1, 256, 64) == 0
