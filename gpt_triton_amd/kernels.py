@@ -17,7 +17,8 @@ K-contiguous image, which `fused_ffn` / `matmul_and_split_qkv` otherwise rebuild
 where the kernels cannot read the weight in place (fp16, K a multiple of 64); a `PackedWeight` may be passed wherever they take `weight`.
 For scoring texts and learning from the scores, which the reference has nothing for: `flash_attention_packed` (prompts of different
 lengths without padding, grouped heads), `token_log_probs` (of rows of logits, with entropy, alternatives and gradient) and
-`distillation_loss` / `distillation_loss_and_grad` (against a teacher's top logits).  Tensors must live on the
+`distillation_loss` / `distillation_loss_and_grad` (against a teacher's top logits).  `flash_attention_packed` and
+`fused_embeddings` have gradients, and `clip_grad_norm_` clips all gradients together.  Tensors must live on the
 GPU: there is no CPU path.  dropout_prob > 0 reproduces the reference's masks: Philox-4x32-10
 (Triton's tl.rand) with the kernels' default seed 1337 and the reference's offsets -- the column
 for the embedding, the flat index m*N + n for fused_ffn, query*Lk + key for the attention
