@@ -906,12 +906,21 @@ static int check_packed(const char* what, const PackedAttention& p, int64_t d, u
   return GPTMI_OK;
 }
 
+// The gradients read the output's rows as they read q's, so a row of it is no longer than a pitch may be.
+static int check_packed_gradients(const char* what, const PackedAttention& p, int64_t d, uintptr_t more, int dtype) {
+  const int rc = check_packed(what, p, d, more, dtype);
+  if (rc || d <= (1 << 24) / p.heads) return rc;
+  set_error("%s: %lld heads of %lld are beyond the supported", what, (long long)p.heads, (long long)d);
+  return GPTMI_ERR_UNSUPPORTED;
+}
+
 static int flash_attn_packed(const char* what, const PackedAttention& p, int64_t d, int dtype, void* stream) {
   if (!p.out) {
     set_error("%s: invalid argument", what);
     return GPTMI_ERR_INVALID;
   }
-  int rc = check_packed(what, p, d, (uintptr_t)p.out, dtype);
+  int rc = p.stats ? check_packed_gradients(what, p, d, (uintptr_t)p.out, dtype)
+                   : check_packed(what, p, d, (uintptr_t)p.out, dtype);
   if (!rc) rc = launch_flash_attn_packed(p, (int)d, (hipStream_t)stream);
   return rc ? rc : check_launch(what);
 }
@@ -958,7 +967,8 @@ int gptmi_flash_attn_packed_backward(const void* q, const void* k, const void* v
   }
   const PackedAttention p{q, k, v, (void*)out, (void*)stats, starts, sequences, T, N, G, q_row, q_head, k_row, k_head, v_row,
                           v_head, scale};
-  int rc = check_packed(what, p, d, (uintptr_t)out | (uintptr_t)d_out | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv, dtype);
+  int rc = check_packed_gradients(
+      what, p, d, (uintptr_t)out | (uintptr_t)d_out | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv, dtype);
   if (rc) return rc;
   const size_t needed = packed_attn_grad_bytes(T, sequences, N, G, d);
   if (!workspace || workspace_bytes < needed || ((uintptr_t)workspace & 255) != 0) {

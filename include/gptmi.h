@@ -407,7 +407,8 @@ int gptmi_flash_attn_packed_train(const void* q, const void* k, const void* v, v
  *   and have gradients of 0.
  * w and u are formed again in fp32 and rounded to fp16 for the products, scaled by powers of two so that they stay normal
  * numbers.  What hidden rows hold, infinities and NaN included, plays no part.  workspace:
- * gptmi_flash_attn_packed_backward_workspace_bytes(...) of the same sizes, 256-byte aligned.
+ * gptmi_flash_attn_packed_backward_workspace_bytes(...) of the same sizes, 256-byte aligned.  N d up to 2^24, here and in
+ * gptmi_flash_attn_packed_train.
  * No counterpart in the reference, which has no gradients.
  */
 size_t gptmi_flash_attn_packed_backward_workspace_bytes(int64_t sequences, int64_t T, int64_t N, int64_t G, int64_t d);

@@ -63,6 +63,16 @@ def test_refusals(lib):
         assert lib.gptmi_flash_attn_packed_backward_workspace_bytes(*args) == 0
 
 
+def test_rows_of_the_output(lib):
+    """Offsets inside a tile of rows of the output and its gradient are 32-bit numbers."""
+    for n, d in ((1 << 20, 256), (1 << 20, 32), ((1 << 18) + 2, 64), ((1 << 16) + 2, 256)):
+        sizes = dict(S=1, T=40, N=n, d=d)
+        assert train(lib, **sizes) == -2, sizes
+        assert backward(lib, **sizes, ws=None) == -2, sizes
+    for n, d in ((1 << 20, 16), (1 << 18, 64), (1 << 16, 256)):
+        assert backward(lib, S=1, T=40, N=n, d=d, ws=None) == -3
+
+
 def test_operator_refuses():
     q, k = (torch.zeros(8, n, 64, dtype=torch.float16, requires_grad=True) for n in (4, 2))
     starts = torch.tensor([0, 3, 8])
