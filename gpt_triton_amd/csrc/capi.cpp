@@ -46,9 +46,10 @@ constexpr int kMaxN = 1 << 26;
 // 64 bits.
 constexpr int64_t kMaxVocab = 1ll << 30, kMaxPitch = 1ll << 40;
 
-// Sizes that the grids of the embedding's gradients take (of the position table its elements); tensors and elements of one
-// clip_grad_norm.
+// Sizes that the grids of the embedding's gradients take (of the tables their elements, too: a workgroup of 1024 threads for each
+// 64 KB of the token table, and a grid's threads are below 2^32); tensors and elements of one clip_grad_norm.
 constexpr int64_t kMaxGradTokens = 1 << 30, kMaxGradVocab = 1 << 26, kMaxGradPositions = 1 << 30, kMaxGradWidth = 1 << 20;
+constexpr int64_t kMaxGradTable = 1ll << 34;
 constexpr int64_t kMaxGradients = 1 << 20, kMaxGradElements = 1ll << 42;
 
 // Workspace plan of one GEMM: where the packed weight and (if needed) the
@@ -431,7 +432,7 @@ int gptmi_embed_backward(const int64_t* ids, const void* dz, void* d_wte, void* 
     set_error("embed_backward: sequence length %lld exceeds the %lld position rows", (long long)L, (long long)P);
     return GPTMI_ERR_INVALID;
   }
-  if (B > kMaxGradTokens / L || V > kMaxGradVocab || P > kMaxGradPositions / H || H > kMaxGradWidth) {
+  if (B > kMaxGradTokens / L || V > kMaxGradVocab || V > kMaxGradTable / H || P > kMaxGradPositions / H || H > kMaxGradWidth) {
     set_error("embed_backward: sizes beyond the supported");
     return GPTMI_ERR_UNSUPPORTED;
   }

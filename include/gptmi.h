@@ -103,8 +103,8 @@ int gptmi_embed(const int64_t* ids, const void* wte, const void* wpe, void* out,
  * same call gives the same bits; one rounding to the storage dtype.
  *   d_wte [V][H], d_wpe [P][H]: one of them may be NULL; they overlap nothing
  *   workspace: gptmi_embed_backward_workspace_bytes(B, L, H) bytes, 256-byte aligned (may be NULL where that is 0, or d_wte is)
- * Up to 2^30 tokens, 2^26 rows of wte, 2^30 elements of wpe, H up to 2^20; any alignment that the element type allows, fastest where rows
- * and addresses are multiples of 16 bytes.
+ * Up to 2^30 tokens, 2^26 rows and 2^34 elements of wte, 2^30 elements of wpe, H up to 2^20; any alignment that the element type allows,
+ * fastest where rows and addresses are multiples of 16 bytes.
  * No counterpart in the reference, which has no gradients.
  */
 size_t gptmi_embed_backward_workspace_bytes(int64_t B, int64_t L, int64_t H);

@@ -42,6 +42,13 @@ def test_embed_backward(lib):
         assert lib.gptmi_embed_backward_workspace_bytes(*args) == 0
 
 
+def test_tables_beyond_the_grid(lib):
+    """The token table's zero rows are a workgroup of 1024 threads for each 64 KB: below 2^32 threads."""
+    for args in (dict(V=1 << 26, H=1 << 10), dict(V=(1 << 24) + 1, H=1 << 10), dict(V=1 << 20, H=1 << 20, P=300)):
+        assert embed(lib, **args, ws=None) == -2, args
+    assert embed(lib, V=1 << 24, H=1 << 10, ws=None) == -3
+
+
 def clip(lib, grads=(4096,), out=None, sizes=(100,), f16=(0,), out_f16=None, n=None, scale=1.0, max_norm=1.0, norm=FAKE, ws=FAKE,
          ws_bytes=1 << 20):
     at = array.array("Q", grads)
