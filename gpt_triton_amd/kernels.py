@@ -197,6 +197,7 @@ def fused_embeddings(x, wte, wpe, dropout_prob=0.0):
 
     Gradients flow to wte and wpe, dense, backward and once: sums over a token's positions and over the batch, in fp32, each
     in one order, so that the same step gives the same bits."""
+    _no_tangents("fused_embeddings", wte, wpe)
     if (wte.requires_grad or wpe.requires_grad) and torch.is_grad_enabled():
         return _EmbeddingsFunction.apply(x, wte, wpe, dropout_prob)
     return _embeddings(x, wte, wpe, dropout_prob)
@@ -229,6 +230,7 @@ def clip_grad_norm_(grads, max_norm, scale=1.0, out=None):
     outs = grads if out is None else list(out)
     assert grads, "no gradients"
     assert len(outs) == len(grads), (len(outs), len(grads))
+    _no_tangents(what, *grads, *outs)
     dev = _on_gpu(*grads) if out is None else _on_gpu(*grads, *outs)
     scale, max_norm = float(scale), float(max_norm)
     if not 0.0 < scale < math.inf or not max_norm > 0.0:
@@ -869,6 +871,7 @@ def flash_attention_packed(q, k, v, starts, scale=None, out=None):
 
     Gradients flow to q, k and v (dense ones, fp16), backward and once; of rows that belong to no sequence they are 0.  Each
     is one sum in one order: the same step gives the same bits.  With `out` given the call is a forward pass only."""
+    _no_tangents("flash_attention_packed", q, k, v)
     if out is None and (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
         return _PackedAttentionFunction.apply(q, k, v, starts, scale)
     return _packed_attention(q, k, v, starts, scale, out, False)[0]
