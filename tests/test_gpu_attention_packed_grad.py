@@ -384,3 +384,100 @@ def test_captured_step(K, gpu_device):
         torch.cuda.synchronize()
         for a, b in zip(got, grads(K, *new, starts_of(some, gpu_device))):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("d", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("heads", [(4, 4), (8, 1)])
+def test_some_of_the_gradients_of_every_size(K, gpu_device, d, heads):
+    """Each walk in a launch of its own, and the heads over a key head divided or not."""
+    r = np.random.default_rng(16)
+    lengths = [150, 1, 70]
+    q, k, v, e = make(r, 221, *heads, d, True, gpu_device)
+    starts = starts_of(lengths, gpu_device)
+    _, *every = grads(K, q, k, v, e, starts)
+    for need in ((True, False, False), (False, True, False), (False, False, True), (False, True, True)):
+        leaves = [t.detach().requires_grad_(n) for t, n in zip((q, k, v), need)]
+        got = torch.autograd.grad(K.flash_attention_packed(*leaves, starts), [t for t in leaves if t.requires_grad], e)
+        assert all(torch.equal(a, b) for a, b in zip(got, [g for g, n in zip(every, need) if n]))
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("far_heads", [False, True])
+def test_offsets_beyond_32_bits(K, gpu_device, d, far_heads):
+    """Rows, or heads, so far apart that their offsets pass 2^32 bytes: the gradients of dense copies."""
+    r = np.random.default_rng(17)
+    dense = make(r, 140, 4, 2, d, False, gpu_device)
+    starts = starts_of([5, 135], gpu_device)
+    far = []
+    if far_heads:
+        wide = torch.empty(4, 1 << 30, dtype=torch.float16, device=gpu_device)
+        for n, t in enumerate(dense[:3]):
+            far.append(wide[:t.shape[1], n << 20:(n << 20) + 140 * d].view(t.shape[1], 140, d).transpose(0, 1))
+    else:
+        wide = torch.empty(140, 1 << 24, dtype=torch.float16, device=gpu_device)
+        for n, t in enumerate(dense[:3]):
+            at = (1 << 24) - (n + 1) * 1024
+            far.append(wide[:, at:at + t.shape[1] * d].view(140, t.shape[1], d))
+    for x, t in zip(far, dense):
+        x.copy_(t)
+    assert all(torch.equal(a, b) for a, b in zip(grads(K, *far, dense[3], starts), grads(K, *dense, starts)))
+
+
+def test_two_streams_at_once(K, gpu_device):
+    r = np.random.default_rng(18)
+    lengths = [700, 300]
+    inputs = [make(r, 1000, 8, 2, 128, True, gpu_device) for _ in range(2)]
+    starts = starts_of(lengths, gpu_device)
+    alone = [grads(K, *t, starts) for t in inputs]
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(3):
+        for n, side in enumerate(sides):
+            with torch.cuda.stream(side):
+                got[n].append(grads(K, *inputs[n], starts))
+    torch.cuda.synchronize()
+    for n in range(2):
+        for one in got[n]:
+            assert all(torch.equal(a, b) for a, b in zip(one, alone[n]))
+
+
+def test_two_graphs_with_one_pool(K, gpu_device):
+    """Replayed by turns: each result stands until its own graph, or one that shares its memory, runs again."""
+    r = np.random.default_rng(20)
+    inputs = [make(r, 200, 4, 1, 64, False, gpu_device) for _ in range(2)]
+    starts = [starts_of(x, gpu_device) for x in ([120, 80], [3, 197])]
+    leaves = [[t.detach().requires_grad_() for t in x[:3]] for x in inputs]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        grads(K, *inputs[0], starts[0])
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, got = [], []
+    for n in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=graphs[0].pool() if graphs else None):
+            out = K.flash_attention_packed(*leaves[n], starts[n])
+            got.append((out, *torch.autograd.grad(out, leaves[n], inputs[n][3])))
+        graphs.append(graph)
+    for turn in range(3):
+        for n in range(2):
+            with torch.no_grad():
+                inputs[n][3].mul_(-1)
+            graphs[n].replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got[n], grads(K, *inputs[n], starts[n])))
+
+
+def test_what_is_changed_behind_the_forward_pass(K, gpu_device):
+    """torch's versions: what the gradients need may not be written in between."""
+    r = np.random.default_rng(21)
+    for which in range(3):
+        q, k, v, e = make(r, 30, 2, 2, 64, False, gpu_device)
+        starts = starts_of([30], gpu_device)
+        q.requires_grad_()
+        out = K.flash_attention_packed(q, k, v, starts)
+        with torch.no_grad():
+            (k, v, starts)[which].add_(0)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            out.backward(e)

@@ -240,3 +240,36 @@ def test_captured_step(K, gpu_device, B, L):
         torch.cuda.synchronize()
         for a, b in zip(got[1:], grads(K, ids.clone(), dz.clone(), 700, L, gpu_device)):
             assert torch.equal(a, b)
+
+
+def test_largest(K, gpu_device):
+    """More than 2^32 bytes and 2^31 elements of the output's gradient: whole numbers, summed without rounding."""
+    B, L, V, H = 2100, 1024, 50257, 1032
+    r = torch.Generator(device=gpu_device).manual_seed(3)
+    ids = torch.randint(0, V, (B, L), device=gpu_device, generator=r)
+    dz = torch.randint(-4, 5, (B, L, H), device=gpu_device, generator=r, dtype=torch.int8).half()
+    got = grads(K, ids, dz, V, L, gpu_device)
+    d_wte, d_wpe = (torch.zeros(n, H, device=gpu_device) for n in (V, L))
+    for i in range(0, B, 100):
+        rows = dz[i:i + 100].float()
+        d_wte.index_add_(0, ids[i:i + 100].reshape(-1), rows.view(-1, H))
+        d_wpe += rows.sum(0)
+    for g, w in zip(got, (d_wte, d_wpe)):
+        assert torch.equal(g, w.half())
+
+
+def test_two_streams_at_once(K, gpu_device):
+    r = np.random.default_rng(22)
+    ids = [torch.from_numpy(texts(r, 40, 300, 1000)).to(gpu_device) for _ in range(2)]
+    dz = [torch.randn(40, 300, 256, device=gpu_device).half() for _ in range(2)]
+    alone = [grads(K, i, x, 1000, 300, gpu_device) for i, x in zip(ids, dz)]
+    torch.cuda.synchronize()
+    sides, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    for _ in range(3):
+        for n, side in enumerate(sides):
+            with torch.cuda.stream(side):
+                got[n].append(grads(K, ids[n], dz[n], 1000, 300, gpu_device))
+    torch.cuda.synchronize()
+    for n in range(2):
+        for one in got[n]:
+            assert all(torch.equal(a, b) for a, b in zip(one, alone[n]))
