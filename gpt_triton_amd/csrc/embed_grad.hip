@@ -7,7 +7,9 @@
 //   more, a stable radix sort of the tokens with their positions, a workgroup a tile of them, whose launches also write the zero rows and
 //   form the position table's sums; then runs of the sorted positions are summed, whoever has a token to itself writes its
 //   row, and what a token has in several runs is joined in a last launch.
-// Bound by memory: dz twice (once for each table), the tables' gradients once.
+// Bound by memory: dz twice (once for each table), the tables' gradients once.  us, 512 x 300 tokens, fp16, 768 wide (236 MB of dz, 77 MB of
+// zero rows and sums): 143, of which the positions' sums and the runs' 55 and 52 at 4.3 and 4.6 TB/s; with one token in all places 175.
+// 16 x 1024, fp32: 59; 2 x 64, one launch: 15, zero rows.
 #include "common.h"
 #include "launch.h"
 

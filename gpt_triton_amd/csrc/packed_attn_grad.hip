@@ -5,14 +5,24 @@
 // over the queries i >= j of all the heads that share a key head.  The weights are formed again from q, k and the
 // statistic that the forward pass keeps of each row, so nothing of the size of the scores goes to memory.
 //
-// Three launches: row sums (delta, and the largest rows of e and v); dk and dv, a workgroup for a block of keys, which walks
-// over the queries; dq, a workgroup for a block of queries, which walks over the keys.  So each sum is formed by one
-// workgroup in one order, without atomics, at the cost of forming w and u twice: 7 products instead of 5.
+// Launches: row sums (delta, and the largest rows of e and v); the walk of the keys (dk and dv: a workgroup has a block of keys and walks
+// over the queries) and the walk of the queries (dq: a block of queries, over the keys), up to d = 64 in one launch; and, where the heads over a
+// key head are divided among workgroups, their sums' join.  So each sum is formed by one workgroup in one order, without atomics, at the
+// cost of forming w and u twice: 7 products instead of 5.
 //
 // Both walks are one kernel: rows x in registers (k and v, or q and e), rows y that pass through LDS (q and e, or k and v).
 // The products are Y . X^T with v_mfma_f32_16x16x32_f16, whose result lane (c, g), c = lane % 16, g = lane / 16, has
 // row c of x and four rows of y; rows 4 g + r of the two 16-row blocks b of a group of 32 are y's rows 8 g + 4 b + r, so
 // that w and u, rounded to fp16, are the second operand of the sums over y as they stand.
+//
+// What bounds it: the matrix pipe and the vector pipe in turn.  us, the row sums and the walks, causal:
+//   25 heads of 64, 1 x 8192 tokens: 750 (7 products of L^2 d operations a head: 1000 TFLOP/s, where a large library product
+//     reaches 1212; MFMA 0.39 and VALU 0.45 busy at 2.2 GHz); two wavefronts a SIMD and two launches 840
+//   32 heads of 128 over 8, texts of 4096, 4095, 2049, 1933, 517 and 64: 1320 (910 TFLOP/s; the keys' walk with one wavefront a SIMD, whose steps overlap; without
+//     overlap 1550); eight narrower wavefronts for it 844 where it takes 834, tiles of 128 rows 949
+//   12 heads of 64, 48 texts of up to 1024, 7276 rows: 72
+// A backward pass with an infinity or a NaN among the output's gradients goes row by row where that reaches, 10 to 50 times as long
+// (12 heads of 64, 1 x 1024: 1400 us, 48 x 300: 560 for one of them, 2000 for nothing else): a step that a training loop skips.
 #include <type_traits>
 #include <utility>
 
