@@ -447,9 +447,9 @@ int gptmi_embed_backward(const int64_t* ids, const void* dz, void* d_wte, void* 
               workspace ? workspace_bytes : (size_t)0);
     return GPTMI_ERR_WORKSPACE;
   }
-  launch_embed_backward(ids, dz, d_wte, d_wpe, B * L, L, V, P, (int)H, Dropout{p, seed}, dtype == GPTMI_F16, workspace,
-                        (hipStream_t)stream);
-  return check_launch("embed_backward");
+  const int rc = launch_embed_backward(ids, dz, d_wte, d_wpe, B * L, L, V, P, (int)H, Dropout{p, seed}, dtype == GPTMI_F16,
+                                       workspace, (hipStream_t)stream);
+  return rc ? rc : check_launch("embed_backward");
 }
 
 size_t gptmi_clip_grad_norm_workspace_bytes(int64_t n) { return n > 0 && n <= kMaxGradients ? clip_grad_bytes(n) : 0; }

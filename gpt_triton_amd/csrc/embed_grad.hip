@@ -4,12 +4,12 @@
 // The sums are formed in fp32, each in one order, in the order of the positions and without atomics, so the same call
 // gives the same bits.  That takes each token's positions one behind the other:
 //   up to 256 tokens, one launch: every workgroup has a range of the vocabulary and looks all tokens through;
-//   more, a stable radix sort of the tokens with their positions, a workgroup a tile of them, whose launches also write the zero rows and
-//   form the position table's sums; then runs of the sorted positions are summed, whoever has a token to itself writes its
-//   row, and what a token has in several runs is joined in a last launch.
+//   more, a stable radix sort of the tokens with their positions, by one workgroup up to 16384 tokens, else a workgroup a tile of them, whose launches
+//   also write the zero rows and form the position table's sums; then runs of the sorted positions are summed, whoever has a
+//   token to itself writes its row, and what a token has in several runs is joined in a last launch.
 // Bound by memory: dz twice (once for each table), the tables' gradients once.  us, 512 x 300 tokens, fp16, 768 wide (236 MB of dz, 77 MB of
 // zero rows and sums): 143, of which the positions' sums and the runs' 55 and 52 at 4.3 and 4.6 TB/s; with one token in all places 175.
-// 16 x 1024, fp32: 59; 2 x 64, one launch: 15, zero rows.
+// 16 x 1024, fp32: 57; 2 x 64, one launch: 15, zero rows.
 #include "common.h"
 #include "launch.h"
 
@@ -18,8 +18,12 @@ namespace {
 
 constexpr int kFew = 256;          // tokens of the single launch
 constexpr int kTile = 4096;        // tokens a workgroup sorts
+// Tokens that one workgroup sorts alone, in registers and 131 KB of LDS, beside the zero rows.  us, kernels / calls, this and by
+// tiles: 16 x 1024 tokens, 768 wide, fp32 57 / 63 and 60 / 71; 8 x 2000, 64 wide, fp16 49 / 63 and 48 / 70.
+constexpr int kOneTile = 16384;
 constexpr int kSortThreads = 1024;
 constexpr int kMaxBits = 9;        // of a digit
+constexpr int kFill = 65536;       // bytes of zero rows a workgroup
 
 // VN elements of a row: 16 bytes, or one element where a row or an address is no multiple of that.
 template <typename T, int VN>
@@ -61,7 +65,9 @@ struct EmbedGradArgs {
   // the sort's
   int tiles, bits;          // workgroups, bits of a digit
   int lanes, across, share;  // of the position table's parts: chunks each, parts a row, groups that share a batch
-  int64_t fill, fills;      // other work of a launch: from which 64 KB on, and how many of them; positions behind
+  // other work of a launch: workgroups of positions, and behind them zero rows, from which 64 KB on, the token table's first
+  int64_t positions, fill, table_fills;
+  int64_t behind;           // elements of the position table behind the first P rows, zeros
   unsigned *keys[2], *at[2];  // tokens (V: none) and positions
   unsigned* hist;           // [tiles][1 << bits]
   // the sums'
@@ -224,18 +230,20 @@ __global__ __launch_bounds__(256) void embed_grad_few_kernel(EmbedGradArgs a, in
 constexpr int kWaves = kSortThreads / kWave, kEach = kTile / kSortThreads;
 struct SortLds {
   unsigned counts[kWaves][1 << kMaxBits];
-  unsigned base[1 << kMaxBits];
   unsigned sums[kWaves];
 };
 
 // Lanes of the wavefront with the same digit.
 __device__ __forceinline__ uint64_t same_digit(unsigned digit, int bits, bool valid) {
-  uint64_t same = __ballot(valid);
+  const uint64_t all = __ballot(valid);
+  unsigned low = (unsigned)all, high = (unsigned)(all >> 32);
   for (int b = 0; b < bits; ++b) {
-    const uint64_t ones = __ballot(digit >> b & 1);
-    same &= digit >> b & 1 ? ones : ~ones;
+    const int set = (int)(digit << (31 - b)) >> 31;  // all ones or none
+    const uint64_t ones = __ballot(set < 0);
+    low &= ~((unsigned)ones ^ (unsigned)set);
+    high &= ~((unsigned)(ones >> 32) ^ (unsigned)set);
   }
-  return same;
+  return (uint64_t)high << 32 | low;
 }
 
 __device__ __forceinline__ unsigned key_of(const EmbedGradArgs& a, int64_t i) {
@@ -247,29 +255,35 @@ __device__ __forceinline__ unsigned key_of(const EmbedGradArgs& a, int64_t i) {
 // table's.  Every launch of the sort has a part of each, in workgroups behind its own.
 template <typename T, int VN>
 __device__ __forceinline__ void other_work(const EmbedGradArgs& a, int64_t item, float* lds) {
-  if (item >= a.fills) {
-    position_parts<T, VN, kSortThreads>(a, item - a.fills, lds);
+  if (item < a.positions) {
+    position_parts<T, VN, kSortThreads>(a, item, lds);
     return;
   }
-  item += a.fill;
-  const int64_t elements = a.V * (int64_t)a.H;
-  constexpr int64_t PER = 65536 / sizeof(T);
+  item += a.fill - a.positions;
+  T* table = (T*)a.d_wte;
+  int64_t elements = a.V * (int64_t)a.H;
+  if (item >= a.table_fills) {
+    item -= a.table_fills;
+    table = (T*)a.d_wpe + a.P * a.H;
+    elements = a.behind;
+  }
+  constexpr int64_t PER = kFill / sizeof(T);
   const int64_t first = item * PER, last = min(first + PER, elements);
   float none[VN];
   clear(none);
-  for (int64_t i = first + threadIdx.x * VN; i < last; i += kSortThreads * VN) put_chunk<T, VN>((T*)a.d_wte + i, none);
+  for (int64_t i = first + threadIdx.x * VN; i < last; i += kSortThreads * VN) put_chunk<T, VN>(table + i, none);
 }
 
-// Where this thread's tokens go by one digit: wavefront w has tokens 64 kEach w .. of the tile, 64 at a time.  place_of: the
+// Where this thread's tokens go by one digit: wavefront w has tokens 64 EACH w .. of the tile, 64 at a time.  place_of: the
 // first place of each digit for this tile, by the threads of the digits.
-template <typename F>
-__device__ __forceinline__ void rank_tile(SortLds& lds, int count, int bits, int shift, const unsigned (&key)[kEach],
-                                          unsigned (&place)[kEach], F place_of) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, digits = 1 << bits, base = wave * (kWave * kEach);
+template <int EACH, typename F>
+__device__ __forceinline__ void rank_tile(SortLds& lds, int count, int bits, int shift, const unsigned (&key)[EACH],
+                                          unsigned (&place)[EACH], F place_of) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, digits = 1 << bits, base = wave * (kWave * EACH);
   for (int i = tid; i < kWaves << bits; i += kSortThreads) lds.counts[i >> bits][i & (digits - 1)] = 0;
   __syncthreads();
 #pragma unroll
-  for (int j = 0; j < kEach; ++j) {
+  for (int j = 0; j < EACH; ++j) {
     const bool valid = base + j * kWave + lane < count;
     const unsigned digit = key[j] >> shift & (digits - 1);
     const uint64_t same = same_digit(digit, bits, valid);
@@ -305,25 +319,31 @@ __device__ __forceinline__ void rank_tile(SortLds& lds, int count, int bits, int
   }
   __syncthreads();
 #pragma unroll
-  for (int j = 0; j < kEach; ++j) place[j] += lds.counts[wave][key[j] >> shift & (digits - 1)];
+  for (int j = 0; j < EACH; ++j) place[j] += lds.counts[wave][key[j] >> shift & (digits - 1)];
 }
 
-// A single tile: all digits in one workgroup.
-template <typename T, int VN>
-__global__ __launch_bounds__(kSortThreads) void embed_grad_sort_kernel(EmbedGradArgs a, int passes) {
-  __shared__ union {
+// A single tile: all digits in one workgroup, EACH tokens a thread.
+template <typename T, int VN, int EACH>
+struct TileLds {
+  union {
     SortLds s;
     float other[kSortThreads * VN];
-  } lds;
-  __shared__ unsigned keys[kTile], at[kTile];
+  };
+  unsigned keys[kSortThreads * EACH];
+  uint16_t at[kSortThreads * EACH];
+};
+template <typename T, int VN, int EACH>
+__global__ __launch_bounds__(kSortThreads) void embed_grad_sort_kernel(EmbedGradArgs a, int passes) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  TileLds<T, VN, EACH>& lds = *reinterpret_cast<TileLds<T, VN, EACH>*>(smem);
   if (blockIdx.x > 0) {
     other_work<T, VN>(a, blockIdx.x - 1, lds.other);
     return;
   }
-  const int count = (int)a.tokens, base = (threadIdx.x >> 6) * (kWave * kEach) + (threadIdx.x & 63);
-  unsigned key[kEach], from[kEach], place[kEach];
+  const int count = (int)a.tokens, base = (threadIdx.x >> 6) * (kWave * EACH) + (threadIdx.x & 63);
+  unsigned key[EACH], from[EACH], place[EACH];
 #pragma unroll
-  for (int j = 0; j < kEach; ++j) {
+  for (int j = 0; j < EACH; ++j) {
     const int i = base + j * kWave;
     key[j] = i < count ? key_of(a, i) : 0;
     from[j] = (unsigned)i;
@@ -331,22 +351,22 @@ __global__ __launch_bounds__(kSortThreads) void embed_grad_sort_kernel(EmbedGrad
   for (int pass = 0; pass < passes; ++pass) {
     rank_tile(lds.s, count, a.bits, pass * a.bits, key, place, [](unsigned mine, unsigned*) { return mine; });
 #pragma unroll
-    for (int j = 0; j < kEach; ++j)
+    for (int j = 0; j < EACH; ++j)
       if (base + j * kWave < count) {
-        keys[place[j]] = key[j];
-        at[place[j]] = from[j];
+        lds.keys[place[j]] = key[j];
+        lds.at[place[j]] = (uint16_t)from[j];
       }
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) {
+    for (int j = 0; j < EACH; ++j) {
       const int i = base + j * kWave;
-      key[j] = i < count ? keys[i] : 0;
-      from[j] = i < count ? at[i] : 0;
+      key[j] = i < count ? lds.keys[i] : 0;
+      from[j] = i < count ? lds.at[i] : 0;
     }
     __syncthreads();
   }
 #pragma unroll
-  for (int j = 0; j < kEach; ++j) {
+  for (int j = 0; j < EACH; ++j) {
     const int i = base + j * kWave;
     if (i < count) {
       a.keys[0][i] = key[j];
@@ -548,16 +568,37 @@ __global__ __launch_bounds__(kSortThreads) void embed_grad_positions_kernel(Embe
   position_parts<T, VN, kSortThreads>(a, blockIdx.x, lds);
 }
 
+template <typename T, int VN, int EACH>
+int launch_sort(const EmbedGradArgs& a, unsigned blocks, int passes, hipStream_t st) {
+  const auto kernel = embed_grad_sort_kernel<T, VN, EACH>;
+  constexpr int lds = sizeof(TileLds<T, VN, EACH>);
+  static bool attr_done = false;  // idempotent; a race only repeats the call
+  if (!attr_done) {
+    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e != hipSuccess) {
+      set_error("hipFuncSetAttribute(%d bytes LDS): %s", lds, hipGetErrorString(e));
+      return -4;
+    }
+    attr_done = true;
+  }
+  hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kSortThreads), lds, st, a, passes);
+  return 0;
+}
+
 int run_of(int64_t tokens) { return tokens >= 1 << 17 ? 128 : tokens >= 1 << 15 ? 64 : 32; }
 
 template <typename T, int VN>
-void launch_as(EmbedGradArgs a, hipStream_t st) {
+int launch_as(EmbedGradArgs a, hipStream_t st) {
   const int chunks = a.H / VN;
   // The batch of a row of the position table is shared, by groups that are narrower then, where the rows alone would be few threads
-  // (us, 583 x 11 tokens, 1280 wide, fp32: 126 as whole rows, 94 shared by 16 groups; 512 x 300 fp16, 768 wide, of which the
-  // launch with them: 57 by 8, 63 by 16).
+  // (us, 583 x 11 tokens, 1280 wide, fp32: 126 as whole rows, 102 shared by 16 groups, 77 with the zero rows behind them filled as the
+  // token table's are; 512 x 300 fp16, 768 wide, of which the launch with them: 57 by 8, 63 by 16).
   const int threads = a.d_wte && a.tokens <= kFew ? 256 : kSortThreads;
   int64_t positions = 0;  // workgroups
+  if (a.d_wte && a.tokens > kFew) {  // rows of the position table that no token has are zero rows as the others
+    a.behind = a.d_wpe ? (a.P - a.L) * a.H : 0;
+    a.P = a.L;
+  }
   const auto share_by = [&](int share) {
     a.share = share;
     a.lanes = lanes_of(chunks, threads / share);
@@ -570,7 +611,7 @@ void launch_as(EmbedGradArgs a, hipStream_t st) {
     share_by(2 * a.share);
   if (!a.d_wte) {
     hipLaunchKernelGGL((embed_grad_positions_kernel<T, VN>), dim3((unsigned)positions), dim3(kSortThreads), 0, st, a);
-    return;
+    return 0;
   }
   if (a.tokens <= kFew) {
     // up to 64 rows a workgroup, fewer where that leaves CUs without one
@@ -579,28 +620,35 @@ void launch_as(EmbedGradArgs a, hipStream_t st) {
     const int64_t blocks = (a.V + rows - 1) / rows;
     hipLaunchKernelGGL((embed_grad_few_kernel<T, VN>), dim3((unsigned)(blocks + positions)), dim3(256), 0, st, a, rows,
                        (int)blocks);
-    return;
+    return 0;
   }
   int width = 1;
   while (a.V >> width) ++width;  // bits of V, the key of no token
   const int passes = (width + kMaxBits - 1) / kMaxBits;
   a.bits = (width + passes - 1) / passes;
   a.tiles = (int)((a.tokens + kTile - 1) / kTile);
-  const int64_t fills = (a.V * a.H * (int64_t)sizeof(T) + 65535) / 65536;
-  if (a.tiles == 1) {
-    a.fills = fills;
-    hipLaunchKernelGGL((embed_grad_sort_kernel<T, VN>), dim3((unsigned)(1 + fills + positions)), dim3(kSortThreads), 0, st, a, passes);
+  const auto fills_of = [](int64_t elements) { return (elements * (int64_t)sizeof(T) + kFill - 1) / kFill; };
+  a.table_fills = fills_of(a.V * a.H);
+  const int64_t fills = a.table_fills + fills_of(a.behind);
+  if (a.tokens <= kOneTile) {
+    a.positions = positions;
+    const unsigned blocks = (unsigned)(1 + fills + positions);
+    const int rc = a.tokens <= kTile ? launch_sort<T, VN, kEach>(a, blocks, passes, st)
+                                     : launch_sort<T, VN, kOneTile / kSortThreads>(a, blocks, passes, st);
+    if (rc) return rc;
     a.sorted = a.keys[0];
     a.order = a.at[0];
   } else {
     // The last launch has the position table's rows, few and long ones; a launch that counts takes about half as long as one
     // that moves, so the others divide the zero rows in thirds a pass.  us, 512 x 300 tokens fp16, the sort's launches with all
     // zero rows in the first and the positions in the second / all divided / this: 91 / 102 / 84.
+    int64_t end = 0;
     const auto part = [&](int third, int pass) {
       const int64_t in = 3 * pass + third, of = 3 * passes - 2;
-      a.fill += a.fills;
-      a.fills = fills * (in < of ? in : of) / of - a.fill;
-      return dim3((unsigned)(a.tiles + a.fills + (in > of ? positions : 0)));
+      a.fill = end;
+      end = fills * (in < of ? in : of) / of;
+      a.positions = in > of ? positions : 0;
+      return dim3((unsigned)(a.tiles + a.positions + end - a.fill));
     };
     for (int pass = 0; pass < passes; ++pass) {
       const int shift = pass * a.bits, from = pass & 1;
@@ -624,6 +672,7 @@ void launch_as(EmbedGradArgs a, hipStream_t st) {
   hipLaunchKernelGGL((embed_grad_sum_kernel<T, VN>), dim3((unsigned)((runs + groups - 1) / groups), across), dim3(256), 0, st, a);
   if (runs > 1)
     hipLaunchKernelGGL((embed_grad_join_kernel<T, VN>), dim3((unsigned)(runs - 1), across), dim3(256), 0, st, a);
+  return 0;
 }
 
 int64_t up(int64_t bytes) { return (bytes + 255) & ~(int64_t)255; }
@@ -636,8 +685,8 @@ size_t embed_grad_bytes(int64_t tokens, int64_t H) {
   return (size_t)(4 * up(tokens * 4) + up(tiles * (4 << kMaxBits)) + up(runs * 2 * H * 4));
 }
 
-void launch_embed_backward(const int64_t* ids, const void* dz, void* d_wte, void* d_wpe, int64_t tokens, int64_t L, int64_t V,
-                           int64_t P, int H, Dropout drop, bool f16, void* workspace, hipStream_t st) {
+int launch_embed_backward(const int64_t* ids, const void* dz, void* d_wte, void* d_wpe, int64_t tokens, int64_t L, int64_t V,
+                          int64_t P, int H, Dropout drop, bool f16, void* workspace, hipStream_t st) {
   EmbedGradArgs a = {};
   a.ids = ids;
   a.dz = dz;
@@ -654,13 +703,8 @@ void launch_embed_backward(const int64_t* ids, const void* dz, void* d_wte, void
   a.hist = (unsigned*)(ws + 4 * up(tokens * 4));
   a.parts = (float*)((char*)a.hist + up((tokens + kTile - 1) / kTile * (4 << kMaxBits)));
   const uintptr_t all = (uintptr_t)dz | (uintptr_t)d_wte | (uintptr_t)d_wpe;
-  if (f16) {
-    if (H % 8 == 0 && (all & 15) == 0) launch_as<_Float16, 8>(a, st);
-    else launch_as<_Float16, 1>(a, st);
-  } else {
-    if (H % 4 == 0 && (all & 15) == 0) launch_as<float, 4>(a, st);
-    else launch_as<float, 1>(a, st);
-  }
+  if (f16) return H % 8 == 0 && (all & 15) == 0 ? launch_as<_Float16, 8>(a, st) : launch_as<_Float16, 1>(a, st);
+  return H % 4 == 0 && (all & 15) == 0 ? launch_as<float, 4>(a, st) : launch_as<float, 1>(a, st);
 }
 
 }  // namespace gptmi

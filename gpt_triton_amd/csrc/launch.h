@@ -23,8 +23,8 @@ int launch_embed(const int64_t* ids, const void* wte, const void* wpe, void* out
 // Gradients of the embedding's tables (embed_grad.hip); one of them may be nullptr.  workspace: embed_grad_bytes, 256-byte
 // aligned.
 size_t embed_grad_bytes(int64_t tokens, int64_t H);
-void launch_embed_backward(const int64_t* ids, const void* dz, void* d_wte, void* d_wpe, int64_t tokens, int64_t L, int64_t V,
-                           int64_t P, int H, Dropout drop, bool f16, void* workspace, hipStream_t st);
+int launch_embed_backward(const int64_t* ids, const void* dz, void* d_wte, void* d_wpe, int64_t tokens, int64_t L, int64_t V,
+                          int64_t P, int H, Dropout drop, bool f16, void* workspace, hipStream_t st);
 bool launch_embed_layernorm(const int64_t* ids, const void* wte, const void* wpe, const void* w,
                             const void* b, void* emb, void* out, int64_t rows, int64_t L,
                             int64_t V, int H, float eps, bool f16, hipStream_t st);

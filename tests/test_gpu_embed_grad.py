@@ -273,3 +273,17 @@ def test_two_streams_at_once(K, gpu_device):
     for n in range(2):
         for one in got[n]:
             assert all(torch.equal(a, b) for a, b in zip(one, alone[n]))
+
+
+@pytest.mark.parametrize("B,L,more", [(4097, 1, 0), (1, 4097, 1), (5461, 3, 1000), (8, 2048, 0), (16385, 1, 70), (2, 150, 3000)])
+@pytest.mark.parametrize("V,H", [(50257, 40), (600, 33), (1 << 18, 8)])
+def test_where_the_sort_changes(K, gpu_device, B, L, more, V, H):
+    """A workgroup that sorts all tokens, of 4 or of 16 a thread, and tiles of them; rows of the position table that no token
+    has are zeros, whole blocks of them and parts."""
+    for dtype in DTYPES:
+        exact(K, gpu_device, B, L, V, L + more, H, dtype)
+
+
+def test_one_token_in_a_large_tile(K, gpu_device):
+    for n in (4098, 16384):
+        exact(K, gpu_device, n // 2, 2, 1000, 2, 24, torch.float32, ids=np.full((n // 2, 2), 999))
