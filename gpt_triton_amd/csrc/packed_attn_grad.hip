@@ -278,8 +278,9 @@ __device__ __forceinline__ void walk(const GradArgs& a, int id, int slots, bool 
 
   // ---- the factor that keeps u in fp16's range: one for all rows where rows are summed over, each row's own otherwise
   float most_e = 0.f, most_v = 0.f;
-  for (int i = lane; i < a.mosts; i += kWave) {
-    const float2 m = a.most[i];
+#pragma unroll
+  for (int i = 0; i < kSums; i += kWave) {  // those that are not there repeat the last one
+    const float2 m = a.most[min(i + lane, a.mosts - 1)];
     most_e = fmaxf(most_e, m.x);
     most_v = fmaxf(most_v, m.y);
   }
