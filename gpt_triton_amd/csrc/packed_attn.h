@@ -24,6 +24,17 @@ __device__ __forceinline__ void load_lds16(const void* base, unsigned lane_off, 
                : "memory", "m0");
 }
 
+// Lane (c, g) has columns 4 g + 0..3 of two blocks of 16 columns of row c.  Rows of lanes exchange halves, so that a lane stores 16
+// bytes and four lanes 64 side by side, not 32 (us, gradients of 48 x 300 tokens, 12 heads of 64: 72, else 77).
+__device__ __forceinline__ void store_blocks(_Float16* at, int g, h4 first, h4 second, bool there) {
+  typedef unsigned u2 __attribute__((ext_vector_type(2)));
+  typedef unsigned u4 __attribute__((ext_vector_type(4)));
+  const u2 p = __builtin_bit_cast(u2, first), q = __builtin_bit_cast(u2, second);
+  const auto low = __builtin_amdgcn_permlane16_swap(p[0], q[0], false, false);
+  const auto high = __builtin_amdgcn_permlane16_swap(p[1], q[1], false, false);
+  if (there) *reinterpret_cast<u4*>(at + 16 * (g & 1) + 8 * (g >> 1)) = u4{low[0], high[0], low[1], high[1]};
+}
+
 // Slots: sequence s, which starts at row a, has its blocks of R queries from slot a / R + s on, which leaves room for
 // every sequence whatever the lengths are (floor(a / R) + floor(len / R) <= floor((a + len) / R)), needs no
 // lengths on the host and no pass over them on the GPU.  Slots that are left over hold nothing.

@@ -393,13 +393,19 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
       }
     }
     if (STATS && g == 0 && q < L) a.stats[head * a.rows + block.first + q] = stat;
-    _Float16* o = a.out + ((block.first + q) * a.heads + head) * D + 4 * g;
-#pragma unroll
-    for (int i = 0; i < DB; ++i) {
+    _Float16* o = a.out + ((block.first + q) * a.heads + head) * D;
+    const auto rounded = [&](int i) {
       h4 x;
 #pragma unroll
       for (int r = 0; r < 4; ++r) x[r] = (_Float16)bounded(oacc[n][i][r]);
-      if (q < L) *reinterpret_cast<h4*>(o + 16 * i) = x;
+      return x;
+    };
+    if constexpr (DB == 1) {
+      const h4 x = rounded(0);
+      if (q < L) *reinterpret_cast<h4*>(o + 4 * g) = x;
+    } else {
+#pragma unroll
+      for (int i = 0; i < DB; i += 2) store_blocks(o + 16 * i, g, rounded(i), rounded(i + 1), q < L);
     }
   }
 }

@@ -20,7 +20,8 @@
 //     reaches 1212; MFMA 0.39 and VALU 0.45 busy at 2.2 GHz); two wavefronts a SIMD and two launches 840
 //   32 heads of 128 over 8, texts of 4096, 4095, 2049, 1933, 517 and 64: 1320 (910 TFLOP/s; the keys' walk with one wavefront a SIMD, whose steps overlap; without
 //     overlap 1550); eight narrower wavefronts for it 844 where it takes 834, tiles of 128 rows 949
-//   12 heads of 64, 48 texts of up to 1024, 7276 rows: 72
+//   12 heads of 64, 48 texts of up to 1024, 7276 rows: 68, 48 x 300: 85, of which the row sums 14, workgroups' starts and finding their rows
+//     10, loads in front of the walks 17, the walks 34, the results 10
 // A backward pass with an infinity or a NaN among the output's gradients goes row by row where that reaches, 10 to 50 times as long
 // (12 heads of 64, 1 x 1024: 1400 us, 48 x 300: 560 for one of them, 2000 for nothing else): a step that a training loop skips.
 #include <type_traits>
@@ -562,14 +563,15 @@ __device__ __forceinline__ void walk(const GradArgs& a, int id, int slots, bool 
   for (int n = 0; n < NB; ++n) {
     const int x = xw0 + 16 * n + c;
     const float f = KEYS ? factor[0] : factor[n], by_a = a.scale * ldexpf(1.f, -kUp) / f, by_b = ldexpf(1.f, -kUp);
-    float none = 0.f;
+    f4 nones = f4(0.f);
 #pragma unroll
     for (int i = 0; i < DB; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        none = fmaf(sa[n][i][r], 0.f, none);
-        if constexpr (KEYS) none = fmaf(sb[n][i][r], 0.f, none);
+        nones[r] = fmaf(sa[n][i][r], 0.f, nones[r]);
+        if constexpr (KEYS) nones[r] = fmaf(sb[n][i][r], 0.f, nones[r]);
       }
+    const float none = (nones[0] + nones[1]) + (nones[2] + nones[3]);
     const int64_t row = block.first + x;
     const int64_t place_a = KEYS ? (row * a.kv_heads + kv_head) * D : (row * a.heads + head0) * D;
     // four numbers of the results, or of this walk's part of them
@@ -585,10 +587,21 @@ __device__ __forceinline__ void walk(const GradArgs& a, int id, int slots, bool 
       if constexpr (KEYS) *reinterpret_cast<h4*>(a.dv + place_a + at) = __builtin_convertvector(rb, h4);
     };
     if (!__any(none != 0.f && x < L)) {
+      if (DB == 1 || (KEYS && a.shares > 1)) {
 #pragma unroll
-      for (int i = 0; i < DB; ++i) {
-        if constexpr (KEYS) store(16 * i + 4 * g, sa[n][i] * by_a, sb[n][i] * by_b);
-        else store(16 * i + 4 * g, sa[n][i] * by_a, f4(0.f));
+        for (int i = 0; i < DB; ++i) {
+          if constexpr (KEYS) store(16 * i + 4 * g, sa[n][i] * by_a, sb[n][i] * by_b);
+          else store(16 * i + 4 * g, sa[n][i] * by_a, f4(0.f));
+        }
+        continue;
+      }
+#pragma unroll
+      for (int i = 0; i + 1 < DB; i += 2) {
+        store_blocks((KEYS ? a.dk : a.dq) + place_a + 16 * i, g, __builtin_convertvector(sa[n][i] * by_a, h4),
+                     __builtin_convertvector(sa[n][i + 1] * by_a, h4), x < L);
+        if constexpr (KEYS)
+          store_blocks(a.dv + place_a + 16 * i, g, __builtin_convertvector(sb[n][i] * by_b, h4),
+                       __builtin_convertvector(sb[n][i + 1] * by_b, h4), x < L);
       }
       continue;
     }
@@ -740,11 +753,12 @@ int launch_d(GradArgs a, hipStream_t st) {
   a.mosts = (int)(items < kSums ? items : kSums);
   if (!deal_slots<NB>(a, a.heads, &a.deal[0]) || !deal_slots<NB>(a, a.kv_heads * a.shares, &a.deal[1])) return -2;
   hipLaunchKernelGGL((packed_sums_kernel<D>), dim3(a.mosts), dim3(256), 0, st, a);
-  static bool done[3];
+  static bool done[2];
   int rc = 0;
-  if (D <= 64 && a.dk && a.dq) {
-    if constexpr (D <= 64)
-      rc = launch(packed_grads_kernel<D, NB>, a, (int64_t)a.deal[0].grid + a.deal[1].grid, lds_of(D, true), &done[2], st);
+  if constexpr (D <= 64) {
+    if (!a.dq) a.deal[0].grid = 0;
+    if (!a.dk) a.deal[1].grid = 0;
+    rc = launch(packed_grads_kernel<D, NB>, a, (int64_t)a.deal[0].grid + a.deal[1].grid, lds_of(D, true), &done[0], st);
   } else {
     if (a.dk) rc = launch(packed_grad_kernel<D, NB, true>, a, a.deal[1].grid, lds_of(D, true), &done[1], st);
     if (a.dq && !rc) rc = launch(packed_grad_kernel<D, NB, false>, a, a.deal[0].grid, lds_of(D, false), &done[0], st);
