@@ -16,9 +16,9 @@
 // that w and u, rounded to fp16, are the second operand of the sums over y as they stand.
 //
 // What bounds it: the matrix pipe and the vector pipe in turn.  us, the row sums and the walks, causal:
-//   25 heads of 64, 1 x 8192 tokens: 750 (7 products of L^2 d operations a head: 1000 TFLOP/s, where a large library product
+//   25 heads of 64, 1 x 8192 tokens: 740 (7 products of L^2 d operations a head: 1015 TFLOP/s, where a large library product
 //     reaches 1212; MFMA 0.39 and VALU 0.45 busy at 2.2 GHz); two wavefronts a SIMD and two launches 840
-//   32 heads of 128 over 8, texts of 4096, 4095, 2049, 1933, 517 and 64: 1320 (910 TFLOP/s; the keys' walk with one wavefront a SIMD, whose steps overlap; without
+//   32 heads of 128 over 8, texts of 4096, 4095, 2049, 1933, 517 and 64: 1310 (915 TFLOP/s; the keys' walk with one wavefront a SIMD, whose steps overlap; without
 //     overlap 1550); eight narrower wavefronts for it 844 where it takes 834, tiles of 128 rows 949
 //   12 heads of 64, 48 texts of up to 1024, 7276 rows: 68, 48 x 300: 85, of which the row sums 14, workgroups' starts and finding their rows
 //     10, loads in front of the walks 17, the walks 34, the results 10
