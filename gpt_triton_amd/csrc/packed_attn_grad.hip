@@ -5,7 +5,7 @@
 // over the queries i >= j of all the heads that share a key head.  The weights are formed again from q, k and the
 // statistic that the forward pass keeps of each row, so nothing of the size of the scores goes to memory.
 //
-// Launches: row sums (delta, and the largest rows of e and v); the walk of the keys (dk and dv: a workgroup has a block of keys and walks
+// Launches: row sums (delta, and the largest rows of e and v); delta of each sequence's first queries once more, as sums over keys; the walk of the keys (dk and dv: a workgroup has a block of keys and walks
 // over the queries) and the walk of the queries (dq: a block of queries, over the keys), up to d = 64 in one launch; and, where the heads over a
 // key head are divided among workgroups, their sums' join.  So each sum is formed by one workgroup in one order, without atomics, at the
 // cost of forming w and u twice: 7 products instead of 5.
@@ -148,6 +148,55 @@ __device__ __forceinline__ void load_lds4(const void* base, unsigned lane_off, u
 
 __device__ __forceinline__ h8 lds_read16(unsigned at) {
   return *(const __attribute__((address_space(3))) h8*)(uintptr_t)at;
+}
+
+// delta of a sequence's first 16 queries as the sum over their keys, a wavefront for a sequence and head.  There e . o is off by what
+// the output and the forward pass's weights were rounded by, which few keys do not average out: dq and dk of a text of 24 tokens are
+// 3.6e-4 off (2-norm, relative) with e . o, this way 3.1e-4, of which 2.1e-4 are the last rounding; single elements of long
+// texts' first rows 0.02 of the largest, this way 0.008.  3 us.
+template <int D>
+__global__ __launch_bounds__(256) void packed_first_kernel(GradArgs a) {
+  constexpr int KS = (D + 31) / 32;
+  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t items = (int64_t)a.sequences * a.heads;
+  for (int64_t item = (int64_t)blockIdx.x * 4 + wave; item < items; item += (int64_t)gridDim.x * 4) {
+    const int64_t sequence = item / a.heads;
+    const int head = (int)(item - sequence * a.heads), kv_head = head / (a.heads / a.kv_heads);
+    const int64_t begin = a.starts[sequence], end = a.starts[sequence + 1];
+    const int64_t first = begin < 0 ? 0 : begin < a.rows ? begin : a.rows;
+    const int64_t last = end < first ? first : end < a.rows ? end : a.rows;
+    if (last - first < 2) continue;
+    const int L = (int)min(last - first, (int64_t)16);
+    const int64_t row = first + min(c, L - 1);
+    const _Float16 *q = a.q + (row * a.q_row + head * a.q_head) + g * 8, *k = a.k + (row * a.k_row + kv_head * a.k_head) + g * 8;
+    const _Float16 *v = a.v + (row * a.v_row + kv_head * a.v_head) + g * 8, *e = a.d_out + (row * a.heads + head) * D + g * 8;
+    f4 s = f4(0.f), p = f4(0.f);  // of query c, keys 4 g + 0..3
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      h8 x[4] = {h8(0), h8(0), h8(0), h8(0)};
+      if (D >= 32 || g < 2) {
+        x[0] = *reinterpret_cast<const h8*>(k + ks * 32);
+        x[1] = *reinterpret_cast<const h8*>(q + ks * 32);
+        x[2] = *reinterpret_cast<const h8*>(v + ks * 32);
+        x[3] = *reinterpret_cast<const h8*>(e + ks * 32);
+      }
+      s = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[0], x[1], s, 0, 0, 0);
+      p = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[2], x[3], p, 0, 0, 0);
+    }
+    const int64_t place = head * a.rows + row;
+    const float lse = a.lse[place];
+    float sum = 0.f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float w = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale * 1.4426950408889634f, -lse));
+      sum = 4 * g + r <= c ? fmaf(w, p[r], sum) : sum;
+    }
+    const LanePair pair = row_swap(half_sum(sum));
+    sum = (pair.a + pair.b) * 0x1p-14f;
+    static_assert(kUp == 14, "of lse");
+    if (g == 0 && c < L && fabsf(sum) < INFINITY) a.minus_delta[place] = -sum;  // else a row that is marked, or none
+  }
 }
 
 // 2^n with 4 < 2^n bound <= 8 for bound = sqrt(ee vv), which |e . v| does not pass: |u| is at most bound / 2, since what
@@ -753,6 +802,8 @@ int launch_d(GradArgs a, hipStream_t st) {
   a.mosts = (int)(items < kSums ? items : kSums);
   if (!deal_slots<NB>(a, a.heads, &a.deal[0]) || !deal_slots<NB>(a, a.kv_heads * a.shares, &a.deal[1])) return -2;
   hipLaunchKernelGGL((packed_sums_kernel<D>), dim3(a.mosts), dim3(256), 0, st, a);
+  const int64_t firsts = ((int64_t)a.sequences * a.heads + 3) / 4;
+  hipLaunchKernelGGL((packed_first_kernel<D>), dim3((unsigned)(firsts < 1 << 16 ? firsts : 1 << 16)), dim3(256), 0, st, a);
   static bool done[2];
   int rc = 0;
   if constexpr (D <= 64) {

@@ -406,7 +406,7 @@ int gptmi_flash_attn_packed_train(const void* q, const void* k, const void* v, v
  *   and scale.  dq, or dk and dv, may be NULL.  The gradients overlap nothing.  Rows that belong to no sequence are not read
  *   and have gradients of 0.
  * w and u are formed again in fp32 and rounded to fp16 for the products, scaled by powers of two so that they stay normal
- * numbers.  What hidden rows hold, infinities and NaN included, plays no part.  workspace:
+ * numbers; delta of a sequence's first 16 queries is the sum over their keys, which the output's rounding does not reach.  What hidden rows hold, infinities and NaN included, plays no part.  workspace:
  * gptmi_flash_attn_packed_backward_workspace_bytes(...) of the same sizes, 256-byte aligned.  N d up to 2^24, here and in
  * gptmi_flash_attn_packed_train.
  * No counterpart in the reference, which has no gradients.

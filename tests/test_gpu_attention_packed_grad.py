@@ -35,8 +35,9 @@ def largest_norm(t):
     return float(n.max().sqrt()) if n.numel() else 0.0
 
 
-def want(q, k, v, e, scale, bound):
-    """((dq, dk, dv), their tolerances) of one sequence in 64 bits."""
+def want(q, k, v, e, scale, bound, summed=0):
+    """((dq, dk, dv), their tolerances) of one sequence in 64 bits.  summed: so many of the first queries' deltas are sums over
+    their keys, off by what their terms are and (summed + 16) u of the sizes'."""
     L, n, d = q.shape
     rep = n // k.shape[1]
     new = lambda like: torch.zeros(like.shape, dtype=torch.float64, device=q.device)
@@ -53,6 +54,8 @@ def want(q, k, v, e, scale, bound):
         p, p_size = mm(g, c.t()), mm(g.abs(), c.abs().t())
         delta = (g * out).sum(1, keepdim=True)
         t_delta = (g.abs() * t_out).sum(1, keepdim=True) + (d + 8) * U * (g * out).abs().sum(1, keepdim=True)
+        few = w * (E * p.abs() + (d + 8) * U * p_size) + (summed + 16) * U * (w * p).abs()
+        t_delta[:summed] = few.sum(1, keepdim=True)[:summed]
         x = w * (p - delta)
         t_w = torch.where(past, (H + E) * w + 2.0**-39, 0.0)
         t_x = torch.where(past, w * (E * (p - delta).abs() + (d + 8) * U * p_size + t_delta) + H * x.abs() + 2.0**-40 * bound, 0.0)
@@ -481,3 +484,37 @@ def test_what_is_changed_behind_the_forward_pass(K, gpu_device):
             (k, v, starts)[which].add_(0)
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             out.backward(e)
+
+
+@pytest.mark.parametrize("d", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("heads", [(12, 12), (8, 2), (7, 1)])
+def test_deltas_of_the_first_queries(K, gpu_device, d, heads):
+    """Of the first 16 queries what the output is rounded by plays no part."""
+    r = np.random.default_rng(23)
+    lengths = [16, 2, 3, 0, 9, 15, 1, 12, 5, 16]
+    q, k, v, e = make(r, sum(lengths) + 3, *heads, d, True, gpu_device)
+    starts = starts_of(lengths, gpu_device, 2)
+    _, *got = grads(K, q, k, v, e, starts)
+    bound, at = largest_norm(e) * largest_norm(v), 2
+    for L in lengths:
+        rows = slice(at, at + L)
+        at += L
+        if L:
+            w, tol = want(q[rows], k[rows], v[rows], e[rows], d**-0.5, bound, summed=16)
+            for name, x, y, t in zip("qkv", got, w, tol):
+                off = (x[rows].double() - y).abs()
+                assert torch.all(off <= t), (name, L, float((off / t).max()))
+
+
+def test_first_queries_of_many_sequences(K, gpu_device):
+    """More sequences and heads than wavefronts of the launch for the first queries."""
+    r = np.random.default_rng(24)
+    n, L = 10000, 3
+    q, k, v, e = make(r, n * L, 32, 4, 16, False, gpu_device)
+    _, *got = grads(K, q, k, v, e, starts_of([L] * n, gpu_device))
+    some = [0, 1, 8191, 8192, 9999]
+    for s in some:
+        rows = slice(s * L, s * L + L)
+        w, tol = want(q[rows], k[rows], v[rows], e[rows], 0.25, largest_norm(e) * largest_norm(v), summed=16)
+        for x, y, t in zip(got, w, tol):
+            assert torch.all((x[rows].double() - y).abs() <= t)
