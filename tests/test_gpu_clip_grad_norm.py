@@ -215,3 +215,24 @@ def test_captured(K, gpu_device):
         assert torch.equal(norm, K.clip_grad_norm_(grads, 1.0, scale=0.5, out=eager))
         assert all(torch.equal(a, b) for a, b in zip(out, eager))
         check(K, grads, 1.0, 0.5, eager)
+
+
+def test_nothing_to_clip(K, gpu_device):
+    """Empty tensors alone, also more than a launch takes, and zeros."""
+    empty = [torch.empty(0, 4, device=gpu_device, dtype=t) for t in (F32, F16) for _ in range(100)]
+    assert float(K.clip_grad_norm_(empty, 1.0)) == 0.0
+    zeros = [torch.zeros(5000, device=gpu_device)]
+    assert float(K.clip_grad_norm_(empty + zeros, 1.0, scale=3.0)) == 0.0 and not zeros[0].any()
+
+
+def test_out_in_place(K, gpu_device):
+    """A gradient itself as its result, beside others that have one of their own."""
+    grads = make([(300, 40), (7,), (20000,)], F32, gpu_device)
+    wanted = want([g.clone() for g in grads], 0.5, 0.25)[1]
+    kept = grads[1].clone()
+    out = [grads[0], torch.empty(7, device=gpu_device, dtype=F16), grads[2]]
+    K.clip_grad_norm_((g for g in grads), 0.5, scale=0.25, out=out)
+    assert torch.equal(kept, grads[1])
+    for o, w in zip(out, wanted):
+        half = o.dtype == F16
+        assert torch.all((o.double() - w).abs() <= (2.0**-22 + (2.0**-11 if half else 0.0)) * w.abs() + (2.0**-25 if half else 0.0))
