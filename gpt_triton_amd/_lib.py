@@ -63,6 +63,8 @@ SIGNATURES = {
                                 _u64, _int, _int, _vp]),
     "gptmi_flash_attn_packed": (_int, [_vp] * 5 + [_i64] * 11 + [_f32, _int, _vp]),
     "gptmi_flash_attn_packed_train": (_int, [_vp] * 6 + [_i64] * 11 + [_f32, _int, _vp]),
+    "gptmi_flash_attn_packed_train_remainder": (_int, [_vp] * 7 + [_i64] * 11 + [_f32, _int, _vp]),
+    "gptmi_flash_attn_packed_backward_remainder": (_int, [_vp] * 11 + [_i64] * 11 + [_f32, _vp, _sz, _int, _vp]),
     "gptmi_flash_attn_packed_backward_workspace_bytes": (_sz, [_i64] * 5),
     "gptmi_flash_attn_packed_backward": (_int, [_vp] * 10 + [_i64] * 11 + [_f32, _vp, _sz, _int, _vp]),
 }

@@ -931,23 +931,43 @@ int gptmi_flash_attn_packed(const void* q, const void* k, const void* v, void* o
                             int64_t q_head, int64_t k_row, int64_t k_head, int64_t v_row, int64_t v_head, float scale,
                             int dtype, void* stream) {
   return flash_attn_packed("flash_attn_packed",
-                           PackedAttention{q, k, v, out, nullptr, starts, sequences, T, N, G, q_row, q_head, k_row, k_head,
-                                           v_row, v_head, scale},
+                           PackedAttention{q, k, v, out, nullptr, nullptr, starts, sequences, T, N, G, q_row, q_head, k_row,
+                                           k_head, v_row, v_head, scale},
                            d, dtype, stream);
+}
+
+static int packed_train(const char* what, const PackedAttention& p, int64_t d, int dtype, void* stream) {
+  if (!p.stats || ((uintptr_t)p.stats & 7) != 0 || ((uintptr_t)p.remainder & 15) != 0) {
+    set_error("%s: invalid argument", what);
+    return GPTMI_ERR_INVALID;
+  }
+  return flash_attn_packed(what, p, d, dtype, stream);
 }
 
 int gptmi_flash_attn_packed_train(const void* q, const void* k, const void* v, void* out, float* stats,
                                   const int64_t* starts, int64_t sequences, int64_t T, int64_t N, int64_t G, int64_t d,
                                   int64_t q_row, int64_t q_head, int64_t k_row, int64_t k_head, int64_t v_row,
                                   int64_t v_head, float scale, int dtype, void* stream) {
-  if (!stats || ((uintptr_t)stats & 7) != 0) {
-    set_error("flash_attn_packed_train: invalid argument");
+  return packed_train("flash_attn_packed_train",
+                      PackedAttention{q, k, v, out, stats, nullptr, starts, sequences, T, N, G, q_row, q_head, k_row, k_head,
+                                      v_row, v_head, scale},
+                      d, dtype, stream);
+}
+
+int gptmi_flash_attn_packed_train_remainder(const void* q, const void* k, const void* v, void* out, float* stats,
+                                            void* remainder, const int64_t* starts, int64_t sequences, int64_t T, int64_t N,
+                                            int64_t G, int64_t d, int64_t q_row, int64_t q_head, int64_t k_row,
+                                            int64_t k_head, int64_t v_row, int64_t v_head, float scale, int dtype,
+                                            void* stream) {
+  const char* what = "flash_attn_packed_train_remainder";
+  if (!remainder) {
+    set_error("%s: invalid argument", what);
     return GPTMI_ERR_INVALID;
   }
-  return flash_attn_packed("flash_attn_packed_train",
-                           PackedAttention{q, k, v, out, stats, starts, sequences, T, N, G, q_row, q_head, k_row, k_head,
-                                           v_row, v_head, scale},
-                           d, dtype, stream);
+  return packed_train(what,
+                      PackedAttention{q, k, v, out, stats, remainder, starts, sequences, T, N, G, q_row, q_head, k_row, k_head,
+                                      v_row, v_head, scale},
+                      d, dtype, stream);
 }
 
 size_t gptmi_flash_attn_packed_backward_workspace_bytes(int64_t sequences, int64_t T, int64_t N, int64_t G, int64_t d) {
@@ -956,28 +976,52 @@ size_t gptmi_flash_attn_packed_backward_workspace_bytes(int64_t sequences, int64
   return ok ? packed_attn_grad_bytes(T, sequences, N, G, d) : 0;
 }
 
+static int packed_backward(const char* what, const PackedAttention& p, const PackedGradients& g, int64_t d, void* workspace,
+                           size_t workspace_bytes, int dtype, void* stream) {
+  if (!p.out || !p.stats || ((uintptr_t)p.stats & 7) != 0 || !g.d_out || (g.dk == nullptr) != (g.dv == nullptr) ||
+      (!g.dq && !g.dk)) {
+    set_error("%s: invalid argument", what);
+    return GPTMI_ERR_INVALID;
+  }
+  const uintptr_t all = (uintptr_t)p.out | (uintptr_t)p.remainder | (uintptr_t)g.d_out | (uintptr_t)g.dq | (uintptr_t)g.dk |
+                        (uintptr_t)g.dv;
+  int rc = check_packed_gradients(what, p, d, all, dtype);
+  if (rc) return rc;
+  const size_t needed = packed_attn_grad_bytes(p.rows, p.sequences, p.heads, p.kv_heads, d);
+  if (!workspace || workspace_bytes < needed || ((uintptr_t)workspace & 255) != 0) {
+    set_error("%s: workspace of %zu bytes needed, 256-byte aligned, %zu given", what, needed, workspace ? workspace_bytes : (size_t)0);
+    return GPTMI_ERR_WORKSPACE;
+  }
+  rc = launch_flash_attn_packed_backward(p, g, (int)d, workspace, (hipStream_t)stream);
+  return rc ? rc : check_launch(what);
+}
+
 int gptmi_flash_attn_packed_backward(const void* q, const void* k, const void* v, const void* out, const float* stats,
                                      const void* d_out, const int64_t* starts, void* dq, void* dk, void* dv,
                                      int64_t sequences, int64_t T, int64_t N, int64_t G, int64_t d, int64_t q_row,
                                      int64_t q_head, int64_t k_row, int64_t k_head, int64_t v_row, int64_t v_head,
                                      float scale, void* workspace, size_t workspace_bytes, int dtype, void* stream) {
-  const char* what = "flash_attn_packed_backward";
-  if (!out || !stats || ((uintptr_t)stats & 7) != 0 || !d_out || (dk == nullptr) != (dv == nullptr) || (!dq && !dk)) {
+  return packed_backward("flash_attn_packed_backward",
+                         PackedAttention{q, k, v, (void*)out, (void*)stats, nullptr, starts, sequences, T, N, G, q_row, q_head,
+                                         k_row, k_head, v_row, v_head, scale},
+                         PackedGradients{d_out, dq, dk, dv}, d, workspace, workspace_bytes, dtype, stream);
+}
+
+int gptmi_flash_attn_packed_backward_remainder(const void* q, const void* k, const void* v, const void* out,
+                                               const float* stats, const void* remainder, const void* d_out,
+                                               const int64_t* starts, void* dq, void* dk, void* dv, int64_t sequences,
+                                               int64_t T, int64_t N, int64_t G, int64_t d, int64_t q_row, int64_t q_head,
+                                               int64_t k_row, int64_t k_head, int64_t v_row, int64_t v_head, float scale,
+                                               void* workspace, size_t workspace_bytes, int dtype, void* stream) {
+  const char* what = "flash_attn_packed_backward_remainder";
+  if (!remainder) {
     set_error("%s: invalid argument", what);
     return GPTMI_ERR_INVALID;
   }
-  const PackedAttention p{q, k, v, (void*)out, (void*)stats, starts, sequences, T, N, G, q_row, q_head, k_row, k_head, v_row,
-                          v_head, scale};
-  int rc = check_packed_gradients(
-      what, p, d, (uintptr_t)out | (uintptr_t)d_out | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv, dtype);
-  if (rc) return rc;
-  const size_t needed = packed_attn_grad_bytes(T, sequences, N, G, d);
-  if (!workspace || workspace_bytes < needed || ((uintptr_t)workspace & 255) != 0) {
-    set_error("%s: workspace of %zu bytes needed, 256-byte aligned, %zu given", what, needed, workspace ? workspace_bytes : (size_t)0);
-    return GPTMI_ERR_WORKSPACE;
-  }
-  rc = launch_flash_attn_packed_backward(p, PackedGradients{d_out, dq, dk, dv}, (int)d, workspace, (hipStream_t)stream);
-  return rc ? rc : check_launch(what);
+  return packed_backward(what,
+                         PackedAttention{q, k, v, (void*)out, (void*)stats, (void*)remainder, starts, sequences, T, N, G,
+                                         q_row, q_head, k_row, k_head, v_row, v_head, scale},
+                         PackedGradients{d_out, dq, dk, dv}, d, workspace, workspace_bytes, dtype, stream);
 }
 
 size_t gptmi_dropout_mask_bytes(int64_t n) {

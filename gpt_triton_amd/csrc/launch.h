@@ -93,6 +93,7 @@ struct PackedAttention {
   const void *q, *k, *v;
   void* out;
   void* stats;  // float2 [heads][rows], what the gradients need of each row, or nullptr
+  void* remainder;  // fp16 [rows][heads][d], 2^10 times what the output's rounding takes, or nullptr
   const int64_t* starts;
   int64_t sequences, rows, heads, kv_heads;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;

@@ -24,6 +24,7 @@ struct PackedArgs {
   const _Float16 *q, *k, *v;
   _Float16* out;
   float2* stats;              // [heads][T], or nullptr: what the gradients need
+  _Float16* remainder;        // [T][heads][D], or nullptr: what the output's rounding takes, 2^10 times
   const int64_t* starts;
   int64_t rows;               // T
   int sequences, heads, kv_heads, slots, longest_first;
@@ -38,6 +39,19 @@ __device__ __forceinline__ float larger(float a, float b) { return __builtin_ele
 // than 1, and what is above 65519 would be an infinity.
 __device__ __forceinline__ float bounded(float x) {
   return fabsf(x) < INFINITY ? __builtin_amdgcn_fmed3f(x, -65504.f, 65504.f) : x;
+}
+
+// sum + the eight numbers of x, one behind the other, each addition one instruction that reads fp16.  us, the forward pass of
+// 1 x 8192 tokens in a training step, 25 heads of 64: 306; as a conversion and an addition 347, by matrix instructions with ones,
+// which cost registers, 328, without these sums and the remainder 278.
+__device__ __forceinline__ void add_halves(float& sum, h8 x) {
+  typedef unsigned u4 __attribute__((ext_vector_type(4)));
+  const u4 pairs = __builtin_bit_cast(u4, x);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    asm("v_fma_mix_f32 %0, %1, 1.0, %0 op_sel_hi:[1,0,0]" : "+v"(sum) : "v"(pairs[i]));
+    asm("v_fma_mix_f32 %0, %1, 1.0, %0 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "+v"(sum) : "v"(pairs[i]));
+  }
 }
 
 // STATS: with what the gradients need of each row (as a branch, 1 % of the others' time).
@@ -158,9 +172,9 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
   // flush subnormal weights / a column of ones in the matrix product, which costs registers: 48 of up to 1024 rows
   // 23.2 / 23.1 / 26.0, 1 x 16384 995 / 988 / 1003.) The key that set the reference weighs 2^6, so a denominator
   // below 2^5 is one whose base was rounded by more than the weights reach, which the end looks for.
-  float ref[QB], limit[QB], base[QB], den[QB];
+  float ref[QB], limit[QB], base[QB], den[QB], den_rounded[QB];  // the last: of the weights as the products have them, for STATS
 #pragma unroll
-  for (int n = 0; n < QB; ++n) ref[n] = limit[n] = base[n] = -INFINITY, den[n] = 0.f;
+  for (int n = 0; n < QB; ++n) ref[n] = limit[n] = base[n] = -INFINITY, den[n] = den_rounded[n] = 0.f;
   const float room = 8.0f / to_exp2;
 
   // One 64-key tile.  MASK: the one that the diagonal cuts, in which query x of the wavefront sees keys 0 .. edge + x;
@@ -214,6 +228,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
         limit[n] = to + room;
         base[n] = next;
         den[n] *= mult;
+        if constexpr (STATS) den_rounded[n] *= mult;
 #pragma unroll
         for (int i = 0; i < DB; ++i) oacc[n][i] *= mult;
       }
@@ -228,6 +243,12 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
           pf[n][kb >> 1][4 * (kb & 1) + r] = (_Float16)p;
           den[n] += p;
         }
+    if constexpr (STATS) {
+#pragma unroll
+      for (int n = 0; n < QB; ++n)
+#pragma unroll
+        for (int kg = 0; kg < KG; ++kg) add_halves(den_rounded[n], pf[n][kg]);
+    }
 #pragma unroll
     for (int n = 0; n < QB; ++n) asm volatile("" : "+v"(den[n]));  // here, not with copies of the weights behind the barrier
   };
@@ -306,7 +327,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
       for (int n = 0; n < QB; ++n) {
 #pragma unroll
         for (int i = 0; i < DB; ++i) sums[(n * (DB + 1) + i) * kWave] = oacc[n][i];
-        sums[(n * (DB + 1) + DB) * kWave] = f4{base[n], den[n], 0.f, 0.f};
+        sums[(n * (DB + 1) + DB) * kWave] = f4{base[n], den[n], den_rounded[n], 0.f};
       }
     }
     __syncthreads();
@@ -317,7 +338,10 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
       const float to = larger(base[n], other[0]);
       const float mine = __builtin_amdgcn_exp2f(base[n] - to), its = __builtin_amdgcn_exp2f(other[0] - to);
       den[n] = fmaf(den[n], mine, other[1] * its);
-      if constexpr (STATS) base[n] = to;
+      if constexpr (STATS) {
+        den_rounded[n] = fmaf(den_rounded[n], mine, other[2] * its);
+        base[n] = to;
+      }
 #pragma unroll
       for (int i = 0; i < DB; ++i) oacc[n][i] = oacc[n][i] * mine + sums[(n * (DB + 1) + i) * kWave] * its;
     }
@@ -342,6 +366,11 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
     // For the gradients: a weight is 2^(t s - x) y; or, y < 0, exp(score - x) -y of the scores key by key, where one rounded
     // base is not as good as an fp16 number.
     float2 stat = {base[n], inv};
+    float normed = 1.0f;  // by which the output's weights, as rounded, add to one
+    if constexpr (STATS) {
+      const LanePair rounded = row_swap(half_sum(den_rounded[n]));
+      normed = sum / (rounded.a + rounded.b);
+    }
     const bool again = __any(none != 0.f && q < L);
     if (again || (STATS && __any(!(fabsf(base[n]) < 8192.f) && q < L))) {
       const int last = min(qw0 + 16 * n + 15, L - 1);
@@ -372,6 +401,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
       const float inv_total = number ? 1.0f / total : NAN;
       stat = {m, -inv_total};
       if (again) {  // the output, too
+        normed = 1.0f;
 #pragma unroll
         for (int i = 0; i < DB; ++i) oacc[n][i] = f4(number ? 0.f : NAN);
       }
@@ -393,20 +423,35 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void packed_attn_kernel(Pack
       }
     }
     if (STATS && g == 0 && q < L) a.stats[head * a.rows + block.first + q] = stat;
-    _Float16* o = a.out + ((block.first + q) * a.heads + head) * D;
+    const int64_t place = ((block.first + q) * a.heads + head) * D;
     const auto rounded = [&](int i) {
       h4 x;
 #pragma unroll
       for (int r = 0; r < 4; ++r) x[r] = (_Float16)bounded(oacc[n][i][r]);
       return x;
     };
-    if constexpr (DB == 1) {
-      const h4 x = rounded(0);
-      if (q < L) *reinterpret_cast<h4*>(o + 4 * g) = x;
-    } else {
+    // What that takes from the output, and what the weights' rounding adds to their sum or takes from it, 2^10 times, no more
+    // than the output itself.  With it e . out is a mean of the e . v, so that an offset of the values is in it as it is in each e . v.
+    const auto taken = [&](int i) {
+      h4 x;
 #pragma unroll
-      for (int i = 0; i < DB; i += 2) store_blocks(o + 16 * i, g, rounded(i), rounded(i + 1), q < L);
-    }
+      for (int r = 0; r < 4; ++r) {
+        const float rest = (oacc[n][i][r] * normed - (float)(_Float16)bounded(oacc[n][i][r])) * 0x1p10f;
+        x[r] = (_Float16)(fabsf(rest) < 65504.f ? rest : 0.f);
+      }
+      return x;
+    };
+    const auto store = [&](_Float16* to, auto of) {
+      if constexpr (DB == 1) {
+        const h4 x = of(0);
+        if (q < L) *reinterpret_cast<h4*>(to + place + 4 * g) = x;
+      } else {
+#pragma unroll
+        for (int i = 0; i < DB; i += 2) store_blocks(to + place + 16 * i, g, of(i), of(i + 1), q < L);
+      }
+    };
+    store(a.out, rounded);
+    if (STATS && a.remainder) store(a.remainder, taken);
   }
 }
 
@@ -484,6 +529,7 @@ int launch_flash_attn_packed(const PackedAttention& p, int d, hipStream_t st) {
   a.v = (const _Float16*)p.v;
   a.out = (_Float16*)p.out;
   a.stats = (float2*)p.stats;
+  a.remainder = (_Float16*)p.remainder;
   a.starts = p.starts;
   a.rows = p.rows;
   a.sequences = (int)p.sequences;

@@ -5,10 +5,18 @@
 // over the queries i >= j of all the heads that share a key head.  The weights are formed again from q, k and the
 // statistic that the forward pass keeps of each row, so nothing of the size of the scores goes to memory.
 //
-// Launches: row sums (delta, and the largest rows of e and v); delta of each sequence's first queries once more, as sums over keys; the walk of the keys (dk and dv: a workgroup has a block of keys and walks
-// over the queries) and the walk of the queries (dq: a block of queries, over the keys), up to d = 64 in one launch; and, where the heads over a
-// key head are divided among workgroups, their sums' join.  So each sum is formed by one workgroup in one order, without atomics, at the
+// Launches: row sums (delta, and the largest rows of e and v); delta of each sequence's first queries as sums over their keys,
+// in place of the row sums'; the walk of the keys (dk and dv: a workgroup has a block of keys and walks over the queries) and the
+// walk of the queries (dq: a block of queries, over the keys), up to d = 64 in one launch; and, where the heads over a key head
+// are divided among workgroups, their sums' join.  So each sum is formed by one workgroup in one order, without atomics, at the
 // cost of forming w and u twice: 7 products instead of 5.
+//
+// u sums to 0 over a row's keys as far as delta is right: an error of delta is one of all of the row's u, and dq has it times
+// the mean of the keys.  So delta comes from the output and what its rounding takes, which the forward pass keeps: 2-norms of dq's
+// errors, 1 x 1024 tokens, 12 heads of 64, of which u's rounding has its part whatever delta is: 3.0e-4 for keys and
+// values of unit spread, 4.0e-4, 8.4e-4 and 2.7e-3 where their channels have offsets of 1, 3 and 10 as well; from the rounded output
+// 3.0e-4, 1.9e-3, 1.7e-2 and 0.19.  dk 2.9e-4 to 3.0e-4; 3.0e-4, 3.5e-4, 6.3e-4, 1.9e-3.  It costs 26 us of the forward pass of
+// 1 x 8192 tokens below and 3 of its row sums.
 //
 // Both walks are one kernel: rows x in registers (k and v, or q and e), rows y that pass through LDS (q and e, or k and v).
 // The products are Y . X^T with v_mfma_f32_16x16x32_f16, whose result lane (c, g), c = lane % 16, g = lane / 16, has
@@ -44,7 +52,7 @@ struct SlotDeal {
   bool longest_first;
 };
 struct GradArgs {
-  const _Float16 *q, *k, *v, *out, *d_out;
+  const _Float16 *q, *k, *v, *out, *remainder, *d_out;  // remainder: the forward pass's, or nullptr
   _Float16 *dq, *dk, *dv;  // dense; dq, or dk and dv, may be nullptr
   const float2* stats;     // [heads][T], the forward pass's
   float *lse, *minus_delta;  // [heads][T]: 2^kUp w = 2^(s t log2(e) - lse); a NaN: see packed_sums_kernel
@@ -79,15 +87,16 @@ __global__ __launch_bounds__(256) void packed_sums_kernel(GradArgs a) {
     const int64_t block = item / a.heads;
     const int head = (int)(item - block * a.heads);
     // all rows' loads first
-    h8 e[PASSES], o[PASSES], v[PASSES];
+    h8 e[PASSES], o[PASSES], rest[PASSES], v[PASSES];
     float2 stat[PASSES];
 #pragma unroll
     for (int pass = 0; pass < PASSES; ++pass) {
       const int64_t row = block * BLOCK + pass * RPP + row_of, at = (row * a.heads + head) * D + in_row * 8;
-      e[pass] = o[pass] = v[pass] = h8(0);
+      e[pass] = o[pass] = rest[pass] = v[pass] = h8(0);
       if (row < from || row >= to || row >= a.rows) continue;
       e[pass] = *reinterpret_cast<const h8*>(a.d_out + at);
       o[pass] = *reinterpret_cast<const h8*>(a.out + at);
+      if (a.remainder) rest[pass] = *reinterpret_cast<const h8*>(a.remainder + at);
       if (head < a.kv_heads) v[pass] = *reinterpret_cast<const h8*>(a.v + row * a.v_row + head * a.v_head + in_row * 8);
       stat[pass] = a.stats[head * a.rows + row];
     }
@@ -104,7 +113,7 @@ __global__ __launch_bounds__(256) void packed_sums_kernel(GradArgs a) {
       float dot = 0.f, ee = 0.f, vv = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        dot = fmaf((float)e[pass][i], (float)o[pass][i], dot);
+        dot = fmaf((float)e[pass][i], fmaf((float)rest[pass][i], 0x1p-10f, (float)o[pass][i]), dot);
         ee = fmaf((float)e[pass][i], (float)e[pass][i], ee);
         vv = fmaf((float)v[pass][i], (float)v[pass][i], vv);
       }
@@ -150,10 +159,9 @@ __device__ __forceinline__ h8 lds_read16(unsigned at) {
   return *(const __attribute__((address_space(3))) h8*)(uintptr_t)at;
 }
 
-// delta of a sequence's first 16 queries as the sum over their keys, a wavefront for a sequence and head.  There e . o is off by what
-// the output and the forward pass's weights were rounded by, which few keys do not average out: dq and dk of a text of 24 tokens are
-// 3.6e-4 off (2-norm, relative) with e . o, this way 3.1e-4, of which 2.1e-4 are the last rounding; single elements of long
-// texts' first rows 0.02 of the largest, this way 0.008.  3 us.
+// delta of a sequence's first 16 queries as the sum over their keys, a wavefront for a sequence and head.  e . o is off by what the
+// forward pass's weights were rounded by, which few keys do not average out: dq of a text of 24 tokens is (2-norm, relative) 2.9e-4
+// off with both, 8.6e-4 and this way 7.7e-4 where the channels of keys and values have offsets of 3.  3 us.
 template <int D>
 __global__ __launch_bounds__(256) void packed_first_kernel(GradArgs a) {
   constexpr int KS = (D + 31) / 32;
@@ -836,6 +844,7 @@ int launch_flash_attn_packed_backward(const PackedAttention& p, const PackedGrad
   a.k = (const _Float16*)p.k;
   a.v = (const _Float16*)p.v;
   a.out = (const _Float16*)p.out;
+  a.remainder = (const _Float16*)p.remainder;
   a.d_out = (const _Float16*)d.d_out;
   a.dq = (_Float16*)d.dq;
   a.dk = (_Float16*)d.dk;

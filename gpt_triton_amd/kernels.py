@@ -782,7 +782,7 @@ def _packed_pitches(q, k, v):
 
 
 def _packed_attention(q, k, v, starts, scale, out, with_stats):
-    """(out, what the gradients need of each row or None, the scale)."""
+    """(out, what the gradients need of each row and what the output's rounding takes or None, the scale)."""
     assert q.dim() == k.dim() == 3 and k.shape == v.shape, (q.shape, k.shape, v.shape)
     T, N, d = q.shape
     G = k.shape[1]
@@ -818,28 +818,28 @@ def _packed_attention(q, k, v, starts, scale, out, with_stats):
                                  (starts.data_ptr(), 8 * starts.shape[0], False)):
             apart = start + size <= at or end <= start
             assert apart or T == 0 or (may and start == at), "out may be a dense q alone"
-    stats = q.new_empty((N, T, 2), dtype=torch.float32) if with_stats else None
+    stats, remainder = (q.new_empty((N, T, 2), dtype=torch.float32), torch.empty_like(out)) if with_stats else (None, None)
     if T > 0:
         lib, sizes = _lib.load(), (starts.data_ptr(), starts.shape[0] - 1, T, N, G, d, *pitches, scale, _lib.GPTMI_F16)
         if with_stats:
-            _call(dev, "flash_attention_packed", lib.gptmi_flash_attn_packed_train, q_at, k_at, v_at, out.data_ptr(),
-                  stats.data_ptr(), *sizes)
+            _call(dev, "flash_attention_packed", lib.gptmi_flash_attn_packed_train_remainder, q_at, k_at, v_at,
+                  out.data_ptr(), stats.data_ptr(), remainder.data_ptr(), *sizes)
         else:
             _call(dev, "flash_attention_packed", lib.gptmi_flash_attn_packed, q_at, k_at, v_at, out.data_ptr(), *sizes)
-    return out, stats, scale
+    return out, stats, remainder, scale
 
 
 class _PackedAttentionFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, starts, scale):
-        out, stats, ctx.scale = _packed_attention(q, k, v, starts, scale, None, True)
-        ctx.save_for_backward(q, k, v, out, stats, starts)
+        out, stats, remainder, ctx.scale = _packed_attention(q, k, v, starts, scale, None, True)
+        ctx.save_for_backward(q, k, v, out, stats, remainder, starts)
         return out
 
     @staticmethod
     def backward(ctx, d_out):
         _first_derivative("flash_attention_packed")
-        q, k, v, out, stats, starts = ctx.saved_tensors
+        q, k, v, out, stats, remainder, starts = ctx.saved_tensors
         (T, N, d), G = q.shape, k.shape[1]
         need_q, need_k, need_v = ctx.needs_input_grad[:3]
         dq = q.new_empty((T, N, d)) if need_q else None
@@ -852,8 +852,8 @@ class _PackedAttentionFunction(torch.autograd.Function):
             lib = _lib.load()
             nbytes = lib.gptmi_flash_attn_packed_backward_workspace_bytes(starts.shape[0] - 1, T, N, G, d)
             workspace = _workspace(nbytes, q)
-            _call(q.get_device(), "flash_attention_packed", lib.gptmi_flash_attn_packed_backward, *addresses,
-                  out.data_ptr(), stats.data_ptr(), d_out.data_ptr(), starts.data_ptr(), _ptr(dq), _ptr(dk), _ptr(dv),
+            _call(q.get_device(), "flash_attention_packed", lib.gptmi_flash_attn_packed_backward_remainder, *addresses,
+                  out.data_ptr(), stats.data_ptr(), remainder.data_ptr(), d_out.data_ptr(), starts.data_ptr(), _ptr(dq), _ptr(dk), _ptr(dv),
                   starts.shape[0] - 1, T, N, G, d, *pitches, ctx.scale, workspace.data_ptr(), nbytes, _lib.GPTMI_F16)
         return dq, dk if need_k else None, dv if need_v else None, None, None
 

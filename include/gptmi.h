@@ -389,8 +389,15 @@ int gptmi_flash_attn_packed(const void* q, const void* k, const void* v, void* o
 
 /*
  * gptmi_flash_attn_packed in a training step: the same output, and in stats [N][T][2] (8-byte aligned) what the gradients need
- * of each row's softmax.
+ * of each row's softmax.  ..._remainder: and in remainder [T][N][d] (16-byte aligned, dense) 2^10 times what the rounding of the
+ * output takes, which makes its gradients exact in delta (below); of rows that belong to no sequence it is not written.
  */
+int gptmi_flash_attn_packed_train_remainder(const void* q, const void* k, const void* v, void* out,
+                                            float* stats, void* remainder, const int64_t* starts,
+                                            int64_t sequences, int64_t T, int64_t N, int64_t G, int64_t d,
+                                            int64_t q_row, int64_t q_head, int64_t k_row, int64_t k_head,
+                                            int64_t v_row, int64_t v_head, float scale, int dtype,
+                                            void* stream);
 int gptmi_flash_attn_packed_train(const void* q, const void* k, const void* v, void* out, float* stats,
                                   const int64_t* starts, int64_t sequences, int64_t T, int64_t N,
                                   int64_t G, int64_t d, int64_t q_row, int64_t q_head, int64_t k_row,
@@ -406,12 +413,23 @@ int gptmi_flash_attn_packed_train(const void* q, const void* k, const void* v, v
  *   and scale.  dq, or dk and dv, may be NULL.  The gradients overlap nothing.  Rows that belong to no sequence are not read
  *   and have gradients of 0.
  * w and u are formed again in fp32 and rounded to fp16 for the products, scaled by powers of two so that they stay normal
- * numbers; delta of a sequence's first 16 queries is the sum over their keys, which the output's rounding does not reach.  What hidden rows hold, infinities and NaN included, plays no part.  workspace:
+ * numbers.  ..._remainder takes delta from the output and its remainder; without it delta takes the output as it is rounded, up to
+ * 2^-11 |e| . |out| off, which dq has times the mean of the row's keys: little where keys and values have a mean of 0, most of
+ * the error where their channels have offsets.  delta of a sequence's first 16 queries is the sum over their keys in both.
+ * What hidden rows hold, infinities and NaN included, plays no part.  workspace:
  * gptmi_flash_attn_packed_backward_workspace_bytes(...) of the same sizes, 256-byte aligned.  N d up to 2^24, here and in
  * gptmi_flash_attn_packed_train.
  * No counterpart in the reference, which has no gradients.
  */
 size_t gptmi_flash_attn_packed_backward_workspace_bytes(int64_t sequences, int64_t T, int64_t N, int64_t G, int64_t d);
+int gptmi_flash_attn_packed_backward_remainder(const void* q, const void* k, const void* v, const void* out,
+                                               const float* stats, const void* remainder,
+                                               const void* d_out, const int64_t* starts, void* dq,
+                                               void* dk, void* dv, int64_t sequences, int64_t T, int64_t N,
+                                               int64_t G, int64_t d, int64_t q_row, int64_t q_head,
+                                               int64_t k_row, int64_t k_head, int64_t v_row, int64_t v_head,
+                                               float scale, void* workspace, size_t workspace_bytes,
+                                               int dtype, void* stream);
 int gptmi_flash_attn_packed_backward(const void* q, const void* k, const void* v, const void* out,
                                      const float* stats, const void* d_out, const int64_t* starts,
                                      void* dq, void* dk, void* dv, int64_t sequences, int64_t T,
