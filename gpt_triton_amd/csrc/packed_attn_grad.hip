@@ -5,8 +5,8 @@
 // over the queries i >= j of all the heads that share a key head.  The weights are formed again from q, k and the
 // statistic that the forward pass keeps of each row, so nothing of the size of the scores goes to memory.
 //
-// Launches: row sums (delta, and the largest rows of e and v); delta of each sequence's first queries as sums over their keys,
-// in place of the row sums'; the walk of the keys (dk and dv: a workgroup has a block of keys and walks over the queries) and the
+// Launches: row sums (delta, and e's and v's squares); what goes by sequences (delta of the first queries as sums over their
+// keys, in place of the row sums'; the largest rows of each key head); the walk of the keys (dk and dv: a workgroup has a block of keys and walks over the queries) and the
 // walk of the queries (dq: a block of queries, over the keys), up to d = 64 in one launch; and, where the heads over a key head
 // are divided among workgroups, their sums' join.  So each sum is formed by one workgroup in one order, without atomics, at the
 // cost of forming w and u twice: 7 products instead of 5.
@@ -45,7 +45,8 @@ namespace {
 // The weights are formed as 2^kUp w and u as 2^kUp f u, f a power of two: fp16 numbers of the size of one that stay
 // normal numbers down to 2^-28 of it.
 constexpr int kUp = 14;
-constexpr int kSums = 1024;  // workgroups of the row sums at most
+constexpr int kSums = 1024;         // workgroups of the row sums at most
+constexpr int kSequenceBlocks = 1 << 16;  // of either part of the sequences' launch
 
 struct SlotDeal {
   int slots, grid;
@@ -56,8 +57,10 @@ struct GradArgs {
   _Float16 *dq, *dk, *dv;  // dense; dq, or dk and dv, may be nullptr
   const float2* stats;     // [heads][T], the forward pass's
   float *lse, *minus_delta;  // [heads][T]: 2^kUp w = 2^(s t log2(e) - lse); a NaN: see packed_sums_kernel
-  float2* most;            // the largest e . e and v . v of each workgroup of the row sums
-  int mosts;
+  float *e_squares, *v_squares;  // e . e [heads][T], v . v [kv_heads][T], 0 where it is no number; behind the launch of the sequences, the
+                                 // first row of a sequence and key head has the largest of all of it
+  int firsts;                    // workgroups of that launch for the first queries, behind them those for the largest rows
+  bool whole;                    // each of which has a sequence and key head, else each wavefront
   const int64_t* starts;
   int64_t rows;  // T
   int sequences, heads, kv_heads;
@@ -69,7 +72,7 @@ struct GradArgs {
 };
 
 // ---------------------------------------------------------------------------
-// delta, lse and the largest rows.  Rows that belong to no sequence get gradients of 0 here.
+// delta, lse, and squares of e's and v's rows.  Rows that belong to no sequence get gradients of 0 here.
 // A row whose statistic is of scores key by key (infinities and NaN, scores of some thousands) gets lse = NaN: what meets it
 // comes out as NaN, and is done again with the statistic itself.
 // ---------------------------------------------------------------------------
@@ -78,11 +81,9 @@ __global__ __launch_bounds__(256) void packed_sums_kernel(GradArgs a) {
   constexpr int LPR = D / 8;          // lanes a row
   constexpr int RPP = 256 / LPR;      // rows a pass
   constexpr int BLOCK = RPP > 64 ? RPP : 64, PASSES = BLOCK / RPP;
-  __shared__ float2 largest[4];
   const int tid = threadIdx.x, in_row = tid % LPR, row_of = tid / LPR;
   const int64_t from = a.starts[0], to = a.starts[a.sequences];
   const int64_t items = (a.rows + BLOCK - 1) / BLOCK * a.heads;
-  float most_e = 0.f, most_v = 0.f;
   for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
     const int64_t block = item / a.heads;
     const int head = (int)(item - block * a.heads);
@@ -123,27 +124,15 @@ __global__ __launch_bounds__(256) void packed_sums_kernel(GradArgs a) {
         ee += __shfl_xor(ee, step);
         vv += __shfl_xor(vv, step);
       }
-      // rows with an infinity or a NaN spoil only what they are part of
-      if (ee < INFINITY) most_e = fmaxf(most_e, ee);
-      if (vv < INFINITY) most_v = fmaxf(most_v, vv);
       if (in_row == 0) {
         const int64_t place = head * a.rows + row;
         a.lse[place] = stat[pass].x - __builtin_amdgcn_logf(stat[pass].y) - kUp;  // to the base 2; NaN where .y < 0
         a.minus_delta[place] = -dot;
+        // rows with an infinity or a NaN spoil only what they are part of
+        a.e_squares[place] = ee < INFINITY ? ee : 0.f;
+        if (head < a.kv_heads) a.v_squares[place] = vv < INFINITY ? vv : 0.f;
       }
     }
-  }
-  most_e = wave_max(most_e);
-  most_v = wave_max(most_v);
-  if ((tid & 63) == 0) largest[tid >> 6] = {most_e, most_v};
-  __syncthreads();
-  if (tid == 0) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      most_e = fmaxf(most_e, largest[i].x);
-      most_v = fmaxf(most_v, largest[i].y);
-    }
-    a.most[blockIdx.x] = {most_e, most_v};
   }
 }
 
@@ -163,12 +152,12 @@ __device__ __forceinline__ h8 lds_read16(unsigned at) {
 // forward pass's weights were rounded by, which few keys do not average out: dq of a text of 24 tokens is (2-norm, relative) 2.9e-4
 // off with both, 8.6e-4 and this way 7.7e-4 where the channels of keys and values have offsets of 3.  3 us.
 template <int D>
-__global__ __launch_bounds__(256) void packed_first_kernel(GradArgs a) {
+__device__ __forceinline__ void first_queries(const GradArgs& a, int block) {
   constexpr int KS = (D + 31) / 32;
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t items = (int64_t)a.sequences * a.heads;
-  for (int64_t item = (int64_t)blockIdx.x * 4 + wave; item < items; item += (int64_t)gridDim.x * 4) {
+  for (int64_t item = (int64_t)block * 4 + wave; item < items; item += (int64_t)a.firsts * 4) {
     const int64_t sequence = item / a.heads;
     const int head = (int)(item - sequence * a.heads), kv_head = head / (a.heads / a.kv_heads);
     const int64_t begin = a.starts[sequence], end = a.starts[sequence + 1];
@@ -207,7 +196,61 @@ __global__ __launch_bounds__(256) void packed_first_kernel(GradArgs a) {
   }
 }
 
-// 2^n with 4 < 2^n bound <= 8 for bound = sqrt(ee vv), which |e . v| does not pass: |u| is at most bound / 2, since what
+// The largest of n numbers, 0 at least, in every thread of THREADS that share them: a wavefront, or the workgroup.
+template <int THREADS>
+__device__ __forceinline__ float largest_of(const float* x, int64_t pitch, int rows, unsigned n, float* lds) {
+  constexpr int U = 8;
+  float most = 0.f;
+  for (int row = 0; row < rows; ++row, x += pitch)
+    for (unsigned i = threadIdx.x % THREADS; i < n; i += U * THREADS) {
+      float some[U];
+#pragma unroll
+      for (int j = 0; j < U; ++j) some[j] = x[min(i + j * THREADS, n - 1)];
+#pragma unroll
+      for (int j = 0; j < U; ++j) most = fmaxf(most, some[j]);
+    }
+  most = wave_max(most);
+  if constexpr (THREADS > kWave) {
+    __syncthreads();
+    lds[threadIdx.x >> 6] = most;
+    __syncthreads();
+    most = fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3]));
+  }
+  return most;
+}
+
+// The largest rows of e and v of each sequence and key head, in its first row's places.
+template <int THREADS>
+__device__ __forceinline__ void largest_rows(const GradArgs& a, int block, int blocks, float* lds) {
+  constexpr int TEAMS = 256 / THREADS;
+  const int team = __builtin_amdgcn_readfirstlane(threadIdx.x / THREADS), per_key = a.heads / a.kv_heads;
+  const int64_t items = (int64_t)a.sequences * a.kv_heads;
+  for (int64_t item = (int64_t)block * TEAMS + team; item < items; item += (int64_t)blocks * TEAMS) {
+    const int64_t sequence = item / a.kv_heads;
+    const int kv_head = (int)(item - sequence * a.kv_heads);
+    const int64_t begin = a.starts[sequence], end = a.starts[sequence + 1];
+    const int64_t first = begin < 0 ? 0 : begin < a.rows ? begin : a.rows;
+    const int64_t last = end < first ? first : end < a.rows ? end : a.rows;
+    if (first == last) continue;
+    float* e = a.e_squares + ((int64_t)kv_head * per_key * a.rows + first);
+    float* v = a.v_squares + (kv_head * a.rows + first);
+    const float most_e = largest_of<THREADS>(e, a.rows, per_key, (unsigned)(last - first), lds);
+    const float most_v = largest_of<THREADS>(v, a.rows, 1, (unsigned)(last - first), lds);
+    if (threadIdx.x % THREADS == 0) *e = most_e, *v = most_v;  // all of them have been read
+  }
+}
+
+// What goes by sequences: their first queries' deltas, and their largest rows.
+template <int D>
+__global__ __launch_bounds__(256) void packed_sequences_kernel(GradArgs a) {
+  __shared__ float lds[4];
+  const int block = blockIdx.x;
+  if (block < a.firsts) first_queries<D>(a, block);
+  else if (a.whole) largest_rows<256>(a, block - a.firsts, (int)gridDim.x - a.firsts, lds);
+  else largest_rows<kWave>(a, block - a.firsts, (int)gridDim.x - a.firsts, lds);
+}
+
+// 2^n with 4 < 2^n bound <= 8 for bound = sqrt(ee vv), which |e . v| of the sequence does not pass: |u| is at most bound / 2, since what
 // w leaves of 1 is the others' part of delta, so 2^kUp 2^n |u| is at most 2^16, which 65519 rounds to.  (A u that is off
 // by more comes out as an infinity, and is done again.)
 __device__ __forceinline__ float factor_of(float ee, float vv) {
@@ -334,18 +377,12 @@ __device__ __forceinline__ void walk(const GradArgs& a, int id, int slots, bool 
     }
   };
 
-  // ---- the factor that keeps u in fp16's range: one for all rows where rows are summed over, each row's own otherwise
-  float most_e = 0.f, most_v = 0.f;
-#pragma unroll
-  for (int i = 0; i < kSums; i += kWave) {  // those that are not there repeat the last one
-    const float2 m = a.most[min(i + lane, a.mosts - 1)];
-    most_e = fmaxf(most_e, m.x);
-    most_v = fmaxf(most_v, m.y);
-  }
-  most_v = wave_max(most_v);
+  // ---- the factor that keeps u in fp16's range, by the largest rows of this sequence and key head: one for all rows where rows
+  // are summed over, each row's own otherwise
+  const float most_v = a.v_squares[kv_head * a.rows + block.first];
   float x_lse[NB], x_less[NB], factor[NB];  // of row c of block n: lse, less the factor's exponent, and -delta
   if constexpr (KEYS) {
-    factor[0] = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, factor_of(wave_max(most_e), most_v))));
+    factor[0] = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, factor_of(a.e_squares[(int64_t)kv_head * per_key * a.rows + block.first], most_v))));
   } else {
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
@@ -807,11 +844,16 @@ int launch_d(GradArgs a, hipStream_t st) {
   constexpr int NB = blocks_of<D>();
   constexpr int BLOCK = 256 / (D / 8) > 64 ? 256 / (D / 8) : 64;
   const int64_t items = (a.rows + BLOCK - 1) / BLOCK * a.heads;
-  a.mosts = (int)(items < kSums ? items : kSums);
   if (!deal_slots<NB>(a, a.heads, &a.deal[0]) || !deal_slots<NB>(a, a.kv_heads * a.shares, &a.deal[1])) return -2;
-  hipLaunchKernelGGL((packed_sums_kernel<D>), dim3(a.mosts), dim3(256), 0, st, a);
-  const int64_t firsts = ((int64_t)a.sequences * a.heads + 3) / 4;
-  hipLaunchKernelGGL((packed_first_kernel<D>), dim3((unsigned)(firsts < 1 << 16 ? firsts : 1 << 16)), dim3(256), 0, st, a);
+  hipLaunchKernelGGL((packed_sums_kernel<D>), dim3((unsigned)(items < kSums ? items : kSums)), dim3(256), 0, st, a);
+  const int64_t firsts = ((int64_t)a.sequences * a.heads + 3) / 4, keys = (int64_t)a.sequences * a.kv_heads;
+  a.firsts = (int)(firsts < kSequenceBlocks ? firsts : kSequenceBlocks);
+  // us, the launch, a workgroup / a wavefront for each sequence and key head: 1 x 8192 tokens, 12 heads 5.5 / 12.9, 16 x 1024, 32
+  // over 8 5.7 / 8.5, 48 x 300, 12 5.5 / 4.3, 400 x 40 14.1 / 10.2, 10000 x 3, 32 over 8 281 / 197
+  a.whole = a.rows >= 512ll * a.sequences;
+  const int64_t largest = a.whole ? keys : (keys + 3) / 4;
+  hipLaunchKernelGGL((packed_sequences_kernel<D>), dim3((unsigned)(a.firsts + (largest < kSequenceBlocks ? largest : kSequenceBlocks))),
+                     dim3(256), 0, st, a);
   static bool done[2];
   int rc = 0;
   if constexpr (D <= 64) {
@@ -829,12 +871,14 @@ int launch_d(GradArgs a, hipStream_t st) {
 
 }  // namespace
 
-// The largest rows' (kSums), lse and -delta, and the parts of dk and dv.
+// lse and -delta, e's and v's squares, and the parts of dk and dv.
+static size_t row_bytes(int64_t rows, int64_t heads, int64_t kv_heads) {
+  return ((size_t)rows * (size_t)(3 * heads + kv_heads) * sizeof(float) + 255) / 256 * 256;
+}
 size_t packed_attn_grad_bytes(int64_t rows, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t d) {
   const int shares = d <= 128 ? shares_of<blocks_of<128>()>(rows, sequences, (int)heads, (int)kv_heads)
                               : shares_of<blocks_of<256>()>(rows, sequences, (int)heads, (int)kv_heads);
-  const size_t stats = kSums * sizeof(float2) + (size_t)rows * (size_t)heads * 2 * sizeof(float);
-  return (stats + 255) / 256 * 256 + (shares > 1 ? (size_t)shares * 2 * (size_t)(rows * kv_heads * d) * sizeof(float) : 0);
+  return row_bytes(rows, heads, kv_heads) + (shares > 1 ? (size_t)shares * 2 * (size_t)(rows * kv_heads * d) * sizeof(float) : 0);
 }
 
 int launch_flash_attn_packed_backward(const PackedAttention& p, const PackedGradients& d, int head_size, void* workspace,
@@ -850,11 +894,11 @@ int launch_flash_attn_packed_backward(const PackedAttention& p, const PackedGrad
   a.dk = (_Float16*)d.dk;
   a.dv = (_Float16*)d.dv;
   a.stats = (const float2*)p.stats;
-  a.most = (float2*)workspace;
-  a.lse = (float*)(a.most + kSums);
+  a.lse = (float*)workspace;
   a.minus_delta = a.lse + p.rows * p.heads;
-  const size_t stats = kSums * sizeof(float2) + (size_t)p.rows * (size_t)p.heads * 2 * sizeof(float);
-  a.parts = (float*)((char*)workspace + (stats + 255) / 256 * 256);
+  a.e_squares = a.minus_delta + p.rows * p.heads;
+  a.v_squares = a.e_squares + p.rows * p.heads;
+  a.parts = (float*)((char*)workspace + row_bytes(p.rows, p.heads, p.kv_heads));
   a.shares = head_size <= 128 ? shares_of<blocks_of<128>()>(p.rows, p.sequences, (int)p.heads, (int)p.kv_heads)
                               : shares_of<blocks_of<256>()>(p.rows, p.sequences, (int)p.heads, (int)p.kv_heads);
   a.starts = p.starts;

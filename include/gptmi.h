@@ -412,8 +412,9 @@ int gptmi_flash_attn_packed_train(const void* q, const void* k, const void* v, v
  *   out, d_out, dq [T][N][d], dk, dv [T][G][d] dense; out, stats: gptmi_flash_attn_packed_train's for these q, k, v, starts
  *   and scale.  dq, or dk and dv, may be NULL.  The gradients overlap nothing.  Rows that belong to no sequence are not read
  *   and have gradients of 0.
- * w and u are formed again in fp32 and rounded to fp16 for the products, scaled by powers of two so that they stay normal
- * numbers.  ..._remainder takes delta from the output and its remainder; without it delta takes the output as it is rounded, up to
+ * w and u are formed again in fp32 and rounded to fp16 for the products, scaled by powers of two: u by the largest rows of e and v
+ * of its sequence and key head (dk) or of v and by its own row of e (dq), whatever else is packed, and down to 2^-28 of what that
+ * bounds it by they are normal numbers.  ..._remainder takes delta from the output and its remainder; without it delta takes the output as it is rounded, up to
  * 2^-11 |e| . |out| off, which dq has times the mean of the row's keys: little where keys and values have a mean of 0, most of
  * the error where their channels have offsets.  delta of a sequence's first 16 queries is the sum over their keys in both.
  * What hidden rows hold, infinities and NaN included, plays no part.  workspace:
