@@ -18,7 +18,8 @@ where the kernels cannot read the weight in place (fp16, K a multiple of 64); a 
 For scoring texts and learning from the scores, which the reference has nothing for: `flash_attention_packed` (prompts of different
 lengths without padding, grouped heads), `token_log_probs` (of rows of logits, with entropy, alternatives and gradient) and
 `distillation_loss` / `distillation_loss_and_grad` (against a teacher's top logits).  `flash_attention_packed` and
-`fused_embeddings` have gradients, and `clip_grad_norm_` clips all gradients together.  Tensors must live on the
+`fused_embeddings` have gradients, and `clip_grad_norm_` clips all gradients together; the other operators have none, and warn
+where an activation that they are given requires one (what their weights require is left alone).  Tensors must live on the
 GPU: there is no CPU path.  dropout_prob > 0 reproduces the reference's masks: Philox-4x32-10
 (Triton's tl.rand) with the kernels' default seed 1337 and the reference's offsets -- the column
 for the embedding, the flat index m*N + n for fused_ffn, query*Lk + key for the attention
@@ -28,6 +29,7 @@ import array
 import collections
 import math
 import os
+import warnings
 
 import torch
 from torch.autograd import forward_ad
@@ -75,6 +77,15 @@ def _ptr(t):
 
 def _workspace(nbytes, like):
     return like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+
+
+def _no_gradient(what, stacklevel=3):
+    """Of an operator without a gradient, called with an activation that requires one.  Its result is in no graph, so a backward
+    pass by the activation's other uses, a residual's for one, ends without an error and without this operator's part."""
+    if torch.is_grad_enabled():
+        warnings.warn(f"{what} has no gradient: its result is cut off from its input, and gradients that reach the input another "
+                      "way lack what would flow through here.  detach() the input, or use torch's operators, to say which is "
+                      "meant", stacklevel=stacklevel)
 
 
 class PackedWeight:
@@ -266,7 +277,9 @@ def clip_grad_norm_(grads, max_norm, scale=1.0, out=None):
 def fused_embeddings_layer_norm(x, wte, wpe, weight, bias):
     """(fused_embeddings(x, wte, wpe), fused_layer_norm(of that, weight, bias)) from one kernel:
     the embedding row is normalised while it is still in registers.  Both results are
-    bit-identical to the two separate calls.  No dropout (eval-mode forward)."""
+    bit-identical to the two separate calls.  No dropout (eval-mode forward), and no gradients."""
+    if wte.requires_grad or wpe.requires_grad:
+        _no_gradient("fused_embeddings_layer_norm")
     assert wte.shape[1] == wpe.shape[1]
     assert x.is_contiguous()
     assert wte.is_contiguous()
@@ -294,6 +307,8 @@ def fused_embeddings_layer_norm(x, wte, wpe, weight, bias):
 
 def fused_layer_norm(x, weight, bias):
     """LayerNorm over the last dim (eps = 1e-5, biased variance), same shape and dtype as x."""
+    if x.requires_grad:
+        _no_gradient("fused_layer_norm")
     assert x.is_contiguous()
     assert weight.is_contiguous()
     assert bias.is_contiguous()
@@ -312,6 +327,8 @@ def fused_layer_norm(x, weight, bias):
 
 def fused_softmax(x):
     """softmax over the last dim with fp32 statistics, same shape and dtype as x."""
+    if x.requires_grad:
+        _no_gradient("fused_softmax")
     assert x.is_contiguous()
     dev = _on_gpu(x)
     H = x.shape[-1]
@@ -352,6 +369,8 @@ def _linear(x, weight, bias, residual, z, gelu, dropout_prob, wlayout, what):
 
 def fused_ffn(x, weight, bias=None, residual=None, add_gelu=False, dropout_prob=0.0):
     """dropout(gelu?(x @ weight + bias)) + residual; weight is [K, N] (in x out)."""
+    if x.requires_grad or residual is not None and residual.requires_grad:
+        _no_gradient("fused_ffn")
     shape = x.shape
     K = shape[-1]
     N = weight.shape[1]
@@ -376,6 +395,8 @@ def lm_head(x, wte):
     """x @ wte^T: logits [*, V].  `wte` is the [V, H] embedding matrix itself (read in place, no
     transposed copy; the result is contiguous) or its `pack_lm_head` image (the result is then
     the [*, :V] view of a buffer whose rows are padded to a multiple of 64 logits)."""
+    if x.requires_grad:
+        _no_gradient("lm_head")
     shape = x.shape
     H = shape[-1]
     assert x.is_contiguous()
@@ -628,6 +649,8 @@ def distillation_loss_and_grad(logits, teacher_tokens, teacher_logits, temperatu
 def matmul_and_split_qkv(x, weight, bias, num_heads):
     """x [B, L, h] @ weight [h, 3h] + bias, returned as q, k, v [B, num_heads, L, h/num_heads],
     each contiguous; the GEMM's store does the head split."""
+    if x.requires_grad:
+        _no_gradient("matmul_and_split_qkv")
     batch_size, seqlen, _ = x.shape
     assert x.is_contiguous()
     assert weight.is_contiguous()
@@ -648,7 +671,7 @@ def matmul_and_split_qkv(x, weight, bias, num_heads):
         raise NotImplementedError("matmul_and_split_qkv: packed weights need head_size % 8 == 0")
     if head_size % 8 != 0:
         # the scatter epilogue stores 8-element groups; other head sizes take the plain GEMM
-        y = fused_ffn(x, weight, bias=bias)
+        y = fused_ffn(x.detach(), weight, bias=bias)
         q, k, v = y.split(hidden_size, dim=2)
         return tuple(t.view(batch_size, seqlen, num_heads, head_size).transpose(1, 2).contiguous()
                      for t in (q, k, v))
@@ -699,9 +722,11 @@ def layer_norm_ffn(x, ln_weight, ln_bias, weight, bias=None, add_gelu=False, the
 
     then=(weight2, bias2), with add_gelu and bias: the MLP's second product behind it in the same
     call -- the result is x + that @ weight2 + bias2 (fused_ffn with x as the residual, same bits)."""
+    if x.requires_grad:
+        _no_gradient("layer_norm_ffn")
     if then is not None:
         assert add_gelu and bias is not None
-        return mlp_block(x, ln_weight, ln_bias, weight, bias, *then, layer_norm_in_gemm=True)
+        return mlp_block(x.detach(), ln_weight, ln_bias, weight, bias, *then, layer_norm_in_gemm=True)
     dev = _check_layer_norm_linear(x, ln_weight, ln_bias, weight, bias, "layer_norm_ffn")
     K, N = weight.shape
     M = x.numel() // K
@@ -715,6 +740,8 @@ def layer_norm_ffn(x, ln_weight, ln_bias, weight, bias=None, add_gelu=False, the
 def layer_norm_matmul_and_split_qkv(x, ln_weight, ln_bias, weight, bias, num_heads):
     """matmul_and_split_qkv(fused_layer_norm(x, ln_weight, ln_bias), weight, bias, num_heads) in
     one launch, same bits; see `layer_norm_ffn`.  x [B, L, h]; head size a multiple of 8."""
+    if x.requires_grad:
+        _no_gradient("layer_norm_matmul_and_split_qkv")
     dev = _check_layer_norm_linear(x, ln_weight, ln_bias, weight, bias,
                                    "layer_norm_matmul_and_split_qkv")
     batch_size, seqlen, K = x.shape
@@ -739,6 +766,8 @@ def flash_attention_v1(q, k, v, dropout_prob=0.0, *, merged_heads_layout=False):
     returns the same values as a [B, N, L, d]-shaped view of a [B, L, N, d] buffer, so the
     caller's `.transpose(1, 2).contiguous()` head merge costs no copy.
     """
+    if q.requires_grad or k.requires_grad or v.requires_grad:
+        _no_gradient("flash_attention_v1")
     assert q.shape[:2] == k.shape[:2]
     assert q.shape[-1] == k.shape[-1]
     assert k.shape == v.shape
@@ -872,8 +901,10 @@ def flash_attention_packed(q, k, v, starts, scale=None, out=None):
     Gradients flow to q, k and v (dense ones, fp16), backward and once; of rows that belong to no sequence they are 0.  Each
     is one sum in one order: the same step gives the same bits.  With `out` given the call is a forward pass only."""
     _no_tangents("flash_attention_packed", q, k, v)
-    if out is None and (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
-        return _PackedAttentionFunction.apply(q, k, v, starts, scale)
+    if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
+        if out is None:
+            return _PackedAttentionFunction.apply(q, k, v, starts, scale)
+        _no_gradient("flash_attention_packed with out")
     return _packed_attention(q, k, v, starts, scale, out, False)[0]
 
 
@@ -936,6 +967,8 @@ def attention_block(x, ln_weight, ln_bias, qkv_weight, qkv_bias, proj_weight, pr
     (False: fp32 blocks of few rows with packed weights all the same; None: in no case); keep: a
     `dropout_mask` for dropout_prob of at least max(x.numel(), L * L) offsets, read instead of
     generating the masks here."""
+    if x.requires_grad or normed is not None and normed.requires_grad:
+        _no_gradient("attention_block")
     B, L, h = x.shape
     dtype = x.dtype
     assert ln_weight.shape[0] == ln_bias.shape[0] == proj_bias.shape[0] == h
@@ -970,6 +1003,8 @@ def mlp_block(x, ln_weight, ln_bias, weight1, bias1, weight2, bias2, dropout_pro
     """x + dropout(W2 . dropout(gelu(W1 . LayerNorm(x)))): the operators of an MLP block
     (gpt.py:91-111) behind one call of the library, with their bits; layer_norm_in_gemm: as in
     `layer_norm_ffn` and `attention_block`; keep: as in `attention_block`, of at least (rows of x) * max(inner, h) offsets."""
+    if x.requires_grad:
+        _no_gradient("mlp_block")
     h = x.shape[-1]
     dtype = x.dtype
     inner = weight1.shape[1]
@@ -1010,6 +1045,8 @@ def block_layers(x, pointers, num_heads, inner, normed=None, layer_norm_in_gemm=
     weights, no dropout; same launches, same bits.  pointers: 12 device addresses a layer, as gptmi_blocks
     lists them, of tensors that the caller has checked and keeps (`FusedGPT.forward` does).  out: where the
     result goes, x itself included; workspace: `blocks_workspace`, if the caller has it."""
+    if x.requires_grad:
+        _no_gradient("block_layers")
     B, L, h = x.shape
     dev = _on_gpu(x, normed, out)
     code = _dtype_code(x, "block_layers")
