@@ -164,8 +164,8 @@ __global__ __launch_bounds__(kThreads) void grad_scale_kernel(ClipArgs a) {
   const double norm = (double)a.scale * sqrt(sum);
   if (blockIdx.x == 0 && a.before == 0 && threadIdx.x == 0) *a.norm = (float)norm;
   if (a.chunks == 0) return;
-  // a NaN is passed on
-  const Factor by((double)a.scale * (norm <= (double)a.limit ? 1.0 : (double)a.limit / norm));
+  // a NaN is passed on, and an infinite norm leaves 0 or NaN whatever the limit is
+  const Factor by((double)a.scale * (norm <= (double)a.limit && norm < (double)INFINITY ? 1.0 : (double)a.limit / norm));
   const bool same = by.first == 1.f;
   if (same && a.in_place) return;
   Cursor cursor(a, a.chunks - 1 - blockIdx.x);

@@ -235,7 +235,8 @@ def clip_grad_norm_(grads, max_norm, scale=1.0, out=None):
     either type and of the order of its gradient, none of which overlaps anything else; a gradient itself may be in its place.
     scale: the inverse of a loss scale; max_norm infinity: the norm, and the gradients times scale.  Squares are summed in 64
     bits.  Gradients in place are written only where the factor is not 1.  An infinity among them makes the norm infinite and
-    the results 0 or NaN, a NaN makes all of them NaN: a step to skip."""
+    the results 0 or NaN, a NaN makes all of them NaN: a step to skip.  With max_norm infinity, scale 1 and all in place the
+    call is for the norm alone, which then is all that says so: no gradient is written, whatever it holds."""
     what = "clip_grad_norm_"
     grads = list(grads)
     outs = grads if out is None else list(out)

@@ -206,8 +206,9 @@ int gptmi_distillation_loss(const void* logits, int64_t ld, const int64_t* teach
 /*
  * The norm of n gradients together, and these at most at max_norm:
  *   norm = scale sqrt(sum g^2) over all elements of all tensors        out = scale min(1, max_norm / norm) g
- * Squares are summed in 64 bits.  An infinity among the gradients makes the norm infinite and out 0, and NaN in its place; a
- * NaN makes all of them NaN.
+ * Squares are summed in 64 bits.  An infinity among the gradients makes the norm infinite and out 0, and NaN in its place (all NaN
+ * where max_norm is infinity); a NaN makes all of them NaN.  With max_norm infinity, scale 1 and all in place nothing but the norm is
+ * written, whatever the gradients hold.
  *   grads, out, sizes, f16, out_f16: host arrays, read during the call: device addresses, elements (0 allowed), and whether the
  *   tensor is of type GPTMI_F16 (else GPTMI_F32).  out[i] may be grads[i], of the same type, which is then written only where it
  *   changes; what is written overlaps nothing else (GPTMI_ERR_INVALID)
