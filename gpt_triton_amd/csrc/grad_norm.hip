@@ -3,8 +3,8 @@
 //
 // Squares are summed in 64 bits, which vector units do at the rate of 32: no square is too large or too small, and the norm does
 // not depend on how the tensors are divided but for its last bits.  Two launches for each kTensors tensors: workgroups' sums over their
-// chunks, each in one order; then every workgroup adds all workgroups' sums (1024 numbers a launch, from the L2) in one order and scales its chunks,
-// the last first, which the memory-side cache still has.  Bound by memory: 148 tensors of a 124M model in fp32 (498 MB), below the limit,
+// chunks, each in one order; then every workgroup adds all workgroups' sums (1024 numbers a launch, from the L2; kJoin) in one order and
+// scales its chunks, the last first, which the memory-side cache still has.  Bound by memory: 148 tensors of a 124M model in fp32 (498 MB), below the limit,
 // 93 us, 5.4 TB/s; 355M elements from fp16 to fp32, 589 us, the squares at 4.3 TB/s and the scaling at 5.0.
 #include "common.h"
 #include "launch.h"
@@ -14,6 +14,10 @@ namespace {
 
 constexpr int kTensors = 152;    // of one launch: what kernel arguments, 4 KB, have room for (a model of 12 layers has 148)
 constexpr int kBlocks = 1024;    // workgroups of one launch at most
+// More workgroups' sums than these are added by a launch of their own, else by every workgroup that scales, work that grows with
+// the square of the launches.  us in a graph, fp32 in place, with that launch / without: 304 tensors of 110000 elements (2048 sums) 55 / 55,
+// 608 102 / 107, 2432 443 / 549, 6000 1084 / 1759; 60000 of 100 2440 / 5190.
+constexpr unsigned kJoin = 2 * kBlocks;
 constexpr int kThreads = 256;
 constexpr int kGroups = 8;       // of 8 elements a thread at a time
 constexpr int64_t kChunk = kThreads * 8 * kGroups;  // elements
@@ -155,12 +159,23 @@ __device__ __forceinline__ void scaled(const S* in, T* out, int n, int front, Fa
   }
 }
 
-__global__ __launch_bounds__(kThreads) void grad_scale_kernel(ClipArgs a) {
-  __shared__ double lds[4];
+__device__ __forceinline__ double sum_of_all(const double* sums, unsigned all, double* lds) {
   double sum = 0.0;
 #pragma unroll 8
-  for (unsigned i = threadIdx.x; i < a.all; i += kThreads) sum += a.sums[i];
-  sum = sum_of(sum, lds);
+  for (unsigned i = threadIdx.x; i < all; i += kThreads) sum += sums[i];
+  return sum_of(sum, lds);
+}
+
+// The sum of all workgroups' in the first one's place, by one workgroup.
+__global__ __launch_bounds__(kThreads) void grad_join_kernel(double* sums, unsigned all) {
+  __shared__ double lds[4];
+  const double sum = sum_of_all(sums, all, lds);  // behind a barrier: all have been read
+  if (threadIdx.x == 0) sums[0] = sum;
+}
+
+__global__ __launch_bounds__(kThreads) void grad_scale_kernel(ClipArgs a) {
+  __shared__ double lds[4];
+  const double sum = sum_of_all(a.sums, a.all, lds);
   const double norm = (double)a.scale * sqrt(sum);
   if (blockIdx.x == 0 && a.before == 0 && threadIdx.x == 0) *a.norm = (float)norm;
   if (a.chunks == 0) return;
@@ -205,6 +220,10 @@ void launch_clip_grad_norm(const Gradients& g, float scale, float limit, float* 
       a.chunks = a.before = 0;
       hipLaunchKernelGGL(grad_scale_kernel, dim3(1), dim3(kThreads), 0, st, a);
       break;
+    }
+    if (scale_them && a.all > kJoin) {
+      hipLaunchKernelGGL(grad_join_kernel, dim3(1), dim3(kThreads), 0, st, a.sums, a.all);
+      a.all = 1;
     }
     int64_t next = 0;
     a.before = 0;
