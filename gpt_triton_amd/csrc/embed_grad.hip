@@ -4,8 +4,9 @@
 // The sums are formed in fp32, each in one order, in the order of the positions and without atomics, so the same call
 // gives the same bits.  That takes each token's positions one behind the other:
 //   up to 256 tokens, one launch: every workgroup has a range of the vocabulary and looks all tokens through;
-//   more, a stable radix sort of the tokens with their positions, by one workgroup up to 16384 tokens, else a workgroup a tile of them, whose launches
-//   also write the zero rows and form the position table's sums; then runs of the sorted positions are summed, whoever has a
+//   more, a stable radix sort of the tokens with their positions, by one workgroup up to 16384 tokens, else a workgroup a tile of
+//   them (from 1.6 million tokens on with two launches a digit that add the tiles' counts), whose launches also write the zero
+//   rows and form the position table's sums; then runs of the sorted positions are summed, whoever has a
 //   token to itself writes its row, and what a token has in several runs is joined in a last launch.
 // Bound by memory: dz twice (once for each table), the tables' gradients once.  us, 512 x 300 tokens, fp16, 768 wide (236 MB of dz, 77 MB of
 // zero rows and sums): 143, of which the positions' sums and the runs' 55 and 52 at 4.3 and 4.6 TB/s; with one token in all places 175.
@@ -22,6 +23,11 @@ constexpr int kTile = 4096;        // tokens a workgroup sorts
 // tiles: 16 x 1024 tokens, 768 wide, fp32 57 / 63 and 60 / 71; 8 x 2000, 64 wide, fp16 49 / 63 and 48 / 70.
 constexpr int kOneTile = 16384;
 constexpr int kSortThreads = 1024;
+// Tiles whose counts each workgroup that moves adds by itself, work that grows with their square; more, and two launches a digit do
+// it for all.  us, calls, 64 wide, fp16, by itself / by the launches: 256 tiles 155 / 182, 512 320 / 302, 1024 778 / 570; 4096, 16 wide
+// 6140 / 2150.
+constexpr int kManyTiles = 400;
+constexpr int kGroupTiles = 256;   // of these a workgroup
 constexpr int kMaxBits = 9;        // of a digit
 constexpr int kFill = 65536;       // bytes of zero rows a workgroup
 
@@ -69,7 +75,9 @@ struct EmbedGradArgs {
   int64_t positions, fill, table_fills;
   int64_t behind;           // elements of the position table behind the first P rows, zeros
   unsigned *keys[2], *at[2];  // tokens (V: none) and positions
-  unsigned* hist;           // [tiles][1 << bits]
+  unsigned* hist;           // [tiles][1 << bits]: counts, or the counts of the tiles in front
+  unsigned* group_counts;   // [groups + 1][1 << bits] where there are many tiles: of kGroupTiles tiles each, and of all
+  bool many;
   // the sums'
   const unsigned *sorted, *order;
   float* parts;             // [runs][2][H]: what a run has of a token that began in front of it, and of one that goes on behind
@@ -232,6 +240,8 @@ struct SortLds {
   unsigned counts[kWaves][1 << kMaxBits];
   unsigned sums[kWaves];
 };
+
+__host__ __device__ __forceinline__ int64_t groups_of(int64_t tiles) { return (tiles + kGroupTiles - 1) / kGroupTiles; }
 
 // Lanes of the wavefront with the same digit.
 __device__ __forceinline__ uint64_t same_digit(unsigned digit, int bits, bool valid) {
@@ -405,6 +415,48 @@ __global__ __launch_bounds__(kSortThreads) void embed_grad_count_kernel(EmbedGra
   if (tid < digits) a.hist[(int64_t)blockIdx.x * digits + tid] = lds.counts[tid];
 }
 
+// Many tiles: the counts of kGroupTiles tiles together,
+__global__ __launch_bounds__(kSortThreads) void embed_grad_group_kernel(EmbedGradArgs a) {
+  __shared__ unsigned other[1 << kMaxBits];
+  constexpr int HALF = kSortThreads / 2;
+  const int digits = 1 << a.bits, digit = threadIdx.x % HALF, half = threadIdx.x / HALF;
+  const int64_t first = (int64_t)blockIdx.x * kGroupTiles, last = min(first + kGroupTiles, (int64_t)a.tiles);
+  unsigned sum = 0;
+  if (digit < digits) {
+#pragma unroll 16
+    for (int64_t t = first + half; t < last; t += 2) sum += a.hist[t * digits + digit];
+  }
+  if (half == 1) other[digit] = sum;
+  __syncthreads();
+  if (half == 0 && digit < digits) a.group_counts[(int64_t)blockIdx.x * digits + digit] = sum + other[digit];
+}
+// and each tile's counts as those of the tiles in front of it.
+__global__ __launch_bounds__(kSortThreads / 2) void embed_grad_in_front_kernel(EmbedGradArgs a) {
+  static_assert(kSortThreads / 2 >= 1 << kMaxBits, "a thread a digit");
+  constexpr int U = 16;
+  const int digits = 1 << a.bits, digit = threadIdx.x, groups = gridDim.x;
+  if (digit >= digits) return;
+  unsigned in_front = 0, total = 0;
+#pragma unroll 16
+  for (int g = 0; g < groups; ++g) {
+    const unsigned n = a.group_counts[(int64_t)g * digits + digit];
+    in_front += g < (int)blockIdx.x ? n : 0;
+    total += n;
+  }
+  if (blockIdx.x == 0) a.group_counts[(int64_t)groups * digits + digit] = total;  // behind what the other workgroups read
+  const int64_t first = (int64_t)blockIdx.x * kGroupTiles, last = min(first + kGroupTiles, (int64_t)a.tiles);
+  for (int64_t t = first; t < last; t += U) {
+    unsigned n[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) n[j] = a.hist[min(t + j, last - 1) * digits + digit];
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      if (t + j < last) a.hist[(t + j) * digits + digit] = in_front;
+      in_front += n[j];
+    }
+  }
+}
+
 // Moves the tokens to their places by one digit.
 template <typename T, int VN, bool FIRST>
 __global__ __launch_bounds__(kSortThreads) void embed_grad_move_kernel(EmbedGradArgs a, int shift, int from) {
@@ -431,7 +483,12 @@ __global__ __launch_bounds__(kSortThreads) void embed_grad_move_kernel(EmbedGrad
   }
   // of each digit, the tokens of all tiles, and of those in front of this one
   unsigned total = 0, in_front = 0;
-  if (tid < digits) {
+  if (a.many) {
+    if (tid < digits) {
+      in_front = a.hist[(int64_t)blockIdx.x * digits + tid];
+      total = a.group_counts[(int64_t)groups_of(a.tiles) * digits + tid];
+    }
+  } else if (tid < digits) {
 #pragma unroll 16
     for (int t = 0; t < a.tiles; ++t) {
       const unsigned n = a.hist[(int64_t)t * digits + tid];
@@ -627,6 +684,7 @@ int launch_as(EmbedGradArgs a, hipStream_t st) {
   const int passes = (width + kMaxBits - 1) / kMaxBits;
   a.bits = (width + passes - 1) / passes;
   a.tiles = (int)((a.tokens + kTile - 1) / kTile);
+  a.many = a.tiles > kManyTiles;
   const auto fills_of = [](int64_t elements) { return (elements * (int64_t)sizeof(T) + kFill - 1) / kFill; };
   a.table_fills = fills_of(a.V * a.H);
   const int64_t fills = a.table_fills + fills_of(a.behind);
@@ -657,6 +715,11 @@ int launch_as(EmbedGradArgs a, hipStream_t st) {
         hipLaunchKernelGGL((embed_grad_count_kernel<T, VN, true>), count, dim3(kSortThreads), 0, st, a, shift, from);
       else
         hipLaunchKernelGGL((embed_grad_count_kernel<T, VN, false>), count, dim3(kSortThreads), 0, st, a, shift, from);
+      if (a.many) {
+        const dim3 groups((unsigned)groups_of(a.tiles));
+        hipLaunchKernelGGL(embed_grad_group_kernel, groups, dim3(kSortThreads), 0, st, a);
+        hipLaunchKernelGGL(embed_grad_in_front_kernel, groups, dim3(kSortThreads / 2), 0, st, a);
+      }
       const dim3 move = part(3, pass);
       if (pass == 0)
         hipLaunchKernelGGL((embed_grad_move_kernel<T, VN, true>), move, dim3(kSortThreads), 0, st, a, shift, from);
@@ -676,13 +739,18 @@ int launch_as(EmbedGradArgs a, hipStream_t st) {
 }
 
 int64_t up(int64_t bytes) { return (bytes + 255) & ~(int64_t)255; }
+// Of the tiles' counts, and the groups' and all together.
+int64_t hist_bytes(int64_t tokens) {
+  const int64_t tiles = (tokens + kTile - 1) / kTile;
+  return up(tiles * (4 << kMaxBits)) + (tiles > kManyTiles ? up((groups_of(tiles) + 1) * (4 << kMaxBits)) : 0);
+}
 
 }  // namespace
 
 size_t embed_grad_bytes(int64_t tokens, int64_t H) {
   if (tokens <= kFew) return 0;
-  const int64_t run = run_of(tokens), runs = (tokens + run - 1) / run, tiles = (tokens + kTile - 1) / kTile;
-  return (size_t)(4 * up(tokens * 4) + up(tiles * (4 << kMaxBits)) + up(runs * 2 * H * 4));
+  const int64_t run = run_of(tokens), runs = (tokens + run - 1) / run;
+  return (size_t)(4 * up(tokens * 4) + hist_bytes(tokens) + up(runs * 2 * H * 4));
 }
 
 int launch_embed_backward(const int64_t* ids, const void* dz, void* d_wte, void* d_wpe, int64_t tokens, int64_t L, int64_t V,
@@ -701,7 +769,8 @@ int launch_embed_backward(const int64_t* ids, const void* dz, void* d_wte, void*
     a.at[i] = (unsigned*)(ws + (2 * i + 1) * up(tokens * 4));
   }
   a.hist = (unsigned*)(ws + 4 * up(tokens * 4));
-  a.parts = (float*)((char*)a.hist + up((tokens + kTile - 1) / kTile * (4 << kMaxBits)));
+  a.group_counts = (unsigned*)((char*)a.hist + up((tokens + kTile - 1) / kTile * (4 << kMaxBits)));
+  a.parts = (float*)((char*)a.hist + hist_bytes(tokens));
   const uintptr_t all = (uintptr_t)dz | (uintptr_t)d_wte | (uintptr_t)d_wpe;
   if (f16) return H % 8 == 0 && (all & 15) == 0 ? launch_as<_Float16, 8>(a, st) : launch_as<_Float16, 1>(a, st);
   return H % 4 == 0 && (all & 15) == 0 ? launch_as<float, 4>(a, st) : launch_as<float, 1>(a, st);
