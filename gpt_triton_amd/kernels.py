@@ -859,9 +859,15 @@ def _packed_attention(q, k, v, starts, scale, out, with_stats):
     return out, stats, remainder, scale
 
 
+# Elements of a row of the output up to which the gradients read it; beyond, the call has an output only.
+_MAX_GRADIENT_ROW = 1 << 24
+
+
 class _PackedAttentionFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, starts, scale):
+        if q.dim() == 3 and q.shape[1] * q.shape[2] > _MAX_GRADIENT_ROW:
+            return _packed_attention(q, k, v, starts, scale, None, False)[0]
         out, stats, remainder, ctx.scale = _packed_attention(q, k, v, starts, scale, None, True)
         ctx.save_for_backward(q, k, v, out, stats, remainder, starts)
         return out
@@ -869,6 +875,8 @@ class _PackedAttentionFunction(torch.autograd.Function):
     @staticmethod
     def backward(ctx, d_out):
         _first_derivative("flash_attention_packed")
+        if not ctx.saved_tensors:
+            raise NotImplementedError(f"flash_attention_packed: rows of more than {_MAX_GRADIENT_ROW} elements have no gradient")
         q, k, v, out, stats, remainder, starts = ctx.saved_tensors
         (T, N, d), G = q.shape, k.shape[1]
         need_q, need_k, need_v = ctx.needs_input_grad[:3]
@@ -900,7 +908,9 @@ def flash_attention_packed(q, k, v, starts, scale=None, out=None):
     nothing else).
 
     Gradients flow to q, k and v (dense ones, fp16), backward and once; of rows that belong to no sequence they are 0.  Each
-    is one sum in one order: the same step gives the same bits.  With `out` given the call is a forward pass only."""
+    is one sum in one order: the same step gives the same bits.  A call that may have to form them keeps q, k, v, the output, as
+    much again for what its rounding takes, and 8 bytes a row and head.  With `out` given the call is a forward pass only, and
+    so it is for rows of more than 2^24 elements (N d), whose backward pass raises NotImplementedError."""
     _no_tangents("flash_attention_packed", q, k, v)
     if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
         if out is None:
