@@ -24,12 +24,15 @@
 // that w and u, rounded to fp16, are the second operand of the sums over y as they stand.
 //
 // What bounds it: the matrix pipe and the vector pipe in turn.  us, the row sums and the walks, causal:
-//   25 heads of 64, 1 x 8192 tokens: 740 (7 products of L^2 d operations a head: 1015 TFLOP/s, where a large library product
-//     reaches 1212; MFMA 0.39 and VALU 0.45 busy at 2.2 GHz); two wavefronts a SIMD and two launches 840
-//   32 heads of 128 over 8, texts of 4096, 4095, 2049, 1933, 517 and 64: 1310 (915 TFLOP/s; the keys' walk with one wavefront a SIMD, whose steps overlap; without
-//     overlap 1550); eight narrower wavefronts for it 844 where it takes 834, tiles of 128 rows 949
-//   12 heads of 64, 48 texts of up to 1024, 7276 rows: 68, 48 x 300: 85, of which the row sums 14, workgroups' starts and finding their rows
-//     10, loads in front of the walks 17, the walks 34, the results 10
+//   25 heads of 64, 1 x 8192 tokens: 775 (7 products of L^2 d operations a head: 970 TFLOP/s, where a large library product
+//     reaches 1212; MFMA 0.44 and VALU 0.51 busy at 2.1 GHz); two wavefronts a SIMD and two launches 13 % more
+//   32 heads of 128 over 8, texts of 4096, 4095, 2049, 1933, 517 and 64: 1400 (855 TFLOP/s; the keys' walk with one wavefront a SIMD,
+//     whose steps overlap; without overlap 18 % more); eight narrower wavefronts for it 844 where it took 834, tiles of 128 rows 949
+//   12 heads of 64, 48 texts of up to 1024, 7276 rows: 62, 48 x 300: 81, of which the row sums 17, the sequences'
+//     launch 4, and more than half of the rest workgroups' starts, finding their rows, first loads and results
+//   12 heads of 32, 16 x 1024: 98, of which the walks 80 to 90; the vector pipe is busy for 45 of these (70 cycles for 64 pairs of a query
+//     and a key in both walks, 32 of them exponentials), the matrix pipe for 18; of 16 91, 46 and 14
+// Registers that are spilled (64 wide 32, 256 wide 13 and 81) are used row by row, which the next lines are about, and behind the walks' loops.
 // A backward pass with an infinity or a NaN among the output's gradients goes row by row where that reaches, 10 to 50 times as long
 // (12 heads of 64, 1 x 1024: 1400 us, 48 x 300: 560 for one of them, 2000 for nothing else): a step that a training loop skips.
 #include <type_traits>
@@ -291,7 +294,7 @@ __device__ __forceinline__ void walk(const GradArgs& a, int id, int slots, bool 
   constexpr int GROUPS = TY / 32, PLACES = places_of(D, KEYS);
   constexpr int ROWS = TY / 2, NDMA = ROWS / RPI;  // rows of a tile that a wavefront brings, and its load instructions
   // Unit u of row r of a tile lies at u ^ key(r).  A row read takes unit g of rows 8 (c / 4) + c % 4 (+ 4 b), served lanes
-  // 0..3, 12..15, 20..27 first, a transposing one two units of rows 8 g + 0..3 (+ 4), two g at a time: in different banks both.
+  // 0..3, 12..15, 20..27 first, a transposing one two units of rows 8 g + 0..3 (+ 4), two g at a time: in different banks both (but for D = 16).
   const auto key = [](int r) {
     return 2 * (CH >= 16 ? (r & 3) | (r >> 3 & 1) << 2 : CH == 8 ? (r >> 1 & 1) | (r >> 3 & 1) << 1 : CH == 4 ? r >> 3 & 1 : 0);
   };
