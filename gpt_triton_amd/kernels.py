@@ -652,6 +652,7 @@ def matmul_and_split_qkv(x, weight, bias, num_heads):
     each contiguous; the GEMM's store does the head split."""
     if x.requires_grad:
         _no_gradient("matmul_and_split_qkv")
+        x = x.detach()
     batch_size, seqlen, _ = x.shape
     assert x.is_contiguous()
     assert weight.is_contiguous()
@@ -672,7 +673,7 @@ def matmul_and_split_qkv(x, weight, bias, num_heads):
         raise NotImplementedError("matmul_and_split_qkv: packed weights need head_size % 8 == 0")
     if head_size % 8 != 0:
         # the scatter epilogue stores 8-element groups; other head sizes take the plain GEMM
-        y = fused_ffn(x.detach(), weight, bias=bias)
+        y = fused_ffn(x, weight, bias=bias)
         q, k, v = y.split(hidden_size, dim=2)
         return tuple(t.view(batch_size, seqlen, num_heads, head_size).transpose(1, 2).contiguous()
                      for t in (q, k, v))
@@ -725,9 +726,10 @@ def layer_norm_ffn(x, ln_weight, ln_bias, weight, bias=None, add_gelu=False, the
     call -- the result is x + that @ weight2 + bias2 (fused_ffn with x as the residual, same bits)."""
     if x.requires_grad:
         _no_gradient("layer_norm_ffn")
+        x = x.detach()
     if then is not None:
         assert add_gelu and bias is not None
-        return mlp_block(x.detach(), ln_weight, ln_bias, weight, bias, *then, layer_norm_in_gemm=True)
+        return mlp_block(x, ln_weight, ln_bias, weight, bias, *then, layer_norm_in_gemm=True)
     dev = _check_layer_norm_linear(x, ln_weight, ln_bias, weight, bias, "layer_norm_ffn")
     K, N = weight.shape
     M = x.numel() // K
