@@ -270,7 +270,7 @@ def clip_grad_norm_(grads, max_norm, scale=1.0, out=None):
     nbytes = lib.gptmi_clip_grad_norm_workspace_bytes(n)
     ws = _workspace(nbytes, norm)
     _call(dev, what, lib.gptmi_clip_grad_norm, at, at if out is None else at + 8 * n, sizes.buffer_info()[0], halves,
-          halves if out is None else halves[n:], n, scale, max_norm, norm.data_ptr(), ws.data_ptr(), nbytes)
+          halves if out is None else halves[n:], n, scale, max_norm, norm.data_ptr(), _ptr(ws), nbytes)
     torch.autograd.graph.increment_version(outs)
     return norm
 

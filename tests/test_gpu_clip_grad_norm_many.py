@@ -50,3 +50,10 @@ def test_captured(K, gpu_device):
         eager = [torch.empty_like(o) for o in out]
         assert torch.equal(norm, K.clip_grad_norm_(grads, 1.0, out=eager))
         assert all(torch.equal(a, b) for a, b in zip(out, eager))
+
+
+def test_too_many(K, gpu_device):
+    empty = torch.empty(0, device=gpu_device)
+    assert float(K.clip_grad_norm_([empty] * 2**20, 1.0)) == 0.0
+    with pytest.raises(NotImplementedError, match="beyond the supported"):
+        K.clip_grad_norm_([empty] * (2**20 + 1), 1.0)
