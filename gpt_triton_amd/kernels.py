@@ -877,9 +877,10 @@ class _PackedAttentionFunction(torch.autograd.Function):
     @staticmethod
     def backward(ctx, d_out):
         _first_derivative("flash_attention_packed")
-        if not ctx.saved_tensors:
+        saved = ctx.saved_tensors  # once: each reading unpacks them, which checkpoints allow no second time
+        if not saved:
             raise NotImplementedError(f"flash_attention_packed: rows of more than {_MAX_GRADIENT_ROW} elements have no gradient")
-        q, k, v, out, stats, remainder, starts = ctx.saved_tensors
+        q, k, v, out, stats, remainder, starts = saved
         (T, N, d), G = q.shape, k.shape[1]
         need_q, need_k, need_v = ctx.needs_input_grad[:3]
         dq = q.new_empty((T, N, d)) if need_q else None
@@ -893,8 +894,8 @@ class _PackedAttentionFunction(torch.autograd.Function):
             nbytes = lib.gptmi_flash_attn_packed_backward_workspace_bytes(starts.shape[0] - 1, T, N, G, d)
             workspace = _workspace(nbytes, q)
             _call(q.get_device(), "flash_attention_packed", lib.gptmi_flash_attn_packed_backward_remainder, *addresses,
-                  out.data_ptr(), stats.data_ptr(), remainder.data_ptr(), d_out.data_ptr(), starts.data_ptr(), _ptr(dq), _ptr(dk), _ptr(dv),
-                  starts.shape[0] - 1, T, N, G, d, *pitches, ctx.scale, workspace.data_ptr(), nbytes, _lib.GPTMI_F16)
+                  out.data_ptr(), stats.data_ptr(), remainder.data_ptr(), d_out.data_ptr(), starts.data_ptr(), _ptr(dq),
+                  _ptr(dk), _ptr(dv), starts.shape[0] - 1, T, N, G, d, *pitches, ctx.scale, workspace.data_ptr(), nbytes, _lib.GPTMI_F16)
         return dq, dk if need_k else None, dv if need_v else None, None, None
 
 
